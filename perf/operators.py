@@ -263,7 +263,7 @@ def run(state):
         return dict(keys=cache.keys, vals=cache.vals, lengths=lengths, kept=kept, weight=weight)
     if case['weights']:
         out, weight = cache.attend(s['q'], s['table'], s['starts'], s['lengths'], most=case['tokens'],
-                                   weight=s['weight'], weight_out=s['weight_out'])
+                                   weight=s['weight'])      # kept in place, pass after pass, as the plain form does
         return dict(out=out, weight=weight)
     return dict(out=cache.attend(s['q'], s['table'], s['starts'], s['lengths'], most=case['tokens']))
 
