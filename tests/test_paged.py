@@ -1,0 +1,193 @@
+"""CPU tests of the paged cache's calls (vesta/paged.py): what is refused, and
+that every launch asked for covers what its kernel indexes. The launches are
+recorded, not made."""
+import contextlib
+
+import pytest
+import torch
+
+from vesta import paged
+from vesta.paged import PagedCache
+
+
+class _Recorder:
+    def __init__(self, log):
+        self.log = log
+
+    def __getattr__(self, name):
+        def launch(grid, block, stream, *vals):
+            assert len(vals) == len(paged.SIGNATURES[name]), name
+            paged.struct.pack('@' + ''.join(paged._CODES[c] for c in paged.SIGNATURES[name]), *vals)
+            self.log.append((name, grid, block, vals))
+        return launch
+
+
+class _Dry(PagedCache):
+    """A cache on the CPU whose launches go into ``log``."""
+
+    def __init__(self, *a, dtype='f16', **kw):
+        kw = {**dict(width=64, layers=1, page=64), **kw}
+        self._shape(*a, kw['width'], kw['layers'], kw['page'], dtype)
+        self._allocate(torch.device('cpu'))
+        self.log = []
+        self._kind = {self.dtype: _Recorder(self.log)}
+        if dtype == 'f16':
+            self._kind[torch.float32] = _Recorder(self.log)
+
+    def _on_device(self):
+        return contextlib.nullcontext()
+
+    def _stream(self):
+        return 0
+
+
+def _ints(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def _batch(B=2, N=3, M=5):
+    return torch.zeros(B, N, dtype=torch.int32), _ints(*[0] * B, M), _ints(*[M] * B)
+
+
+def _rows(M, H, E=64, dtype=torch.float16):
+    return torch.zeros(M, H, E, dtype=dtype)
+
+
+@pytest.mark.parametrize('bad', [dict(pages=0), dict(heads=0), dict(layers=0), dict(page=0), dict(page=48),
+                                 dict(page=1 << 17), dict(width=80), dict(dtype='f32'), dict(pages=1 << 25)])
+def test_shapes_refused(bad):
+    with pytest.raises(ValueError):
+        PagedCache(**{**dict(pages=4, heads=2), **bad})
+
+
+def test_no_gpu_raises():
+    if torch.cuda.is_available():
+        pytest.skip('a GPU is present')
+    with pytest.raises(RuntimeError, match='no GPU'):
+        PagedCache(4, 2)
+
+
+def test_append_refusals():
+    c = _Dry(8, 3)
+    table, starts, lengths = _batch()
+    k = _rows(5, 3)
+    c.append(k, k, table, starts, lengths)
+    assert [e[0] for e in c.log] == ['pg_append16']
+    c.append(k.float(), k.float(), table, starts, lengths)
+    assert c.log[-1][0] == 'pg_append32' and c.log[-1][1] * 256 >= 5 * 3 * 8
+    n = len(c.log)
+    for args, err in (((k.double(), k, table, starts, lengths), TypeError),
+                      ((k.bfloat16(), k, table, starts, lengths), TypeError),
+                      ((k, k.float(), table, starts, lengths), TypeError),
+                      ((k, _rows(4, 3), table, starts, lengths), ValueError),
+                      ((_rows(5, 2), _rows(5, 2), table, starts, lengths), ValueError),
+                      ((_rows(5, 3, 32), _rows(5, 3, 32), table, starts, lengths), ValueError),
+                      ((k[0], k[0], table, starts, lengths), ValueError),
+                      ((k, k, table.long(), starts, lengths), TypeError),
+                      ((k, k, table.t(), starts, lengths), TypeError),
+                      ((k, k, table[0], starts, lengths), ValueError),
+                      ((k, k, table, starts[:2], lengths), ValueError),
+                      ((k, k, table, starts, lengths[:1]), ValueError),
+                      ((k, k, table, starts, lengths.long()), TypeError),
+                      ((k, k, table, starts, lengths, 1), ValueError),
+                      ((k, k, table, starts, lengths, -1), ValueError)):
+        with pytest.raises(err):
+            c.append(*args)
+    assert len(c.log) == n
+
+
+def test_strides():
+    """Any strides of the rows and heads, as the columns of one product's output; not of the values in a row."""
+    c = _Dry(8, 3)
+    table, starts, lengths = _batch()
+    qkv = torch.zeros(5, 9, 64, dtype=torch.float16)
+    q, k, v = qkv[:, :3], qkv[:, 3:6], qkv[:, 6:]
+    c.append(k, v, table, starts, lengths)
+    assert c.log[-1][3][2:6] == (9 * 64, 64, 9 * 64, 64)
+    c.attend(q, table, starts, lengths)
+    assert c.log[-1][3][1:3] == (9 * 64, 64)
+    c.attend(torch.zeros(3, 5, 64, dtype=torch.float16).transpose(0, 1), table, starts, lengths)
+    assert c.log[-1][3][1:3] == (64, 5 * 64)
+    odd = torch.zeros(5 * 3 * 64 + 4, dtype=torch.float16)
+    for bad in (odd[4:].view(5, 3, 64), torch.zeros(5, 3, 128, dtype=torch.float16)[:, :, ::2],
+                torch.zeros(5, 3, 68, dtype=torch.float16)[:, :, :64]):
+        with pytest.raises(ValueError):
+            c.append(bad, k, table, starts, lengths)
+        with pytest.raises(ValueError):
+            c.attend(bad, table, starts, lengths)
+        with pytest.raises(ValueError):
+            c.attend(q, table, starts, lengths, out=bad)
+
+
+def test_attend_refusals():
+    c = _Dry(8, 3)
+    table, starts, lengths = _batch()
+    q = _rows(5, 6)
+    w = torch.zeros(2, 3, 3 * 64)
+    for kw, err in ((dict(q=_rows(5, 4)), ValueError), (dict(q=_rows(5, 0)), ValueError),
+                    (dict(q=q.bfloat16()), TypeError), (dict(q=q.double()), TypeError), (dict(scale=0.0), ValueError),
+                    (dict(scale=-1.0), ValueError), (dict(scale=float('nan')), ValueError),
+                    (dict(scale=float('inf')), ValueError), (dict(most=0), ValueError),
+                    (dict(out=q.float()), TypeError), (dict(out=_rows(4, 6)), ValueError),
+                    (dict(weight=w.half()), TypeError), (dict(weight=w[:, :, :-1]), TypeError),
+                    (dict(weight=w[:, :, :-1].contiguous()), ValueError), (dict(weight=w[:1]), ValueError),
+                    (dict(weight=w[None]), ValueError), (dict(weight_out=w), ValueError),
+                    (dict(weight=w, weight_out=w[:, :, :64].contiguous()), ValueError)):
+        with pytest.raises(err):
+            c.attend(**{**dict(q=q, table=table, starts=starts, lengths=lengths), **kw})
+    assert not c.log
+    with pytest.raises(TypeError):
+        _Dry(8, 3, dtype='bf16').attend(q.float(), table, starts, lengths)
+
+
+def test_attend_results():
+    c = _Dry(8, 3)
+    table, starts, lengths = _batch()
+    for dtype in (torch.float16, torch.float32):
+        q = _rows(5, 6, dtype=dtype)
+        out = c.attend(q, table, starts, lengths)
+        assert out.shape == q.shape and out.dtype == dtype
+        assert c.attend(q, table, starts, lengths, out=out) is out
+    w = torch.zeros(2, 3, 3 * 64)
+    assert c.attend(q, table, starts, lengths, weight=w)[1] is w
+    w2 = torch.zeros(2, 3, 200)
+    assert c.attend(q, table, starts, lengths, weight=w, weight_out=w2)[1] is w2
+
+
+def test_nothing_to_do():
+    """No tokens, no sequences, no pages in the table: no launch that would read what is not there."""
+    c = _Dry(8, 3)
+    for B, M, N in ((2, 0, 3), (0, 0, 3), (0, 4, 3), (2, 4, 0)):
+        table = torch.zeros(B, N, dtype=torch.int32)
+        starts, lengths = torch.zeros(B + 1, dtype=torch.int32), torch.zeros(B, dtype=torch.int32)
+        c.append(_rows(M, 3), _rows(M, 3), table, starts, lengths)
+        assert not c.log
+        assert c.attend(_rows(M, 6), table, starts, lengths).shape == (M, 6, 64)
+        assert all(name == 'pg_attn' and M and B for name, *_ in c.log)
+        c.log.clear()
+
+
+def test_evict_refusals():
+    c = _Dry(8, 3, layers=2)
+    table, _, lengths = _batch()
+    to = torch.zeros(2, 1, dtype=torch.int32)
+    w = torch.zeros(2, 2, 3, 192)
+    ok = dict(weight=w, table=table, lengths=lengths, keep=50, to=to)
+    new, wo, kept = c.evict(**ok)
+    assert new.shape == (2,) and wo.shape == (2, 2, 3, 64) and kept.shape == (2, 2, 3, 50)
+    assert [e[0] for e in c.log] == ['pg_select', 'pg_move']
+    for kw, err in ((dict(keep=0), ValueError), (dict(keep=65), ValueError), (dict(recent=-1), ValueError),
+                    (dict(weight=w[:1]), ValueError), (dict(weight=w[..., :100].contiguous()), ValueError),
+                    (dict(weight=w.half()), TypeError), (dict(to=to[:1]), ValueError), (dict(to=to.long()), TypeError),
+                    (dict(weight_out=w[..., :32].contiguous()), ValueError), (dict(weight_out=w), ValueError),
+                    (dict(lengths=lengths[:1]), ValueError)):
+        with pytest.raises(err):
+            c.evict(**{**ok, **kw})
+    assert len(c.log) == 2
+
+
+@pytest.mark.parametrize('kind', paged.KINDS)
+@pytest.mark.parametrize('width', paged.WIDTHS)
+def test_kernels_compile(width, kind):
+    from vesta.launch import code_spills, compile_code
+    assert code_spills(compile_code(paged.paged_source(width, kind))) == 0

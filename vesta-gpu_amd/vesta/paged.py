@@ -1,0 +1,378 @@
+"""A key/value cache in pages, for sequences of different lengths, and its operators.
+
+    cache = PagedCache(pages=512, heads=12, width=64, layers=12, page=64, dtype='f16')
+    cache.append(k, v, table, starts, lengths, layer)             # new tokens' rows into their pages
+    out = cache.attend(q, table, starts, lengths, layer)          # their attention over all positions
+    out, w = cache.attend(q, ..., layer, weight=w[layer])         # ... counting the weight each receives
+    lengths, w, kept = cache.evict(w, table, lengths, keep, to)   # the positions of least weight go
+    cache.check()                                                 # raises if a call met a bad page (syncs)
+
+A batch is B sequences in the same three int32 device tensors throughout:
+
+* ``table`` [B, N]: the pages of each sequence, position s in page
+  ``table[b, s // page]``, slot ``s % page``. Entries past a sequence's length
+  are not looked at. Which page is whose is the caller's: pages may be shared
+  where only read (a common prompt), not where two sequences write.
+* ``lengths`` [B]: each sequence's positions, its new tokens included.
+* ``starts`` [B + 1]: sequence b's new tokens are rows ``starts[b]`` ..
+  ``starts[b + 1] - 1`` of the call's tensors, any number of each, none too.
+  Rows behind ``starts[B]`` are left as they are.
+
+New token j of c is at position ``lengths[b] - c + j`` and attends to the
+positions up to its own. A token at a negative position (a padded row: length
+0 in a batch of fixed size) is not stored, its output is 0.
+
+Everything stays on the device and on torch's current stream, so a call can be
+captured in a HIP graph and replayed with other contents of its tensors.
+Calls allocate their workspaces from torch's allocator, none is shared between
+two calls. Tensors are checked on the host (``TypeError``, ``ValueError``);
+what lies in ``table``, ``starts`` and ``lengths`` is checked on the device,
+where an impossible value is replaced by a possible one and raises an error
+word that ``check()`` reads.
+
+The decode cache of ``VestaGPT2`` [B, L, tmax, H, 64] (reference
+``vesta/gpt2.py:31-33``) holds one position for all its rows; this one is for
+programs whose rows come and go.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+import struct
+import threading
+from pathlib import Path
+
+from .launch import compile_code, lib, ok, track, unload
+from .prefill import PRELUDE_SRC
+
+PAGED_SRC = Path(__file__).resolve().parent / 'hip' / 'paged.hip'
+BLOCK = 256
+WIDTHS = (64, 128)
+KINDS = ('f16', 'bf16', 'f32')         # kernels' queries: the cache's type, or f32 over an f16 cache
+PAGE_MAX = 1 << 16
+ROWS = 16                              # query rows of a pg_attn block
+WEIGH = 128                            # positions of a pg_weigh block
+ERRORS = {1: 'a page id outside the pool', 2: 'starts that do not ascend, or lie past the rows',
+          4: 'a length past its table', 8: 'a sequence with more new tokens than `most`'}
+
+# parameters of the kernels: p a pointer, l a 64-bit, i a 32-bit whole number, f an fp32
+_SEQS = 'iipipp'                       # pages, shift, table, its columns, starts, lengths
+SIGNATURES = {
+    'pg_append16': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
+    'pg_append32': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
+    'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iif' + 'pllpp',
+    'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipii',
+    'pg_select': 'pipiiiiippipp',
+    'pg_move': 'ppiipipipiiiip',
+}
+_CODES = {'p': 'P', 'l': 'q', 'i': 'i', 'f': 'f'}
+
+
+def paged_source(width: int, kind: str) -> str:
+    return (f'#define VBLOCK {BLOCK}\n#define PG_E {width}\n#define PG_KIND {KINDS.index(kind)}\n'
+            + PRELUDE_SRC.read_text() + '\n' + PAGED_SRC.read_text())
+
+
+class _Launcher:
+    """One kernel with a buffer for its arguments: filled and read by one call
+    at a time."""
+
+    def __init__(self, fn, name):
+        self.fn, self.name = fn, name
+        self.lock = threading.Lock()
+        codes = '@' + ''.join(_CODES[c] for c in SIGNATURES[name])
+        self.pack = struct.Struct(codes)
+        self.buf = ctypes.create_string_buffer(self.pack.size)
+        base = ctypes.addressof(self.buf)
+        offs = [struct.calcsize(codes[:k + 1]) - struct.calcsize(codes[k]) for k in range(1, len(codes))]
+        self.args = (ctypes.c_void_p * len(offs))(*[base + o for o in offs])
+
+    def __call__(self, grid, block, stream, *vals):
+        with self.lock:
+            self.pack.pack_into(self.buf, 0, *vals)
+            status = lib().vh_launch(self.fn, grid, block, 0, stream, self.args)
+        ok(status, self.name)
+
+
+class _Kernels:
+    """The kernels of one head width and kind, loaded on one device."""
+
+    def __init__(self, device, width, kind):
+        import torch
+        self.mod = ctypes.c_void_p()
+        with torch.cuda.device(device):
+            ok(lib().vh_module_load(compile_code(paged_source(width, kind)), ctypes.byref(self.mod)),
+               'paged cache module load')
+            track(self)
+            for name in SIGNATURES:
+                fn = ctypes.c_void_p()
+                ok(lib().vh_module_get_function(self.mod, name.encode(), ctypes.byref(fn)), name)
+                setattr(self, name, _Launcher(fn, name))
+
+    def close(self):
+        if self.mod is not None and self.mod.value:
+            mod, self.mod = self.mod, None
+            unload(mod)
+
+
+_loaded = {}
+_loaded_lock = threading.Lock()
+
+
+def _kernels(device, width, kind):
+    with _loaded_lock:
+        key = (device, width, kind)
+        if key not in _loaded:
+            _loaded[key] = _Kernels(device, width, kind)
+        return _loaded[key]
+
+
+def _blocks8(n):
+    """Blocks of a grid whose kernel deals n tasks to the device's eight XCDs."""
+    return 8 * -(-n // 8)
+
+
+class PagedCache:
+    """``pages`` pages of ``page`` rows (a power of two) in each of ``layers``
+    layers, for ``heads`` key heads of ``width`` 64 or 128. ``keys`` and
+    ``vals`` are [layers, pages, page, heads, width] tensors of ``dtype``
+    ('f16' or 'bf16'), zeroed."""
+
+    def __init__(self, pages, heads, width=64, layers=1, page=64, dtype='f16', device=None):
+        """``device``: a CUDA device or its index, the current one by default."""
+        self._shape(pages, heads, width, layers, page, dtype)
+        import torch
+        if not torch.cuda.is_available():
+            raise RuntimeError('no GPU: the paged cache needs a ROCm device')
+        device = torch.device('cuda', device) if isinstance(device, int) else torch.device(device or 'cuda')
+        if device.type != 'cuda':
+            raise ValueError(f'device {device}: a CUDA device')
+        self._allocate(torch.device('cuda', torch.cuda.current_device() if device.index is None else device.index))
+        self._kind = {self.dtype: _kernels(self.device.index, width, dtype)}
+        if dtype == 'f16':
+            self._kind[torch.float32] = _kernels(self.device.index, width, 'f32')
+
+    def _shape(self, pages, heads, width, layers, page, dtype):
+        if dtype not in ('f16', 'bf16'):
+            raise ValueError(f"dtype {dtype!r}: the cache is 'f16' or 'bf16'")
+        if width not in WIDTHS:
+            raise ValueError(f'heads of {width}: their width is one of {WIDTHS}')
+        if not (1 <= page <= PAGE_MAX and page & (page - 1) == 0):
+            raise ValueError(f'pages of {page} rows: a power of two up to {PAGE_MAX}')
+        if min(pages, heads, layers) < 1:
+            raise ValueError(f'{pages} pages, {heads} heads, {layers} layers: one at least of each')
+        if pages * page >= 1 << 31:
+            raise ValueError(f'{pages} pages of {page} rows: fewer than 2^31 rows a layer')
+        self.pages, self.heads, self.width, self.layers, self.page = pages, heads, width, layers, page
+        self._shift = page.bit_length() - 1
+        self._dt = dtype
+
+    def _allocate(self, device):
+        import torch
+        self.device = device
+        self.dtype = torch.float16 if self._dt == 'f16' else torch.bfloat16
+        shape = (self.layers, self.pages, self.page, self.heads, self.width)
+        self.keys = torch.zeros(shape, dtype=self.dtype, device=self.device)
+        self.vals = torch.zeros(shape, dtype=self.dtype, device=self.device)
+        self._layer_bytes = self.keys[0].numel() * 2
+        self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+
+    # ------------------------------------------------------------ checks
+    def _ints(self, name, t, shape):
+        import torch
+        if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == self.device
+                and t.is_contiguous()):
+            raise TypeError(f'{name}: need a contiguous int32 tensor on {self.device}')
+        if t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
+            raise ValueError(f'{name}: shape {tuple(t.shape)}, need {tuple("any" if w is None else w for w in shape)}')
+
+    def _batch(self, table, starts, lengths):
+        self._ints('table', table, (None, None))
+        B, N = table.shape
+        if N * self.page >= 1 << 31:
+            raise ValueError(f'table: {N} pages of {self.page} rows a sequence, fewer than 2^31 rows are possible')
+        if starts is not None:
+            self._ints('starts', starts, (B + 1,))
+        self._ints('lengths', lengths, (B,))
+        return B, N
+
+    def _rows(self, name, t, dtypes, heads=None, like=None):
+        """New tokens' rows [M, heads, width]: any strides but the last, 16-byte aligned."""
+        import torch
+        if not (isinstance(t, torch.Tensor) and t.device == self.device and t.dtype in dtypes):
+            raise TypeError(f'{name}: need a tensor of {" or ".join(str(d)[6:] for d in dtypes)} on {self.device}')
+        shape = t.shape
+        if len(shape) != 3 or shape[2] != self.width or (heads is not None and shape[1] != heads) \
+                or (like is not None and shape != like):
+            raise ValueError(f'{name}: shape {tuple(shape)}, need '
+                             f'{tuple(like) if like is not None else ("rows", heads or "heads", self.width)}')
+        row, head, one = t.stride()
+        unit = 16 // t.element_size()
+        if t.numel() and (one != 1 or row % unit or head % unit or t.data_ptr() % 16):
+            raise ValueError(f'{name}: rows of consecutive, 16-byte aligned values needed (strides {t.stride()})')
+        return row, head
+
+    def _layer(self, layer):
+        if not 0 <= layer < self.layers:
+            raise ValueError(f'layer {layer} of {self.layers}')
+        return layer * self._layer_bytes
+
+    def _on_device(self):
+        import torch
+        return torch.cuda.device(self.device)
+
+    def _stream(self):
+        import torch
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    # ------------------------------------------------------------ operators
+    def append(self, k, v, table, starts, lengths, layer=0):
+        """The new tokens' key and value rows ``k``, ``v`` [M, heads, width]
+        into their pages of ``layer``. They are of the cache's type or f32
+        (rounded to nearest). Rows of other sequences' slots stay as they are;
+        a page that two of the new rows' sequences share gets either's."""
+        import torch
+        B, N = self._batch(table, starts, lengths)
+        at = self._layer(layer)
+        ks = self._rows('k', k, (self.dtype, torch.float32), self.heads)
+        vs = self._rows('v', v, (k.dtype,), like=k.shape)
+        M = k.shape[0]
+        if M == 0 or B == 0 or N == 0:
+            return
+        kn = self._kind[self.dtype]
+        launch = kn.pg_append32 if k.dtype == torch.float32 else kn.pg_append16
+        grid = -(-M * self.heads * (self.width // 8) // BLOCK)
+        if grid >= 1 << 31:
+            raise ValueError(f'k: {M} rows are too many for one call')
+        with self._on_device():
+            launch(grid, BLOCK, self._stream(), k.data_ptr(), v.data_ptr(), *ks, *vs, self.keys.data_ptr() + at,
+                   self.vals.data_ptr() + at, self.pages, self._shift, table.data_ptr(), N, starts.data_ptr(),
+                   lengths.data_ptr(), B, M, self.heads, self.err.data_ptr())
+
+    def attend(self, q, table, starts, lengths, layer=0, scale=None, out=None, weight=None, weight_out=None, most=None):
+        """Attention of the new tokens' queries ``q`` [M, G * heads, width]
+        (query heads G h .. G h + G - 1 read key head h) over their sequences'
+        positions in ``layer``: softmax(``scale`` q . k), 1 / sqrt(width) by
+        default, times the values. ``q`` is of the cache's type or, over an f16
+        cache, f32; the result is of q's type: ``out`` [M, G * heads, width],
+        made if not given. A token that sees no position gets zeros.
+
+        ``weight`` [B, heads, S] (f32, contiguous, S at least the table's
+        positions): the softmax weight that each position has received so far.
+        Then the call returns (out, weight_out), where weight_out [B, heads, S'] is
+        weight plus what the new tokens give, over the query heads of the key
+        head; the new positions start at 0, and past the lengths it is 0.
+        ``weight_out`` may be given, ``weight`` itself is updated if it is not.
+
+        ``most``: a bound of the new tokens of a sequence that the program
+        knows (1 for a decode step); the work is laid out by it."""
+        import torch
+        B, N = self._batch(table, starts, lengths)
+        at = self._layer(layer)
+        qs = self._rows('q', q, tuple(self._kind))
+        M, Hq, _ = q.shape
+        if Hq == 0 or Hq % self.heads:
+            raise ValueError(f'q: {Hq} heads are not a multiple of the {self.heads} key heads')
+        G = Hq // self.heads
+        scale = 1.0 / math.sqrt(self.width) if scale is None else float(scale)
+        if not 0.0 < scale < math.inf:
+            raise ValueError(f'scale {scale}: positive and finite')
+        if most is not None and most < 1:
+            raise ValueError(f'most {most}: at least 1')
+        if out is None:
+            out = torch.empty((M, Hq, self.width), dtype=q.dtype, device=self.device)
+            os = (Hq * self.width, self.width)
+        else:
+            os = self._rows('out', out, (q.dtype,), like=q.shape)
+        S = So = 0
+        if weight is not None:
+            weight_out = weight if weight_out is None else weight_out
+            S, So = (self._weights(n, w, (B, self.heads), N * self.page)
+                     for n, w in (('weight', weight), ('weight_out', weight_out)))
+        elif weight_out is not None:
+            raise ValueError('weight_out: no weight given')
+        most = M if most is None else min(most, M)
+        kn = self._kind[q.dtype]
+        scale2 = scale * 1.4426950408889634
+        with self._on_device():
+            stream = self._stream()
+            seqs = (self.pages, self._shift, table.data_ptr(), N, starts.data_ptr(), lengths.data_ptr())
+            lse = None if weight is None else torch.empty(M * Hq, dtype=torch.float32, device=self.device)
+            if M and B:
+                tiles = -(-most * G // ROWS)
+                if B * self.heads * tiles >= 1 << 30:
+                    raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
+                kn.pg_attn(_blocks8(B * self.heads * tiles), BLOCK, stream, q.data_ptr(), *qs,
+                           self.keys.data_ptr() + at, self.vals.data_ptr() + at, *seqs, B, M, self.heads, G, tiles,
+                           most, scale2, out.data_ptr(), *os, 0 if lse is None else lse.data_ptr(),
+                           self.err.data_ptr())
+            if weight is not None and B:
+                blocks = -(-So // WEIGH)
+                kn.pg_weigh(_blocks8(B * self.heads * blocks), BLOCK, stream, q.data_ptr(), *qs,
+                            self.keys.data_ptr() + at, *seqs, B, M, self.heads, G, scale2, lse.data_ptr(),
+                            weight.data_ptr(), S, weight_out.data_ptr(), So, blocks)
+        return out if weight is None else (out, weight_out)
+
+    def _weights(self, name, w, lead, least):
+        import torch
+        if not (isinstance(w, torch.Tensor) and w.dtype == torch.float32 and w.device == self.device
+                and w.is_contiguous()):
+            raise TypeError(f'{name}: need a contiguous float32 tensor on {self.device}')
+        if w.dim() != len(lead) + 1 or tuple(w.shape[:-1]) != lead or w.shape[-1] < least:
+            raise ValueError(f'{name}: shape {tuple(w.shape)}, need {lead} and {least} positions at least')
+        return w.shape[-1]
+
+    def evict(self, weight, table, lengths, keep, to, recent=0, weight_out=None):
+        """Keep ``keep`` positions of each sequence (all where it has no more):
+        its ``recent`` last ones and, of the others, those of largest
+        ``weight`` [layers, B, heads, S] (f32, contiguous; a tie goes to the
+        lowest position, NaN counts as the largest), chosen for each layer and
+        head on its own. They go, in their order, into the pages ``to`` [B, N']
+        (int32, N' pages of at least ``keep`` rows in all), which must be none
+        of the pages that the call reads; ``table``'s pages stay as they are,
+        for their owner to hand out again.
+
+        Returns (lengths [B], weight_out [layers, B, heads, S'], kept [layers,
+        B, heads, keep]): the new lengths, the kept positions' weights (0
+        behind them) and which positions they were (-1 behind them)."""
+        import torch
+        B, N = self._batch(table, None, lengths)
+        self._ints('to', to, (B, None))
+        No = to.shape[1]
+        if keep < 1 or recent < 0:
+            raise ValueError(f'keep {keep} of at least 1 position, recent {recent} of at least 0')
+        if No * self.page < keep:
+            raise ValueError(f'to: {No} pages of {self.page} rows cannot hold {keep} positions')
+        lead = (self.layers, B, self.heads)
+        S = self._weights('weight', weight, lead, N * self.page)
+        if weight_out is None:
+            weight_out = torch.empty(lead + (No * self.page,), dtype=torch.float32, device=self.device)
+        So = self._weights('weight_out', weight_out, lead, No * self.page)
+        if B and weight_out.data_ptr() == weight.data_ptr():
+            raise ValueError('weight_out: a tensor other than weight')
+        kept = torch.empty(lead + (keep,), dtype=torch.int32, device=self.device)
+        new = torch.empty(B, dtype=torch.int32, device=self.device)
+        if B == 0:
+            return new, weight_out, kept
+        kn = self._kind[self.dtype]
+        blocks = -(-keep * self.heads * (self.width // 8) // BLOCK)
+        if self.layers * B * max(blocks, self.heads) >= 1 << 31:
+            raise ValueError(f'{self.layers} layers of {B} sequences are too many for one call')
+        with self._on_device():
+            stream = self._stream()
+            kn.pg_select(self.layers * B * self.heads, 1024, stream, weight.data_ptr(), S, lengths.data_ptr(),
+                         N * self.page, B, self.heads, keep, recent, kept.data_ptr(), weight_out.data_ptr(), So,
+                         new.data_ptr(), self.err.data_ptr())
+            kn.pg_move(self.layers * B * blocks, BLOCK, stream, self.keys.data_ptr(), self.vals.data_ptr(), self.pages,
+                       self._shift, table.data_ptr(), N, to.data_ptr(), No, kept.data_ptr(), keep, B, self.heads,
+                       blocks, self.err.data_ptr())
+        return new, weight_out, kept
+
+    def check(self):
+        """Raise if an earlier call met a page, a length or starts that cannot
+        be (one synchronisation); the word is cleared first."""
+        word = int(self.err.item())
+        if word:
+            self.err.zero_()
+            why = ', '.join(text for bit, text in ERRORS.items() if word & bit)
+            raise RuntimeError(f'paged cache: {why}; the results are invalid')
