@@ -284,90 +284,234 @@ __device__ __forceinline__ unsigned pg_wild2(unsigned x) {
 // of four each). The softmax is a running one in powers of two, statistics in
 // fp32; weights are rounded to the cache's type for the second product, as
 // their values are (fp32 queries: 24 bits in three planes).
+//
+// A block that has a part of the positions only (pg_work) leaves its rows'
+// maxima, sums and weighted values in `ws` for pg_join.
 #define PG_STEP (PG_E == 64 ? 64 : 32)
 #define PG_VROW (PG_E + 16)                // halves of a value row in LDS: 16 past a multiple of 32 banks
+#define PG_WS(rows) ((rows) * (PG_E + 2))  // floats of a tile's part: maxima, sums, rows of E
+
+// How the work is dealt to blocks. A sequence's rows come in tiles of ROWS, its
+// positions in steps of STEP; a part is `each` steps of one (sequence, key
+// head, tile), `each` such that there are about `target` parts in all (0: one
+// part a tile). So parts are of one size whatever the lengths, and a block of
+// the grid is a part: the grid holds target + H (M G / ROWS + B) + 64, every
+// number of parts that can come out, and is dealt to the XCDs in contiguous
+// runs. A sequence's parts follow each other, in each its heads, whose rows lie
+// side by side, in each its tiles, which read the same rows.
+struct PgWork {
+  PgSeq sq;
+  int b, h, R, x0, tile, tiles, part, each, at;   // x0: the tile's first row of R; at: the part's place in ws
+};
+template <int ROWS, int STEP>
+__device__ __forceinline__ void pg_count(const PgSeq& s, int G, int& tiles, int& steps) {
+  tiles = (s.count * G + ROWS - 1) / ROWS;
+  steps = max((s.len + STEP - 1) / STEP, 1);
+}
+__device__ __forceinline__ int pg_scan(int v, int lane) {          // sums over the lanes up to each
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int u = __shfl_up(v, d, 64);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+// The steps of a part: the same in every wave that asks.
+template <int ROWS, int STEP>
+__device__ __forceinline__ int pg_each(const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
+                                       int cap, int H, int G, int target, int least) {
+  if (target == 0) return 0x7fffffff;
+  const int lane = threadIdx.x & 63;
+  float w = 0.0f;
+  for (int b = lane; b < B; b += 64) {
+    int tiles, steps;
+    pg_count<ROWS, STEP>(pg_seq(starts, lengths, b, M, cap), G, tiles, steps);
+    w += (float)tiles * (float)steps;
+  }
+  w = wave_red_sum(w);
+  return max((int)fminf(w * (float)H / (float)target, 1e9f) + 1, least);
+}
+// Block `at`'s part, where `joined` one of all (sequence, head, tile)s of a
+// grid of those instead (its parts' first place in ws is then `at`).
+template <int ROWS, int STEP>
+__device__ __forceinline__ bool pg_work(PgWork& o, int block, bool joined, const int* __restrict__ starts,
+                                        const int* __restrict__ lengths, int B, int M, int cap, int H, int G,
+                                        int target, int least, unsigned* __restrict__ err, int most) {
+  const int lane = threadIdx.x & 63;
+  o.each = pg_each<ROWS, STEP>(starts, lengths, B, M, cap, H, G, target, least);
+  auto mine = [&](int b, PgSeq& s, int& tiles, int& parts) -> int {
+    tiles = parts = 0;
+    if (b >= B) return 0;
+    s = pg_seq(starts, lengths, b, M, cap);
+    int steps;
+    pg_count<ROWS, STEP>(s, G, tiles, steps);
+    parts = (steps - 1) / o.each + 1;
+    return tiles * H * (joined ? 1 : parts);
+  };
+  PgSeq s = {};
+  int tiles, parts, n = mine(lane, s, tiles, parts), sum = pg_scan(n, lane);
+  int total = __builtin_amdgcn_readlane(sum, 63);
+  for (int base = 64; base < B; base += 64) {
+    PgSeq u;
+    int x, y;
+    total += __builtin_amdgcn_readlane(pg_scan(mine(base + lane, u, x, y), lane), 63);
+  }
+  if (err && block == 0 && threadIdx.x < 64) {                     // once a call: what is wrong with any sequence
+    unsigned bad = lane < B ? s.bad | (s.count > most ? PG_ERR_MOST : 0u) : 0u;
+    for (int b = 64 + lane; b < B; b += 64) {
+      const PgSeq u = pg_seq(starts, lengths, b, M, cap);
+      bad |= u.bad | (u.count > most ? PG_ERR_MOST : 0u);
+    }
+    if (bad) pg_raise(err, bad);
+  }
+  const int per = (total + 7) / 8;
+  const int at = joined ? block : (block & 7) * per + (block >> 3);
+  if (at >= total || (!joined && (block >> 3) >= per)) return false;
+  int before = 0, places = 0;                                      // in the chunks of 64 sequences already passed
+  for (int base = 0;; base += 64) {
+    if (base) {
+      n = mine(base + lane, s, tiles, parts);
+      sum = pg_scan(n, lane);
+    }
+    const int all = __builtin_amdgcn_readlane(sum, 63);
+    if (at < before + all) {
+      const int l = __builtin_ctzll(__ballot(before + sum > at));  // the sequence's lane
+      o.b = base + l;
+      o.sq.first = __builtin_amdgcn_readlane(s.first, l);
+      o.sq.count = __builtin_amdgcn_readlane(s.count, l);
+      o.sq.len = __builtin_amdgcn_readlane(s.len, l);
+      o.tiles = __builtin_amdgcn_readlane(tiles, l);
+      const int rest = at - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
+      o.tile = o.tiles - 1 - rest % o.tiles;                       // the longest first
+      o.h = rest / o.tiles % H;
+      o.part = rest / o.tiles / H;
+      o.at = at;
+      if (joined) {
+        const int p = pg_scan(n * parts, lane);
+        o.at = places + __builtin_amdgcn_readlane(p, l) - __builtin_amdgcn_readlane(n * parts, l) + rest;
+      }
+      o.R = o.sq.count * G;
+      o.x0 = o.tile * ROWS;
+      return true;
+    }
+    before += all;
+    if (joined) places += __builtin_amdgcn_readlane(pg_scan(n * parts, lane), 63);
+  }
+}
+// A tile's last position (-1: its rows see none), its steps and its parts that have steps.
+template <int ROWS, int STEP>
+__device__ __forceinline__ void pg_span(const PgWork& w, int G, int& last, int& steps, int& parts) {
+  last = w.sq.len - w.sq.count + min(w.x0 + ROWS - 1, w.R - 1) / G;
+  steps = last < 0 ? 0 : last / STEP + 1;
+  parts = max((steps - 1) / w.each + 1, 1);
+}
+
+// Four consecutive results of a row, rounded to the queries' type.
+__device__ __forceinline__ void pg_store4(pg_q* p, const float* v) {
+#if PG_KIND == PG_F32
+  *(vh_f32x4*)p = vh_f32x4{v[0], v[1], v[2], v[3]};
+#else
+  const vh_u32x4 w = pg_pack8(pg_f8{v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f});
+  *(vh_u32x2*)p = vh_u32x2{w[0], w[1]};
+#endif
+}
+
 extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,
     const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
-    const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int tiles, int most,
-    float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse, unsigned* __restrict__ err) {
+    const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
+    int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
+    float* __restrict__ ws, unsigned* __restrict__ err) {
   constexpr int KS = PG_E / 32, NG = PG_STEP / 16, NV = PG_STEP * PG_E / 512, DT = PG_E / 16;
+  constexpr int VL = PG_E / 8, VR = 64 / VL;                       // lanes of a value row; rows of a wave's load
   __shared__ __attribute__((aligned(16))) unsigned short lv[4][PG_STEP * PG_VROW];
   __shared__ float om[4][2][16];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, q = lane >> 4;
-  const int T = B * H * tiles, per = (T + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || id >= T) return;
-  const int h = id / tiles % H, b = id / tiles / H;
-  const PgSeq sq = pg_seq(starts, lengths, b, M, N << shift);
-  const int R = sq.count * G, x0 = (tiles - 1 - id % tiles) * 16;  // the longest first
-  unsigned bad = sq.bad | (sq.count > most ? PG_ERR_MOST : 0u);
-  if (x0 == 0 && bad && tid == 0) pg_raise(err, bad);
-  bad = 0;
-  if (x0 >= R) return;
+  PgWork wk;
+  if (!pg_work<16, PG_STEP>(wk, blockIdx.x, false, starts, lengths, B, M, N << shift, H, G, target, least, err, most)) return;
+  int last, steps, parts;
+  pg_span<16, PG_STEP>(wk, G, last, steps, parts);
+  if (wk.part >= parts) return;
+  const PgSeq sq = wk.sq;
+  const int R = wk.R, x0 = wk.x0, h = wk.h;
+  const int t0 = min(wk.part * wk.each, steps), t1 = wk.each < steps - t0 ? t0 + wk.each : steps;
+  unsigned bad = 0;
   const int x = min(x0 + r, R - 1), tok = x / G, head = h * G + x % G;
   const bool live = x0 + r < R;
   const int lim = sq.len - sq.count + tok;                         // this lane's last position
-  const int last = sq.len - sq.count + min(x0 + 15, R - 1) / G, first = sq.len - sq.count + x0 / G;
-  const int nt = last < 0 ? 0 : last / PG_STEP + 1;
+  const int first = sq.len - sq.count + x0 / G;                    // the first row's
   const pg_q* qp = Q + (sq.first + tok) * qrow + head * qhead;
-  PgQuery qf;
-  pg_query(qf, qp, q, scale2);
   const size_t rowlen = (size_t)H * PG_E;
-  const int* tb = table + (size_t)b * N;
-  auto row = [&](int s) -> size_t {                                // element offset of position s's row
-    const int page = tb[s >> shift];
+  const int* tb = table + (size_t)wk.b * N;
+  const unsigned short *kh = kp + h * PG_E + 8 * q, *vh = vp + h * PG_E + lane % VL * 8;
+  // the pool rows of a step's positions, one a lane
+  auto rows = [&](int t) -> unsigned {
+    const int s = min(t * PG_STEP + lane % PG_STEP, last), page = tb[s >> shift];
     const bool in = (unsigned)page < (unsigned)pages;
     if (!in) bad = PG_ERR_PAGE;
-    return (((size_t)(in ? page : 0) << shift) + (s & ((1 << shift) - 1))) * rowlen + h * PG_E;
+    return ((unsigned)(in ? page : 0) << shift) + (unsigned)(s & ((1 << shift) - 1));
+  };
+  vh_u32x4 kr[NG][KS], vr[NV];
+  auto load = [&](unsigned rw) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const unsigned short* p = kh + (unsigned)__shfl((int)rw, 16 * i + r, 64) * rowlen;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) kr[i][k] = ld16(p + 32 * k);
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) vr[n] = ld16(vh + (unsigned)__shfl((int)rw, n * VR + lane / VL, 64) * rowlen);
   };
   float o[DT][4] = {};
   float m2 = -INFINITY, sum = 0.0f;
   unsigned short* V = lv[wave];
-  for (int t = wave; t < nt; t += 4) {
+  unsigned rw = 0;
+  PgQuery qf;
+  pg_query(qf, qp, q, scale2);
+  if (t0 + wave < t1) {
+    load(rows(t0 + wave));
+    rw = rows(min(t0 + wave + 4, t1 - 1));
+  }
+  for (int t = t0 + wave; t < t1; t += 4) {
     const int p0 = t * PG_STEP;
-    vh_u32x4 vr[NV];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {                                 // positions past the last: zeros
-      const int s = p0 + n * (512 / PG_E) + lane / (PG_E / 8);
-      vr[n] = ld16(vp + row(min(s, last)) + lane % (PG_E / 8) * 8);
-      if (s > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
-    }
     float s[NG][4];
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      vh_u32x4 kf[KS];
-      const unsigned short* kr = kp + row(min(p0 + 16 * i + r, last)) + 8 * q;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) kf[k] = ld16(kr + 32 * k);
-      pg_scores(kf, qf, qp, lane, s[i]);
-    }
-    const bool part = p0 + PG_STEP - 1 > first;                    // some row sees it in part
-    // values that are not finite are left out of the product where a row may
-    // not see their position, or a plane of its weight may be 0: 0 * inf ...
+    for (int i = 0; i < NG; ++i) pg_scores(kr[i], qf, qp, lane, s[i]);
+    const bool seen = p0 + PG_STEP - 1 > first;                    // not the whole step by every row
+    // values past the last position are 0; ones that are not finite are left
+    // out of the product where a row may not see their position, or a plane of
+    // its weight may be 0: 0 * inf ...
     bool wild = false;
-    if (part || PG_KIND == PG_F32) {
+    if (p0 + PG_STEP - 1 > last) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+        if (p0 + n * VR + lane / VL > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
+    }
+    if (seen || PG_KIND == PG_F32) {
       unsigned any = 0u;
 #pragma unroll
       for (int n = 0; n < NV; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
       wild = __any(any != 0u);
     }
-    if (part) {
+    pg_wave_sync();                                                // the step before is read
+#pragma unroll
+    for (int n = 0; n < NV; ++n) *(vh_u32x4*)(V + (n * VR + lane / VL) * PG_VROW + lane % VL * 8) = vr[n];
+    pg_wave_sync();
+    if (t + 4 < t1) {
+      load(rw);
+      rw = rows(min(t + 8, t1 - 1));
+    }
+    if (seen) {
 #pragma unroll
       for (int i = 0; i < NG; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = p0 + 16 * i + 4 * q + j <= lim ? s[i][j] : -INFINITY;
     }
-    pg_wave_sync();
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-      *(vh_u32x4*)(V + (n * (512 / PG_E) + lane / (PG_E / 8)) * PG_VROW + lane % (PG_E / 8) * 8) = vr[n];
-    pg_wave_sync();
     float bm = s[0][0];
 #pragma unroll
     for (int n = 1; n < 4 * NG; ++n) bm = fmaxf(bm, s[n >> 2][n & 3]);
-    bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
-    bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+    bm = vh_pair32(vh_pair16(bm, op_max), op_max);
     const float n2 = fmaxf(m2, bm * qf.k2);
     const float ref = n2 == -INFINITY ? 0.0f : n2;                 // no score above -inf yet: all weights 0
     const float c = __builtin_amdgcn_exp2f(m2 - ref);
@@ -387,7 +531,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
     for (int d = 0; d < DT; ++d) {
       vh_f32x4 th = {0.0f, 0.0f, 0.0f, 0.0f};
 #if PG_KIND == PG_F32
-      vh_f32x4 tl = th;
+      vh_f32x4 tw = th;
 #endif
 #pragma unroll
       for (int k = 0; k < NG / 2; ++k) {
@@ -405,14 +549,14 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
         const vh_u32x4 vf = __builtin_bit_cast(vh_u32x4, f);
         th = pg_mfma(vf, pf[k][0], th);
 #if PG_KIND == PG_F32
-        tl = pg_mfma(vf, pf[k][1], tl);
-        tl = pg_mfma(vf, pf[k][2], tl);
+        tw = pg_mfma(vf, pf[k][1], tw);
+        tw = pg_mfma(vf, pf[k][2], tw);
 #endif
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #if PG_KIND == PG_F32
-        o[d][j] = fmaf(o[d][j], c, vh_hilo(th[j], tl[j]));
+        o[d][j] = fmaf(o[d][j], c, vh_hilo(th[j], tw[j]));
 #else
         o[d][j] = fmaf(o[d][j], c, th[j]);
 #endif
@@ -430,8 +574,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
     }
   }
   if (__any(bad != 0) && lane == 0) pg_raise(err, PG_ERR_PAGE);
-  sum += __shfl_xor(sum, 16, 64);
-  sum += __shfl_xor(sum, 32, 64);
+  sum = vh_pair32(vh_pair16(sum, op_sum), op_sum);
   // each wave's maximum, sum and output, rescaled to the common maximum and
   // added in wave order; wave w then makes every fourth dim tile
   float* ow = (float*)lv;                                          // [wave][dim tile][j][lane]
@@ -457,7 +600,9 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
     sum = fmaf(om[w][1][r], f[w], sum);
   }
   if (!live) return;
+  const bool whole = parts == 1;
   pg_q* op = out + (sq.first + tok) * orow + head * ohead;
+  float* wp = ws + (size_t)wk.at * PG_WS(16);
 #pragma unroll
   for (int d = wave; d < DT; d += 4) {
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -465,20 +610,313 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
     for (int w = 0; w < 4; ++w)
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = fmaf(ow[((w * DT + d) * 4 + j) * 64 + lane], f[w], v[j]);
+    if (whole) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = lim < 0 ? 0.0f : v[j] / sum;
-#if PG_KIND == PG_F32
-    *(vh_f32x4*)(op + 16 * d + 4 * q) = vh_f32x4{v[0], v[1], v[2], v[3]};
-#else
-    const vh_u32x4 w = pg_pack8(pg_f8{v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f});
-    *(vh_u32x2*)(op + 16 * d + 4 * q) = vh_u32x2{w[0], w[1]};
-#endif
+      for (int j = 0; j < 4; ++j) v[j] = lim < 0 ? 0.0f : v[j] / sum;
+      pg_store4(op + 16 * d + 4 * q, v);
+    } else {
+      *(vh_f32x4*)(wp + 32 + r * PG_E + 16 * d + 4 * q) = vh_f32x4{v[0], v[1], v[2], v[3]};
+    }
   }
-  // log2 of the row's sum of 2^score: +inf for a row that sees nothing, so
-  // that all its weights are 0
-  if (lse && wave == 0 && q == 0)
-    lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : m + __builtin_amdgcn_logf(sum);
+  if (wave == 0 && q == 0) {
+    if (!whole) {
+      wp[r] = m;
+      wp[16 + r] = sum;
+    } else if (lse) {
+      // log2 of the row's sum of 2^score: +inf for a row that sees nothing, so
+      // that all its weights are 0
+      lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : m + __builtin_amdgcn_logf(sum);
+    }
+  }
 }
+
+// Attention of many rows of 16-bit queries. A block makes 128 rows of one
+// (sequence, key head), 32 to a wave, over steps of 64 positions that its four
+// waves share: key and value rows lie in LDS (double-buffered; the loads of the
+// step after next are in flight while one is used). Products in tiles of
+// 32 x 32 x 16: lane 32 g + r holds row r, fold positions 8 g .. + 7 of an
+// operand; column r, rows 8 (i / 4) + 4 g + i % 4 of the result, i < 16. As in
+// pg_attn, scores are K Q^T, outputs V^T P^T, and the weights feed the second
+// product from the registers they are in: fold position 8 g + e stands for
+// position 4 g + e (e < 4) or 8 + 4 g + e - 4 of 16. The weighted values
+// accumulate in the matrix cores' own registers; they are rescaled only when a
+// row's maximum has grown by more than 2^PG_SLACK since (weights up to that
+// are exact in the sums and rounded as finely).
+#if PG_KIND != PG_F32
+#define PG_SLACK 8.0f
+#define PG_WROW (PG_E + 32)                // halves of a value row in LDS: 64 bytes past a multiple of all banks
+typedef float pg_f16v __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ pg_f16v pg_mfma32(vh_u32x4 a, vh_u32x4 b, pg_f16v c) {
+#if PG_KIND == PG_BF16
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_b8, a), __builtin_bit_cast(pg_b8, b), c, 0, 0, 0);
+#else
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vh_h8, a), __builtin_bit_cast(vh_h8, b), c, 0, 0, 0);
+#endif
+}
+
+extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
+    const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,
+    const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
+    const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
+    int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
+    float* __restrict__ ws, unsigned* __restrict__ err) {
+  constexpr int KS = PG_E / 16, DT = PG_E / 32, CH = PG_E / 8, NL = 64 * CH / 256;   // k-steps, dim tiles, 16-byte
+  constexpr int RS = 256 / CH;                                     // pieces of a row; a thread's pieces and rows apart
+  __shared__ __attribute__((aligned(16))) vh_u32x4 lk[2][64 * CH];
+  __shared__ __attribute__((aligned(16))) unsigned short lv[2][64 * PG_WROW];
+  __shared__ int lwild[2];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int r = lane & 31, g = lane >> 5;
+  PgWork wk;
+  if (!pg_work<128, 64>(wk, blockIdx.x, false, starts, lengths, B, M, N << shift, H, G, target, least, err, most)) return;
+  int last, steps, parts;
+  pg_span<128, 64>(wk, G, last, steps, parts);
+  if (wk.part >= parts) return;
+  const PgSeq sq = wk.sq;
+  const int R = wk.R, x0 = wk.x0 + 32 * wave, h = wk.h, new0 = sq.len - sq.count;
+  const int t0 = min(wk.part * wk.each, steps), t1 = wk.each < steps - t0 ? t0 + wk.each : steps;
+  const int x = min(x0 + r, R - 1), tok = x / G, head = h * G + x % G;
+  const bool live = x0 + r < R;
+  const int lim = new0 + tok;                                      // this lane's last position
+  const int bfirst = new0 + wk.x0 / G;                             // the block's first row's
+  const int wfirst = new0 + min(x0, R - 1) / G, wlast = new0 + min(x0 + 31, R - 1) / G;
+  unsigned bad = 0;
+  vh_u32x4 qf[KS];
+  {
+    const pg_q* qp = Q + (sq.first + tok) * qrow + head * qhead + 8 * g;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qf[k] = ld16(qp + 16 * k);
+  }
+  // staging: thread t takes piece t % CH of rows t / CH + RS n
+  const size_t rowlen = (size_t)H * PG_E;
+  const int* tb = table + (size_t)wk.b * N;
+  const int c8 = tid % CH, r8 = tid / CH;
+  const unsigned short *kh = kp + h * PG_E + 8 * c8, *vh = vp + h * PG_E + 8 * c8;
+  unsigned rw[NL];
+  auto rows = [&](int t) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int s = min(64 * t + r8 + RS * n, last), page = tb[s >> shift];
+      const bool in = (unsigned)page < (unsigned)pages;
+      if (!in) bad = PG_ERR_PAGE;
+      rw[n] = ((unsigned)(in ? page : 0) << shift) + (unsigned)(s & ((1 << shift) - 1));
+    }
+  };
+  vh_u32x4 kr[NL], vr[NL];
+  auto load = [&]() {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      kr[n] = ld16(kh + rw[n] * rowlen);
+      vr[n] = ld16(vh + rw[n] * rowlen);
+    }
+  };
+  // Key pieces are permuted within their row by its number, so that a column of
+  // them falls on all banks. Values past the last position are 0; whether a
+  // step that some row sees in part holds one that is not finite is noted.
+  auto put = [&](int t) {
+    const int buf = t & 1;
+    const bool end = 64 * t + 63 > last;
+    unsigned any = 0u;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int row = r8 + RS * n;
+      lk[buf][row * CH + (c8 ^ (row & 7))] = kr[n];
+      if (end && 64 * t + row > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
+      *(vh_u32x4*)(lv[buf] + row * PG_WROW + 8 * c8) = vr[n];
+    }
+    if (64 * t + 63 > bfirst) {
+#pragma unroll
+      for (int n = 0; n < NL; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
+      if (any) lwild[buf] = t + 1;
+    }
+  };
+  pg_f16v o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[d][j] = 0.0f;
+  float m2 = -INFINITY, sum = 0.0f;
+  if (tid < 2) lwild[tid] = 0;
+  vh_lds_sync();                                                   // noted as none before a step may be noted
+  if (t0 < t1) {
+    rows(t0);
+    load();
+    rows(min(t0 + 1, t1 - 1));
+    put(t0);
+    if (t0 + 1 < t1) {
+      load();
+      rows(min(t0 + 2, t1 - 1));
+    }
+  }
+  for (int t = t0; t < t1; ++t) {
+    vh_lds_sync();                       // step t is staged; the other buffer's step is read
+    if (t + 1 < t1) {
+      put(t + 1);
+      if (t + 2 < t1) {
+        load();
+        rows(min(t + 3, t1 - 1));
+      }
+    }
+    const int p0 = 64 * t, buf = t & 1;
+    if (x0 >= R || p0 > wlast) continue;
+    const vh_u32x4* K = lk[buf];
+    const unsigned short* V = lv[buf];
+    pg_f16v s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) s[i] = pg_mfma32(K[(32 * i + r) * CH + ((2 * k + g) ^ (r & 7))], qf[k], s[i]);
+    }
+    const bool seen = p0 + 63 > wfirst;                            // not the whole step by every row
+    if (seen) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[i][j] = p0 + 32 * i + 8 * (j >> 2) + 4 * g + (j & 3) <= lim ? s[i][j] : -INFINITY;
+    }
+    float bm = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int j = 1; j < 16; ++j) bm = fmaxf(bm, fmaxf(s[0][j], s[1][j]));
+    bm = vh_pair32(bm, op_max);
+    const float n2 = bm * scale2;
+    if (__any(n2 > m2 + PG_SLACK || (n2 > m2 && m2 == -INFINITY))) {
+      const float m = fmaxf(m2, n2);
+      const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - m);
+      m2 = m;
+      sum *= c;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[d][j] *= c;
+    }
+    const float ref = m2 == -INFINITY ? 0.0f : m2;                 // no score above -inf yet: all weights 0
+    vh_u32x4 pf[2][2];
+    float ts[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(s[i][8 * k + j], scale2, -ref));
+        ts[2 * i + k] = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        pf[i][k] = pg_pack8(pg_f8{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]});
+      }
+    sum += (ts[0] + ts[1]) + (ts[2] + ts[3]);
+    const bool wild = lwild[buf] == t + 1 && seen;                 // as in pg_attn
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s4 lds4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const unsigned short* vb = V + (32 * i + 16 * k + 4 * g + ((lane & 15) >> 2)) * PG_WROW + 32 * d
+                                     + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+          const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vb);
+          const s4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vb + 8 * PG_WROW));
+          s8 f = __builtin_shufflevector(a, e, 0, 1, 2, 3, 4, 5, 6, 7);
+          if (wild) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = pg_wild((unsigned short)f[j]) ? 0 : f[j];
+          }
+          o[d] = pg_mfma32(__builtin_bit_cast(vh_u32x4, f), pf[i][k], o[d]);
+        }
+    if (wild) {
+      for (int s = p0; s <= min(p0 + 63, last); ++s)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const unsigned short v = V[(s - p0) * PG_WROW + 32 * d + 8 * (j >> 2) + 4 * g + (j & 3)];
+            if (pg_wild(v) && s <= lim) o[d][j] += pg_to_f(v);
+          }
+    }
+  }
+  if (__any(bad != 0) && lane == 0) pg_raise(err, PG_ERR_PAGE);
+  if (!live) return;
+  sum = vh_pair32(sum, op_sum);
+  const bool whole = parts == 1;
+  pg_q* op = out + (sq.first + tok) * orow + head * ohead;
+  float* wp = ws + (size_t)wk.at * PG_WS(128);
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = !whole ? o[d][4 * i + j] : lim < 0 ? 0.0f : o[d][4 * i + j] / sum;
+      if (whole) pg_store4(op + 32 * d + 8 * i + 4 * g, v);
+      else *(vh_f32x4*)(wp + 256 + (32 * wave + r) * PG_E + 32 * d + 8 * i + 4 * g) = vh_f32x4{v[0], v[1], v[2], v[3]};
+    }
+  if (g == 0) {
+    if (!whole) {
+      wp[32 * wave + r] = m2;
+      wp[128 + 32 * wave + r] = sum;
+    } else if (lse) {
+      lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : m2 + __builtin_amdgcn_logf(sum);
+    }
+  }
+}
+#endif
+
+// The parts of a tile of ROWS rows put together, in their order: a block makes
+// 16 rows of it, 16 lanes a row.
+template <int ROWS, int STEP>
+__device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, const int* __restrict__ lengths, int B,
+                                             int cap, int M, int H, int G, int target, int least,
+                                             const float* __restrict__ ws, pg_q* __restrict__ out, long orow,
+                                             long ohead, float* __restrict__ lse) {
+  const int tid = threadIdx.x, c = tid & 15, y = blockIdx.x % (ROWS / 16) * 16 + (tid >> 4);
+  PgWork wk;                                                       // grid: H (M G / ROWS + B) tiles or more
+  if (!pg_work<ROWS, STEP>(wk, blockIdx.x / (ROWS / 16), true, starts, lengths, B, M, cap, H, G, target, least, nullptr,
+                           0))
+    return;
+  int last, steps, parts;
+  pg_span<ROWS, STEP>(wk, G, last, steps, parts);
+  if (parts == 1 || wk.x0 + y >= wk.R) return;
+  const int x = wk.x0 + y, tok = x / G, head = wk.h * G + x % G, lim = wk.sq.len - wk.sq.count + tok;
+  const size_t next = (size_t)H * wk.tiles * PG_WS(ROWS);          // the tile's next part
+  const float* wp = ws + (size_t)wk.at * PG_WS(ROWS);
+  float m = -INFINITY;
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, wp[p * next + y]);
+  float sum = 0.0f, v[PG_E / 16] = {};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float* w = wp + p * next;
+    const float f = w[y] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w[y] - m);       // no score: 0
+    sum = fmaf(w[ROWS + y], f, sum);
+#pragma unroll
+    for (int d = 0; d < PG_E / 64; ++d) {
+      const vh_f32x4 a = *(const vh_f32x4*)(w + 2 * ROWS + y * PG_E + 64 * d + 4 * c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * d + j] = fmaf(a[j], f, v[4 * d + j]);
+    }
+  }
+  pg_q* op = out + (wk.sq.first + tok) * orow + head * ohead;
+#pragma unroll
+  for (int d = 0; d < PG_E / 64; ++d) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[4 * d + j] = lim < 0 ? 0.0f : v[4 * d + j] / sum;
+    pg_store4(op + 64 * d + 4 * c, v + 4 * d);
+  }
+  if (lse && c == 0) lse[(size_t)(wk.sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : m + __builtin_amdgcn_logf(sum);
+}
+#define PG_JOIN(name, rows, step)                                                                                  \
+  extern "C" __global__ __launch_bounds__(256) void name(                                                          \
+      const int* __restrict__ starts, const int* __restrict__ lengths, int B, int cap, int M, int H, int G,        \
+      int target, int least, const float* __restrict__ ws, pg_q* __restrict__ out, long orow, long ohead,          \
+      float* __restrict__ lse) {                                                                                   \
+    pg_join_body<rows, step>(starts, lengths, B, cap, M, H, G, target, least, ws, out, orow, ohead, lse);          \
+  }
+PG_JOIN(pg_join, 16, PG_STEP)
+#if PG_KIND != PG_F32
+PG_JOIN(pg_wide_join, 128, 64)
+#endif
 
 // ---------------------------------------------------------------- weights
 // out[b, h, s] = old[b, h, s] (0 for the chunk's own positions) + the sum over

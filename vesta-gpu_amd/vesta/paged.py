@@ -51,6 +51,10 @@ WIDTHS = (64, 128)
 KINDS = ('f16', 'bf16', 'f32')         # kernels' queries: the cache's type, or f32 over an f16 cache
 PAGE_MAX = 1 << 16
 ROWS = 16                              # query rows of a pg_attn block
+FEW_ROWS = 32                          # rows of a sequence (its most) from which pg_wide makes them
+WIDE_TARGET, WIDE_PART_STEPS = 512, 8
+TARGET = 1024                          # parts that the positions of all row tiles are cut into, about, ...
+PART_STEPS = 8                         # ... each of at least so many steps
 WEIGH = 128                            # positions of a pg_weigh block
 ERRORS = {1: 'a page id outside the pool', 2: 'starts that do not ascend, or lie past the rows',
           4: 'a length past its table', 8: 'a sequence with more new tokens than `most`'}
@@ -60,11 +64,15 @@ _SEQS = 'iipipp'                       # pages, shift, table, its columns, start
 SIGNATURES = {
     'pg_append16': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
     'pg_append32': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
-    'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iif' + 'pllpp',
+    'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiif' + 'pllppp',
+    'pg_join': 'ppiiiiiiippllp',
+    'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiif' + 'pllppp',
+    'pg_wide_join': 'ppiiiiiiippllp',
     'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipii',
     'pg_select': 'pipiiiiippipp',
     'pg_move': 'ppiipipipiiiip',
 }
+_WIDE = ('pg_wide', 'pg_wide_join')    # for 16-bit queries only
 _CODES = {'p': 'P', 'l': 'q', 'i': 'i', 'f': 'f'}
 
 
@@ -104,7 +112,7 @@ class _Kernels:
             ok(lib().vh_module_load(compile_code(paged_source(width, kind)), ctypes.byref(self.mod)),
                'paged cache module load')
             track(self)
-            for name in SIGNATURES:
+            for name in SIGNATURES if kind != 'f32' else set(SIGNATURES) - set(_WIDE):
                 fn = ctypes.c_void_p()
                 ok(lib().vh_module_get_function(self.mod, name.encode(), ctypes.byref(fn)), name)
                 setattr(self, name, _Launcher(fn, name))
@@ -299,13 +307,26 @@ class PagedCache:
             seqs = (self.pages, self._shift, table.data_ptr(), N, starts.data_ptr(), lengths.data_ptr())
             lse = None if weight is None else torch.empty(M * Hq, dtype=torch.float32, device=self.device)
             if M and B:
-                tiles = -(-most * G // ROWS)
-                if B * self.heads * tiles >= 1 << 30:
+                # a launch's tiles of rows, as many as there can be, and its parts
+                wide = most * G > FEW_ROWS and q.dtype != torch.float32
+                rows, aim = (128, WIDE_TARGET) if wide else (ROWS, TARGET)
+                tiles = self.heads * (M * G // rows + B)
+                target = aim if tiles < 2 * aim else 0
+                blocks = target + tiles + 64
+                if blocks >= 1 << 28 or M * G >= 1 << 30:
                     raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
-                kn.pg_attn(_blocks8(B * self.heads * tiles), BLOCK, stream, q.data_ptr(), *qs,
-                           self.keys.data_ptr() + at, self.vals.data_ptr() + at, *seqs, B, M, self.heads, G, tiles,
-                           most, scale2, out.data_ptr(), *os, 0 if lse is None else lse.data_ptr(),
-                           self.err.data_ptr())
+                ws = None if target == 0 else torch.empty(blocks * rows * (self.width + 2), dtype=torch.float32,
+                                                          device=self.device)
+                to = (out.data_ptr(), *os, 0 if lse is None else lse.data_ptr())
+                least = WIDE_PART_STEPS if wide else PART_STEPS
+                (kn.pg_wide if wide else kn.pg_attn)(
+                    _blocks8(blocks), BLOCK, stream, q.data_ptr(), *qs, self.keys.data_ptr() + at,
+                    self.vals.data_ptr() + at, *seqs, B, M, self.heads, G, target, least, most, scale2, *to,
+                    0 if ws is None else ws.data_ptr(), self.err.data_ptr())
+                if target:
+                    (kn.pg_wide_join if wide else kn.pg_join)(
+                        tiles * (rows // 16), BLOCK, stream, starts.data_ptr(), lengths.data_ptr(), B, N * self.page, M,
+                        self.heads, G, target, least, ws.data_ptr(), *to)
             if weight is not None and B:
                 blocks = -(-So // WEIGH)
                 kn.pg_weigh(_blocks8(B * self.heads * blocks), BLOCK, stream, q.data_ptr(), *qs,
