@@ -421,7 +421,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
     const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
     const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
     int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
-    float* __restrict__ ws, unsigned* __restrict__ err) {
+    float* __restrict__ ws, float* __restrict__ sc, long pitch, unsigned* __restrict__ err) {
   constexpr int KS = PG_E / 32, NG = PG_STEP / 16, NV = PG_STEP * PG_E / 512, DT = PG_E / 16;
   constexpr int VL = PG_E / 8, VR = 64 / VL;                       // lanes of a value row; rows of a wave's load
   __shared__ __attribute__((aligned(16))) unsigned short lv[4][PG_STEP * PG_VROW];
@@ -445,15 +445,16 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
   const size_t rowlen = (size_t)H * PG_E;
   const int* tb = table + (size_t)wk.b * N;
   const unsigned short *kh = kp + h * PG_E + 8 * q, *vh = vp + h * PG_E + lane % VL * 8;
-  // the pool rows of a step's positions, one a lane
-  auto rows = [&](int t) -> unsigned {
-    const int s = min(t * PG_STEP + lane % PG_STEP, last), page = tb[s >> shift];
+  // the page of a step's positions, one a lane: looked up a step ahead of its
+  // rows, and looked at only then (a wait for it would be one for the rows
+  // asked for before it)
+  auto look = [&](int t) { return tb[min(t * PG_STEP + lane % PG_STEP, last) >> shift]; };
+  vh_u32x4 kr[NG][KS], vr[NV];
+  auto load = [&](int t, int page) {
     const bool in = (unsigned)page < (unsigned)pages;
     if (!in) bad = PG_ERR_PAGE;
-    return ((unsigned)(in ? page : 0) << shift) + (unsigned)(s & ((1 << shift) - 1));
-  };
-  vh_u32x4 kr[NG][KS], vr[NV];
-  auto load = [&](unsigned rw) {
+    const unsigned rw = ((unsigned)(in ? page : 0) << shift)
+                        + (unsigned)(min(t * PG_STEP + lane % PG_STEP, last) & ((1 << shift) - 1));
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       const unsigned short* p = kh + (unsigned)__shfl((int)rw, 16 * i + r, 64) * rowlen;
@@ -466,12 +467,13 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
   float o[DT][4] = {};
   float m2 = -INFINITY, sum = 0.0f;
   unsigned short* V = lv[wave];
-  unsigned rw = 0;
+  int page = 0;
+  if (t0 + wave < t1) page = look(t0 + wave);
   PgQuery qf;
   pg_query(qf, qp, q, scale2);
   if (t0 + wave < t1) {
-    load(rows(t0 + wave));
-    rw = rows(min(t0 + wave + 4, t1 - 1));
+    load(t0 + wave, page);
+    page = look(min(t0 + wave + 4, t1 - 1));
   }
   for (int t = t0 + wave; t < t1; t += 4) {
     const int p0 = t * PG_STEP;
@@ -499,14 +501,20 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
     for (int n = 0; n < NV; ++n) *(vh_u32x4*)(V + (n * VR + lane / VL) * PG_VROW + lane % VL * 8) = vr[n];
     pg_wave_sync();
     if (t + 4 < t1) {
-      load(rw);
-      rw = rows(min(t + 8, t1 - 1));
+      load(t + 4, page);
+      page = look(min(t + 8, t1 - 1));
     }
     if (seen) {
 #pragma unroll
       for (int i = 0; i < NG; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = p0 + 16 * i + 4 * q + j <= lim ? s[i][j] : -INFINITY;
+    }
+    if (sc && live) {                                              // for pg_given, in powers of 2
+      float* to = sc + ((long)(sq.first + tok) * (H * G) + head) * pitch + p0 + 4 * q;
+#pragma unroll
+      for (int i = 0; i < NG; ++i)
+        *(vh_f32x4*)(to + 16 * i) = vh_f32x4{s[i][0] * qf.k2, s[i][1] * qf.k2, s[i][2] * qf.k2, s[i][3] * qf.k2};
     }
     float bm = s[0][0];
 #pragma unroll
@@ -662,7 +670,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     float* __restrict__ ws, unsigned* __restrict__ err) {
   constexpr int KS = PG_E / 16, DT = PG_E / 32, CH = PG_E / 8, NL = 64 * CH / 256;   // k-steps, dim tiles, 16-byte
   constexpr int RS = 256 / CH;                                     // pieces of a row; a thread's pieces and rows apart
-  __shared__ __attribute__((aligned(16))) vh_u32x4 lk[2][64 * CH];
+  __shared__ __attribute__((aligned(16))) vh_u32x4 lk[2][64 * (CH + 1)];
   __shared__ __attribute__((aligned(16))) unsigned short lv[2][64 * PG_WROW];
   __shared__ int lwild[2];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -692,36 +700,40 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
   const int* tb = table + (size_t)wk.b * N;
   const int c8 = tid % CH, r8 = tid / CH;
   const unsigned short *kh = kp + h * PG_E + 8 * c8, *vh = vp + h * PG_E + 8 * c8;
-  unsigned rw[NL];
-  auto rows = [&](int t) {
+  int page[NL];
+  auto look = [&](int t) {                                         // as in pg_attn
 #pragma unroll
-    for (int n = 0; n < NL; ++n) {
-      const int s = min(64 * t + r8 + RS * n, last), page = tb[s >> shift];
-      const bool in = (unsigned)page < (unsigned)pages;
-      if (!in) bad = PG_ERR_PAGE;
-      rw[n] = ((unsigned)(in ? page : 0) << shift) + (unsigned)(s & ((1 << shift) - 1));
-    }
+    for (int n = 0; n < NL; ++n) page[n] = tb[min(64 * t + r8 + RS * n, last) >> shift];
   };
   vh_u32x4 kr[NL], vr[NL];
-  auto load = [&]() {
+  auto load = [&](int t) {
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      kr[n] = ld16(kh + rw[n] * rowlen);
-      vr[n] = ld16(vh + rw[n] * rowlen);
+      const bool in = (unsigned)page[n] < (unsigned)pages;
+      if (!in) bad = PG_ERR_PAGE;
+      const size_t at = (((unsigned)(in ? page[n] : 0) << shift)
+                         + (unsigned)(min(64 * t + r8 + RS * n, last) & ((1 << shift) - 1))) * rowlen;
+      kr[n] = ld16(kh + at);
+      vr[n] = ld16(vh + at);
     }
   };
-  // Key pieces are permuted within their row by its number, so that a column of
-  // them falls on all banks. Values past the last position are 0; whether a
-  // step that some row sees in part holds one that is not finite is noted.
+  // Key rows are 16 bytes past a multiple of all banks apart, so that a column
+  // of their pieces falls on all of them. Values past the last position are 0;
+  // whether a step that some row sees in part holds one that is not finite is
+  // noted.
   auto put = [&](int t) {
     const int buf = t & 1;
-    const bool end = 64 * t + 63 > last;
     unsigned any = 0u;
+    if (64 * t + 63 > last) {
+#pragma unroll
+      for (int n = 0; n < NL; ++n)
+        if (64 * t + r8 + RS * n > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
+      asm volatile("" ::: "memory");                               // kept a branch
+    }
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
       const int row = r8 + RS * n;
-      lk[buf][row * CH + (c8 ^ (row & 7))] = kr[n];
-      if (end && 64 * t + row > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
+      lk[buf][row * (CH + 1) + c8] = kr[n];
       *(vh_u32x4*)(lv[buf] + row * PG_WROW + 8 * c8) = vr[n];
     }
     if (64 * t + 63 > bfirst) {
@@ -739,13 +751,13 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
   if (tid < 2) lwild[tid] = 0;
   vh_lds_sync();                                                   // noted as none before a step may be noted
   if (t0 < t1) {
-    rows(t0);
-    load();
-    rows(min(t0 + 1, t1 - 1));
+    look(t0);
+    load(t0);
+    look(min(t0 + 1, t1 - 1));
     put(t0);
     if (t0 + 1 < t1) {
-      load();
-      rows(min(t0 + 2, t1 - 1));
+      load(t0 + 1);
+      look(min(t0 + 2, t1 - 1));
     }
   }
   for (int t = t0; t < t1; ++t) {
@@ -753,8 +765,8 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     if (t + 1 < t1) {
       put(t + 1);
       if (t + 2 < t1) {
-        load();
-        rows(min(t + 3, t1 - 1));
+        load(t + 2);
+        look(min(t + 3, t1 - 1));
       }
     }
     const int p0 = 64 * t, buf = t & 1;
@@ -767,7 +779,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) s[i] = pg_mfma32(K[(32 * i + r) * CH + ((2 * k + g) ^ (r & 7))], qf[k], s[i]);
+      for (int k = 0; k < KS; ++k) s[i] = pg_mfma32(K[(32 * i + r) * (CH + 1) + 2 * k + g], qf[k], s[i]);
     }
     const bool seen = p0 + 63 > wfirst;                            // not the whole step by every row
     if (seen) {
@@ -776,9 +788,21 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[i][j] = p0 + 32 * i + 8 * (j >> 2) + 4 * g + (j & 3) <= lim ? s[i][j] : -INFINITY;
     }
-    float bm = fmaxf(s[0][0], s[1][0]);
+    // The largest as a whole number of the same bits, right wherever one is
+    // positive (fmaxf asks for a canonical form of every score first: 48
+    // operations more); where none is, in floats.
+    int bi = 0x80000000;
 #pragma unroll
-    for (int j = 1; j < 16; ++j) bm = fmaxf(bm, fmaxf(s[0][j], s[1][j]));
+    for (int j = 0; j < 16; ++j) {
+      const float a = s[0][j], e = s[1][j];                        // (a bit_cast of a vector's element takes its first)
+      bi = max(bi, max(__builtin_bit_cast(int, a), __builtin_bit_cast(int, e)));
+    }
+    float bm = __builtin_bit_cast(float, bi);
+    if (__any(bi < 0)) {
+      bm = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int j = 1; j < 16; ++j) bm = fmaxf(bm, fmaxf(s[0][j], s[1][j]));
+    }
     bm = vh_pair32(bm, op_max);
     const float n2 = bm * scale2;
     if (__any(n2 > m2 + PG_SLACK || (n2 > m2 && m2 == -INFINITY))) {
@@ -864,50 +888,98 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 }
 #endif
 
-// The parts of a tile of ROWS rows put together, in their order: a block makes
-// 16 rows of it, 16 lanes a row.
+// The parts of a tile of ROWS rows put together: a block of 512 threads makes
+// up to 16 rows of it, E / 4 lanes a row; where there are fewer rows their
+// parts are dealt to the lane groups left, whose results are added in order
+// (128 parts of four rows, one group a row: 60 us; dealt out: 4).
 template <int ROWS, int STEP>
 __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, const int* __restrict__ lengths, int B,
                                              int cap, int M, int H, int G, int target, int least,
                                              const float* __restrict__ ws, pg_q* __restrict__ out, long orow,
                                              long ohead, float* __restrict__ lse) {
-  const int tid = threadIdx.x, c = tid & 15, y = blockIdx.x % (ROWS / 16) * 16 + (tid >> 4);
+  constexpr int LR = PG_E / 4, NGR = 512 / LR;
+  __shared__ float jm[NGR], js[NGR];
+  __shared__ vh_f32x4 jv[512];
+  const int tid = threadIdx.x, c = tid % LR, grp = tid / LR, y0 = blockIdx.x % (ROWS / 16) * 16;
   PgWork wk;                                                       // grid: H (M G / ROWS + B) tiles or more
   if (!pg_work<ROWS, STEP>(wk, blockIdx.x / (ROWS / 16), true, starts, lengths, B, M, cap, H, G, target, least, nullptr,
                            0))
     return;
   int last, steps, parts;
   pg_span<ROWS, STEP>(wk, G, last, steps, parts);
-  if (parts == 1 || wk.x0 + y >= wk.R) return;
-  const int x = wk.x0 + y, tok = x / G, head = wk.h * G + x % G, lim = wk.sq.len - wk.sq.count + tok;
+  const int n = min(16, wk.R - wk.x0 - y0);                        // rows
+  if (parts == 1 || n <= 0) return;
+  const int n2 = n == 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)), slices = NGR / n2;
+  const int y = y0 + grp % n2, slice = grp / n2;
   const size_t next = (size_t)H * wk.tiles * PG_WS(ROWS);          // the tile's next part
   const float* wp = ws + (size_t)wk.at * PG_WS(ROWS);
-  float m = -INFINITY;
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, wp[p * next + y]);
-  float sum = 0.0f, v[PG_E / 16] = {};
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float* w = wp + p * next;
-    const float f = w[y] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w[y] - m);       // no score: 0
-    sum = fmaf(w[ROWS + y], f, sum);
+  float m = -INFINITY, sum = 0.0f;
+  vh_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (grp % n2 < n) {
+    for (int p0 = slice; p0 < parts; p0 += 8 * slices) {
+      float pm[8], ps[8];
+      vh_f32x4 pv[8];
 #pragma unroll
-    for (int d = 0; d < PG_E / 64; ++d) {
-      const vh_f32x4 a = *(const vh_f32x4*)(w + 2 * ROWS + y * PG_E + 64 * d + 4 * c);
+      for (int u = 0; u < 8; ++u) {                                // past the last: the last again, without weight
+        const int p = p0 + u * slices;
+        const float* w = wp + min(p, parts - 1) * next;
+        pm[u] = p < parts ? w[y] : -INFINITY;
+        ps[u] = w[ROWS + y];
+        pv[u] = *(const vh_f32x4*)(w + 2 * ROWS + y * PG_E + 4 * c);
+      }
+      float mm = m;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * d + j] = fmaf(a[j], f, v[4 * d + j]);
+      for (int u = 0; u < 8; ++u) mm = fmaxf(mm, pm[u]);
+      const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mm);       // no score: 0
+      m = mm;
+      sum *= old;
+      v *= old;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        // a part without a score has no weight, unless its sum is a NaN, which it keeps
+        const float f = p0 + u * slices >= parts ? 0.0f : pm[u] == -INFINITY ? (ps[u] == ps[u] ? 0.0f : 1.0f)
+                                                                             : __builtin_amdgcn_exp2f(pm[u] - mm);
+        if (f != 0.0f) {
+          sum = fmaf(ps[u], f, sum);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = fmaf(pv[u][j], f, v[j]);
+        }
+      }
     }
   }
-  pg_q* op = out + (wk.sq.first + tok) * orow + head * ohead;
+  if (slices > 1) {
+    if (c == 0) {
+      jm[grp] = m;
+      js[grp] = sum;
+    }
+    jv[tid] = v;
+    __syncthreads();
+    if (slice > 0) return;
+    float mm = m;
+    for (int k = 1; k < slices; ++k) mm = fmaxf(mm, jm[grp + k * n2]);
+    const float old = m == -INFINITY ? (sum == sum ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - mm);
+    sum *= old;
+    v *= old;
+    for (int k = 1; k < slices; ++k) {
+      const float km = jm[grp + k * n2], ks = js[grp + k * n2];
+      const float f = km == -INFINITY ? (ks == ks ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(km - mm);
+      if (f == 0.0f) continue;
+      sum = fmaf(ks, f, sum);
 #pragma unroll
-  for (int d = 0; d < PG_E / 64; ++d) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[4 * d + j] = lim < 0 ? 0.0f : v[4 * d + j] / sum;
-    pg_store4(op + 64 * d + 4 * c, v + 4 * d);
+      for (int j = 0; j < 4; ++j) v[j] = fmaf(jv[tid + k * n2 * LR][j], f, v[j]);
+    }
+    m = mm;
   }
+  if (grp % n2 >= n || slice > 0) return;
+  const int x = wk.x0 + y, tok = x / G, head = wk.h * G + x % G, lim = wk.sq.len - wk.sq.count + tok;
+  float w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = lim < 0 ? 0.0f : v[j] / sum;
+  pg_store4(out + (wk.sq.first + tok) * orow + head * ohead + 4 * c, w);
   if (lse && c == 0) lse[(size_t)(wk.sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : m + __builtin_amdgcn_logf(sum);
 }
 #define PG_JOIN(name, rows, step)                                                                                  \
-  extern "C" __global__ __launch_bounds__(256) void name(                                                          \
+  extern "C" __global__ __launch_bounds__(512) void name(                                                          \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int cap, int M, int H, int G,        \
       int target, int least, const float* __restrict__ ws, pg_q* __restrict__ out, long orow, long ohead,          \
       float* __restrict__ lse) {                                                                                   \
@@ -924,12 +996,13 @@ PG_JOIN(pg_wide_join, 128, 64)
 // s; 0 past the length. A block takes 128 positions of one (sequence, key
 // head), 32 to a wave, their key rows in registers, and goes through the rows
 // that see them, 16 at a time, in order: no atomics, the same sums each time.
+// `out` may be `old`: a thread reads an element before it writes it.
 // Scores are made again (as in pg_attn), the weight is 2^(score - lse).
 extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
     const int* __restrict__ table, int N, const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
-    int H, int G, float scale2, const float* __restrict__ lse, const float* __restrict__ old, int S,
-    float* __restrict__ out, int So, int blocks) {
+    int H, int G, float scale2, const float* __restrict__ lse, const float* old, int S, float* out, int So,
+    int blocks) {
   constexpr int KS = PG_E / 32;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, q = lane >> 4;
@@ -981,6 +1054,155 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh(
       if (r == 0 && s < So) out[bh * So + s] = w + (s < new0 ? old[bh * S + s] : 0.0f);
     }
 }
+
+// The same where pg_attn left its scores (rows of `pitch` in `sc`): a thread
+// takes every 256th of 1024 positions.
+extern "C" __global__ __launch_bounds__(256) void pg_given(const float* __restrict__ sc, long pitch,
+                                                           const int* __restrict__ starts,
+                                                           const int* __restrict__ lengths, int cap, int M, int H, int G,
+                                                           const float* __restrict__ lse, const float* old, int S,
+                                                           float* out, int So, int blocks) {
+  const int bh = blockIdx.x / blocks, b = bh / H, h = bh % H;      // grid: B * H * blocks
+  const int p0 = blockIdx.x % blocks * 1024 + threadIdx.x;
+  const PgSeq sq = pg_seq(starts, lengths, b, M, cap);
+  const int new0 = sq.len - sq.count;
+  float acc[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) acc[u] = p0 + 256 * u < min(new0, So) ? old[(size_t)bh * S + p0 + 256 * u] : 0.0f;
+  for (int j = max(p0 - (int)threadIdx.x - new0, 0); j < sq.count; ++j)   // tokens that see some of the 1024
+    for (int g = 0; g < G; ++g) {
+      const long row = (long)(sq.first + j) * (H * G) + h * G + g;
+      const float z = lse[row];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int s = p0 + 256 * u;
+        if (s <= new0 + j) acc[u] += __builtin_amdgcn_exp2f(sc[row * pitch + s] - z);
+      }
+    }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (p0 + 256 * u < So) out[(size_t)bh * So + p0 + 256 * u] = acc[u];
+}
+
+// The same for many rows of 16-bit queries: a block takes 256 positions of one
+// (sequence, key head), 64 to a wave, their key rows in registers, and a slice
+// of the rows that see them, 32 at a time through LDS (double-buffered, with
+// the rows' lse), on tiles of 32 x 32 x 16 as in pg_wide. A wave's sums stay in
+// registers over all rows. Several slices (few positions, many rows) leave
+// their sums in `part` [slice][B H So] for pg_total.
+#if PG_KIND != PG_F32
+extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
+    const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
+    const int* __restrict__ table, int N, const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
+    int H, int G, float scale2, const float* __restrict__ lse, const float* old, int S,
+    float* out, int So, int blocks, int slices, float* __restrict__ part) {
+  constexpr int KS = PG_E / 16, CH = PG_E / 8, NL = 32 * CH / 256, RS = 256 / CH;
+  __shared__ __attribute__((aligned(16))) vh_u32x4 lq[2][32 * CH];
+  __shared__ float lz[2][32];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int r = lane & 31, g = lane >> 5;
+  const int T = B * H * blocks * slices, per = (T + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || id >= T) return;
+  const int slice = id % slices, bh = id / slices / blocks, b = bh / H, h = bh % H;
+  const int b0 = id / slices % blocks * 256, p0 = b0 + 64 * wave;
+  const PgSeq sq = pg_seq(starts, lengths, b, M, N << shift);
+  const int new0 = sq.len - sq.count, R = sq.count * G;
+  // the slice's rows: its share of the 32-row tiles from the first token that sees the block's first position
+  const int tile0 = max(b0 - new0, 0) * G / 32, tiles = b0 < sq.len ? max((R + 31) / 32 - tile0, 0) : 0;
+  const int share = (tiles + slices - 1) / slices;
+  const int x0 = (tile0 + min(slice * share, tiles)) * 32, x1 = (tile0 + min((slice + 1) * share, tiles)) * 32;
+  float acc[2][16] = {};
+  vh_u32x4 kf[2][KS];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = min(p0 + 32 * i + r, sq.len - 1), page = x0 < x1 ? table[(size_t)b * N + (max(s, 0) >> shift)] : 0;
+    const size_t at = ((size_t)((unsigned)page < (unsigned)pages ? page : 0) << shift) + (max(s, 0) & ((1 << shift) - 1));
+#pragma unroll
+    for (int k = 0; k < KS; ++k) kf[i][k] = ld16(kp + (at * H + h) * PG_E + 16 * k + 8 * g);
+  }
+  const int c8 = tid % CH, r8 = tid / CH;
+  vh_u32x4 qr[NL];
+  float zr = 0.0f;
+  auto load = [&](int x) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int y = min(x + r8 + RS * n, R - 1), tok = y / G;
+      qr[n] = ld16(Q + (sq.first + tok) * qrow + (h * G + y % G) * qhead + 8 * c8);
+    }
+    if (tid < 32) {                                                // past the last row: no weight
+      const int y = min(x + tid, R - 1);
+      zr = x + tid < R ? lse[(size_t)(sq.first + y / G) * (H * G) + h * G + y % G] : INFINITY;
+    }
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) lq[buf][(r8 + RS * n) * CH + (c8 ^ ((r8 + RS * n) & 7))] = qr[n];
+    if (tid < 32) lz[buf][tid] = zr;
+  };
+  if (x0 < x1) {
+    load(x0);
+    put(0);
+    if (x0 + 32 < x1) load(x0 + 32);
+  }
+  for (int x = x0, buf = 0; x < x1; x += 32, buf ^= 1) {
+    vh_lds_sync();
+    if (x + 32 < x1) {
+      put(buf ^ 1);
+      if (x + 64 < x1) load(x + 64);
+    }
+    if (new0 + min(x + 31, R - 1) / G < p0) continue;              // no row sees the wave's positions
+    const float z = lz[buf][r];
+    pg_f16v s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const vh_u32x4 qf = lq[buf][r * CH + ((2 * k + g) ^ (r & 7))];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i] = pg_mfma32(kf[i][k], qf, s[i]);
+    }
+    if (p0 + 63 > new0 + x / G) {                                  // not all of them by every row
+      const int lim = new0 + min(x + r, R - 1) / G;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[i][j] = p0 + 32 * i + 8 * (j >> 2) + 4 * g + (j & 3) <= lim ? s[i][j] : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[i][j] += __builtin_amdgcn_exp2f(fmaf(s[i][j], scale2, -z));
+  }
+  // over the rows: lane 32 g + r keeps position 32 (r / 16) + 8 (r % 16 / 4) + 4 g + r % 4
+  float w = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float v = group_red_sum(acc[i][j], 32);
+      if (r == 16 * i + j) w = v;
+    }
+  const int s = p0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * g + (r & 3);
+  if (s >= So) return;
+  if (slices > 1) part[((size_t)slice * B * H + bh) * So + s] = w;
+  else out[(size_t)bh * So + s] = w + (s < new0 ? old[(size_t)bh * S + s] : 0.0f);
+}
+
+// The slices' sums added to the old ones, in order.
+extern "C" __global__ __launch_bounds__(256) void pg_total(const float* __restrict__ part, int slices,
+                                                           const int* __restrict__ starts,
+                                                           const int* __restrict__ lengths, int cap, int B, int M, int H,
+                                                           const float* old, int S, float* out, int So, int blocks) {
+  const int bh = blockIdx.x / blocks, s = blockIdx.x % blocks * 256 + threadIdx.x;     // grid: B * H * blocks
+  if (s >= So) return;
+  const PgSeq sq = pg_seq(starts, lengths, bh / H, M, cap);
+  float w = 0.0f;
+  for (int k = 0; k < slices; ++k) w += part[((size_t)k * B * H + bh) * So + s];
+  out[(size_t)bh * So + s] = w + (s < sq.len - sq.count ? old[(size_t)bh * S + s] : 0.0f);
+}
+#endif
 
 // ---------------------------------------------------------------- eviction
 // pg_select: a block per (layer, sequence, head) finds which positions stay:

@@ -53,7 +53,11 @@ PAGE_MAX = 1 << 16
 ROWS = 16                              # query rows of a pg_attn block
 FEW_ROWS = 32                          # rows of a sequence (its most) from which pg_wide makes them
 WIDE_TARGET, WIDE_PART_STEPS = 512, 8
-TARGET = 1024                          # parts that the positions of all row tiles are cut into, about, ...
+JOIN_BLOCK = 512
+WEIGH_BLOCKS = 1024
+SCORES_MAX = 1 << 27                   # scores (512 MB) that a call may keep for its weights' pass
+SPLIT, WIDE_SPLIT = 2048, 1024
+TARGET = 1536                          # parts that the positions of all row tiles are cut into, about, ...
 PART_STEPS = 8                         # ... each of at least so many steps
 WEIGH = 128                            # positions of a pg_weigh block
 ERRORS = {1: 'a page id outside the pool', 2: 'starts that do not ascend, or lie past the rows',
@@ -64,15 +68,18 @@ _SEQS = 'iipipp'                       # pages, shift, table, its columns, start
 SIGNATURES = {
     'pg_append16': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
     'pg_append32': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
-    'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiif' + 'pllppp',
+    'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiif' + 'pllpp' + 'plp',
     'pg_join': 'ppiiiiiiippllp',
     'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiif' + 'pllppp',
     'pg_wide_join': 'ppiiiiiiippllp',
     'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipii',
+    'pg_given': 'plppiiiippipii',
+    'pg_weigh_wide': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiiip',
+    'pg_total': 'pippiiiipipii',
     'pg_select': 'pipiiiiippipp',
     'pg_move': 'ppiipipipiiiip',
 }
-_WIDE = ('pg_wide', 'pg_wide_join')    # for 16-bit queries only
+_WIDE = ('pg_wide', 'pg_wide_join', 'pg_weigh_wide', 'pg_total')    # for 16-bit queries only
 _CODES = {'p': 'P', 'l': 'q', 'i': 'i', 'f': 'f'}
 
 
@@ -133,6 +140,11 @@ def _kernels(device, width, kind):
         if key not in _loaded:
             _loaded[key] = _Kernels(device, width, kind)
         return _loaded[key]
+
+
+def _at(t):
+    """A tensor's address, 0 for none."""
+    return 0 if t is None else t.data_ptr()
 
 
 def _blocks8(n):
@@ -305,34 +317,63 @@ class PagedCache:
         with self._on_device():
             stream = self._stream()
             seqs = (self.pages, self._shift, table.data_ptr(), N, starts.data_ptr(), lengths.data_ptr())
-            lse = None if weight is None else torch.empty(M * Hq, dtype=torch.float32, device=self.device)
+            lse = scores = None
+            pitch = 0
+            # a launch's tiles of rows, as many as there can be, and its parts
+            wide = most * G > FEW_ROWS and q.dtype != torch.float32
+            if weight is not None:
+                lse = torch.empty(M * Hq, dtype=torch.float32, device=self.device)
+                pitch = -(-N * self.page // 64) * 64
+                if not wide and 0 < M * Hq * pitch <= SCORES_MAX:
+                    scores = torch.empty(M * Hq * pitch, dtype=torch.float32, device=self.device)
             if M and B:
-                # a launch's tiles of rows, as many as there can be, and its parts
-                wide = most * G > FEW_ROWS and q.dtype != torch.float32
                 rows, aim = (128, WIDE_TARGET) if wide else (ROWS, TARGET)
                 tiles = self.heads * (M * G // rows + B)
-                target = aim if tiles < 2 * aim else 0
+                target = aim if tiles < 2 * aim and N * self.page > (WIDE_SPLIT if wide else SPLIT) else 0
                 blocks = target + tiles + 64
                 if blocks >= 1 << 28 or M * G >= 1 << 30:
                     raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
                 ws = None if target == 0 else torch.empty(blocks * rows * (self.width + 2), dtype=torch.float32,
                                                           device=self.device)
-                to = (out.data_ptr(), *os, 0 if lse is None else lse.data_ptr())
+                to = (out.data_ptr(), *os, _at(lse))
                 least = WIDE_PART_STEPS if wide else PART_STEPS
-                (kn.pg_wide if wide else kn.pg_attn)(
-                    _blocks8(blocks), BLOCK, stream, q.data_ptr(), *qs, self.keys.data_ptr() + at,
-                    self.vals.data_ptr() + at, *seqs, B, M, self.heads, G, target, least, most, scale2, *to,
-                    0 if ws is None else ws.data_ptr(), self.err.data_ptr())
+                args = (_blocks8(blocks), BLOCK, stream, q.data_ptr(), *qs, self.keys.data_ptr() + at,
+                        self.vals.data_ptr() + at, *seqs, B, M, self.heads, G, target, least, most, scale2, *to, _at(ws))
+                if wide:
+                    kn.pg_wide(*args, self.err.data_ptr())
+                else:
+                    kn.pg_attn(*args, _at(scores), pitch, self.err.data_ptr())
                 if target:
                     (kn.pg_wide_join if wide else kn.pg_join)(
-                        tiles * (rows // 16), BLOCK, stream, starts.data_ptr(), lengths.data_ptr(), B, N * self.page, M,
-                        self.heads, G, target, least, ws.data_ptr(), *to)
+                        tiles * (rows // 16), JOIN_BLOCK, stream, starts.data_ptr(), lengths.data_ptr(), B,
+                        N * self.page, M, self.heads, G, target, least, ws.data_ptr(), *to)
             if weight is not None and B:
-                blocks = -(-So // WEIGH)
-                kn.pg_weigh(_blocks8(B * self.heads * blocks), BLOCK, stream, q.data_ptr(), *qs,
-                            self.keys.data_ptr() + at, *seqs, B, M, self.heads, G, scale2, lse.data_ptr(),
-                            weight.data_ptr(), S, weight_out.data_ptr(), So, blocks)
+                self._receive(kn, stream, (q.data_ptr(), *qs, self.keys.data_ptr() + at), seqs, (B, M, G), most, wide,
+                              scale2, lse, scores, pitch, (weight.data_ptr(), S, weight_out.data_ptr(), So))
         return out if weight is None else (out, weight_out)
+
+    def _receive(self, kn, stream, keys, seqs, extents, most, wide, scale2, lse, scores, pitch, to):
+        """The weights' pass after ``attend``'s: from the scores it left, or making them again."""
+        import torch
+        B, M, G = extents
+        bh, So, cap = B * self.heads, to[-1], seqs[3] * self.page
+        if scores is not None:
+            blocks = -(-So // 1024)
+            kn.pg_given(bh * blocks, BLOCK, stream, scores.data_ptr(), pitch, *seqs[4:], cap, M, self.heads, G,
+                        lse.data_ptr(), *to, blocks)
+        elif not wide:
+            blocks = -(-So // WEIGH)
+            kn.pg_weigh(_blocks8(bh * blocks), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2, lse.data_ptr(),
+                        *to, blocks)
+        else:
+            blocks = -(-So // 256)
+            slices = max(1, min(WEIGH_BLOCKS // (bh * blocks), most * G // 256))
+            part = None if slices == 1 else torch.empty(slices * bh * So, dtype=torch.float32, device=self.device)
+            kn.pg_weigh_wide(_blocks8(bh * blocks * slices), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2,
+                             lse.data_ptr(), *to, blocks, slices, _at(part))
+            if slices > 1:
+                kn.pg_total(bh * blocks, BLOCK, stream, part.data_ptr(), slices, *seqs[4:], cap, B, M, self.heads, *to,
+                            blocks)
 
     def _weights(self, name, w, lead, least):
         import torch
