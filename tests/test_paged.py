@@ -135,6 +135,9 @@ def test_attend_refusals():
                     (dict(scale=-1.0), ValueError), (dict(scale=float('nan')), ValueError),
                     (dict(scale=float('inf')), ValueError), (dict(most=0), ValueError),
                     (dict(out=q.float()), TypeError), (dict(out=_rows(4, 6)), ValueError),
+                    (dict(out=_rows(1, 6).expand(5, 6, 64)), ValueError),
+                    (dict(out=_rows(5, 1).expand(5, 6, 64)), ValueError), (dict(q=None), TypeError),
+                    (dict(table=None), TypeError), (dict(lengths=[1, 2]), TypeError), (dict(weight=3), TypeError),
                     (dict(weight=w.half()), TypeError), (dict(weight=w[:, :, :-1]), TypeError),
                     (dict(weight=w[:, :, :-1].contiguous()), ValueError), (dict(weight=w[:1]), ValueError),
                     (dict(weight=w[None]), ValueError), (dict(weight_out=w), ValueError),

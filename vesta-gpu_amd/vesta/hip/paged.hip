@@ -1208,24 +1208,31 @@ extern "C" __global__ __launch_bounds__(256) void pg_total(const float* __restri
 // pg_select: a block per (layer, sequence, head) finds which positions stay:
 // the `recent` last and, of the others, those of largest weight, ties to the
 // lowest position, min(keep, length) in all. The weight of the last one to stay
-// is found eight bits at a time (histograms of an order-preserving integer
-// key), then the positions are listed in order. A NaN counts as the largest.
+// is found 11, 11 and 10 bits at a time (histograms in LDS of an
+// order-preserving whole number: with fewer bits at once the first digit, an
+// exponent, takes few values, whose adds wait for each other), ending early
+// where all that share a prefix stay; then the positions are listed in order,
+// four consecutive ones a thread. A NaN counts as the largest. What bounds it:
+// the chain of passes over a block's weights, not bytes.
+#define PG_BINS 2048
 __device__ __forceinline__ unsigned pg_key(float w) {
   const unsigned u = __builtin_bit_cast(unsigned, w + 0.0f);       // -0 as 0
   if (w != w) return 0xffffffffu;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+#define PG_HELD 8                          // groups of four consecutive weights a thread holds in registers
+
 extern "C" __global__ __launch_bounds__(1024) void pg_select(const float* __restrict__ weight, int S,
                                                              const int* __restrict__ lengths, int cap, int B, int H,
                                                              int keep, int recent, int* __restrict__ kept,
                                                              float* __restrict__ wout, int So,
                                                              int* __restrict__ lout, unsigned* __restrict__ err) {
-  __shared__ int hist[256];
-  __shared__ int wsum[16][2];
-  __shared__ unsigned s_prefix;
-  __shared__ int s_need;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int hist[PG_BINS];
+  __shared__ int part[PG_HELD][16];
+  __shared__ int found[3];                                         // the digit, how many of it stay, how many have it
+  const int tid = threadIdx.x, threads = blockDim.x;               // 256 or 1024
+  const int lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
   const int b = blockIdx.x / H % B;                                // grid: layers * B * H
   const int len = lengths[b], n = min(max(len, 0), cap);
   const int m = min(keep, n), last = min(recent, m), C = n - last, take = m - last;
@@ -1234,68 +1241,118 @@ extern "C" __global__ __launch_bounds__(1024) void pg_select(const float* __rest
     if (n != len) pg_raise(err, PG_ERR_LENGTH);
   }
   const float* w = weight + (size_t)blockIdx.x * S;
+  // Group c of a thread: positions 4 (c threads + tid) .. + 3. The first
+  // PG_HELD groups are loaded once, the rest (a long sequence's) in each pass.
+  const int block = 4 * threads, held = PG_HELD * block;
+  float x[PG_HELD][4];
+  auto get = [&](int base) {
+#pragma unroll
+    for (int c = 0; c < PG_HELD; ++c)
+      if (base + c * block < n)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[c][u] = w[min(base + c * block + 4 * tid + u, n - 1)];
+  };
+  get(0);
+  // of those whose key's bits from `bit` on are `prefix`, the first `need` stay,
+  // and all above
   unsigned prefix = 0;
-  int need = take;                                                 // of those with the prefix so far
-  for (int bit = 24; bit >= 0; bit -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  int need = take, bit = 32;
+  while (bit > 0 && take > 0 && take < C) {                        // the same for all threads
+    const int bits = bit == 10 ? 10 : 11, low = bit - bits;
+    for (int v = tid; v < PG_BINS; v += threads) hist[v] = 0;
     __syncthreads();
-    for (int s = tid; s < C; s += 1024) {
-      const unsigned k = pg_key(w[s]);
-      if (bit == 24 || (k >> (bit + 8)) == prefix) atomicAdd(&hist[(k >> bit) & 255u], 1);
+    for (int base = 0; base < C; base += held) {
+      if (n > held) get(base);
+#pragma unroll
+      for (int c = 0; c < PG_HELD; ++c)
+        if (base + c * block < C)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const unsigned k = pg_key(x[c][u]);
+            if (base + c * block + 4 * tid + u < C && (bit == 32 || k >> (bit & 31) == prefix))
+              atomicAdd(&hist[(k >> low) & ((1u << bits) - 1u)], 1);
+          }
     }
     __syncthreads();
-    if (tid == 0) {
-      int v = 255, left = need;
-      while (v > 0 && left > hist[v]) left -= hist[v--];
-      s_prefix = prefix << 8 | (unsigned)v;
-      s_need = left;
+    // thread t takes the bins from the top, PG_BINS / threads each
+    const int each = PG_BINS / threads, top = PG_BINS - 1 - tid * each;
+    int mine = 0;
+    for (int v = 0; v < each; ++v) mine += hist[top - v];
+    const int upto = pg_scan(mine, lane);
+    if (lane == 63) part[0][wave] = upto;
+    __syncthreads();
+    int above = upto - mine;
+    for (int i = 0; i < wave; ++i) above += part[0][i];
+    if (above < need && need <= above + mine) {                    // one thread's
+      int v = top;
+      while (above + hist[v] < need) above += hist[v--];
+      found[0] = v;
+      found[1] = need - above;
+      found[2] = hist[v];
     }
     __syncthreads();
-    prefix = s_prefix;
-    need = s_need;
+    prefix = prefix << bits | (unsigned)found[0];
+    need = found[1];
+    bit = low;
+    if (need == found[2]) break;
+    __syncthreads();                                               // found is read
   }
-  // positions in order: those above the key stay, and the first `need` that equal it
+  if (take >= C) need = C;                                         // all of them
+  // positions in order
   int* kp = kept + (size_t)blockIdx.x * keep;
   float* wp = wout + (size_t)blockIdx.x * So;
-  int above0 = 0, same0 = 0;
-  for (int base = 0; base < n; base += 1024) {
-    const int s = base + tid;
-    float x = 0.0f;
-    bool above = false, same = false;
-    if (s < n) {
-      x = w[s];
-      const unsigned k = pg_key(x);
-      above = s >= C || (take > 0 && k > prefix);
-      same = s < C && take > 0 && k == prefix;
-    }
-    const unsigned long long am = __ballot(above), sm = __ballot(same), below = (1ull << lane) - 1ull;
-    if (lane == 0) {
-      wsum[wave][0] = __popcll(am);
-      wsum[wave][1] = __popcll(sm);
-    }
-    __syncthreads();
-    int a = above0, e = same0;
-    for (int i = 0; i < 16; ++i) {
-      if (i < wave) {
-        a += wsum[i][0];
-        e += wsum[i][1];
-      }
-      above0 += wsum[i][0];
-      same0 += wsum[i][1];
-    }
-    a += __popcll(am & below);
-    e += __popcll(sm & below);
-    if (above || (same && e < need)) {
-      const int to = a + min(e, need);
-      if (to < keep) {
-        kp[to] = s;
-        wp[to] = x;
+  int above0 = 0, same0 = 0;                                       // in the groups before
+  for (int base = 0; base < n; base += held) {
+    if (n > held) get(base);
+    unsigned stay[PG_HELD];                                        // bits u: above, 4 + u: same
+    int upto[PG_HELD];                                             // above: low half, same: high half
+    __syncthreads();                                               // part is read
+#pragma unroll
+    for (int c = 0; c < PG_HELD; ++c) {
+      stay[c] = 0;
+      upto[c] = 0;
+      if (base + c * block < n) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int s = base + c * block + 4 * tid + u;
+          const unsigned k = bit == 32 ? 0u : pg_key(x[c][u]) >> bit;
+          if (s < n && (s >= C || (take > 0 && k > prefix))) stay[c] |= 1u << u;
+          if (s < C && take > 0 && k == prefix) stay[c] |= 16u << u;
+        }
+        upto[c] = pg_scan(__builtin_popcount(stay[c] & 15u) + (__builtin_popcount(stay[c] & 240u) << 16), lane);
+        if (lane == 63) part[c][wave] = upto[c];
       }
     }
     __syncthreads();
+#pragma unroll
+    for (int c = 0; c < PG_HELD; ++c) {
+      if (base + c * block >= n) continue;
+      int before = 0, total = 0;
+      for (int i = 0; i < waves; ++i) {
+        if (i < wave) before += part[c][i];
+        total += part[c][i];
+      }
+      before += upto[c] - __builtin_popcount(stay[c] & 15u) - (__builtin_popcount(stay[c] & 240u) << 16);
+      int a = above0 + (before & 0xffff), e = same0 + (before >> 16);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool above = stay[c] >> u & 1u, same = stay[c] >> (4 + u) & 1u;
+        if (above || (same && e < need)) {
+          const int to = a + min(e, need);
+          if (to < keep) {
+            kp[to] = base + c * block + 4 * tid + u;
+            wp[to] = x[c][u];
+          }
+        }
+        a += above ? 1 : 0;
+        e += same ? 1 : 0;
+      }
+      above0 += total & 0xffff;
+      same0 += total >> 16;
+    }
   }
-  for (int s = m + tid; s < keep; s += 1024) kp[s] = -1;
-  for (int s = m + tid; s < So; s += 1024) wp[s] = 0.0f;
+  for (int s = m + tid; s < keep; s += threads) kp[s] = -1;
+  for (int s = m + tid; s < So; s += threads) wp[s] = 0.0f;
 }
 
 // pg_move: the kept rows of all layers into the pages of the other table, 16

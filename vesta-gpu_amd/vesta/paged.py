@@ -36,6 +36,7 @@ programs whose rows come and go.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import struct
@@ -54,6 +55,7 @@ ROWS = 16                              # query rows of a pg_attn block
 FEW_ROWS = 32                          # rows of a sequence (its most) from which pg_wide makes them
 WIDE_TARGET, WIDE_PART_STEPS = 512, 8
 JOIN_BLOCK = 512
+SELECT_FEW = 4096
 WEIGH_BLOCKS = 1024
 SCORES_MAX = 1 << 27                   # scores (512 MB) that a call may keep for its weights' pass
 SPLIT, WIDE_SPLIT = 2048, 1024
@@ -101,12 +103,14 @@ class _Launcher:
         base = ctypes.addressof(self.buf)
         offs = [struct.calcsize(codes[:k + 1]) - struct.calcsize(codes[k]) for k in range(1, len(codes))]
         self.args = (ctypes.c_void_p * len(offs))(*[base + o for o in offs])
+        self.launch = lib().vh_launch
 
     def __call__(self, grid, block, stream, *vals):
         with self.lock:
             self.pack.pack_into(self.buf, 0, *vals)
-            status = lib().vh_launch(self.fn, grid, block, 0, stream, self.args)
-        ok(status, self.name)
+            status = self.launch(self.fn, grid, block, 0, stream, self.args)
+        if status:
+            ok(status, self.name)
 
 
 class _Kernels:
@@ -130,6 +134,8 @@ class _Kernels:
             unload(mod)
 
 
+_HERE = contextlib.nullcontext()       # the cache's device is the current one
+_ANY2 = (None, None)
 _loaded = {}
 _loaded_lock = threading.Lock()
 
@@ -185,6 +191,7 @@ class PagedCache:
             raise ValueError(f'{pages} pages of {page} rows: fewer than 2^31 rows a layer')
         self.pages, self.heads, self.width, self.layers, self.page = pages, heads, width, layers, page
         self._shift = page.bit_length() - 1
+        self._scale = 1.0 / math.sqrt(width)
         self._dt = dtype
 
     def _allocate(self, device):
@@ -195,42 +202,56 @@ class PagedCache:
         self.keys = torch.zeros(shape, dtype=self.dtype, device=self.device)
         self.vals = torch.zeros(shape, dtype=self.dtype, device=self.device)
         self._layer_bytes = self.keys[0].numel() * 2
+        # what every call needs (a call's checks cost about as much as its launch)
+        self._pools = self.keys.data_ptr(), self.vals.data_ptr()
+        self._index = self.keys.get_device()
+        self._i32, self._f32, self._empty = torch.int32, torch.float32, torch.empty
+        self._new = self.dtype, self._f32                          # types of new rows, and of queries
+        self._queries = self._new if self._dt == 'f16' else (self.dtype,)
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._err = self.err.data_ptr()
 
     # ------------------------------------------------------------ checks
     def _ints(self, name, t, shape):
-        import torch
-        if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == self.device
-                and t.is_contiguous()):
+        try:
+            fits = t.dtype is self._i32 and t.get_device() == self._index and t.is_contiguous()
+            got = t.shape
+        except AttributeError:
+            fits = False
+        if not fits:
             raise TypeError(f'{name}: need a contiguous int32 tensor on {self.device}')
-        if t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
-            raise ValueError(f'{name}: shape {tuple(t.shape)}, need {tuple("any" if w is None else w for w in shape)}')
+        if got != shape and (shape[-1] is not None or len(got) != 2 or shape[0] not in (None, got[0])):
+            raise ValueError(f'{name}: shape {tuple(got)}, need {tuple("any" if w is None else w for w in shape)}')
+        return t.data_ptr()
 
     def _batch(self, table, starts, lengths):
-        self._ints('table', table, (None, None))
+        """B, N and the kernels' arguments for a batch."""
+        at = self._ints('table', table, _ANY2)
         B, N = table.shape
         if N * self.page >= 1 << 31:
             raise ValueError(f'table: {N} pages of {self.page} rows a sequence, fewer than 2^31 rows are possible')
-        if starts is not None:
-            self._ints('starts', starts, (B + 1,))
-        self._ints('lengths', lengths, (B,))
-        return B, N
+        return B, N, (self.pages, self._shift, at, N, 0 if starts is None else self._ints('starts', starts, (B + 1,)),
+                      self._ints('lengths', lengths, (B,)))
 
     def _rows(self, name, t, dtypes, heads=None, like=None):
-        """New tokens' rows [M, heads, width]: any strides but the last, 16-byte aligned."""
-        import torch
-        if not (isinstance(t, torch.Tensor) and t.device == self.device and t.dtype in dtypes):
+        """New tokens' rows [M, heads, width]: any strides but the last, 16-byte aligned. Returns their address and
+        strides."""
+        try:
+            fits = t.dtype in dtypes and t.get_device() == self._index
+            shape = t.shape
+        except AttributeError:
+            fits = False
+        if not fits:
             raise TypeError(f'{name}: need a tensor of {" or ".join(str(d)[6:] for d in dtypes)} on {self.device}')
-        shape = t.shape
         if len(shape) != 3 or shape[2] != self.width or (heads is not None and shape[1] != heads) \
                 or (like is not None and shape != like):
             raise ValueError(f'{name}: shape {tuple(shape)}, need '
                              f'{tuple(like) if like is not None else ("rows", heads or "heads", self.width)}')
         row, head, one = t.stride()
-        unit = 16 // t.element_size()
-        if t.numel() and (one != 1 or row % unit or head % unit or t.data_ptr() % 16):
+        at = t.data_ptr()
+        if (one != 1 or (row | head) & (3 if t.dtype is self._f32 else 7) or at & 15) and t.numel():
             raise ValueError(f'{name}: rows of consecutive, 16-byte aligned values needed (strides {t.stride()})')
-        return row, head
+        return at, row, head
 
     def _layer(self, layer):
         if not 0 <= layer < self.layers:
@@ -239,7 +260,7 @@ class PagedCache:
 
     def _on_device(self):
         import torch
-        return torch.cuda.device(self.device)
+        return _HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self.device)
 
     def _stream(self):
         import torch
@@ -251,23 +272,21 @@ class PagedCache:
         into their pages of ``layer``. They are of the cache's type or f32
         (rounded to nearest). Rows of other sequences' slots stay as they are;
         a page that two of the new rows' sequences share gets either's."""
-        import torch
-        B, N = self._batch(table, starts, lengths)
+        B, N, seqs = self._batch(table, starts, lengths)
         at = self._layer(layer)
-        ks = self._rows('k', k, (self.dtype, torch.float32), self.heads)
-        vs = self._rows('v', v, (k.dtype,), like=k.shape)
+        k_at, *ks = self._rows('k', k, self._new, self.heads)
+        v_at, *vs = self._rows('v', v, (k.dtype,), like=k.shape)
         M = k.shape[0]
         if M == 0 or B == 0 or N == 0:
             return
         kn = self._kind[self.dtype]
-        launch = kn.pg_append32 if k.dtype == torch.float32 else kn.pg_append16
+        launch = kn.pg_append32 if k.dtype is self._f32 else kn.pg_append16
         grid = -(-M * self.heads * (self.width // 8) // BLOCK)
         if grid >= 1 << 31:
             raise ValueError(f'k: {M} rows are too many for one call')
         with self._on_device():
-            launch(grid, BLOCK, self._stream(), k.data_ptr(), v.data_ptr(), *ks, *vs, self.keys.data_ptr() + at,
-                   self.vals.data_ptr() + at, self.pages, self._shift, table.data_ptr(), N, starts.data_ptr(),
-                   lengths.data_ptr(), B, M, self.heads, self.err.data_ptr())
+            launch(grid, BLOCK, self._stream(), k_at, v_at, *ks, *vs, self._pools[0] + at, self._pools[1] + at, *seqs, B,
+                   M, self.heads, self._err)
 
     def attend(self, q, table, starts, lengths, layer=0, scale=None, out=None, weight=None, weight_out=None, most=None):
         """Attention of the new tokens' queries ``q`` [M, G * heads, width]
@@ -286,24 +305,25 @@ class PagedCache:
 
         ``most``: a bound of the new tokens of a sequence that the program
         knows (1 for a decode step); the work is laid out by it."""
-        import torch
-        B, N = self._batch(table, starts, lengths)
+        B, N, seqs = self._batch(table, starts, lengths)
         at = self._layer(layer)
-        qs = self._rows('q', q, tuple(self._kind))
+        qs = self._rows('q', q, self._queries)
         M, Hq, _ = q.shape
-        if Hq == 0 or Hq % self.heads:
+        G, odd = divmod(Hq, self.heads)
+        if Hq == 0 or odd:
             raise ValueError(f'q: {Hq} heads are not a multiple of the {self.heads} key heads')
-        G = Hq // self.heads
-        scale = 1.0 / math.sqrt(self.width) if scale is None else float(scale)
+        scale = self._scale if scale is None else float(scale)
         if not 0.0 < scale < math.inf:
             raise ValueError(f'scale {scale}: positive and finite')
         if most is not None and most < 1:
             raise ValueError(f'most {most}: at least 1')
         if out is None:
-            out = torch.empty((M, Hq, self.width), dtype=q.dtype, device=self.device)
-            os = (Hq * self.width, self.width)
+            out = self._empty((M, Hq, self.width), dtype=q.dtype, device=self.device)
+            to = out.data_ptr(), Hq * self.width, self.width
         else:
-            os = self._rows('out', out, (q.dtype,), like=q.shape)
+            to = self._rows('out', out, (q.dtype,), like=q.shape)
+            if M > 1 and to[1] == 0 or Hq > 1 and to[2] == 0:
+                raise ValueError(f'out: rows that lie on one another (strides {out.stride()})')
         S = So = 0
         if weight is not None:
             weight_out = weight if weight_out is None else weight_out
@@ -316,16 +336,15 @@ class PagedCache:
         scale2 = scale * 1.4426950408889634
         with self._on_device():
             stream = self._stream()
-            seqs = (self.pages, self._shift, table.data_ptr(), N, starts.data_ptr(), lengths.data_ptr())
             lse = scores = None
             pitch = 0
             # a launch's tiles of rows, as many as there can be, and its parts
-            wide = most * G > FEW_ROWS and q.dtype != torch.float32
+            wide = most * G > FEW_ROWS and q.dtype is not self._f32
             if weight is not None:
-                lse = torch.empty(M * Hq, dtype=torch.float32, device=self.device)
+                lse = self._floats(M * Hq)
                 pitch = -(-N * self.page // 64) * 64
                 if not wide and 0 < M * Hq * pitch <= SCORES_MAX:
-                    scores = torch.empty(M * Hq * pitch, dtype=torch.float32, device=self.device)
+                    scores = self._floats(M * Hq * pitch)
             if M and B:
                 rows, aim = (128, WIDE_TARGET) if wide else (ROWS, TARGET)
                 tiles = self.heads * (M * G // rows + B)
@@ -333,28 +352,29 @@ class PagedCache:
                 blocks = target + tiles + 64
                 if blocks >= 1 << 28 or M * G >= 1 << 30:
                     raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
-                ws = None if target == 0 else torch.empty(blocks * rows * (self.width + 2), dtype=torch.float32,
-                                                          device=self.device)
-                to = (out.data_ptr(), *os, _at(lse))
+                ws = self._floats(blocks * rows * (self.width + 2)) if target else None
                 least = WIDE_PART_STEPS if wide else PART_STEPS
-                args = (_blocks8(blocks), BLOCK, stream, q.data_ptr(), *qs, self.keys.data_ptr() + at,
-                        self.vals.data_ptr() + at, *seqs, B, M, self.heads, G, target, least, most, scale2, *to, _at(ws))
+                args = (_blocks8(blocks), BLOCK, stream, *qs, self._pools[0] + at, self._pools[1] + at, *seqs, B, M,
+                        self.heads, G, target, least, most, scale2, *to, _at(lse), _at(ws))
                 if wide:
-                    kn.pg_wide(*args, self.err.data_ptr())
+                    kn.pg_wide(*args, self._err)
                 else:
-                    kn.pg_attn(*args, _at(scores), pitch, self.err.data_ptr())
+                    kn.pg_attn(*args, _at(scores), pitch, self._err)
                 if target:
                     (kn.pg_wide_join if wide else kn.pg_join)(
-                        tiles * (rows // 16), JOIN_BLOCK, stream, starts.data_ptr(), lengths.data_ptr(), B,
-                        N * self.page, M, self.heads, G, target, least, ws.data_ptr(), *to)
+                        tiles * (rows // 16), JOIN_BLOCK, stream, *seqs[4:], B, N * self.page, M, self.heads, G, target,
+                        least, ws.data_ptr(), *to, _at(lse))
             if weight is not None and B:
-                self._receive(kn, stream, (q.data_ptr(), *qs, self.keys.data_ptr() + at), seqs, (B, M, G), most, wide,
-                              scale2, lse, scores, pitch, (weight.data_ptr(), S, weight_out.data_ptr(), So))
+                self._receive(kn, stream, (*qs, self._pools[0] + at), seqs, (B, M, G), most, wide, scale2, lse, scores,
+                              pitch, (weight.data_ptr(), S, weight_out.data_ptr(), So))
         return out if weight is None else (out, weight_out)
+
+    def _floats(self, n):
+        """A workspace of a call."""
+        return self._empty(n, dtype=self._f32, device=self.device)
 
     def _receive(self, kn, stream, keys, seqs, extents, most, wide, scale2, lse, scores, pitch, to):
         """The weights' pass after ``attend``'s: from the scores it left, or making them again."""
-        import torch
         B, M, G = extents
         bh, So, cap = B * self.heads, to[-1], seqs[3] * self.page
         if scores is not None:
@@ -368,7 +388,7 @@ class PagedCache:
         else:
             blocks = -(-So // 256)
             slices = max(1, min(WEIGH_BLOCKS // (bh * blocks), most * G // 256))
-            part = None if slices == 1 else torch.empty(slices * bh * So, dtype=torch.float32, device=self.device)
+            part = None if slices == 1 else self._floats(slices * bh * So)
             kn.pg_weigh_wide(_blocks8(bh * blocks * slices), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2,
                              lse.data_ptr(), *to, blocks, slices, _at(part))
             if slices > 1:
@@ -376,13 +396,16 @@ class PagedCache:
                             blocks)
 
     def _weights(self, name, w, lead, least):
-        import torch
-        if not (isinstance(w, torch.Tensor) and w.dtype == torch.float32 and w.device == self.device
-                and w.is_contiguous()):
+        try:
+            fits = w.dtype is self._f32 and w.get_device() == self._index and w.is_contiguous()
+            shape = w.shape
+        except AttributeError:
+            fits = False
+        if not fits:
             raise TypeError(f'{name}: need a contiguous float32 tensor on {self.device}')
-        if w.dim() != len(lead) + 1 or tuple(w.shape[:-1]) != lead or w.shape[-1] < least:
-            raise ValueError(f'{name}: shape {tuple(w.shape)}, need {lead} and {least} positions at least')
-        return w.shape[-1]
+        if tuple(shape[:-1]) != lead or shape[-1] < least:
+            raise ValueError(f'{name}: shape {tuple(shape)}, need {lead} and {least} positions at least')
+        return shape[-1]
 
     def evict(self, weight, table, lengths, keep, to, recent=0, weight_out=None):
         """Keep ``keep`` positions of each sequence (all where it has no more):
@@ -397,9 +420,8 @@ class PagedCache:
         Returns (lengths [B], weight_out [layers, B, heads, S'], kept [layers,
         B, heads, keep]): the new lengths, the kept positions' weights (0
         behind them) and which positions they were (-1 behind them)."""
-        import torch
-        B, N = self._batch(table, None, lengths)
-        self._ints('to', to, (B, None))
+        B, N, seqs = self._batch(table, None, lengths)
+        to_at = self._ints('to', to, (B, None))
         No = to.shape[1]
         if keep < 1 or recent < 0:
             raise ValueError(f'keep {keep} of at least 1 position, recent {recent} of at least 0')
@@ -408,12 +430,12 @@ class PagedCache:
         lead = (self.layers, B, self.heads)
         S = self._weights('weight', weight, lead, N * self.page)
         if weight_out is None:
-            weight_out = torch.empty(lead + (No * self.page,), dtype=torch.float32, device=self.device)
+            weight_out = self._empty(lead + (No * self.page,), dtype=self._f32, device=self.device)
         So = self._weights('weight_out', weight_out, lead, No * self.page)
         if B and weight_out.data_ptr() == weight.data_ptr():
             raise ValueError('weight_out: a tensor other than weight')
-        kept = torch.empty(lead + (keep,), dtype=torch.int32, device=self.device)
-        new = torch.empty(B, dtype=torch.int32, device=self.device)
+        kept = self._empty(lead + (keep,), dtype=self._i32, device=self.device)
+        new = self._empty(B, dtype=self._i32, device=self.device)
         if B == 0:
             return new, weight_out, kept
         kn = self._kind[self.dtype]
@@ -422,12 +444,11 @@ class PagedCache:
             raise ValueError(f'{self.layers} layers of {B} sequences are too many for one call')
         with self._on_device():
             stream = self._stream()
-            kn.pg_select(self.layers * B * self.heads, 1024, stream, weight.data_ptr(), S, lengths.data_ptr(),
-                         N * self.page, B, self.heads, keep, recent, kept.data_ptr(), weight_out.data_ptr(), So,
-                         new.data_ptr(), self.err.data_ptr())
-            kn.pg_move(self.layers * B * blocks, BLOCK, stream, self.keys.data_ptr(), self.vals.data_ptr(), self.pages,
-                       self._shift, table.data_ptr(), N, to.data_ptr(), No, kept.data_ptr(), keep, B, self.heads,
-                       blocks, self.err.data_ptr())
+            kn.pg_select(self.layers * B * self.heads, 256 if N * self.page <= SELECT_FEW else 1024, stream, weight.data_ptr(), S, seqs[5], N * self.page, B,
+                         self.heads, keep, recent, kept.data_ptr(), weight_out.data_ptr(), So, new.data_ptr(),
+                         self._err)
+            kn.pg_move(self.layers * B * blocks, BLOCK, stream, *self._pools, *seqs[:4], to_at, No, kept.data_ptr(), keep,
+                       B, self.heads, blocks, self._err)
         return new, weight_out, kept
 
     def check(self):
