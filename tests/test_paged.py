@@ -1,8 +1,6 @@
 """CPU tests of the paged cache's calls (vesta/paged.py): what is refused, and
 that every launch asked for covers what its kernel indexes. The launches are
 recorded, not made."""
-import contextlib
-
 import pytest
 import torch
 
@@ -34,11 +32,8 @@ class _Dry(PagedCache):
         if dtype == 'f16':
             self._kind[torch.float32] = _Recorder(self.log)
 
-    def _on_device(self):
-        return contextlib.nullcontext()
-
-    def _stream(self):
-        return 0
+    def _enter(self):
+        return 0, None
 
 
 def _last(c, *names):
@@ -110,7 +105,7 @@ def test_strides():
     c.append(k, v, table, starts, lengths)
     assert c.log[-1][3][2:6] == (9 * 64, 64, 9 * 64, 64)
     c.attend(q, table, starts, lengths)
-    attn = ('pg_attn', 'pg_wide')
+    attn = ('pg_attn', 'pg_attn8', 'pg_wide')
     assert _last(c, *attn)[1:3] == (9 * 64, 64)
     c.attend(torch.zeros(3, 5, 64, dtype=torch.float16).transpose(0, 1), table, starts, lengths)
     assert _last(c, *attn)[1:3] == (64, 5 * 64)

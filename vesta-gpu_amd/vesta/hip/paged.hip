@@ -273,9 +273,29 @@ __device__ __forceinline__ unsigned pg_wild2(unsigned x) {
   return ((x & (PG_EXP << 16 | PG_EXP)) + (0x80008000u - (PG_EXP << 16 | PG_EXP))) & 0x80008000u;
 }
 
+// Eight values with 0 for those that are not finite.
+__device__ __forceinline__ vh_u32x4 pg_tame(vh_u32x4 v) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned w = pg_wild2(v[j]);
+    v[j] &= ~((w & 0x8000u ? 0xffffu : 0u) | (w >> 31 ? 0xffff0000u : 0u));
+  }
+  return v;
+}
+// What pg_tame took out of row s of a head's values (rows of `rowlen`, the
+// table's and the pool's as the kernels have them), added to a row's outputs
+// that see it: dim `dim` of it.
+__device__ __forceinline__ float pg_taken(const unsigned short* __restrict__ vh, size_t rowlen,
+                                          const int* __restrict__ tb, int pages, int shift, int s, int dim) {
+  const int page = tb[s >> shift];
+  const size_t at = (((size_t)((unsigned)page < (unsigned)pages ? page : 0)) << shift) + (s & ((1 << shift) - 1));
+  const unsigned short v = vh[at * rowlen + dim];
+  return pg_wild(v) ? pg_to_f(v) : 0.0f;
+}
+
 // A block makes 16 rows of one (sequence, key head): row x stands for new
-// token x / G, query head G h + x % G. Its four waves take every fourth step
-// of PG_STEP positions each and combine at the end. Scores are K Q^T, outputs
+// token x / G, query head G h + x % G. Its W waves take every W-th step of
+// PG_STEP positions each and combine at the end. Scores are K Q^T, outputs
 // V^T P^T, so that a lane holds values of one row (lane % 16) in both, and the
 // weights feed the second product from the registers the first left them in:
 // the instruction's fold position 8 q + e stands for position 4 q + e (e < 4)
@@ -296,13 +316,18 @@ __device__ __forceinline__ unsigned pg_wild2(unsigned x) {
 // head, tile), `each` such that there are about `target` parts in all (0: one
 // part a tile). So parts are of one size whatever the lengths, and a block of
 // the grid is a part: the grid holds target + H (M G / ROWS + B) + 64, every
-// number of parts that can come out, and is dealt to the XCDs in contiguous
-// runs. A sequence's parts follow each other, in each its heads, whose rows lie
+// number of parts that can come out (a multiple of 8 runs), and is dealt to the
+// eight XCDs in runs of `run`, which share an L2. A sequence's parts follow each other, in each its heads, whose rows lie
 // side by side, in each its tiles, which read the same rows.
 struct PgWork {
   PgSeq sq;
   int b, h, R, x0, tile, tiles, part, each, at;   // x0: the tile's first row of R; at: the part's place in ws
 };
+__device__ __forceinline__ int pg_deal(int block, int run) {       // the block's place: blocks go to XCD block % 8
+  const int j = block >> 3;
+  return (j / run * 8 + (block & 7)) * run + j % run;
+}
+#define PG_RUN_LONG 64
 template <int ROWS, int STEP>
 __device__ __forceinline__ void pg_count(const PgSeq& s, int G, int& tiles, int& steps) {
   tiles = (s.count * G + ROWS - 1) / ROWS;
@@ -334,7 +359,7 @@ __device__ __forceinline__ int pg_each(const int* __restrict__ starts, const int
 // Block `at`'s part, where `joined` one of all (sequence, head, tile)s of a
 // grid of those instead (its parts' first place in ws is then `at`).
 template <int ROWS, int STEP>
-__device__ __forceinline__ bool pg_work(PgWork& o, int block, bool joined, const int* __restrict__ starts,
+__device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool joined, const int* __restrict__ starts,
                                         const int* __restrict__ lengths, int B, int M, int cap, int H, int G,
                                         int target, int least, unsigned* __restrict__ err, int most) {
   const int lane = threadIdx.x & 63;
@@ -364,9 +389,8 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, bool joined, const
     }
     if (bad) pg_raise(err, bad);
   }
-  const int per = (total + 7) / 8;
-  const int at = joined ? block : (block & 7) * per + (block >> 3);
-  if (at >= total || (!joined && (block >> 3) >= per)) return false;
+  const int at = joined ? block : pg_deal(block, run);
+  if (at >= total) return false;
   int before = 0, places = 0;                                      // in the chunks of 64 sequences already passed
   for (int base = 0;; base += 64) {
     if (base) {
@@ -382,9 +406,11 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, bool joined, const
       o.sq.len = __builtin_amdgcn_readlane(s.len, l);
       o.tiles = __builtin_amdgcn_readlane(tiles, l);
       const int rest = at - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
-      o.tile = o.tiles - 1 - rest % o.tiles;                       // the longest first
-      o.h = rest / o.tiles % H;
-      o.part = rest / o.tiles / H;
+      o.part = rest / (o.tiles * H);
+      const bool by_head = run >= PG_RUN_LONG || o.tiles <= 8;
+      const int ht = rest % (o.tiles * H);
+      o.h = by_head ? ht / o.tiles : ht % H;
+      o.tile = o.tiles - 1 - (by_head ? ht % o.tiles : ht / H);    // the longest first
       o.at = at;
       if (joined) {
         const int p = pg_scan(n * parts, lane);
@@ -416,20 +442,21 @@ __device__ __forceinline__ void pg_store4(pg_q* p, const float* v) {
 #endif
 }
 
-extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
+template <int W>
+__device__ __forceinline__ void pg_attn_body(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,
     const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
     const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
-    int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
+    int run, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
     float* __restrict__ ws, float* __restrict__ sc, long pitch, unsigned* __restrict__ err) {
   constexpr int KS = PG_E / 32, NG = PG_STEP / 16, NV = PG_STEP * PG_E / 512, DT = PG_E / 16;
   constexpr int VL = PG_E / 8, VR = 64 / VL;                       // lanes of a value row; rows of a wave's load
-  __shared__ __attribute__((aligned(16))) unsigned short lv[4][PG_STEP * PG_VROW];
-  __shared__ float om[4][2][16];
+  __shared__ __attribute__((aligned(16))) unsigned short lv[W][PG_STEP * PG_VROW];
+  __shared__ float om[W][2][16];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, q = lane >> 4;
   PgWork wk;
-  if (!pg_work<16, PG_STEP>(wk, blockIdx.x, false, starts, lengths, B, M, N << shift, H, G, target, least, err, most)) return;
+  if (!pg_work<16, PG_STEP>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, err, most)) return;
   int last, steps, parts;
   pg_span<16, PG_STEP>(wk, G, last, steps, parts);
   if (wk.part >= parts) return;
@@ -473,9 +500,9 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
   pg_query(qf, qp, q, scale2);
   if (t0 + wave < t1) {
     load(t0 + wave, page);
-    page = look(min(t0 + wave + 4, t1 - 1));
+    page = look(min(t0 + wave + W, t1 - 1));
   }
-  for (int t = t0 + wave; t < t1; t += 4) {
+  for (int t = t0 + wave; t < t1; t += W) {
     const int p0 = t * PG_STEP;
     float s[NG][4];
 #pragma unroll
@@ -495,14 +522,18 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
 #pragma unroll
       for (int n = 0; n < NV; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
       wild = __any(any != 0u);
+      if (wild) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) vr[n] = pg_tame(vr[n]);
+      }
     }
     pg_wave_sync();                                                // the step before is read
 #pragma unroll
     for (int n = 0; n < NV; ++n) *(vh_u32x4*)(V + (n * VR + lane / VL) * PG_VROW + lane % VL * 8) = vr[n];
     pg_wave_sync();
-    if (t + 4 < t1) {
-      load(t + 4, page);
-      page = look(min(t + 8, t1 - 1));
+    if (t + W < t1) {
+      load(t + W, page);
+      page = look(min(t + 2 * W, t1 - 1));
     }
     if (seen) {
 #pragma unroll
@@ -535,6 +566,8 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
       pg_split(w, pf[k]);
     }
     sum = fmaf(sum, c, ts);
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds4;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       vh_f32x4 th = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -543,18 +576,10 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
 #endif
 #pragma unroll
       for (int k = 0; k < NG / 2; ++k) {
-        typedef short s4 __attribute__((ext_vector_type(4)));
-        typedef short s8 __attribute__((ext_vector_type(8)));
-        typedef __attribute__((address_space(3))) s4 lds4;
         unsigned short* vb = V + (32 * k + 4 * q + r / 4) * PG_VROW + 16 * d + 4 * (r & 3);
         const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vb);
         const s4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vb + 16 * PG_VROW));
-        s8 f = __builtin_shufflevector(a, e, 0, 1, 2, 3, 4, 5, 6, 7);
-        if (wild) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = pg_wild((unsigned short)f[j]) ? 0 : f[j];
-        }
-        const vh_u32x4 vf = __builtin_bit_cast(vh_u32x4, f);
+        const vh_u32x4 vf = __builtin_bit_cast(vh_u32x4, __builtin_shufflevector(a, e, 0, 1, 2, 3, 4, 5, 6, 7));
         th = pg_mfma(vf, pf[k][0], th);
 #if PG_KIND == PG_F32
         tw = pg_mfma(vf, pf[k][1], tw);
@@ -571,13 +596,14 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
       }
     }
     if (wild) {                                                    // ... and go to the rows that see them
+#pragma nounroll
       for (int s = p0; s <= min(p0 + PG_STEP - 1, last); ++s)
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const unsigned short v = V[(s - p0) * PG_VROW + 16 * d + 4 * q + j];
-            if (pg_wild(v) && s <= lim) o[d][j] += pg_to_f(v);
+            const float v = pg_taken(vp + h * PG_E, rowlen, tb, pages, shift, s, 16 * d + 4 * q + j);
+            o[d][j] += s <= lim ? v : 0.0f;
           }
     }
   }
@@ -586,7 +612,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
   // each wave's maximum, sum and output, rescaled to the common maximum and
   // added in wave order; wave w then makes every fourth dim tile
   float* ow = (float*)lv;                                          // [wave][dim tile][j][lane]
-  static_assert(sizeof(lv) >= 4 * DT * 4 * 64 * 4, "the value tiles hold the waves' outputs");
+  static_assert(sizeof(lv) >= W * DT * 4 * 64 * 4, "the value tiles hold the waves' outputs");
   __syncthreads();
   if (q == 0) {
     om[wave][0][r] = m2;
@@ -599,11 +625,11 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
   __syncthreads();
   float m = om[0][0][r];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) m = fmaxf(m, om[w][0][r]);
+  for (int w = 1; w < W; ++w) m = fmaxf(m, om[w][0][r]);
   sum = 0.0f;
-  float f[4];
+  float f[W];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < W; ++w) {
     f[w] = om[w][0][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(om[w][0][r] - m);   // no score: 0
     sum = fmaf(om[w][1][r], f[w], sum);
   }
@@ -612,10 +638,10 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
   pg_q* op = out + (sq.first + tok) * orow + head * ohead;
   float* wp = ws + (size_t)wk.at * PG_WS(16);
 #pragma unroll
-  for (int d = wave; d < DT; d += 4) {
+  for (int d = wave; d < DT; d += W) {
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < W; ++w)
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = fmaf(ow[((w * DT + d) * 4 + j) * 64 + lane], f[w], v[j]);
     if (whole) {
@@ -637,6 +663,19 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_attn(
     }
   }
 }
+
+#define PG_ATTN(name, waves) \
+  extern "C" __global__ __launch_bounds__(64 * waves, 2) void name( \
+      const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, \
+      const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N, \
+      const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least, \
+      int run, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse, \
+      float* __restrict__ ws, float* __restrict__ sc, long pitch, unsigned* __restrict__ err) { \
+    pg_attn_body<waves>(Q, qrow, qhead, kp, vp, pages, shift, table, N, starts, lengths, B, M, H, \
+                        G, target, least, run, most, scale2, out, orow, ohead, lse, ws, sc, pitch, err); \
+  }
+PG_ATTN(pg_attn, 4)
+PG_ATTN(pg_attn8, 8)
 
 // Attention of many rows of 16-bit queries. A block makes 128 rows of one
 // (sequence, key head), 32 to a wave, over steps of 64 positions that its four
@@ -666,7 +705,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,
     const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
     const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
-    int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
+    int run, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
     float* __restrict__ ws, unsigned* __restrict__ err) {
   constexpr int KS = PG_E / 16, DT = PG_E / 32, CH = PG_E / 8, NL = 64 * CH / 256;   // k-steps, dim tiles, 16-byte
   constexpr int RS = 256 / CH;                                     // pieces of a row; a thread's pieces and rows apart
@@ -676,7 +715,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
   PgWork wk;
-  if (!pg_work<128, 64>(wk, blockIdx.x, false, starts, lengths, B, M, N << shift, H, G, target, least, err, most)) return;
+  if (!pg_work<128, 64>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, err, most)) return;
   int last, steps, parts;
   pg_span<128, 64>(wk, G, last, steps, parts);
   if (wk.part >= parts) return;
@@ -718,28 +757,32 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     }
   };
   // Key rows are 16 bytes past a multiple of all banks apart, so that a column
-  // of their pieces falls on all of them. Values past the last position are 0;
-  // whether a step that some row sees in part holds one that is not finite is
-  // noted.
+  // of their pieces falls on all of them. Values past the last position are 0,
+  // and where some row sees a step in part so are those that are not finite
+  // (0 * inf); that there are such is noted.
   auto put = [&](int t) {
     const int buf = t & 1;
-    unsigned any = 0u;
     if (64 * t + 63 > last) {
 #pragma unroll
       for (int n = 0; n < NL; ++n)
         if (64 * t + r8 + RS * n > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
       asm volatile("" ::: "memory");                               // kept a branch
     }
+    if (64 * t + 63 > bfirst) {
+      unsigned any = 0u;
+#pragma unroll
+      for (int n = 0; n < NL; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
+      if (any) {
+        lwild[buf] = t + 1;
+#pragma unroll
+        for (int n = 0; n < NL; ++n) vr[n] = pg_tame(vr[n]);
+      }
+    }
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
       const int row = r8 + RS * n;
       lk[buf][row * (CH + 1) + c8] = kr[n];
       *(vh_u32x4*)(lv[buf] + row * PG_WROW + 8 * c8) = vr[n];
-    }
-    if (64 * t + 63 > bfirst) {
-#pragma unroll
-      for (int n = 0; n < NL; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
-      if (any) lwild[buf] = t + 1;
     }
   };
   pg_f16v o[DT];
@@ -771,16 +814,22 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     }
     const int p0 = 64 * t, buf = t & 1;
     if (x0 >= R || p0 > wlast) continue;
+    // the matrix cores' share of a step goes before the other block's softmax
+    // (4096 tokens after 27001, width 128: 2147 -> 2050 us; width 64, where the
+    // softmax is most of a step, 27 -> 30)
+    if (PG_E == 128) __builtin_amdgcn_s_setprio(1);
     const vh_u32x4* K = lk[buf];
     const unsigned short* V = lv[buf];
     pg_f16v s[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) s[i] = pg_mfma32(K[(32 * i + r) * (CH + 1) + 2 * k + g], qf[k], s[i]);
-    }
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i] = pg_mfma32(K[(32 * i + r) * (CH + 1) + 2 * k + g], qf[k], s[i]);
+    if (PG_E == 128) __builtin_amdgcn_s_setprio(0);
     const bool seen = p0 + 63 > wfirst;                            // not the whole step by every row
     if (seen) {
 #pragma unroll
@@ -829,35 +878,34 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
         pf[i][k] = pg_pack8(pg_f8{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]});
       }
     sum += (ts[0] + ts[1]) + (ts[2] + ts[3]);
-    const bool wild = lwild[buf] == t + 1 && seen;                 // as in pg_attn
+    if (PG_E == 128) __builtin_amdgcn_s_setprio(1);
+    const bool wild = lwild[buf] == t + 1;                         // added back below
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef short s8 __attribute__((ext_vector_type(8)));
     typedef __attribute__((address_space(3))) s4 lds4;
+    auto value = [&](int i, int k, int d) {
+      const unsigned short* vb = V + (32 * i + 16 * k + 4 * g + ((lane & 15) >> 2)) * PG_WROW + 32 * d
+                                 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vb);
+      const s4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vb + 8 * PG_WROW));
+      return __builtin_shufflevector(a, e, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const unsigned short* vb = V + (32 * i + 16 * k + 4 * g + ((lane & 15) >> 2)) * PG_WROW + 32 * d
-                                     + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-          const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vb);
-          const s4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vb + 8 * PG_WROW));
-          s8 f = __builtin_shufflevector(a, e, 0, 1, 2, 3, 4, 5, 6, 7);
-          if (wild) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = pg_wild((unsigned short)f[j]) ? 0 : f[j];
-          }
-          o[d] = pg_mfma32(__builtin_bit_cast(vh_u32x4, f), pf[i][k], o[d]);
-        }
+        for (int d = 0; d < DT; ++d) o[d] = pg_mfma32(__builtin_bit_cast(vh_u32x4, value(i, k, d)), pf[i][k], o[d]);
+    if (PG_E == 128) __builtin_amdgcn_s_setprio(0);
     if (wild) {
+#pragma nounroll
       for (int s = p0; s <= min(p0 + 63, last); ++s)
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const unsigned short v = V[(s - p0) * PG_WROW + 32 * d + 8 * (j >> 2) + 4 * g + (j & 3)];
-            if (pg_wild(v) && s <= lim) o[d][j] += pg_to_f(v);
+            const float v = pg_taken(vp + h * PG_E, rowlen, tb, pages, shift, s, 32 * d + 8 * (j >> 2) + 4 * g + (j & 3));
+            o[d][j] += s <= lim ? v : 0.0f;
           }
     }
   }
@@ -894,7 +942,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 // (128 parts of four rows, one group a row: 60 us; dealt out: 4).
 template <int ROWS, int STEP>
 __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, const int* __restrict__ lengths, int B,
-                                             int cap, int M, int H, int G, int target, int least,
+                                             int cap, int M, int H, int G, int target, int least, int run,
                                              const float* __restrict__ ws, pg_q* __restrict__ out, long orow,
                                              long ohead, float* __restrict__ lse) {
   constexpr int LR = PG_E / 4, NGR = 512 / LR;
@@ -902,7 +950,7 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
   __shared__ vh_f32x4 jv[512];
   const int tid = threadIdx.x, c = tid % LR, grp = tid / LR, y0 = blockIdx.x % (ROWS / 16) * 16;
   PgWork wk;                                                       // grid: H (M G / ROWS + B) tiles or more
-  if (!pg_work<ROWS, STEP>(wk, blockIdx.x / (ROWS / 16), true, starts, lengths, B, M, cap, H, G, target, least, nullptr,
+  if (!pg_work<ROWS, STEP>(wk, blockIdx.x / (ROWS / 16), run, true, starts, lengths, B, M, cap, H, G, target, least, nullptr,
                            0))
     return;
   int last, steps, parts;
@@ -981,9 +1029,9 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
 #define PG_JOIN(name, rows, step)                                                                                  \
   extern "C" __global__ __launch_bounds__(512) void name(                                                          \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int cap, int M, int H, int G,        \
-      int target, int least, const float* __restrict__ ws, pg_q* __restrict__ out, long orow, long ohead,          \
+      int target, int least, int run, const float* __restrict__ ws, pg_q* __restrict__ out, long orow, long ohead, \
       float* __restrict__ lse) {                                                                                   \
-    pg_join_body<rows, step>(starts, lengths, B, cap, M, H, G, target, least, ws, out, orow, ohead, lse);          \
+    pg_join_body<rows, step>(starts, lengths, B, cap, M, H, G, target, least, run, ws, out, orow, ohead, lse);        \
   }
 PG_JOIN(pg_join, 16, PG_STEP)
 #if PG_KIND != PG_F32
@@ -1002,12 +1050,12 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
     const int* __restrict__ table, int N, const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
     int H, int G, float scale2, const float* __restrict__ lse, const float* old, int S, float* out, int So,
-    int blocks) {
+    int blocks, int run) {
   constexpr int KS = PG_E / 32;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, q = lane >> 4;
-  const int T = B * H * blocks, per = (T + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || id >= T) return;
+  const int id = pg_deal(blockIdx.x, run);
+  if (id >= B * H * blocks) return;
   const int h = id / blocks % H, b = id / blocks / H, p0 = id % blocks * 128 + 32 * wave;
   if (p0 >= So) return;
   const PgSeq sq = pg_seq(starts, lengths, b, M, N << shift);
@@ -1095,14 +1143,14 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
     const int* __restrict__ table, int N, const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
     int H, int G, float scale2, const float* __restrict__ lse, const float* old, int S,
-    float* out, int So, int blocks, int slices, float* __restrict__ part) {
+    float* out, int So, int blocks, int run, int slices, float* __restrict__ part) {
   constexpr int KS = PG_E / 16, CH = PG_E / 8, NL = 32 * CH / 256, RS = 256 / CH;
   __shared__ __attribute__((aligned(16))) vh_u32x4 lq[2][32 * CH];
   __shared__ float lz[2][32];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
-  const int T = B * H * blocks * slices, per = (T + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || id >= T) return;
+  const int id = pg_deal(blockIdx.x, run);
+  if (id >= B * H * blocks * slices) return;
   const int slice = id % slices, bh = id / slices / blocks, b = bh / H, h = bh % H;
   const int b0 = id / slices % blocks * 256, p0 = b0 + 64 * wave;
   const PgSeq sq = pg_seq(starts, lengths, b, M, N << shift);

@@ -36,7 +36,6 @@ programs whose rows come and go.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 import struct
@@ -55,8 +54,10 @@ ROWS = 16                              # query rows of a pg_attn block
 FEW_ROWS = 32                          # rows of a sequence (its most) from which pg_wide makes them
 WIDE_TARGET, WIDE_PART_STEPS = 512, 8
 JOIN_BLOCK = 512
+EIGHT_WAVES = 256
+RUN, RUN_LONG = 8, 64
 SELECT_FEW = 4096
-WEIGH_BLOCKS = 1024
+WEIGH_BLOCKS = 1536
 SCORES_MAX = 1 << 27                   # scores (512 MB) that a call may keep for its weights' pass
 SPLIT, WIDE_SPLIT = 2048, 1024
 TARGET = 1536                          # parts that the positions of all row tiles are cut into, about, ...
@@ -70,13 +71,14 @@ _SEQS = 'iipipp'                       # pages, shift, table, its columns, start
 SIGNATURES = {
     'pg_append16': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
     'pg_append32': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
-    'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiif' + 'pllpp' + 'plp',
-    'pg_join': 'ppiiiiiiippllp',
-    'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiif' + 'pllppp',
-    'pg_wide_join': 'ppiiiiiiippllp',
-    'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipii',
+    'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllpp' + 'plp',
+    'pg_attn8': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllpp' + 'plp',
+    'pg_join': 'ppiiiiiiiippllp',
+    'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllppp',
+    'pg_wide_join': 'ppiiiiiiiippllp',
+    'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiii',
     'pg_given': 'plppiiiippipii',
-    'pg_weigh_wide': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiiip',
+    'pg_weigh_wide': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiiiip',
     'pg_total': 'pippiiiipipii',
     'pg_select': 'pipiiiiippipp',
     'pg_move': 'ppiipipipiiiip',
@@ -134,7 +136,6 @@ class _Kernels:
             unload(mod)
 
 
-_HERE = contextlib.nullcontext()       # the cache's device is the current one
 _ANY2 = (None, None)
 _loaded = {}
 _loaded_lock = threading.Lock()
@@ -153,9 +154,9 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _blocks8(n):
-    """Blocks of a grid whose kernel deals n tasks to the device's eight XCDs."""
-    return 8 * -(-n // 8)
+def _dealt(n, run):
+    """Blocks of a grid whose kernel deals n tasks to the device's eight XCDs in runs."""
+    return 8 * run * -(-n // (8 * run))
 
 
 class PagedCache:
@@ -174,6 +175,9 @@ class PagedCache:
         if device.type != 'cuda':
             raise ValueError(f'device {device}: a CUDA device')
         self._allocate(torch.device('cuda', torch.cuda.current_device() if device.index is None else device.index))
+        # torch.cuda's own, without the stream object around the handle
+        self._current = torch._C._cuda_getDevice
+        self._raw_stream = torch._C._cuda_getCurrentRawStream
         self._kind = {self.dtype: _kernels(self.device.index, width, dtype)}
         if dtype == 'f16':
             self._kind[torch.float32] = _kernels(self.device.index, width, 'f32')
@@ -258,13 +262,20 @@ class PagedCache:
             raise ValueError(f'layer {layer} of {self.layers}')
         return layer * self._layer_bytes
 
-    def _on_device(self):
+    def _enter(self):
+        """The stream to launch on, with the cache's device the current one; and the device to go back to, or None."""
+        if self._current() == self._index:
+            return self._raw_stream(self._index), None
         import torch
-        return _HERE if torch.cuda.current_device() == self._index else torch.cuda.device(self.device)
+        back = torch.cuda.current_device()
+        torch.cuda.set_device(self._index)
+        return self._raw_stream(self._index), back
 
-    def _stream(self):
-        import torch
-        return torch.cuda.current_stream(self.device).cuda_stream
+    @staticmethod
+    def _leave(back):
+        if back is not None:
+            import torch
+            torch.cuda.set_device(back)
 
     # ------------------------------------------------------------ operators
     def append(self, k, v, table, starts, lengths, layer=0):
@@ -284,9 +295,12 @@ class PagedCache:
         grid = -(-M * self.heads * (self.width // 8) // BLOCK)
         if grid >= 1 << 31:
             raise ValueError(f'k: {M} rows are too many for one call')
-        with self._on_device():
-            launch(grid, BLOCK, self._stream(), k_at, v_at, *ks, *vs, self._pools[0] + at, self._pools[1] + at, *seqs, B,
+        stream, back = self._enter()
+        try:
+            launch(grid, BLOCK, stream, k_at, v_at, *ks, *vs, self._pools[0] + at, self._pools[1] + at, *seqs, B,
                    M, self.heads, self._err)
+        finally:
+            self._leave(back)
 
     def attend(self, q, table, starts, lengths, layer=0, scale=None, out=None, weight=None, weight_out=None, most=None):
         """Attention of the new tokens' queries ``q`` [M, G * heads, width]
@@ -334,8 +348,8 @@ class PagedCache:
         most = M if most is None else min(most, M)
         kn = self._kind[q.dtype]
         scale2 = scale * 1.4426950408889634
-        with self._on_device():
-            stream = self._stream()
+        stream, back = self._enter()
+        try:
             lse = scores = None
             pitch = 0
             # a launch's tiles of rows, as many as there can be, and its parts
@@ -354,19 +368,23 @@ class PagedCache:
                     raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
                 ws = self._floats(blocks * rows * (self.width + 2)) if target else None
                 least = WIDE_PART_STEPS if wide else PART_STEPS
-                args = (_blocks8(blocks), BLOCK, stream, *qs, self._pools[0] + at, self._pools[1] + at, *seqs, B, M,
-                        self.heads, G, target, least, most, scale2, *to, _at(lse), _at(ws))
+                run = RUN if not wide or M * G < 128 * RUN_LONG * B else M * G // (128 * B)
+                block, attn = (BLOCK, kn.pg_attn) if wide or target or tiles > EIGHT_WAVES else (2 * BLOCK, kn.pg_attn8)
+                args = (_dealt(blocks, run), block, stream, *qs, self._pools[0] + at, self._pools[1] + at, *seqs, B, M,
+                        self.heads, G, target, least, run, most, scale2, *to, _at(lse), _at(ws))
                 if wide:
                     kn.pg_wide(*args, self._err)
                 else:
-                    kn.pg_attn(*args, _at(scores), pitch, self._err)
+                    attn(*args, _at(scores), pitch, self._err)
                 if target:
                     (kn.pg_wide_join if wide else kn.pg_join)(
                         tiles * (rows // 16), JOIN_BLOCK, stream, *seqs[4:], B, N * self.page, M, self.heads, G, target,
-                        least, ws.data_ptr(), *to, _at(lse))
+                        least, run, ws.data_ptr(), *to, _at(lse))
             if weight is not None and B:
                 self._receive(kn, stream, (*qs, self._pools[0] + at), seqs, (B, M, G), most, wide, scale2, lse, scores,
                               pitch, (weight.data_ptr(), S, weight_out.data_ptr(), So))
+        finally:
+            self._leave(back)
         return out if weight is None else (out, weight_out)
 
     def _floats(self, n):
@@ -383,14 +401,14 @@ class PagedCache:
                         lse.data_ptr(), *to, blocks)
         elif not wide:
             blocks = -(-So // WEIGH)
-            kn.pg_weigh(_blocks8(bh * blocks), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2, lse.data_ptr(),
-                        *to, blocks)
+            kn.pg_weigh(_dealt(bh * blocks, RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2, lse.data_ptr(),
+                        *to, blocks, RUN)
         else:
             blocks = -(-So // 256)
             slices = max(1, min(WEIGH_BLOCKS // (bh * blocks), most * G // 256))
             part = None if slices == 1 else self._floats(slices * bh * So)
-            kn.pg_weigh_wide(_blocks8(bh * blocks * slices), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2,
-                             lse.data_ptr(), *to, blocks, slices, _at(part))
+            kn.pg_weigh_wide(_dealt(bh * blocks * slices, RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2,
+                             lse.data_ptr(), *to, blocks, RUN, slices, _at(part))
             if slices > 1:
                 kn.pg_total(bh * blocks, BLOCK, stream, part.data_ptr(), slices, *seqs[4:], cap, B, M, self.heads, *to,
                             blocks)
@@ -442,13 +460,15 @@ class PagedCache:
         blocks = -(-keep * self.heads * (self.width // 8) // BLOCK)
         if self.layers * B * max(blocks, self.heads) >= 1 << 31:
             raise ValueError(f'{self.layers} layers of {B} sequences are too many for one call')
-        with self._on_device():
-            stream = self._stream()
+        stream, back = self._enter()
+        try:
             kn.pg_select(self.layers * B * self.heads, 256 if N * self.page <= SELECT_FEW else 1024, stream, weight.data_ptr(), S, seqs[5], N * self.page, B,
                          self.heads, keep, recent, kept.data_ptr(), weight_out.data_ptr(), So, new.data_ptr(),
                          self._err)
             kn.pg_move(self.layers * B * blocks, BLOCK, stream, *self._pools, *seqs[:4], to_at, No, kept.data_ptr(), keep,
                        B, self.heads, blocks, self._err)
+        finally:
+            self._leave(back)
         return new, weight_out, kept
 
     def check(self):
