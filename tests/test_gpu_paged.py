@@ -533,3 +533,65 @@ def test_serving_run():
             assert (out[i0:i0 + c].double() - want).abs().max().item() < 4e-4 if c else True
             i0 += c
     cache.check()
+
+
+@pytest.mark.parametrize('dtype,query', KINDS)
+@pytest.mark.parametrize('width', (64, 128))
+def test_every_variant(monkeypatch, dtype, query, width):
+    """The same batch through every kernel that a rule may pick: four or eight waves, positions dealt to parts or not,
+    blocks of 16 or 128 rows, weights from kept scores or made again, in slices of the rows or not."""
+    from vesta import paged
+    b = Batch([1, 40, 1, 3], [700, 333, 2500, 3], 2, 2, width, 16, dtype, query)
+    want, bound, got, gerr = b.want()
+    base = dict(EIGHT_WAVES=0, SPLIT={64: 1 << 30, 128: 1 << 30}, WIDE_SPLIT=1 << 30, FEW_ROWS=1 << 20)
+    parts = dict(SPLIT={64: 0, 128: 0}, WIDE_SPLIT=0)
+    for kw in ({}, dict(EIGHT_WAVES=1 << 20), parts, {**parts, 'TARGET': 16, 'PART_STEPS': 1}, dict(SCORES_MAX=0),
+               dict(FEW_ROWS=0), dict(FEW_ROWS=0, **parts), dict(FEW_ROWS=0, WEIGH_BLOCKS=1),
+               dict(FEW_ROWS=0, WIDE_TARGET=1 << 12, WIDE_PART_STEPS=1, WEIGH_BLOCKS=1 << 20, **parts),
+               dict(RUN=1), dict(RUN=64, FEW_ROWS=0), dict(RUN_LONG=0, FEW_ROWS=0)):
+        for name, value in {**base, **kw}.items():
+            monkeypatch.setattr(paged, name, value)
+        out, w = b.attend(weight=torch.zeros_like(got, dtype=torch.float32))
+        _close(out, want, bound)
+        _close(w, got, gerr)
+        _close(b.attend(), want, bound)
+        monkeypatch.undo()
+    b.cache.check()
+
+
+def test_many_sequences():
+    """More sequences than a wave has lanes, most of them without new tokens."""
+    n = 150
+    counts = [1 if i % 3 == 0 else 0 for i in range(n)]
+    counts[149], counts[64] = 40, 5
+    lengths = [3 * i + c for i, c in enumerate(counts)]
+    b = Batch(counts, lengths, 1, 1, 64, 16)
+    want, bound, got, gerr = b.want()
+    for most in (None, 40):
+        out, w = b.attend(most=most, weight=torch.zeros_like(got, dtype=torch.float32))
+        _close(out, want, bound)
+        _close(w, got, gerr)
+    counts = [1] * n
+    b = Batch(counts, [40 * i + 1 for i in range(n)], 1, 2, 64, 16)
+    want, bound, got, gerr = b.want()
+    _close(b.attend(most=1), want, bound)
+    b.cache.check()
+
+
+@pytest.mark.parametrize('n', (9000, 40000))
+def test_evict_long(n):
+    """More positions than a block holds in registers."""
+    b = Batch([0, 0], [n, 300], 1, 1, 64, 64, to_rows=n // 2)
+    w = torch.randn(1, 2, 1, b.table.shape[1] * 64, generator=b.gen, device='cuda').exp_()
+    w[0, 0, 0, 17::5] = 0.5
+    w[0, 0, 0, 16::3] = 0.0
+    for keep, recent in ((n // 2, 100), (n // 2 - 5, 0), (301, 7)):
+        new, wo, kept = b.cache.evict(w, b.table, b.lengths, keep, b.to, recent=recent)
+        for i in range(2):
+            want = _evicted(w[0, i, 0].cpu(), b.lens[i], keep, recent)
+            assert int(new[i]) == len(want) and kept[0, i, 0, :len(want)].tolist() == want
+            src, dst = torch.tensor(want, device='cuda'), torch.arange(len(want), device='cuda')
+            assert torch.equal(wo[0, i, 0, :len(want)], w[0, i, 0][src])
+            assert torch.equal(b.cache.keys[0, b.to[i].long()[dst // 64], dst % 64],
+                               b.cache.keys[0, b.table[i].long()[src // 64], src % 64])
+    b.cache.check()

@@ -134,7 +134,7 @@ class VestaGPT2:
                                              outputs=('logit', 'next'),
                                              feedback={'x': 'next', 't': 1} if feedback else None, grid=grid))
         self._R, self._bps, self._timing = R, blocks_per_sm, timing
-        self.low, self.k, self._pf = None, None, None
+        self.low, self.k, self._pf, self._paged = None, None, None, None
         self._variants = {}
         self._know_pos(0)
         self.engine, self.why_layered = 'persistent', None
@@ -314,6 +314,51 @@ class VestaGPT2:
         self.x.copy_(ins[0])
         self._prefill_kernel().launch(P, tokens, ins)
         self._take_outputs()
+
+    def extend(self, cache, tokens, positions, table, starts, lengths, weight=None, most=None):
+        """New tokens of sequences of different lengths whose key and value
+        rows lie in ``cache``, a ``vesta.paged.PagedCache`` of this model's
+        layers and heads (f16), instead of this object's own: ``tokens`` and
+        ``positions`` (int32 device tensors [M]; which learned position each
+        has, its count in the conversation whatever has been evicted) are the
+        rows of the batch that ``table``, ``starts`` and ``lengths`` describe
+        (``vesta.paged``). Chunks of prompts and single tokens may be mixed.
+        Returns (logits [B, vocabulary], next [B]) of each sequence's last new
+        token (of no meaning for a sequence without one), which the next call
+        overwrites. ``weight`` (f32 [layers, B, heads, S]) counts the
+        attention that each position receives, in place, for
+        ``cache.evict``; ``most`` bounds the new tokens of a sequence (1 for a
+        decode step).
+
+        Nothing is read back, so a call can be captured in a HIP graph.
+        ``check()`` and ``cache.check()`` report what went wrong."""
+        import torch
+        from .paged import PagedCache, PagedPass
+        from .prefill import Prefill, supported
+        if not isinstance(cache, PagedCache):
+            raise TypeError('cache: need a vesta.paged.PagedCache')
+        want = (self.L, self.H, self.E, self.W['wte'].dtype)
+        have = (cache.layers, cache.heads, cache.width, cache.dtype)
+        if have != want:
+            raise ValueError(f'cache of (layers, heads, width, type) {have}, the model has {want}')
+        if not supported(self.D, self.H, self.W['fcw'].shape[2]):
+            raise ValueError('extend needs 64-wide heads and widths that are multiples of 64')
+        for name, t in (('tokens', tokens), ('positions', positions)):
+            if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == cache.device
+                    and t.is_contiguous()):
+                raise TypeError(f'{name}: need a contiguous int32 tensor on {cache.device}')
+        if tokens.dim() != 1 or tokens.shape[0] < 1 or positions.shape != tokens.shape:
+            raise ValueError(f'tokens {tuple(tokens.shape)}, positions {tuple(positions.shape)}: need two of [M], M >= 1')
+        B, N, _ = cache._batch(table, starts, lengths)
+        if B < 1 or N < 1:
+            raise ValueError(f'table {tuple(table.shape)}: one sequence and one page at least')
+        if weight is not None:
+            cache._weights('weight', weight, (self.L, B, self.H), N * cache.page)
+        if self._paged is None:
+            if self._pf is None:
+                self._pf = Prefill(self)
+            self._paged = PagedPass(self, self._pf)
+        return self._paged.run(cache, tokens, positions, table, starts, lengths, weight, most)
 
     def warm(self, n):
         """n decode steps through the prefill kernel (untimed warm-up)."""

@@ -1107,6 +1107,21 @@ extern "C" __global__ __launch_bounds__(256) void pf_reduce_frag(const float* __
   if (bad) stc_u(err, VH_ERR_RANGE);
 }
 
+// Rows of fp32 in fragment order (an attention over a paged cache leaves its
+// outputs as rows): one thread per eight consecutive columns of a row.
+extern "C" __global__ __launch_bounds__(256) void pf_frag_rows(const float* __restrict__ X, int M, int D,
+                                                                vh_half* __restrict__ F, int MT,
+                                                                unsigned* __restrict__ err) {
+  const int e = blockIdx.x * blockDim.x + threadIdx.x;
+  if (e >= M * (D / 8)) return;
+  const int m = e / (D / 8), k8 = 8 * (e % (D / 8));
+  float v[8];
+  pf_ld8f(X + (size_t)m * D + k8, v);
+  bool bad = false;
+  pf_frag_put8(F, MT, D / 32, m, k8, v, bad);
+  if (bad) stc_u(err, VH_ERR_RANGE);
+}
+
 // ---------------------------------------------------------------- attention
 // Prefill attention on the matrix cores: a block of four waves makes 64 queries
 // of one (batch row, head), 16 to a wave, over the cache positions up to its

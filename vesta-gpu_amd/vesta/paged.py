@@ -40,10 +40,12 @@ import ctypes
 import math
 import struct
 import threading
+import types
 from pathlib import Path
 
 from .launch import compile_code, lib, ok, track, unload
-from .prefill import PRELUDE_SRC
+from .prefill import (ARGMAX_SPLIT, BLOCK as PF_BLOCK, FEW_ROWS as MHEAD_ROWS, LNM_ROWS, MODE_GELU, MODE_PLAIN, MODE_QKV,
+                      MODE_RESID, PRELUDE_SRC, Prefill, _i, _mtiles, _p)
 
 PAGED_SRC = Path(__file__).resolve().parent / 'hip' / 'paged.hip'
 BLOCK = 256
@@ -59,7 +61,8 @@ RUN, RUN_LONG = 8, 64
 SELECT_FEW = 4096
 WEIGH_BLOCKS = 1536
 SCORES_MAX = 1 << 27                   # scores (512 MB) that a call may keep for its weights' pass
-SPLIT, WIDE_SPLIT = 2048, 1024
+SPLIT = {64: 2048, 128: 1024}
+WIDE_SPLIT = 1024
 TARGET = 1536                          # parts that the positions of all row tiles are cut into, about, ...
 PART_STEPS = 8                         # ... each of at least so many steps
 WEIGH = 128                            # positions of a pg_weigh block
@@ -362,13 +365,13 @@ class PagedCache:
             if M and B:
                 rows, aim = (128, WIDE_TARGET) if wide else (ROWS, TARGET)
                 tiles = self.heads * (M * G // rows + B)
-                target = aim if tiles < 2 * aim and N * self.page > (WIDE_SPLIT if wide else SPLIT) else 0
+                target = aim if tiles < 2 * aim and N * self.page > (WIDE_SPLIT if wide else SPLIT[self.width]) else 0
                 blocks = target + tiles + 64
                 if blocks >= 1 << 28 or M * G >= 1 << 30:
                     raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
                 ws = self._floats(blocks * rows * (self.width + 2)) if target else None
                 least = WIDE_PART_STEPS if wide else PART_STEPS
-                run = RUN if not wide or M * G < 128 * RUN_LONG * B else M * G // (128 * B)
+                run = RUN if not wide or M * G < 128 * RUN_LONG * B else max(RUN, M * G // (128 * B))
                 block, attn = (BLOCK, kn.pg_attn) if wide or target or tiles > EIGHT_WAVES else (2 * BLOCK, kn.pg_attn8)
                 args = (_dealt(blocks, run), block, stream, *qs, self._pools[0] + at, self._pools[1] + at, *seqs, B, M,
                         self.heads, G, target, least, run, most, scale2, *to, _at(lse), _at(ws))
@@ -479,3 +482,125 @@ class PagedCache:
             self.err.zero_()
             why = ', '.join(text for bit, text in ERRORS.items() if word & bit)
             raise RuntimeError(f'paged cache: {why}; the results are invalid')
+
+
+PLANS = 8                              # row counts whose launches a PagedPass keeps recorded
+
+
+class PagedPass(Prefill):
+    """One pass of a GPT-2 over ragged new tokens and a paged cache
+    (``VestaGPT2.extend``): the layered engine's products and LayerNorms
+    (``base``, whose module and packed weights are used), with the cache's
+    ``append`` and ``attend`` in the place of its attention. The qkv product
+    writes its key and value rows where ``append`` takes them from: to a
+    product's epilogue the staging rows are M caches of one position.
+    Activation buffers grow to the largest call and are kept."""
+
+    def __init__(self, model, base):
+        import torch
+        self.base, self.fn, self._own, self.err = base, base.fn, base._own, base.err
+        self.layers = model.L
+        self.m = types.SimpleNamespace(W=model.W, D=model.D, H=model.H, L=1, tmax=1, keys=None, vals=None,
+                                       weight_bytes=model.weight_bytes,
+                                       t=torch.zeros(1, dtype=torch.int32, device=self.err.device))
+        self._ws, self._ws_at, self._graph, self._plan, self.mod = None, ctypes.c_void_p(), None, [], None
+        self._held, self._buf, self._plans = (0, 0), None, {}
+
+    def _room(self, M, B):
+        """Buffers for M rows of B sequences (rows past M reach discarded outputs only)."""
+        import torch
+        if M <= self._held[0] and B <= self._held[1]:
+            return
+        M, B = self._held = max(M, self._held[0]), max(B, self._held[1])
+        m, dev = self.m, self.err.device
+        F, V = m.W['fcw'].shape[2], m.W['wte'].shape[0]
+        f32, f16, i32 = (dict(dtype=t, device=dev) for t in (torch.float32, torch.float16, torch.int32))
+        rows, last = 16 * _mtiles(M), 16 * _mtiles(B)
+        self._buf = types.SimpleNamespace(
+            tok=torch.zeros(M, **i32), wpe=torch.empty(M, m.D, **f16), Z=torch.empty(M, m.D, **f32),
+            Q=torch.empty(M, m.D, **f32), O=torch.zeros(M, m.D, **f32), K=torch.empty(M, m.D, **f16),
+            V=torch.empty(M, m.D, **f16), AF=torch.zeros(2 * rows * m.D, **f16), GF=torch.zeros(2 * rows * F, **f16),
+            ZL=torch.empty(B, m.D, **f32), CF=torch.zeros(2 * last * m.D, **f16), logit=torch.empty(B, V, **f32),
+            x=torch.zeros(B, **i32), next=torch.zeros(B, **f32), apv=torch.empty(B * ARGMAX_SPLIT, **f32),
+            api=torch.empty(B * ARGMAX_SPLIT, **i32))
+        self._plans = {}
+
+    def _record(self, build):
+        self._plan = []
+        build()
+        plan, self._plan = self._plan, []
+        return plan
+
+    def _norm(self, X, w, b, to, rows):
+        D, mt = self.m.D, _mtiles(rows)
+        if rows >= LNM_ROWS:
+            self._launch('pf_lnm8' if D <= 1024 else 'pf_lnm16', -(-rows // 16),
+                         [_p(X), _i(rows), _i(D), _p(w), _p(b), _p(to), _i(mt), _p(self.err)])
+        else:
+            self._launch('pf_ln', rows, [_p(X), _i(0), _i(1), _p(w), _p(b), _i(D), _p(to), _i(mt), _p(self.err)])
+
+    def _launches(self, M, B):
+        """The recorded launches of a pass of M rows: embedding; each layer's qkv product; each layer's rest; head."""
+        key = (M, B)
+        if key in self._plans:
+            return self._plans[key]
+        while len(self._plans) >= PLANS:
+            del self._plans[next(iter(self._plans))]
+        m, b, W, err = self.m, self._buf, self.m.W, self.err
+        D, F, V, mt = m.D, W['fcw'].shape[2], W['wte'].shape[0], _mtiles(M)
+
+        def embed():                     # (the positions' rows are gathered: row m's is row m)
+            self._launch('pf_embed_ln', M, [_p(b.tok), _i(M), _p(m.t), _p(W['wte']), _p(b.wpe), _p(b.Z), _i(D), _i(V),
+                                            _i(M), _p(W['ln1w'][0]), _p(W['ln1b'][0]), _p(b.AF), _i(mt), _p(err)])
+
+        def qkv(layer):                  # row i of layer l is row i + l to the epilogue
+            m.keys, m.vals = (ctypes.c_void_p(t.data_ptr() - 2 * layer * D) for t in (b.K, b.V))
+            self._product(b.AF, D, 'qkvw', layer, 3 * D, MODE_QKV, bias=W['qkvb'][layer], out=b.Q, ldo=D, M=M, P=1)
+
+        def rest(layer):
+            self._launch('pf_frag_rows', -(-M * (D // 8) // PF_BLOCK), [_p(b.O), _i(M), _i(D), _p(b.AF), _i(mt), _p(err)])
+            ln2 = W['ln2w'][layer], W['ln2b'][layer], b.AF
+            if not self._product(b.AF, D, 'ow', layer, D, MODE_RESID, bias=W['ob'][layer], out=b.Z, ldo=D, ln=ln2, M=M):
+                self._norm(b.Z, *ln2, M)
+            self._product(b.AF, D, 'fcw', layer, F, MODE_GELU, bias=W['fcb'][layer], F=b.GF, M=M)
+            last = layer + 1 == self.layers
+            ln1 = None if last else (W['ln1w'][layer + 1], W['ln1b'][layer + 1], b.AF)
+            if not self._product(b.GF, F, 'pw', layer, D, MODE_RESID, bias=W['pb'][layer], out=b.Z, ldo=D, ln=ln1, M=M) \
+                    and not last:
+                self._norm(b.Z, *ln1, M)
+
+        def head():
+            self._norm(b.ZL, W['lnfw'], W['lnfb'], b.CF, B)
+            if B <= MHEAD_ROWS:
+                self._mhead(b.CF, D, V, b.logit, B)
+            else:
+                self._pgemm(b.CF, D, 'wte', None, V, MODE_PLAIN, out=b.logit, ldo=V, M=B)
+            self._launch('pf_argmax_part', B * ARGMAX_SPLIT, [_p(b.logit), _i(V), _i(ARGMAX_SPLIT), _p(b.apv), _p(b.api)])
+            self._launch('pf_argmax', B, [_p(b.apv), _p(b.api), _i(ARGMAX_SPLIT), _p(b.x), _p(b.next), _p(m.t), _i(0)])
+
+        self._plans[key] = (self._record(embed), [self._record(lambda n=n: qkv(n)) for n in range(self.layers)],
+                            [self._record(lambda n=n: rest(n)) for n in range(self.layers)], self._record(head))
+        return self._plans[key]
+
+    def run(self, cache, tokens, positions, table, starts, lengths, weight=None, most=None):
+        """The new tokens' pass; returns the logits of each sequence's last
+        row and the largest's id, which the next call overwrites."""
+        import torch
+        M, B, H = tokens.shape[0], table.shape[0], self.m.H
+        self._room(M, B)
+        embed, qkv, rest, head = self._launches(M, B)
+        b = self._buf
+        wpe = self.m.W['wpe']
+        b.tok[:M].copy_(tokens)
+        torch.index_select(wpe, 0, positions.clamp(0, wpe.shape[0] - 1), out=b.wpe[:M])
+        q, o, k, v = (t[:M].view(M, H, -1) for t in (b.Q, b.O, b.K, b.V))
+        self._replay(embed)
+        for layer in range(self.layers):
+            self._replay(qkv[layer])
+            cache.append(k, v, table, starts, lengths, layer)
+            cache.attend(q, table, starts, lengths, layer, out=o, most=most,
+                         weight=None if weight is None else weight[layer])
+            self._replay(rest[layer])
+        torch.index_select(b.Z, 0, (starts[1:] - 1).clamp(0, M - 1), out=b.ZL[:B])
+        self._replay(head)
+        return b.logit[:B], b.x[:B]

@@ -36,8 +36,8 @@ CHUNK = 64                    # products' fold lengths are multiples of this (tw
 HEAD = 64
 KERNELS = ('pf_embed_ln', 'pf_ln', 'pf_lnm8', 'pf_lnm16', 'pf_mgemm1', 'pf_mgemm2', 'pf_mgemm4', 'pf_mgemm1n',
            'pf_mgemm2n', 'pf_mgemm4n', 'pf_pgemm128', 'pf_pgemm64', 'pf_pgemm64w', 'pf_pgemm32', 'pf_pgemm32o',
-           'pf_reduce', 'pf_reduce_ln', 'pf_reduce_frag', 'pf_attn', 'pf_attn16', 'pf_attn1', 'pf_attn1s', 'pf_mhead1',
-           'pf_mhead2', 'pf_mhead4', 'pf_argmax_part', 'pf_argmax')
+           'pf_reduce', 'pf_reduce_ln', 'pf_reduce_frag', 'pf_frag_rows', 'pf_attn', 'pf_attn16', 'pf_attn1',
+           'pf_attn1s', 'pf_mhead1', 'pf_mhead2', 'pf_mhead4', 'pf_argmax_part', 'pf_argmax')
 ARGMAX_SPLIT = 32             # blocks per row of the output-head argmax (same box, 16 -> 32: GPT-2 small 32 rows
                               # 547.6 -> 545.8 us per step, 8 rows 396.3 -> 395.5, XL 64 rows even)
 # output tiles of the products beyond FEW_ROWS rows: 16-row tiles, 16-column tiles and waves of a block
