@@ -333,12 +333,18 @@ __device__ __forceinline__ void pg_count(const PgSeq& s, int G, int& tiles, int&
   tiles = (s.count * G + ROWS - 1) / ROWS;
   steps = max((s.len + STEP - 1) / STEP, 1);
 }
-__device__ __forceinline__ int pg_scan(int v, int lane) {          // sums over the lanes up to each
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int u = __shfl_up(v, d, 64);
-    if (lane >= d) v += u;
-  }
+// Sums over the lanes up to each.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int pg_dpp(int v) {                     // a lane of another row or column, 0 where there is none
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+__device__ __forceinline__ int pg_scan(int v) {                    // (row_shr 1, 2, 4, 8, then row_bcast 15, 31)
+  v += pg_dpp<0x111, 0xF>(v);
+  v += pg_dpp<0x112, 0xF>(v);
+  v += pg_dpp<0x114, 0xF>(v);
+  v += pg_dpp<0x118, 0xF>(v);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
   return v;
 }
 // The steps of a part: the same in every wave that asks.
@@ -374,12 +380,12 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
     return tiles * H * (joined ? 1 : parts);
   };
   PgSeq s = {};
-  int tiles, parts, n = mine(lane, s, tiles, parts), sum = pg_scan(n, lane);
+  int tiles, parts, n = mine(lane, s, tiles, parts), sum = pg_scan(n);
   int total = __builtin_amdgcn_readlane(sum, 63);
   for (int base = 64; base < B; base += 64) {
     PgSeq u;
     int x, y;
-    total += __builtin_amdgcn_readlane(pg_scan(mine(base + lane, u, x, y), lane), 63);
+    total += __builtin_amdgcn_readlane(pg_scan(mine(base + lane, u, x, y)), 63);
   }
   if (err && block == 0 && threadIdx.x < 64) {                     // once a call: what is wrong with any sequence
     unsigned bad = lane < B ? s.bad | (s.count > most ? PG_ERR_MOST : 0u) : 0u;
@@ -395,7 +401,7 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
   for (int base = 0;; base += 64) {
     if (base) {
       n = mine(base + lane, s, tiles, parts);
-      sum = pg_scan(n, lane);
+      sum = pg_scan(n);
     }
     const int all = __builtin_amdgcn_readlane(sum, 63);
     if (at < before + all) {
@@ -413,7 +419,7 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
       o.tile = o.tiles - 1 - (by_head ? ht % o.tiles : ht / H);    // the longest first
       o.at = at;
       if (joined) {
-        const int p = pg_scan(n * parts, lane);
+        const int p = pg_scan(n * parts);
         o.at = places + __builtin_amdgcn_readlane(p, l) - __builtin_amdgcn_readlane(n * parts, l) + rest;
       }
       o.R = o.sq.count * G;
@@ -421,7 +427,7 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
       return true;
     }
     before += all;
-    if (joined) places += __builtin_amdgcn_readlane(pg_scan(n * parts, lane), 63);
+    if (joined) places += __builtin_amdgcn_readlane(pg_scan(n * parts), 63);
   }
 }
 // A tile's last position (-1: its rows see none), its steps and its parts that have steps.
@@ -1134,7 +1140,7 @@ extern "C" __global__ __launch_bounds__(256) void pg_given(const float* __restri
 
 // The same for many rows of 16-bit queries: a block takes 256 positions of one
 // (sequence, key head), 64 to a wave, their key rows in registers, and a slice
-// of the rows that see them, 32 at a time through LDS (double-buffered, with
+// of the rows that see them, 64 at a time through LDS (double-buffered, with
 // the rows' lse), on tiles of 32 x 32 x 16 as in pg_wide. A wave's sums stay in
 // registers over all rows. Several slices (few positions, many rows) leave
 // their sums in `part` [slice][B H So] for pg_total.
@@ -1144,21 +1150,22 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
     const int* __restrict__ table, int N, const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
     int H, int G, float scale2, const float* __restrict__ lse, const float* old, int S,
     float* out, int So, int blocks, int run, int slices, float* __restrict__ part) {
-  constexpr int KS = PG_E / 16, CH = PG_E / 8, NL = 32 * CH / 256, RS = 256 / CH;
-  __shared__ __attribute__((aligned(16))) vh_u32x4 lq[2][32 * CH];
-  __shared__ float lz[2][32];
+  constexpr int KS = PG_E / 16, CH = PG_E / 8, NL = 64 * CH / 256, RS = 256 / CH;
+  __shared__ __attribute__((aligned(16))) vh_u32x4 lq[2][64 * (CH + 1)];
+  __shared__ float lz[2][64];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
   const int id = pg_deal(blockIdx.x, run);
   if (id >= B * H * blocks * slices) return;
-  const int slice = id % slices, bh = id / slices / blocks, b = bh / H, h = bh % H;
-  const int b0 = id / slices % blocks * 256, p0 = b0 + 64 * wave;
+  // the first positions of all heads first: most rows see them
+  const int slice = id % slices, bh = id / slices % (B * H), b = bh / H, h = bh % H;
+  const int b0 = id / slices / (B * H) * 256, p0 = b0 + 64 * wave;
   const PgSeq sq = pg_seq(starts, lengths, b, M, N << shift);
   const int new0 = sq.len - sq.count, R = sq.count * G;
-  // the slice's rows: its share of the 32-row tiles from the first token that sees the block's first position
-  const int tile0 = max(b0 - new0, 0) * G / 32, tiles = b0 < sq.len ? max((R + 31) / 32 - tile0, 0) : 0;
+  // the slice's rows: its share of the 64-row tiles from the first token that sees the block's first position
+  const int tile0 = max(b0 - new0, 0) * G / 64, tiles = b0 < sq.len ? max((R + 63) / 64 - tile0, 0) : 0;
   const int share = (tiles + slices - 1) / slices;
-  const int x0 = (tile0 + min(slice * share, tiles)) * 32, x1 = (tile0 + min((slice + 1) * share, tiles)) * 32;
+  const int x0 = (tile0 + min(slice * share, tiles)) * 64, x1 = (tile0 + min((slice + 1) * share, tiles)) * 64;
   float acc[2][16] = {};
   vh_u32x4 kf[2][KS];
 #pragma unroll
@@ -1168,60 +1175,78 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
 #pragma unroll
     for (int k = 0; k < KS; ++k) kf[i][k] = ld16(kp + (at * H + h) * PG_E + 16 * k + 8 * g);
   }
-  const int c8 = tid % CH, r8 = tid / CH;
+  // Staging: row x + r8 + RS n is head `gr`, token `tr` of the sequence, both
+  // carried on from 64 rows before (a division each cost a third of the loop).
+  const int c8 = tid % CH, r8 = tid / CH, step_t = 64 / G, step_g = 64 % G;
+  int tr[NL + 1], gr[NL + 1];                                      // the last: of the lse's row, x + tid
+#pragma unroll
+  for (int n = 0; n <= NL; ++n) {
+    const int y = x0 + (n < NL ? r8 + RS * n : tid & 63);
+    tr[n] = y / G;
+    gr[n] = y % G;
+  }
   vh_u32x4 qr[NL];
   float zr = 0.0f;
-  auto load = [&](int x) {
+  auto load = [&]() {                                              // past the last row: the last token, without weight
 #pragma unroll
-    for (int n = 0; n < NL; ++n) {
-      const int y = min(x + r8 + RS * n, R - 1), tok = y / G;
-      qr[n] = ld16(Q + (sq.first + tok) * qrow + (h * G + y % G) * qhead + 8 * c8);
-    }
-    if (tid < 32) {                                                // past the last row: no weight
-      const int y = min(x + tid, R - 1);
-      zr = x + tid < R ? lse[(size_t)(sq.first + y / G) * (H * G) + h * G + y % G] : INFINITY;
+    for (int n = 0; n < NL; ++n)
+      qr[n] = ld16(Q + (sq.first + min(tr[n], sq.count - 1)) * qrow + (h * G + gr[n]) * qhead + 8 * c8);
+    if (tid < 64)
+      zr = tr[NL] < sq.count ? lse[(size_t)(sq.first + tr[NL]) * (H * G) + h * G + gr[NL]] : INFINITY;
+#pragma unroll
+    for (int n = 0; n <= NL; ++n) {
+      gr[n] += step_g;
+      tr[n] += step_t;
+      if (gr[n] >= G) {
+        gr[n] -= G;
+        ++tr[n];
+      }
     }
   };
   auto put = [&](int buf) {
 #pragma unroll
-    for (int n = 0; n < NL; ++n) lq[buf][(r8 + RS * n) * CH + (c8 ^ ((r8 + RS * n) & 7))] = qr[n];
-    if (tid < 32) lz[buf][tid] = zr;
+    for (int n = 0; n < NL; ++n) lq[buf][(r8 + RS * n) * (CH + 1) + c8] = qr[n];
+    if (tid < 64) lz[buf][tid] = zr;
   };
   if (x0 < x1) {
-    load(x0);
+    load();
     put(0);
-    if (x0 + 32 < x1) load(x0 + 32);
+    if (x0 + 64 < x1) load();
   }
-  for (int x = x0, buf = 0; x < x1; x += 32, buf ^= 1) {
+  for (int x = x0, buf = 0; x < x1; x += 64, buf ^= 1) {
     vh_lds_sync();
-    if (x + 32 < x1) {
+    if (x + 64 < x1) {
       put(buf ^ 1);
-      if (x + 64 < x1) load(x + 64);
+      if (x + 128 < x1) load();
     }
-    if (new0 + min(x + 31, R - 1) / G < p0) continue;              // no row sees the wave's positions
-    const float z = lz[buf][r];
-    pg_f16v s[2];
+    if (new0 + min(x + 63, R - 1) / G < p0) continue;              // no row sees the wave's positions
+    const bool part = p0 + 63 > new0 + x / G;                      // not all of them by every row
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const vh_u32x4 qf = lq[buf][r * CH + ((2 * k + g) ^ (r & 7))];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) s[i] = pg_mfma32(kf[i][k], qf, s[i]);
-    }
-    if (p0 + 63 > new0 + x / G) {                                  // not all of them by every row
-      const int lim = new0 + min(x + r, R - 1) / G;
+    for (int u = 0; u < 2; ++u) {
+      const float z = lz[buf][32 * u + r];
+      pg_f16v s[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[i][j] = p0 + 32 * i + 8 * (j >> 2) + 4 * g + (j & 3) <= lim ? s[i][j] : -INFINITY;
+        for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const vh_u32x4 qf = lq[buf][(32 * u + r) * (CH + 1) + 2 * k + g];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[i] = pg_mfma32(kf[i][k], qf, s[i]);
+      }
+      if (part) {
+        const int lim = new0 + min(x + 32 * u + r, R - 1) / G;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[i][j] = p0 + 32 * i + 8 * (j >> 2) + 4 * g + (j & 3) <= lim ? s[i][j] : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[i][j] += __builtin_amdgcn_exp2f(fmaf(s[i][j], scale2, -z));
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) acc[i][j] += __builtin_amdgcn_exp2f(fmaf(s[i][j], scale2, -z));
   }
   // over the rows: lane 32 g + r keeps position 32 (r / 16) + 8 (r % 16 / 4) + 4 g + r % 4
   float w = 0.0f;
@@ -1326,7 +1351,7 @@ extern "C" __global__ __launch_bounds__(1024) void pg_select(const float* __rest
     const int each = PG_BINS / threads, top = PG_BINS - 1 - tid * each;
     int mine = 0;
     for (int v = 0; v < each; ++v) mine += hist[top - v];
-    const int upto = pg_scan(mine, lane);
+    const int upto = pg_scan(mine);
     if (lane == 63) part[0][wave] = upto;
     __syncthreads();
     int above = upto - mine;
@@ -1367,7 +1392,7 @@ extern "C" __global__ __launch_bounds__(1024) void pg_select(const float* __rest
           if (s < n && (s >= C || (take > 0 && k > prefix))) stay[c] |= 1u << u;
           if (s < C && take > 0 && k == prefix) stay[c] |= 16u << u;
         }
-        upto[c] = pg_scan(__builtin_popcount(stay[c] & 15u) + (__builtin_popcount(stay[c] & 240u) << 16), lane);
+        upto[c] = pg_scan(__builtin_popcount(stay[c] & 15u) + (__builtin_popcount(stay[c] & 240u) << 16));
         if (lane == 63) part[c][wave] = upto[c];
       }
     }

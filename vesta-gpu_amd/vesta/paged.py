@@ -59,7 +59,7 @@ JOIN_BLOCK = 512
 EIGHT_WAVES = 256
 RUN, RUN_LONG = 8, 64
 SELECT_FEW = 4096
-WEIGH_BLOCKS = 1536
+WEIGH_BLOCKS = 2048
 SCORES_MAX = 1 << 27                   # scores (512 MB) that a call may keep for its weights' pass
 SPLIT = {64: 2048, 128: 1024}
 WIDE_SPLIT = 1024
