@@ -538,14 +538,14 @@ def test_serving_run():
 @pytest.mark.parametrize('dtype,query', KINDS)
 @pytest.mark.parametrize('width', (64, 128))
 def test_every_variant(monkeypatch, dtype, query, width):
-    """The same batch through every kernel that a rule may pick: four or eight waves, positions dealt to parts or not,
+    """The same batch through every kernel that a rule may pick: two, four or eight waves, positions dealt to parts or not,
     blocks of 16 or 128 rows, weights from kept scores or made again, in slices of the rows or not."""
     from vesta import paged
     b = Batch([1, 40, 1, 3], [700, 333, 2500, 3], 2, 2, width, 16, dtype, query)
     want, bound, got, gerr = b.want()
-    base = dict(EIGHT_WAVES=0, SPLIT={64: 1 << 30, 128: 1 << 30}, WIDE_SPLIT=1 << 30, FEW_ROWS=1 << 20)
+    base = dict(EIGHT_WAVES=0, TWO_WAVES=0, SPLIT={64: 1 << 30, 128: 1 << 30}, WIDE_SPLIT=1 << 30, FEW_ROWS=1 << 20)
     parts = dict(SPLIT={64: 0, 128: 0}, WIDE_SPLIT=0)
-    for kw in ({}, dict(EIGHT_WAVES=1 << 20), parts, {**parts, 'TARGET': 16, 'PART_STEPS': 1}, dict(SCORES_MAX=0),
+    for kw in ({}, dict(EIGHT_WAVES=1 << 20), dict(TWO_WAVES=1 << 20), parts, {**parts, 'TARGET': 16, 'PART_STEPS': 1}, dict(SCORES_MAX=0),
                dict(FEW_ROWS=0), dict(FEW_ROWS=0, **parts), dict(FEW_ROWS=0, WEIGH_BLOCKS=1),
                dict(FEW_ROWS=0, WIDE_TARGET=1 << 12, WIDE_PART_STEPS=1, WEIGH_BLOCKS=1 << 20, **parts),
                dict(RUN=1), dict(RUN=64, FEW_ROWS=0), dict(RUN_LONG=0, FEW_ROWS=0)):

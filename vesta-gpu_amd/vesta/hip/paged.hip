@@ -680,6 +680,7 @@ __device__ __forceinline__ void pg_attn_body(
     pg_attn_body<waves>(Q, qrow, qhead, kp, vp, pages, shift, table, N, starts, lengths, B, M, H, \
                         G, target, least, run, most, scale2, out, orow, ohead, lse, ws, sc, pitch, err); \
   }
+PG_ATTN(pg_attn2, 2)
 PG_ATTN(pg_attn, 4)
 PG_ATTN(pg_attn8, 8)
 

@@ -57,13 +57,15 @@ FEW_ROWS = 32                          # rows of a sequence (its most) from whic
 WIDE_TARGET, WIDE_PART_STEPS = 512, 8
 JOIN_BLOCK = 512
 EIGHT_WAVES = 256
+TWO_WAVES = 8
+STEP = {64: 64, 128: 32}               # positions of a wave's step in pg_attn, by width
 RUN, RUN_LONG = 8, 64
 SELECT_FEW = 4096
 WEIGH_BLOCKS = 2048
 SCORES_MAX = 1 << 27                   # scores (512 MB) that a call may keep for its weights' pass
 SPLIT = {64: 2048, 128: 1024}
 WIDE_SPLIT = 1024
-TARGET = 1536                          # parts that the positions of all row tiles are cut into, about, ...
+TARGET = 2048                          # parts that the positions of all row tiles are cut into, about, ...
 PART_STEPS = 8                         # ... each of at least so many steps
 WEIGH = 128                            # positions of a pg_weigh block
 ERRORS = {1: 'a page id outside the pool', 2: 'starts that do not ascend, or lie past the rows',
@@ -75,6 +77,7 @@ SIGNATURES = {
     'pg_append16': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
     'pg_append32': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
     'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllpp' + 'plp',
+    'pg_attn2': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllpp' + 'plp',
     'pg_attn8': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllpp' + 'plp',
     'pg_join': 'ppiiiiiiiippllp',
     'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllppp',
@@ -363,20 +366,29 @@ class PagedCache:
                 if not wide and 0 < M * Hq * pitch <= SCORES_MAX:
                     scores = self._floats(M * Hq * pitch)
             if M and B:
-                rows, aim = (128, WIDE_TARGET) if wide else (ROWS, TARGET)
+                if wide:
+                    rows, aim, most_tiles, least, split = 128, WIDE_TARGET, 2 * WIDE_TARGET, WIDE_PART_STEPS, WIDE_SPLIT
+                else:
+                    rows, aim, most_tiles, least, split = ROWS, TARGET, 16 * TARGET, PART_STEPS, SPLIT[self.width]
                 tiles = self.heads * (M * G // rows + B)
-                target = aim if tiles < 2 * aim and N * self.page > (WIDE_SPLIT if wide else SPLIT[self.width]) else 0
+                target = aim if tiles < most_tiles and N * self.page * 256 > split * max(tiles, 256) else 0
                 blocks = target + tiles + 64
                 if blocks >= 1 << 28 or M * G >= 1 << 30:
                     raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
                 ws = self._floats(blocks * rows * (self.width + 2)) if target else None
-                least = WIDE_PART_STEPS if wide else PART_STEPS
                 run = RUN if not wide or M * G < 128 * RUN_LONG * B else max(RUN, M * G // (128 * B))
-                block, attn = (BLOCK, kn.pg_attn) if wide or target or tiles > EIGHT_WAVES else (2 * BLOCK, kn.pg_attn8)
+                if wide or target:
+                    attn, block = kn.pg_wide if wide else kn.pg_attn, BLOCK
+                elif tiles <= EIGHT_WAVES:
+                    attn, block = kn.pg_attn8, 2 * BLOCK
+                elif N * self.page <= TWO_WAVES * STEP[self.width]:
+                    attn, block = kn.pg_attn2, BLOCK // 2
+                else:
+                    attn, block = kn.pg_attn, BLOCK
                 args = (_dealt(blocks, run), block, stream, *qs, self._pools[0] + at, self._pools[1] + at, *seqs, B, M,
                         self.heads, G, target, least, run, most, scale2, *to, _at(lse), _at(ws))
                 if wide:
-                    kn.pg_wide(*args, self._err)
+                    attn(*args, self._err)
                 else:
                     attn(*args, _at(scores), pitch, self._err)
                 if target:
