@@ -10,6 +10,8 @@ import torch
 pytestmark = pytest.mark.gpu
 
 DT = {'f16': torch.float16, 'bf16': torch.bfloat16, 'f32': torch.float32}
+# pg_wide wherever it is made (not for f32 queries of width 128)
+WIDE = {(64, False): (0, 0, 0), (128, False): (0, 0, 0), (64, True): (0, 0, 0), (128, True): (1 << 30, 1 << 30, 0)}
 KINDS = [('f16', 'f16'), ('bf16', 'bf16'), ('f16', 'f32')]        # cache, queries
 
 
@@ -17,6 +19,15 @@ KINDS = [('f16', 'f16'), ('bf16', 'bf16'), ('f16', 'f32')]        # cache, queri
 def _gpu():
     if not torch.cuda.is_available():
         pytest.skip('no GPU')
+
+
+@pytest.fixture(params=('rule', 'rows of 16', 'rows of 128'))
+def blocks(request, monkeypatch):
+    """Attention as the rule has it, or by the kernel for few or for many rows throughout."""
+    from vesta import paged
+    if request.param != 'rule':
+        monkeypatch.setattr(paged, 'FEW_ROWS', 0 if request.param == 'rows of 128' else 1 << 30)
+        monkeypatch.setattr(paged, 'WIDE_FROM', WIDE)
 
 
 def _gen(*seed):
@@ -153,7 +164,7 @@ SHAPES = [
 @pytest.mark.parametrize('dtype,query', KINDS)
 @pytest.mark.parametrize('width,group,page', [(64, 1, 16), (128, 4, 64), (64, 3, 8), (128, 1, 1), (64, 16, 128)])
 @pytest.mark.parametrize('shape', range(len(SHAPES)))
-def test_attend(dtype, query, width, group, page, shape):
+def test_attend(blocks, dtype, query, width, group, page, shape):
     counts, lengths = SHAPES[shape]
     b = Batch(counts, lengths, 2, group, width, page, dtype, query, seed=shape)
     want, bound, got, gerr = b.want()
@@ -174,7 +185,7 @@ def test_attend(dtype, query, width, group, page, shape):
 
 
 @pytest.mark.parametrize('dtype,query', KINDS)
-def test_attend_long(dtype, query):
+def test_attend_long(blocks, dtype, query):
     """Contexts of some thousands, few and many sequences, and a scale of the caller's."""
     for counts, lengths, heads, group in (([1], [5000], 1, 1), ([1, 1], [3001, 64], 4, 4), ([7], [4100], 2, 2),
                                           ([1] * 40, [50 * i for i in range(40)], 2, 1), ([300], [2300], 1, 2)):
@@ -190,7 +201,7 @@ def test_attend_long(dtype, query):
 @pytest.mark.parametrize('dtype,query', KINDS)
 @pytest.mark.parametrize('width', (64, 128))
 @pytest.mark.parametrize('counts,lengths', [([5, 20], [40, 70]), ([140], [200])])
-def test_values_not_finite(dtype, query, width, counts, lengths):
+def test_values_not_finite(blocks, dtype, query, width, counts, lengths):
     """An infinity or a NaN in a key or value reaches the tokens that see its position, and no other: the outputs of
     those that see none of it are what they are without it, those that do see it get what the formula gives."""
     b = Batch(counts, lengths, 2, 2, width, 16, dtype, query)
@@ -211,7 +222,7 @@ def test_values_not_finite(dtype, query, width, counts, lengths):
 
 
 @pytest.mark.parametrize('dtype,query', KINDS)
-def test_infinite_value_seen_by_all(dtype, query):
+def test_infinite_value_seen_by_all(blocks, dtype, query):
     b = Batch([1, 40], [70, 200], 2, 1, 64, 16, dtype, query)
     for i in range(2):
         b.cache.vals[0, b.table[i, 0], 3, 1, 5] = -math.inf
@@ -220,7 +231,7 @@ def test_infinite_value_seen_by_all(dtype, query):
     _close(b.attend(), want, bound)
 
 
-def test_infinite_key_fp32():
+def test_infinite_key_fp32(blocks):
     """A key with an infinity: scores of +-inf, whatever the planes of the query hold: weight 0, or all NaN."""
     b = Batch([9], [100], 1, 1, 64, 16, 'f16', 'f32')
     b.cache.keys[0, b.table[0, 1], 2, 0, 7] = math.inf
@@ -236,7 +247,7 @@ def test_infinite_key_fp32():
 
 
 @pytest.mark.parametrize('scale', (1e-30, 1e30))
-def test_fp32_queries_of_any_size(scale):
+def test_fp32_queries_of_any_size(blocks, scale):
     b = Batch([4, 1], [60, 33], 2, 1, 128, 16, 'f16', 'f32')
     b.q.mul_(scale)
     want, bound, *_ = b.want(scale=0.1 / scale)
@@ -244,7 +255,7 @@ def test_fp32_queries_of_any_size(scale):
 
 
 @pytest.mark.parametrize('dtype,query', KINDS)
-def test_rows_behind_the_last_are_left(dtype, query):
+def test_rows_behind_the_last_are_left(blocks, dtype, query):
     counts, lengths = [3, 1], [10, 70]
     b = Batch(counts, lengths, 2, 2, 64, 16, dtype, query)
     want, bound, *_ = b.want()
@@ -261,7 +272,7 @@ def test_rows_behind_the_last_are_left(dtype, query):
     b.cache.check()
 
 
-def test_strided_queries_and_outputs():
+def test_strided_queries_and_outputs(blocks):
     """Queries that are a part of a fused projection, outputs into a wider row."""
     b = Batch([3, 20, 1], [3, 50, 90], 2, 2, 64, 16)
     want, bound, *_ = b.want()
@@ -380,7 +391,7 @@ def test_bad_contents_raise_after():
         b.cache.check()
 
 
-def test_pages_shared_to_read():
+def test_pages_shared_to_read(blocks):
     """Two sequences with the same first pages; each appends to its own."""
     b = Batch([1, 1], [33, 33], 2, 1, 64, 16)
     b.table[1, :2] = b.table[0, :2]
@@ -390,7 +401,7 @@ def test_pages_shared_to_read():
     _close(b.attend(), want, bound)
 
 
-def test_a_long_pool():
+def test_a_long_pool(blocks):
     """Row offsets past 2^31 bytes and elements in a layer."""
     from vesta.paged import PagedCache
     c = PagedCache(pages=40000, heads=8, width=128, page=64, dtype='bf16')     # 2.6e9 elements
@@ -543,7 +554,7 @@ def test_every_variant(monkeypatch, dtype, query, width):
     from vesta import paged
     b = Batch([1, 40, 1, 3], [700, 333, 2500, 3], 2, 2, width, 16, dtype, query)
     want, bound, got, gerr = b.want()
-    base = dict(EIGHT_WAVES=0, TWO_WAVES=0, SPLIT={64: 1 << 30, 128: 1 << 30}, WIDE_SPLIT=1 << 30, FEW_ROWS=1 << 20)
+    base = dict(EIGHT_WAVES=0, TWO_WAVES=0, WIDE_FROM=WIDE, SPLIT={64: 1 << 30, 128: 1 << 30}, WIDE_SPLIT=1 << 30, FEW_ROWS=1 << 20)
     parts = dict(SPLIT={64: 0, 128: 0}, WIDE_SPLIT=0)
     for kw in ({}, dict(EIGHT_WAVES=1 << 20), dict(TWO_WAVES=1 << 20), parts, {**parts, 'TARGET': 16, 'PART_STEPS': 1}, dict(SCORES_MAX=0),
                dict(FEW_ROWS=0), dict(FEW_ROWS=0, **parts), dict(FEW_ROWS=0, WEIGH_BLOCKS=1),
@@ -559,7 +570,7 @@ def test_every_variant(monkeypatch, dtype, query, width):
     b.cache.check()
 
 
-def test_many_sequences():
+def test_many_sequences(blocks):
     """More sequences than a wave has lanes, most of them without new tokens."""
     n = 150
     counts = [1 if i % 3 == 0 else 0 for i in range(n)]

@@ -197,4 +197,4 @@ def test_kernels_compile(width, kind):
     code = compile_code(paged.paged_source(width, kind))
     key = b'.vgpr_spill_count'                        # of every kernel: a MessagePack number after the key
     spills = [code[i + len(key)] for i in range(len(code)) if code.startswith(key, i)]
-    assert len(spills) == len(paged.SIGNATURES) - (len(paged._WIDE) if kind == 'f32' else 0) and not any(spills)
+    assert len(spills) == len(paged.kernels_of(width, kind)) and not any(spills)

@@ -684,8 +684,7 @@ PG_ATTN(pg_attn2, 2)
 PG_ATTN(pg_attn, 4)
 PG_ATTN(pg_attn8, 8)
 
-// Attention of many rows of 16-bit queries. A block makes 128 rows of one
-// (sequence, key head), 32 to a wave, over steps of 64 positions that its four
+// Attention of many rows. A block makes 128 rows of one (sequence, key head), 32 to a wave, over steps of 64 positions that its four
 // waves share: key and value rows lie in LDS (double-buffered; the loads of the
 // step after next are in flight while one is used). Products in tiles of
 // 32 x 32 x 16: lane 32 g + r holds row r, fold positions 8 g .. + 7 of an
@@ -695,8 +694,12 @@ PG_ATTN(pg_attn8, 8)
 // position 4 g + e (e < 4) or 8 + 4 g + e - 4 of 16. The weighted values
 // accumulate in the matrix cores' own registers; they are rescaled only when a
 // row's maximum has grown by more than 2^PG_SLACK since (weights up to that
-// are exact in the sums and rounded as finely).
-#if PG_KIND != PG_F32
+// are exact in the sums and rounded as finely). fp32 queries and weights go in
+// three planes, 32 positions at a time, and each 32 positions' weighted values
+// are summed on their own and added in fp32, so that no sum is a chain over all
+// positions; they take this kernel at width 64 only (at 128 their planes leave
+// one block a CU, no faster than pg_attn: 32 x 768 1169 us against 1171).
+#if PG_KIND != PG_F32 || PG_E == 64
 #define PG_SLACK 8.0f
 #define PG_WROW (PG_E + 32)                // halves of a value row in LDS: 64 bytes past a multiple of all banks
 typedef float pg_f16v __attribute__((ext_vector_type(16)));
@@ -735,12 +738,39 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
   const int bfirst = new0 + wk.x0 / G;                             // the block's first row's
   const int wfirst = new0 + min(x0, R - 1) / G, wlast = new0 + min(x0 + 31, R - 1) / G;
   unsigned bad = 0;
-  vh_u32x4 qf[KS];
+  const pg_q* qp = Q + (sq.first + tok) * qrow + head * qhead;
+#if PG_KIND == PG_F32
+  vh_u32x4 qf[KS][3];
+  float k2;                                                        // as in pg_query
   {
-    const pg_q* qp = Q + (sq.first + tok) * qrow + head * qhead + 8 * g;
+    float v[KS][8], mx = 0.0f;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) qf[k] = ld16(qp + 16 * k);
+    for (int k = 0; k < KS; ++k) {
+      const vh_f32x4 a = *(const vh_f32x4*)(qp + 16 * k + 8 * g), c = *(const vh_f32x4*)(qp + 16 * k + 8 * g + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[k][j] = a[j];
+        v[k][4 + j] = c[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, __builtin_fabsf(v[k][j]));
+    }
+    mx = vh_pair32(mx, op_max);
+    int e = 0;
+    if (mx > 0.0f && mx < INFINITY) e = max(__builtin_amdgcn_frexp_expf(mx), -100);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[k][j] = __builtin_ldexpf(v[k][j], -e);
+      pg_split(v[k], qf[k]);
+    }
+    k2 = __builtin_ldexpf(scale2, e);
   }
+#else
+  vh_u32x4 qf[KS];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) qf[k] = ld16(qp + 16 * k + 8 * g);
+#endif
   // staging: thread t takes piece t % CH of rows t / CH + RS n
   const size_t rowlen = (size_t)H * PG_E;
   const int* tb = table + (size_t)wk.b * N;
@@ -775,7 +805,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
         if (64 * t + r8 + RS * n > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
       asm volatile("" ::: "memory");                               // kept a branch
     }
-    if (64 * t + 63 > bfirst) {
+    if (PG_KIND == PG_F32 || 64 * t + 63 > bfirst) {               // (fp32: a plane of a weight may be 0)
       unsigned any = 0u;
 #pragma unroll
       for (int n = 0; n < NL; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
@@ -821,12 +851,24 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     }
     const int p0 = 64 * t, buf = t & 1;
     if (x0 >= R || p0 > wlast) continue;
+    const vh_u32x4* K = lk[buf];
+    const unsigned short* V = lv[buf];
+    const bool seen = p0 + 63 > wfirst;                            // not the whole step by every row
+    const bool wild = lwild[buf] == t + 1;                         // added back below
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds4;
+    auto value = [&](int i, int k, int d) {
+      const unsigned short* vb = V + (32 * i + 16 * k + 4 * g + ((lane & 15) >> 2)) * PG_WROW + 32 * d
+                                 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vb);
+      const s4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vb + 8 * PG_WROW));
+      return __builtin_shufflevector(a, e, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+#if PG_KIND != PG_F32
     // the matrix cores' share of a step goes before the other block's softmax
     // (4096 tokens after 27001, width 128: 2147 -> 2050 us; width 64, where the
     // softmax is most of a step, 27 -> 30)
     if (PG_E == 128) __builtin_amdgcn_s_setprio(1);
-    const vh_u32x4* K = lk[buf];
-    const unsigned short* V = lv[buf];
     pg_f16v s[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -837,7 +879,6 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 #pragma unroll
       for (int i = 0; i < 2; ++i) s[i] = pg_mfma32(K[(32 * i + r) * (CH + 1) + 2 * k + g], qf[k], s[i]);
     if (PG_E == 128) __builtin_amdgcn_s_setprio(0);
-    const bool seen = p0 + 63 > wfirst;                            // not the whole step by every row
     if (seen) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -886,17 +927,6 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
       }
     sum += (ts[0] + ts[1]) + (ts[2] + ts[3]);
     if (PG_E == 128) __builtin_amdgcn_s_setprio(1);
-    const bool wild = lwild[buf] == t + 1;                         // added back below
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    typedef short s8 __attribute__((ext_vector_type(8)));
-    typedef __attribute__((address_space(3))) s4 lds4;
-    auto value = [&](int i, int k, int d) {
-      const unsigned short* vb = V + (32 * i + 16 * k + 4 * g + ((lane & 15) >> 2)) * PG_WROW + 32 * d
-                                 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vb);
-      const s4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vb + 8 * PG_WROW));
-      return __builtin_shufflevector(a, e, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -904,6 +934,79 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = pg_mfma32(__builtin_bit_cast(vh_u32x4, value(i, k, d)), pf[i][k], o[d]);
     if (PG_E == 128) __builtin_amdgcn_s_setprio(0);
+#else
+#pragma nounroll
+    for (int i = 0; i < 2; ++i) {
+      pg_f16v hi, lo;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) hi[j] = lo[j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const vh_u32x4 kf = K[(32 * i + r) * (CH + 1) + 2 * k + g];
+        hi = pg_mfma32(kf, qf[k][0], hi);
+        lo = pg_mfma32(kf, qf[k][1], lo);
+        lo = pg_mfma32(kf, qf[k][2], lo);
+      }
+      float s[16], fin = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        s[j] = vh_hilo(hi[j], lo[j]);
+        fin = fmaf(hi[j], 0.0f, fin);
+      }
+      if (__any(fin != fin)) {                                     // as in pg_scores
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float acc = 0.0f;
+#pragma nounroll
+          for (int c = 0; c < CH; ++c) {
+            float kv[8];
+            unpack8(K[(32 * i + 8 * (j >> 2) + 4 * g + (j & 3)) * (CH + 1) + c], kv);
+#pragma unroll
+            for (int d = 0; d < 8; ++d) acc = fmaf(qp[8 * c + d], kv[d], acc);
+          }
+          if (!(__builtin_fabsf(hi[j]) < INFINITY)) s[j] = acc;
+        }
+      }
+      if (seen) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = p0 + 32 * i + 8 * (j >> 2) + 4 * g + (j & 3) <= lim ? s[j] : -INFINITY;
+      }
+      float bm = s[0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) bm = fmaxf(bm, s[j]);
+      bm = vh_pair32(bm, op_max);
+      const float n2 = fmaxf(m2, bm * k2);
+      const float ref = n2 == -INFINITY ? 0.0f : n2;               // no score above -inf yet: all weights 0
+      const float c = __builtin_amdgcn_exp2f(m2 - ref);
+      m2 = n2;
+      vh_u32x4 pf[2][3];
+      float ts[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * k + j], k2, -ref));
+        ts[k] = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        pg_split(w, pf[k]);
+      }
+      sum = fmaf(sum, c, ts[0] + ts[1]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        pg_f16v th, tw;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) th[j] = tw[j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const vh_u32x4 vf = __builtin_bit_cast(vh_u32x4, value(i, k, d));
+          th = pg_mfma32(vf, pf[k][0], th);
+          tw = pg_mfma32(vf, pf[k][1], tw);
+          tw = pg_mfma32(vf, pf[k][2], tw);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[d][j] = fmaf(o[d][j], c, vh_hilo(th[j], tw[j]));
+      }
+    }
+#endif
     if (wild) {
 #pragma nounroll
       for (int s = p0; s <= min(p0 + 63, last); ++s)
@@ -1041,7 +1144,7 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
     pg_join_body<rows, step>(starts, lengths, B, cap, M, H, G, target, least, run, ws, out, orow, ohead, lse);        \
   }
 PG_JOIN(pg_join, 16, PG_STEP)
-#if PG_KIND != PG_F32
+#if PG_KIND != PG_F32 || PG_E == 64
 PG_JOIN(pg_wide_join, 128, 64)
 #endif
 

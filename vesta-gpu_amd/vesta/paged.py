@@ -55,6 +55,8 @@ PAGE_MAX = 1 << 16
 ROWS = 16                              # query rows of a pg_attn block
 FEW_ROWS = 32                          # rows of a sequence (its most) from which pg_wide makes them
 WIDE_TARGET, WIDE_PART_STEPS = 512, 8
+WIDE_FROM = {(64, False): (128, 64, 4096), (128, False): (64, 64, 1024), (64, True): (256, 256, 4096),
+             (128, True): (1 << 30, 1 << 30, 0)}
 JOIN_BLOCK = 512
 EIGHT_WAVES = 256
 TWO_WAVES = 8
@@ -89,7 +91,17 @@ SIGNATURES = {
     'pg_select': 'pipiiiiippipp',
     'pg_move': 'ppiipipipiiiip',
 }
-_WIDE = ('pg_wide', 'pg_wide_join', 'pg_weigh_wide', 'pg_total')    # for 16-bit queries only
+
+
+def kernels_of(width: int, kind: str) -> set:
+    """The kernels of a module: attention of many rows and its weights are not made for f32 queries, but the former at
+    width 64."""
+    without = set()
+    if kind == 'f32':
+        without = {'pg_weigh_wide', 'pg_total'} | ({'pg_wide', 'pg_wide_join'} if width != 64 else set())
+    return set(SIGNATURES) - without
+
+
 _CODES = {'p': 'P', 'l': 'q', 'i': 'i', 'f': 'f'}
 
 
@@ -131,7 +143,7 @@ class _Kernels:
             ok(lib().vh_module_load(compile_code(paged_source(width, kind)), ctypes.byref(self.mod)),
                'paged cache module load')
             track(self)
-            for name in SIGNATURES if kind != 'f32' else set(SIGNATURES) - set(_WIDE):
+            for name in kernels_of(width, kind):
                 fn = ctypes.c_void_p()
                 ok(lib().vh_module_get_function(self.mod, name.encode(), ctypes.byref(fn)), name)
                 setattr(self, name, _Launcher(fn, name))
@@ -359,7 +371,7 @@ class PagedCache:
             lse = scores = None
             pitch = 0
             # a launch's tiles of rows, as many as there can be, and its parts
-            wide = most * G > FEW_ROWS and q.dtype is not self._f32
+            wide = self._wide(B, N, M, G, most, q.dtype is self._f32) and not (q.dtype is self._f32 and weight is not None)
             if weight is not None:
                 lse = self._floats(M * Hq)
                 pitch = -(-N * self.page // 64) * 64
@@ -401,6 +413,12 @@ class PagedCache:
         finally:
             self._leave(back)
         return out if weight is None else (out, weight_out)
+
+    def _wide(self, B, N, M, G, most, f32):
+        """Whether blocks of 128 rows make the call's (``WIDE_FROM``)."""
+        tiles, rows, positions = WIDE_FROM[self.width, f32]
+        return most * G > FEW_ROWS and (self.heads * max(B, M * G // 128) >= tiles
+                                        or most * G >= rows and N * self.page > positions)
 
     def _floats(self, n):
         """A workspace of a call."""
