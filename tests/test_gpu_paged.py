@@ -356,7 +356,7 @@ def test_evict(dtype, width, page, to_spare, keep, recent):
     b.cache.check()
 
 
-def test_bad_contents_raise_after():
+def test_bad_contents_raise_after(blocks):
     """What the host cannot see: replaced by something possible, and check() says so (once)."""
     b = Batch([2, 3], [40, 20], 2, 1, 64, 16)
     good = b.table, b.starts, b.lengths
@@ -374,11 +374,20 @@ def test_bad_contents_raise_after():
                        ((good[0], _ints([0, 2, 900]), good[2]), 'starts'),
                        ((good[0], _ints([0, 4, 2]), good[2]), 'starts'),
                        ((good[0], _ints([-1, 2, 5]), good[2]), 'starts'),
+                       ((good[0], _ints([0, 5, 0]), good[2]), 'starts'),
                        ((*good[:2], _ints([40, 1 << 30])), 'length'), ((*good[:2], _ints([-3, 20])), 'length')):
         calls(*args)
         with pytest.raises(RuntimeError, match=text):
             b.cache.check()
         b.cache.check()
+    # starts that ask for more parts than there can be: left out, none past the workspaces
+    n = 70
+    many = Batch([1] * n, [300] * n, 2, 1, 64, 16)
+    odd = _ints([0 if i % 2 else n for i in range(n + 1)])
+    w = torch.zeros(n, 2, many.table.shape[1] * 16, device='cuda')
+    many.cache.attend(many.q, many.table, odd, many.lengths, weight=w)
+    with pytest.raises(RuntimeError, match='starts'):
+        many.cache.check()
     b.cache.attend(b.q, *good, most=1)
     with pytest.raises(RuntimeError, match='most'):
         b.cache.check()

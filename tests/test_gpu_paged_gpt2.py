@@ -207,6 +207,31 @@ def test_a_captured_step(hf, alone):
     s.cache.check()
 
 
+def test_capture_needs_room(hf, alone):
+    """Buffers are made before a capture, and a graph outlives a larger call's."""
+    from vesta.gpt2 import VestaGPT2
+    m = VestaGPT2(hf, batch=1, tmax=32, engine='layered')
+    s = Server(m, 2)
+    args = (s.cache, _ints([1, 2]), _ints([0, 0]), _ints([[0], [1]]), _ints([0, 1, 2]), _ints([1, 1]))
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='before capturing'):
+        with torch.cuda.graph(g):
+            m.extend(*args)
+    want = [t.clone() for t in m.extend(*args)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = m.extend(*args)
+    prompt = _prompt(200, 1)
+    big, _ = Server(m, 1, room=16).feed([prompt])
+    _same(big[0], 0, _alone(alone, prompt, 0)[0][0], 0)
+    for _ in range(3):
+        got[0].zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        m.extend(*args)
+
+
 def test_refusals(hf):
     from vesta.gpt2 import VestaGPT2
     from vesta.paged import PagedCache

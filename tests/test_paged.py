@@ -128,7 +128,9 @@ def test_attend_refusals():
     for kw, err in ((dict(q=_rows(5, 4)), ValueError), (dict(q=_rows(5, 0)), ValueError),
                     (dict(q=q.bfloat16()), TypeError), (dict(q=q.double()), TypeError), (dict(scale=0.0), ValueError),
                     (dict(scale=-1.0), ValueError), (dict(scale=float('nan')), ValueError),
-                    (dict(scale=float('inf')), ValueError), (dict(most=0), ValueError),
+                    (dict(scale=float('inf')), ValueError), (dict(most=0), ValueError), (dict(most=1.5), TypeError),
+                    (dict(scale=1e39), ValueError), (dict(scale=1e-40), ValueError), (dict(out=q), ValueError),
+                    (dict(layer=0.0), TypeError),
                     (dict(out=q.float()), TypeError), (dict(out=_rows(4, 6)), ValueError),
                     (dict(out=_rows(1, 6).expand(5, 6, 64)), ValueError),
                     (dict(out=_rows(5, 1).expand(5, 6, 64)), ValueError), (dict(q=None), TypeError),
@@ -169,6 +171,10 @@ def test_nothing_to_do():
         assert c.attend(_rows(M, 6), table, starts, lengths).shape == (M, 6, 64)
         assert not c.log or M and B
         c.log.clear()
+        w = torch.zeros(B, 3, N * 64)
+        c.attend(_rows(M, 6), table, starts, lengths, weight=w)
+        assert all(grid for _, grid, *_ in c.log) and (w.numel() or not any('weigh' in e[0] or 'given' in e[0] for e in c.log))
+        c.log.clear()
 
 
 def test_evict_refusals():
@@ -180,7 +186,8 @@ def test_evict_refusals():
     new, wo, kept = c.evict(**ok)
     assert new.shape == (2,) and wo.shape == (2, 2, 3, 64) and kept.shape == (2, 2, 3, 50)
     assert [e[0] for e in c.log] == ['pg_select', 'pg_move']
-    for kw, err in ((dict(keep=0), ValueError), (dict(keep=65), ValueError), (dict(recent=-1), ValueError),
+    for kw, err in ((dict(to=table), ValueError), (dict(keep=2.0), TypeError), (dict(recent=None), TypeError),
+                    (dict(keep=0), ValueError), (dict(keep=65), ValueError), (dict(recent=-1), ValueError),
                     (dict(weight=w[:1]), ValueError), (dict(weight=w[..., :100].contiguous()), ValueError),
                     (dict(weight=w.half()), TypeError), (dict(to=to[:1]), ValueError), (dict(to=to.long()), TypeError),
                     (dict(weight_out=w[..., :32].contiguous()), ValueError), (dict(weight_out=w), ValueError),

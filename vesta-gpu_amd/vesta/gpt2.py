@@ -330,7 +330,9 @@ class VestaGPT2:
         ``cache.evict``; ``most`` bounds the new tokens of a sequence (1 for a
         decode step).
 
-        Nothing is read back, so a call can be captured in a HIP graph.
+        Nothing is read back, so a call can be captured in a HIP graph, after
+        one call of as many tokens and sequences. Calls share this object's
+        activation buffers, those of two streams must not overlap.
         ``check()`` and ``cache.check()`` report what went wrong."""
         import torch
         from .paged import PagedCache, PagedPass
@@ -355,6 +357,8 @@ class VestaGPT2:
         if weight is not None:
             cache._weights('weight', weight, (self.L, B, self.H), N * cache.page)
         if self._paged is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('extend: call once before capturing such a call')
             if self._pf is None:
                 self._pf = Prefill(self)
             self._paged = PagedPass(self, self._pf)

@@ -317,8 +317,11 @@ __device__ __forceinline__ float pg_taken(const unsigned short* __restrict__ vh,
 // part a tile). So parts are of one size whatever the lengths, and a block of
 // the grid is a part: the grid holds target + H (M G / ROWS + B) + 64, every
 // number of parts that can come out (a multiple of 8 runs), and is dealt to the
-// eight XCDs in runs of `run`, which share an L2. A sequence's parts follow each other, in each its heads, whose rows lie
-// side by side, in each its tiles, which read the same rows.
+// eight XCDs in runs of `run`, which share an L2. A sequence's parts follow
+// each other; in each come its tiles from the longest, all heads of a tile, or
+// (few tiles, or runs of many) its heads, all tiles of a head, which read the
+// same rows. Starts that do not ascend can ask for more parts than there can
+// be: those past `limit`, the places of ws, are left out.
 struct PgWork {
   PgSeq sq;
   int b, h, R, x0, tile, tiles, part, each, at;   // x0: the tile's first row of R; at: the part's place in ws
@@ -367,7 +370,7 @@ __device__ __forceinline__ int pg_each(const int* __restrict__ starts, const int
 template <int ROWS, int STEP>
 __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool joined, const int* __restrict__ starts,
                                         const int* __restrict__ lengths, int B, int M, int cap, int H, int G,
-                                        int target, int least, unsigned* __restrict__ err, int most) {
+                                        int target, int least, int limit, unsigned* __restrict__ err, int most) {
   const int lane = threadIdx.x & 63;
   o.each = pg_each<ROWS, STEP>(starts, lengths, B, M, cap, H, G, target, least);
   auto mine = [&](int b, PgSeq& s, int& tiles, int& parts) -> int {
@@ -396,9 +399,9 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
     if (bad) pg_raise(err, bad);
   }
   const int at = joined ? block : pg_deal(block, run);
-  if (at >= total) return false;
+  if (at >= total || (!joined && at >= limit)) return false;
   int before = 0, places = 0;                                      // in the chunks of 64 sequences already passed
-  for (int base = 0;; base += 64) {
+  for (int base = 0; base < B; base += 64) {
     if (base) {
       n = mine(base + lane, s, tiles, parts);
       sum = pg_scan(n);
@@ -421,6 +424,7 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
       if (joined) {
         const int p = pg_scan(n * parts);
         o.at = places + __builtin_amdgcn_readlane(p, l) - __builtin_amdgcn_readlane(n * parts, l) + rest;
+        if (o.at < 0 || o.at + (__builtin_amdgcn_readlane(parts, l) - 1) * (o.tiles * H) >= limit) return false;
       }
       o.R = o.sq.count * G;
       o.x0 = o.tile * ROWS;
@@ -429,6 +433,7 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
     before += all;
     if (joined) places += __builtin_amdgcn_readlane(pg_scan(n * parts), 63);
   }
+  return false;
 }
 // A tile's last position (-1: its rows see none), its steps and its parts that have steps.
 template <int ROWS, int STEP>
@@ -453,7 +458,7 @@ __device__ __forceinline__ void pg_attn_body(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,
     const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
     const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
-    int run, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
+    int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
     float* __restrict__ ws, float* __restrict__ sc, long pitch, unsigned* __restrict__ err) {
   constexpr int KS = PG_E / 32, NG = PG_STEP / 16, NV = PG_STEP * PG_E / 512, DT = PG_E / 16;
   constexpr int VL = PG_E / 8, VR = 64 / VL;                       // lanes of a value row; rows of a wave's load
@@ -462,7 +467,7 @@ __device__ __forceinline__ void pg_attn_body(
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, q = lane >> 4;
   PgWork wk;
-  if (!pg_work<16, PG_STEP>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, err, most)) return;
+  if (!pg_work<16, PG_STEP>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, limit, err, most)) return;
   int last, steps, parts;
   pg_span<16, PG_STEP>(wk, G, last, steps, parts);
   if (wk.part >= parts) return;
@@ -675,10 +680,10 @@ __device__ __forceinline__ void pg_attn_body(
       const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, \
       const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N, \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least, \
-      int run, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse, \
+      int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse, \
       float* __restrict__ ws, float* __restrict__ sc, long pitch, unsigned* __restrict__ err) { \
     pg_attn_body<waves>(Q, qrow, qhead, kp, vp, pages, shift, table, N, starts, lengths, B, M, H, \
-                        G, target, least, run, most, scale2, out, orow, ohead, lse, ws, sc, pitch, err); \
+                        G, target, least, run, limit, most, scale2, out, orow, ohead, lse, ws, sc, pitch, err); \
   }
 PG_ATTN(pg_attn2, 2)
 PG_ATTN(pg_attn, 4)
@@ -715,7 +720,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,
     const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
     const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
-    int run, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
+    int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
     float* __restrict__ ws, unsigned* __restrict__ err) {
   constexpr int KS = PG_E / 16, DT = PG_E / 32, CH = PG_E / 8, NL = 64 * CH / 256;   // k-steps, dim tiles, 16-byte
   constexpr int RS = 256 / CH;                                     // pieces of a row; a thread's pieces and rows apart
@@ -725,7 +730,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
   PgWork wk;
-  if (!pg_work<128, 64>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, err, most)) return;
+  if (!pg_work<128, 64>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, limit, err, most)) return;
   int last, steps, parts;
   pg_span<128, 64>(wk, G, last, steps, parts);
   if (wk.part >= parts) return;
@@ -1052,7 +1057,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 // (128 parts of four rows, one group a row: 60 us; dealt out: 4).
 template <int ROWS, int STEP>
 __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, const int* __restrict__ lengths, int B,
-                                             int cap, int M, int H, int G, int target, int least, int run,
+                                             int cap, int M, int H, int G, int target, int least, int run, int limit,
                                              const float* __restrict__ ws, pg_q* __restrict__ out, long orow,
                                              long ohead, float* __restrict__ lse) {
   constexpr int LR = PG_E / 4, NGR = 512 / LR;
@@ -1060,8 +1065,8 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
   __shared__ vh_f32x4 jv[512];
   const int tid = threadIdx.x, c = tid % LR, grp = tid / LR, y0 = blockIdx.x % (ROWS / 16) * 16;
   PgWork wk;                                                       // grid: H (M G / ROWS + B) tiles or more
-  if (!pg_work<ROWS, STEP>(wk, blockIdx.x / (ROWS / 16), run, true, starts, lengths, B, M, cap, H, G, target, least, nullptr,
-                           0))
+  if (!pg_work<ROWS, STEP>(wk, blockIdx.x / (ROWS / 16), run, true, starts, lengths, B, M, cap, H, G, target, least, limit,
+                           nullptr, 0))
     return;
   int last, steps, parts;
   pg_span<ROWS, STEP>(wk, G, last, steps, parts);
@@ -1139,9 +1144,9 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
 #define PG_JOIN(name, rows, step)                                                                                  \
   extern "C" __global__ __launch_bounds__(512) void name(                                                          \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int cap, int M, int H, int G,        \
-      int target, int least, int run, const float* __restrict__ ws, pg_q* __restrict__ out, long orow, long ohead, \
-      float* __restrict__ lse) {                                                                                   \
-    pg_join_body<rows, step>(starts, lengths, B, cap, M, H, G, target, least, run, ws, out, orow, ohead, lse);        \
+      int target, int least, int run, int limit, const float* __restrict__ ws, pg_q* __restrict__ out, long orow,  \
+      long ohead, float* __restrict__ lse) {                                                                       \
+    pg_join_body<rows, step>(starts, lengths, B, cap, M, H, G, target, least, run, limit, ws, out, orow, ohead, lse);        \
   }
 PG_JOIN(pg_join, 16, PG_STEP)
 #if PG_KIND != PG_F32 || PG_E == 64

@@ -38,6 +38,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import struct
 import threading
 import types
@@ -78,12 +79,12 @@ _SEQS = 'iipipp'                       # pages, shift, table, its columns, start
 SIGNATURES = {
     'pg_append16': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
     'pg_append32': 'ppllll' + 'pp' + _SEQS + 'iii' + 'p',
-    'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllpp' + 'plp',
-    'pg_attn2': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllpp' + 'plp',
-    'pg_attn8': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllpp' + 'plp',
-    'pg_join': 'ppiiiiiiiippllp',
-    'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiif' + 'pllppp',
-    'pg_wide_join': 'ppiiiiiiiippllp',
+    'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllpp' + 'plp',
+    'pg_attn2': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllpp' + 'plp',
+    'pg_attn8': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllpp' + 'plp',
+    'pg_join': 'ppiiiiiiiiippllp',
+    'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllppp',
+    'pg_wide_join': 'ppiiiiiiiiippllp',
     'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiii',
     'pg_given': 'plppiiiippipii',
     'pg_weigh_wide': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiiiip',
@@ -276,7 +277,7 @@ class PagedCache:
         return at, row, head
 
     def _layer(self, layer):
-        if not 0 <= layer < self.layers:
+        if not 0 <= operator.index(layer) < self.layers:
             raise ValueError(f'layer {layer} of {self.layers}')
         return layer * self._layer_bytes
 
@@ -344,10 +345,10 @@ class PagedCache:
         G, odd = divmod(Hq, self.heads)
         if Hq == 0 or odd:
             raise ValueError(f'q: {Hq} heads are not a multiple of the {self.heads} key heads')
-        scale = self._scale if scale is None else float(scale)
-        if not 0.0 < scale < math.inf:
-            raise ValueError(f'scale {scale}: positive and finite')
-        if most is not None and most < 1:
+        scale2 = 1.4426950408889634 * (self._scale if scale is None else float(scale))
+        if not 2.0 ** -126 <= scale2 < 2.0 ** 127:
+            raise ValueError(f'scale {scale}: positive and finite in 32 bits')
+        if most is not None and operator.index(most) < 1:
             raise ValueError(f'most {most}: at least 1')
         if out is None:
             out = self._empty((M, Hq, self.width), dtype=q.dtype, device=self.device)
@@ -356,6 +357,8 @@ class PagedCache:
             to = self._rows('out', out, (q.dtype,), like=q.shape)
             if M > 1 and to[1] == 0 or Hq > 1 and to[2] == 0:
                 raise ValueError(f'out: rows that lie on one another (strides {out.stride()})')
+            if to[0] == qs[0] and M:
+                raise ValueError('out: a tensor other than q (which a second pass may read again)')
         S = So = 0
         if weight is not None:
             weight_out = weight if weight_out is None else weight_out
@@ -365,7 +368,6 @@ class PagedCache:
             raise ValueError('weight_out: no weight given')
         most = M if most is None else min(most, M)
         kn = self._kind[q.dtype]
-        scale2 = scale * 1.4426950408889634
         stream, back = self._enter()
         try:
             lse = scores = None
@@ -398,7 +400,7 @@ class PagedCache:
                 else:
                     attn, block = kn.pg_attn, BLOCK
                 args = (_dealt(blocks, run), block, stream, *qs, self._pools[0] + at, self._pools[1] + at, *seqs, B, M,
-                        self.heads, G, target, least, run, most, scale2, *to, _at(lse), _at(ws))
+                        self.heads, G, target, least, run, blocks, most, scale2, *to, _at(lse), _at(ws))
                 if wide:
                     attn(*args, self._err)
                 else:
@@ -406,8 +408,8 @@ class PagedCache:
                 if target:
                     (kn.pg_wide_join if wide else kn.pg_join)(
                         tiles * (rows // 16), JOIN_BLOCK, stream, *seqs[4:], B, N * self.page, M, self.heads, G, target,
-                        least, run, ws.data_ptr(), *to, _at(lse))
-            if weight is not None and B:
+                        least, run, blocks, ws.data_ptr(), *to, _at(lse))
+            if weight is not None and B and So:
                 self._receive(kn, stream, (*qs, self._pools[0] + at), seqs, (B, M, G), most, wide, scale2, lse, scores,
                               pitch, (weight.data_ptr(), S, weight_out.data_ptr(), So))
         finally:
@@ -474,7 +476,9 @@ class PagedCache:
         B, N, seqs = self._batch(table, None, lengths)
         to_at = self._ints('to', to, (B, None))
         No = to.shape[1]
-        if keep < 1 or recent < 0:
+        if to_at == seqs[2] and B and N:
+            raise ValueError('to: pages other than those that are read')
+        if operator.index(keep) < 1 or operator.index(recent) < 0:
             raise ValueError(f'keep {keep} of at least 1 position, recent {recent} of at least 0')
         if No * self.page < keep:
             raise ValueError(f'to: {No} pages of {self.page} rows cannot hold {keep} positions')
@@ -535,13 +539,18 @@ class PagedPass(Prefill):
                                        t=torch.zeros(1, dtype=torch.int32, device=self.err.device))
         self._ws, self._ws_at, self._graph, self._plan, self.mod = None, ctypes.c_void_p(), None, [], None
         self._held, self._buf, self._plans = (0, 0), None, {}
+        self._outgrown = []              # buffers that a captured graph may hold
 
     def _room(self, M, B):
         """Buffers for M rows of B sequences (rows past M reach discarded outputs only)."""
         import torch
         if M <= self._held[0] and B <= self._held[1]:
             return
-        M, B = self._held = max(M, self._held[0]), max(B, self._held[1])
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f'extend: call once with at least {M} tokens of {B} sequences before capturing such a call')
+        # (doubled at least, so that all that were outgrown are no more than the present ones)
+        M, B = self._held = tuple(h if n <= h else 1 << (n - 1).bit_length() for n, h in zip((M, B), self._held))
+        self._outgrown.append(self._buf)
         m, dev = self.m, self.err.device
         F, V = m.W['fcw'].shape[2], m.W['wte'].shape[0]
         f32, f16, i32 = (dict(dtype=t, device=dev) for t in (torch.float32, torch.float16, torch.int32))
@@ -554,6 +563,12 @@ class PagedPass(Prefill):
             x=torch.zeros(B, **i32), next=torch.zeros(B, **f32), apv=torch.empty(B * ARGMAX_SPLIT, **f32),
             api=torch.empty(B * ARGMAX_SPLIT, **i32))
         self._plans = {}
+
+    def _workspace(self, n):
+        if self._ws is None or self._ws.numel() < n:
+            self._outgrown.append(self._ws)
+            n = 1 << (n - 1).bit_length()
+        return super()._workspace(n)
 
     def _record(self, build):
         self._plan = []
