@@ -68,7 +68,8 @@ __device__ __forceinline__ vh_u32x4 pg_pack8(pg_f8 v) {
 
 // ---------------------------------------------------------------- append
 // New key and value rows into their pages, eight elements a thread (fp32 ones
-// rounded to the pool's type).
+// rounded to the pool's type). Bound by memory: 12,900 rows of 8 heads of 128,
+// 106 MB read and written, 19.0 us (5.6 TB/s); eight rows 3.1 us, a launch.
 template <typename T>
 __device__ __forceinline__ vh_u32x4 pg_load8(const T* p);
 template <>
@@ -307,6 +308,14 @@ __device__ __forceinline__ float pg_taken(const unsigned short* __restrict__ vh,
 //
 // A block that has a part of the positions only (pg_work) leaves its rows'
 // maxima, sums and weighted values in `ws` for pg_join.
+//
+// What bounds it: over long contexts the cache's bytes: two tokens of 32 heads
+// after 100,003 positions of 8 heads of 128, 818 MB in 162 us (5.05 TB/s, a
+// copy's rate), 64 ragged sequences of up to 4000 603 MB in 125 (4.8 TB/s);
+// over short ones the chain of dependent loads (lengths, pages, rows: 5.5 us
+// with one position, 1.4 us for each further step of a wave). A wave's next
+// step is in flight while it uses one: 16 KB, 128 KB a CU at two waves a SIMD
+// (three waves a SIMD spill: 134 -> 200 us).
 #define PG_STEP (PG_E == 64 ? 64 : 32)
 #define PG_VROW (PG_E + 16)                // halves of a value row in LDS: 16 past a multiple of 32 banks
 #define PG_WS(rows) ((rows) * (PG_E + 2))  // floats of a tile's part: maxima, sums, rows of E
@@ -467,7 +476,9 @@ __device__ __forceinline__ void pg_attn_body(
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, q = lane >> 4;
   PgWork wk;
-  if (!pg_work<16, PG_STEP>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, limit, err, most)) return;
+  if (!pg_work<16, PG_STEP>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, limit,
+                            err, most))
+    return;
   int last, steps, parts;
   pg_span<16, PG_STEP>(wk, G, last, steps, parts);
   if (wk.part >= parts) return;
@@ -689,8 +700,8 @@ PG_ATTN(pg_attn2, 2)
 PG_ATTN(pg_attn, 4)
 PG_ATTN(pg_attn8, 8)
 
-// Attention of many rows. A block makes 128 rows of one (sequence, key head), 32 to a wave, over steps of 64 positions that its four
-// waves share: key and value rows lie in LDS (double-buffered; the loads of the
+// Attention of many rows. A block makes 128 rows of one (sequence, key head),
+// 32 to a wave, over steps of 64 positions that its four waves share: key and value rows lie in LDS (double-buffered; the loads of the
 // step after next are in flight while one is used). Products in tiles of
 // 32 x 32 x 16: lane 32 g + r holds row r, fold positions 8 g .. + 7 of an
 // operand; column r, rows 8 (i / 4) + 4 g + i % 4 of the result, i < 16. As in
@@ -704,6 +715,14 @@ PG_ATTN(pg_attn8, 8)
 // are summed on their own and added in fp32, so that no sum is a chain over all
 // positions; they take this kernel at width 64 only (at 128 their planes leave
 // one block a CU, no faster than pg_attn: 32 x 768 1169 us against 1171).
+//
+// What bounds it: at width 128 the matrix cores (1024 cycles of a wave's step)
+// and LDS (each operand read serves 32 rows: 32 KB a wave's step, as many
+// cycles of the CU's LDS as of its matrix cores) about evenly: 4096 tokens after
+// 27,001, 1.95 TFLOP in 2060-2110 us (925-945 TFLOP/s, 68% of a large library
+// product's rate). At width 64 the softmax on the vector units (about 1400
+// cycles a step against 512), and for short chunks the blocks' starts and ends
+// (10 us): six chunks of up to 512 tokens 27 us (200 TFLOP/s).
 #if PG_KIND != PG_F32 || PG_E == 64
 #define PG_SLACK 8.0f
 #define PG_WROW (PG_E + 32)                // halves of a value row in LDS: 64 bytes past a multiple of all banks
@@ -730,7 +749,9 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
   PgWork wk;
-  if (!pg_work<128, 64>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, limit, err, most)) return;
+  if (!pg_work<128, 64>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, limit, err,
+                        most))
+    return;
   int last, steps, parts;
   pg_span<128, 64>(wk, G, last, steps, parts);
   if (wk.part >= parts) return;
@@ -1160,7 +1181,8 @@ PG_JOIN(pg_wide_join, 128, 64)
 // head), 32 to a wave, their key rows in registers, and goes through the rows
 // that see them, 16 at a time, in order: no atomics, the same sums each time.
 // `out` may be `old`: a thread reads an element before it writes it.
-// Scores are made again (as in pg_attn), the weight is 2^(score - lse).
+// Scores are made again (as in pg_attn), the weight is 2^(score - lse). For fp32
+// queries, and where the scores would be too many to keep.
 extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
     const int* __restrict__ table, int N, const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
@@ -1252,7 +1274,9 @@ extern "C" __global__ __launch_bounds__(256) void pg_given(const float* __restri
 // of the rows that see them, 64 at a time through LDS (double-buffered, with
 // the rows' lse), on tiles of 32 x 32 x 16 as in pg_wide. A wave's sums stay in
 // registers over all rows. Several slices (few positions, many rows) leave
-// their sums in `part` [slice][B H So] for pg_total.
+// their sums in `part` [slice][B H So] for pg_total. 4 x 1999 tokens of 32 heads
+// (8 of 128 keyed): 79 us, of which 45 the rows and 34 the blocks' starts and
+// ends; slices of one size for all positions instead: 99.
 #if PG_KIND != PG_F32
 extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
@@ -1395,7 +1419,9 @@ extern "C" __global__ __launch_bounds__(256) void pg_total(const float* __restri
 // exponent, takes few values, whose adds wait for each other), ending early
 // where all that share a prefix stay; then the positions are listed in order,
 // four consecutive ones a thread. A NaN counts as the largest. What bounds it:
-// the chain of passes over a block's weights, not bytes.
+// LDS adds, about one a cycle and CU whatever their addresses (four or eight
+// copies of the histogram are no faster): 30,000 positions 31 us, of which 14
+// the first digit's; 1152 times 1024 positions 13 us.
 #define PG_BINS 2048
 __device__ __forceinline__ unsigned pg_key(float w) {
   const unsigned u = __builtin_bit_cast(unsigned, w + 0.0f);       // -0 as 0
@@ -1538,7 +1564,8 @@ extern "C" __global__ __launch_bounds__(1024) void pg_select(const float* __rest
 }
 
 // pg_move: the kept rows of all layers into the pages of the other table, 16
-// bytes of a key and of a value row a thread.
+// bytes of a key and of a value row a thread: 393 MB in 79 us (5.0 TB/s, a
+// copy's rate).
 extern "C" __global__ __launch_bounds__(256) void pg_move(unsigned short* __restrict__ kp, unsigned short* __restrict__ vp,
                                                           int pages, int shift, const int* __restrict__ table, int N,
                                                           const int* __restrict__ to, int No,

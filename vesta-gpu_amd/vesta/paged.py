@@ -25,8 +25,8 @@ positions up to its own. A token at a negative position (a padded row: length
 Everything stays on the device and on torch's current stream, so a call can be
 captured in a HIP graph and replayed with other contents of its tensors.
 Calls allocate their workspaces from torch's allocator, none is shared between
-two calls. Tensors are checked on the host (``TypeError``, ``ValueError``);
-what lies in ``table``, ``starts`` and ``lengths`` is checked on the device,
+two calls, which may come from several threads and streams. Tensors are checked
+on the host (``TypeError``, ``ValueError``); what lies in ``table``, ``starts`` and ``lengths`` is checked on the device,
 where an impossible value is replaced by a possible one and raises an error
 word that ``check()`` reads.
 
@@ -45,32 +45,52 @@ import types
 from pathlib import Path
 
 from .launch import compile_code, lib, ok, track, unload
-from .prefill import (ARGMAX_SPLIT, BLOCK as PF_BLOCK, FEW_ROWS as MHEAD_ROWS, LNM_ROWS, MODE_GELU, MODE_PLAIN, MODE_QKV,
-                      MODE_RESID, PRELUDE_SRC, Prefill, _i, _mtiles, _p)
+from .prefill import (ARGMAX_SPLIT, BLOCK as PF_BLOCK, FEW_ROWS as MHEAD_ROWS, LNM_ROWS, MODE_GELU, MODE_PLAIN,
+                      MODE_QKV, MODE_RESID, PRELUDE_SRC, Prefill, _i, _mtiles, _p)
 
 PAGED_SRC = Path(__file__).resolve().parent / 'hip' / 'paged.hip'
 BLOCK = 256
 WIDTHS = (64, 128)
 KINDS = ('f16', 'bf16', 'f32')         # kernels' queries: the cache's type, or f32 over an f16 cache
 PAGE_MAX = 1 << 16
-ROWS = 16                              # query rows of a pg_attn block
-FEW_ROWS = 32                          # rows of a sequence (its most) from which pg_wide makes them
-WIDE_TARGET, WIDE_PART_STEPS = 512, 8
+STEP = {64: 64, 128: 32}               # positions of a wave's step in pg_attn, by width
+JOIN_BLOCK = 512
+
+# How a call's work is laid out; us a call (GPU time) on both sides of each rule.
+ROWS = 16                     # query rows of a pg_attn block; pg_wide's have 128
+FEW_ROWS = 32                 # a sequence of up to so many rows (new tokens times heads of a group) is pg_attn's
+# More are pg_wide's, by (width, whether the queries are f32), from so many of its tiles on, or from so many rows a
+# sequence where the tables have more than so many positions. pg_attn / pg_wide, width 64, 16 bits: 8 x 128 after 900
+# (96 tiles) 25.7 / 28.9, 16 x 128 (192) 42.1 / 30.5, 1 x 64 after 8000 22.2 / 20.9, 1 x 256 52.2 / 28.1; width 128,
+# four heads a group: 1 x 128 (32 tiles) 7.0 / 12.0, 4 x 128 after 500 (128) 33.3 / 26.8, 2 x 16 after 30000 91 / 59;
+# f32, width 64: 16 x 128 after 900 53.7 / 55.3, 24 x 128 76.7 / 75.2, 32 x 768 321 / 178, 1 x 64 after 8000 25.7 /
+# 33.5, 1 x 256 63.3 / 48.6; f32, width 128: even at best, so it is not made.
 WIDE_FROM = {(64, False): (128, 64, 4096), (128, False): (64, 64, 1024), (64, True): (256, 256, 4096),
              (128, True): (1 << 30, 1 << 30, 0)}
-JOIN_BLOCK = 512
-EIGHT_WAVES = 256
-TWO_WAVES = 8
-STEP = {64: 64, 128: 32}               # positions of a wave's step in pg_attn, by width
-RUN, RUN_LONG = 8, 64
-SELECT_FEW = 4096
-WEIGH_BLOCKS = 2048
-SCORES_MAX = 1 << 27                   # scores (512 MB) that a call may keep for its weights' pass
+# A tile's positions go to several blocks, and a second launch puts them together, where the tables have more than
+# SPLIT positions times tiles / 256. One token, 12 heads, whole / in parts: width 64 after 1024 9.6 / 14.0, 2048 15.4 /
+# 14.0, 16384 86.9 / 21.3; width 128 after 700 12.1 / 13.0, 1024 15.9 / 13.0, 16384 176 / 27.7; 64 sequences after up
+# to 900 (512 tiles, width 128) 31.5 / 36.1, 256 after up to 2000 (2048 tiles) 258 / 274, 64 after up to 4000 142 / 125.
 SPLIT = {64: 2048, 128: 1024}
-WIDE_SPLIT = 1024
-TARGET = 2048                          # parts that the positions of all row tiles are cut into, about, ...
-PART_STEPS = 8                         # ... each of at least so many steps
-WEIGH = 128                            # positions of a pg_weigh block
+TARGET = 2048                 # parts in all, about (64 after up to 4000, 1024 / 1536 / 2048 / 3072: 131.0 / 128.5 / 125.3
+                              # / 126.3; 2 after 100003: 160.2 / 162.4 / 162.0 / 167.1) ...
+PART_STEPS = 8                # ... each of at least so many steps: two a wave
+# The same of pg_wide, where it has fewer tiles than fill the chip twice (two blocks a CU are resident).
+WIDE_SPLIT, WIDE_TARGET, WIDE_PART_STEPS = 1024, 512, 8
+EIGHT_WAVES = 256             # pg_attn of up to so many tiles (a block a CU) in blocks of eight waves (one token after
+                              # 700, four / eight waves: 11.1 / 10.4; 8 x 128, 864 tiles: 13.4 / 19.1) ...
+TWO_WAVES = 8                 # ... and of more, where the tables have up to so many steps, of two (f32, four / two waves:
+                              # 8 x 128 13.2 / 8.4, 64 tokens after 256 18.6 / 16.0, after 512 24.6 / 24.6; 64 after
+                              # 600 of width 128, 19 steps, 22.4 / 23.5)
+RUN = 8                       # neighbouring blocks that go to one XCD (4 x 1999 in 4 / 16 / 64: 234 / 246 / 269) ...
+RUN_LONG = 64                 # ... but all tiles of a head where they are so many or more, which read the head's rows
+                              # together (4096 tokens after 27001, 16 / 64 / all 128 tiles: 2369 / 2261 / 2114)
+SCORES_MAX = 1 << 27          # scores (512 MB) that pg_attn keeps for the weights' pass (32 tokens after up to 1000: 24;
+                              # made again by pg_weigh: 37)
+WEIGH = 128                   # positions of a pg_weigh block
+WEIGH_BLOCKS = 2048           # blocks of pg_weigh_wide, about, by slices of the rows (4 x 1999, 512 / 1024 / 1536 / 2048 /
+                              # 3072: 319 / 205 / 198 / 197 / 204)
+SELECT_FEW = 4096             # positions up to which pg_select has 256 threads, not 1024 (1152 times 1024: 13 / 38)
 ERRORS = {1: 'a page id outside the pool', 2: 'starts that do not ascend, or lie past the rows',
           4: 'a length past its table', 8: 'a sequence with more new tokens than `most`'}
 
@@ -351,7 +371,7 @@ class PagedCache:
         if most is not None and operator.index(most) < 1:
             raise ValueError(f'most {most}: at least 1')
         if out is None:
-            out = self._empty((M, Hq, self.width), dtype=q.dtype, device=self.device)
+            out = q.new_empty((M, Hq, self.width))
             to = out.data_ptr(), Hq * self.width, self.width
         else:
             to = self._rows('out', out, (q.dtype,), like=q.shape)
@@ -370,45 +390,37 @@ class PagedCache:
         kn = self._kind[q.dtype]
         stream, back = self._enter()
         try:
-            lse = scores = None
-            pitch = 0
-            # a launch's tiles of rows, as many as there can be, and its parts
-            wide = self._wide(B, N, M, G, most, q.dtype is self._f32) and not (q.dtype is self._f32 and weight is not None)
+            f32 = q.dtype is self._f32
+            wide = self._wide(B, N, M, G, most, f32) and not (f32 and weight is not None)
+            lse = scores = pitch = target = 0
+            floats = 0                   # of the one workspace: lse, scores, parts
             if weight is not None:
-                lse = self._floats(M * Hq)
                 pitch = -(-N * self.page // 64) * 64
+                floats = -(-M * Hq // 4) * 4
                 if not wide and 0 < M * Hq * pitch <= SCORES_MAX:
-                    scores = self._floats(M * Hq * pitch)
+                    scores = 4 * floats
+                    floats += M * Hq * pitch
             if M and B:
-                if wide:
-                    rows, aim, most_tiles, least, split = 128, WIDE_TARGET, 2 * WIDE_TARGET, WIDE_PART_STEPS, WIDE_SPLIT
-                else:
-                    rows, aim, most_tiles, least, split = ROWS, TARGET, 16 * TARGET, PART_STEPS, SPLIT[self.width]
-                tiles = self.heads * (M * G // rows + B)
-                target = aim if tiles < most_tiles and N * self.page * 256 > split * max(tiles, 256) else 0
-                blocks = target + tiles + 64
-                if blocks >= 1 << 28 or M * G >= 1 << 30:
-                    raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
-                ws = self._floats(blocks * rows * (self.width + 2)) if target else None
-                run = RUN if not wide or M * G < 128 * RUN_LONG * B else max(RUN, M * G // (128 * B))
-                if wide or target:
-                    attn, block = kn.pg_wide if wide else kn.pg_attn, BLOCK
-                elif tiles <= EIGHT_WAVES:
-                    attn, block = kn.pg_attn8, 2 * BLOCK
-                elif N * self.page <= TWO_WAVES * STEP[self.width]:
-                    attn, block = kn.pg_attn2, BLOCK // 2
-                else:
-                    attn, block = kn.pg_attn, BLOCK
+                attn, block, rows, tiles, target, blocks, least, run = self._layout(kn, B, N, M, G, wide)
+                ws = 4 * floats
+                floats += blocks * rows * (self.width + 2) if target else 0
+            if floats:
+                held = self._floats(floats)
+                base = held.data_ptr()
+                lse = base if weight is not None else 0
+                scores = scores and base + scores
+            if M and B:
+                to = (*to, lse)
                 args = (_dealt(blocks, run), block, stream, *qs, self._pools[0] + at, self._pools[1] + at, *seqs, B, M,
-                        self.heads, G, target, least, run, blocks, most, scale2, *to, _at(lse), _at(ws))
+                        self.heads, G, target, least, run, blocks, most, scale2, *to, base + ws if target else 0)
                 if wide:
                     attn(*args, self._err)
                 else:
-                    attn(*args, _at(scores), pitch, self._err)
+                    attn(*args, scores, pitch, self._err)
                 if target:
                     (kn.pg_wide_join if wide else kn.pg_join)(
                         tiles * (rows // 16), JOIN_BLOCK, stream, *seqs[4:], B, N * self.page, M, self.heads, G, target,
-                        least, run, blocks, ws.data_ptr(), *to, _at(lse))
+                        least, run, blocks, base + ws, *to)
             if weight is not None and B and So:
                 self._receive(kn, stream, (*qs, self._pools[0] + at), seqs, (B, M, G), most, wide, scale2, lse, scores,
                               pitch, (weight.data_ptr(), S, weight_out.data_ptr(), So))
@@ -422,6 +434,34 @@ class PagedCache:
         return most * G > FEW_ROWS and (self.heads * max(B, M * G // 128) >= tiles
                                         or most * G >= rows and N * self.page > positions)
 
+    def _layout(self, kn, B, N, M, G, wide):
+        """The kernel and threads of a block, its rows, the tiles of so many rows there can be, the parts asked for (0:
+        one a tile) and those there can be, the least steps of one, the blocks to an XCD in turn."""
+        positions = N * self.page
+        if wide:
+            rows, aim, most_tiles, least, split = 128, WIDE_TARGET, 2 * WIDE_TARGET, WIDE_PART_STEPS, WIDE_SPLIT
+        else:
+            rows, aim, most_tiles, least, split = ROWS, TARGET, 16 * TARGET, PART_STEPS, SPLIT[self.width]
+        tiles = self.heads * (M * G // rows + B)
+        target = aim if tiles < most_tiles and positions * 256 > split * max(tiles, 256) else 0
+        blocks = target + tiles + 64
+        if blocks >= 1 << 28 or M * G >= 1 << 30:
+            raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
+        run = RUN
+        if wide:
+            attn, block = kn.pg_wide, BLOCK
+            if M * G >= 128 * RUN_LONG * B:
+                run = M * G // (128 * B)
+        elif target:
+            attn, block = kn.pg_attn, BLOCK
+        elif tiles <= EIGHT_WAVES:
+            attn, block = kn.pg_attn8, 2 * BLOCK
+        elif positions <= TWO_WAVES * STEP[self.width]:
+            attn, block = kn.pg_attn2, BLOCK // 2
+        else:
+            attn, block = kn.pg_attn, BLOCK
+        return attn, block, rows, tiles, target, blocks, least, max(run, 1)
+
     def _floats(self, n):
         """A workspace of a call."""
         return self._empty(n, dtype=self._f32, device=self.device)
@@ -430,20 +470,19 @@ class PagedCache:
         """The weights' pass after ``attend``'s: from the scores it left, or making them again."""
         B, M, G = extents
         bh, So, cap = B * self.heads, to[-1], seqs[3] * self.page
-        if scores is not None:
+        if scores:
             blocks = -(-So // 1024)
-            kn.pg_given(bh * blocks, BLOCK, stream, scores.data_ptr(), pitch, *seqs[4:], cap, M, self.heads, G,
-                        lse.data_ptr(), *to, blocks)
+            kn.pg_given(bh * blocks, BLOCK, stream, scores, pitch, *seqs[4:], cap, M, self.heads, G, lse, *to, blocks)
         elif not wide:
             blocks = -(-So // WEIGH)
-            kn.pg_weigh(_dealt(bh * blocks, RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2, lse.data_ptr(),
-                        *to, blocks, RUN)
+            kn.pg_weigh(_dealt(bh * blocks, RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2, lse, *to,
+                        blocks, RUN)
         else:
             blocks = -(-So // 256)
             slices = max(1, min(WEIGH_BLOCKS // (bh * blocks), most * G // 256))
             part = None if slices == 1 else self._floats(slices * bh * So)
             kn.pg_weigh_wide(_dealt(bh * blocks * slices, RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2,
-                             lse.data_ptr(), *to, blocks, RUN, slices, _at(part))
+                             lse, *to, blocks, RUN, slices, _at(part))
             if slices > 1:
                 kn.pg_total(bh * blocks, BLOCK, stream, part.data_ptr(), slices, *seqs[4:], cap, B, M, self.heads, *to,
                             blocks)
@@ -499,9 +538,9 @@ class PagedCache:
             raise ValueError(f'{self.layers} layers of {B} sequences are too many for one call')
         stream, back = self._enter()
         try:
-            kn.pg_select(self.layers * B * self.heads, 256 if N * self.page <= SELECT_FEW else 1024, stream, weight.data_ptr(), S, seqs[5], N * self.page, B,
-                         self.heads, keep, recent, kept.data_ptr(), weight_out.data_ptr(), So, new.data_ptr(),
-                         self._err)
+            kn.pg_select(self.layers * B * self.heads, 256 if N * self.page <= SELECT_FEW else 1024, stream,
+                         weight.data_ptr(), S, seqs[5], N * self.page, B, self.heads, keep, recent, kept.data_ptr(),
+                         weight_out.data_ptr(), So, new.data_ptr(), self._err)
             kn.pg_move(self.layers * B * blocks, BLOCK, stream, *self._pools, *seqs[:4], to_at, No, kept.data_ptr(), keep,
                        B, self.heads, blocks, self._err)
         finally:
