@@ -32,6 +32,15 @@ __device__ __forceinline__ void pg_raise(unsigned* err, unsigned bits) {
   __hip_atomic_fetch_or(err, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// x / d of whole numbers, x >= 0 and d > 0: the compiler's 32-bit division is
+// some 35 dependent operations, and a small call waits for half a dozen. Below
+// 2^22 the reciprocal's quotient is off by one at most.
+__device__ __forceinline__ int pg_div(int x, int d) {
+  if (x >= 1 << 22) return x / d;
+  const int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d)), r = x - q * d;
+  return q + (r >= d ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+
 // Sequence b: its first row, new tokens and length.
 struct PgSeq {
   int first, count, len;
@@ -337,7 +346,8 @@ struct PgWork {
 };
 __device__ __forceinline__ int pg_deal(int block, int run) {       // the block's place: blocks go to XCD block % 8
   const int j = block >> 3;
-  return (j / run * 8 + (block & 7)) * run + j % run;
+  const int n = pg_div(j, run);
+  return (n * 8 + (block & 7)) * run + j - n * run;
 }
 #define PG_RUN_LONG 64
 template <int ROWS, int STEP>
@@ -388,7 +398,7 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
     s = pg_seq(starts, lengths, b, M, cap);
     int steps;
     pg_count<ROWS, STEP>(s, G, tiles, steps);
-    parts = (steps - 1) / o.each + 1;
+    parts = target ? pg_div(steps - 1, o.each) + 1 : 1;
     return tiles * H * (joined ? 1 : parts);
   };
   PgSeq s = {};
@@ -424,11 +434,12 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
       o.sq.len = __builtin_amdgcn_readlane(s.len, l);
       o.tiles = __builtin_amdgcn_readlane(tiles, l);
       const int rest = at - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
-      o.part = rest / (o.tiles * H);
       const bool by_head = run >= PG_RUN_LONG || o.tiles <= 8;
-      const int ht = rest % (o.tiles * H);
-      o.h = by_head ? ht / o.tiles : ht % H;
-      o.tile = o.tiles - 1 - (by_head ? ht % o.tiles : ht / H);    // the longest first
+      o.part = target ? pg_div(rest, o.tiles * H) : 0;
+      const int ht = rest - o.part * (o.tiles * H), inner = by_head ? o.tiles : H;
+      const int major = pg_div(ht, inner), minor = ht - major * inner;
+      o.h = by_head ? major : minor;
+      o.tile = o.tiles - 1 - (by_head ? minor : major);            // the longest first
       o.at = at;
       if (joined) {
         const int p = pg_scan(n * parts);
@@ -447,9 +458,9 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
 // A tile's last position (-1: its rows see none), its steps and its parts that have steps.
 template <int ROWS, int STEP>
 __device__ __forceinline__ void pg_span(const PgWork& w, int G, int& last, int& steps, int& parts) {
-  last = w.sq.len - w.sq.count + min(w.x0 + ROWS - 1, w.R - 1) / G;
+  last = w.sq.len - w.sq.count + pg_div(min(w.x0 + ROWS - 1, w.R - 1), G);
   steps = last < 0 ? 0 : last / STEP + 1;
-  parts = max((steps - 1) / w.each + 1, 1);
+  parts = steps > w.each ? pg_div(steps - 1, w.each) + 1 : 1;
 }
 
 // Four consecutive results of a row, rounded to the queries' type.
@@ -486,10 +497,10 @@ __device__ __forceinline__ void pg_attn_body(
   const int R = wk.R, x0 = wk.x0, h = wk.h;
   const int t0 = min(wk.part * wk.each, steps), t1 = wk.each < steps - t0 ? t0 + wk.each : steps;
   unsigned bad = 0;
-  const int x = min(x0 + r, R - 1), tok = x / G, head = h * G + x % G;
+  const int x = min(x0 + r, R - 1), tok = pg_div(x, G), head = h * G + x - tok * G;
   const bool live = x0 + r < R;
   const int lim = sq.len - sq.count + tok;                         // this lane's last position
-  const int first = sq.len - sq.count + x0 / G;                    // the first row's
+  const int first = sq.len - sq.count + pg_div(x0, G);                    // the first row's
   const pg_q* qp = Q + (sq.first + tok) * qrow + head * qhead;
   const size_t rowlen = (size_t)H * PG_E;
   const int* tb = table + (size_t)wk.b * N;
@@ -758,11 +769,11 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
   const PgSeq sq = wk.sq;
   const int R = wk.R, x0 = wk.x0 + 32 * wave, h = wk.h, new0 = sq.len - sq.count;
   const int t0 = min(wk.part * wk.each, steps), t1 = wk.each < steps - t0 ? t0 + wk.each : steps;
-  const int x = min(x0 + r, R - 1), tok = x / G, head = h * G + x % G;
+  const int x = min(x0 + r, R - 1), tok = pg_div(x, G), head = h * G + x - tok * G;
   const bool live = x0 + r < R;
   const int lim = new0 + tok;                                      // this lane's last position
-  const int bfirst = new0 + wk.x0 / G;                             // the block's first row's
-  const int wfirst = new0 + min(x0, R - 1) / G, wlast = new0 + min(x0 + 31, R - 1) / G;
+  const int bfirst = new0 + pg_div(wk.x0, G);                             // the block's first row's
+  const int wfirst = new0 + pg_div(min(x0, R - 1), G), wlast = new0 + pg_div(min(x0 + 31, R - 1), G);
   unsigned bad = 0;
   const pg_q* qp = Q + (sq.first + tok) * qrow + head * qhead;
 #if PG_KIND == PG_F32
@@ -1049,6 +1060,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
   if (!live) return;
   sum = vh_pair32(sum, op_sum);
   const bool whole = parts == 1;
+  const float inv = 1.0f / sum;        // (exact enough for results of 16 bits: a division each was 0.5 us of a block's end)
   pg_q* op = out + (sq.first + tok) * orow + head * ohead;
   float* wp = ws + (size_t)wk.at * PG_WS(128);
 #pragma unroll
@@ -1057,7 +1069,8 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     for (int i = 0; i < 4; ++i) {
       float v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = !whole ? o[d][4 * i + j] : lim < 0 ? 0.0f : o[d][4 * i + j] / sum;
+      for (int j = 0; j < 4; ++j)
+        v[j] = !whole ? o[d][4 * i + j] : lim < 0 ? 0.0f : PG_KIND == PG_F32 ? o[d][4 * i + j] / sum : o[d][4 * i + j] * inv;
       if (whole) pg_store4(op + 32 * d + 8 * i + 4 * g, v);
       else *(vh_f32x4*)(wp + 256 + (32 * wave + r) * PG_E + 32 * d + 8 * i + 4 * g) = vh_f32x4{v[0], v[1], v[2], v[3]};
     }
@@ -1155,7 +1168,7 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
     m = mm;
   }
   if (grp % n2 >= n || slice > 0) return;
-  const int x = wk.x0 + y, tok = x / G, head = wk.h * G + x % G, lim = wk.sq.len - wk.sq.count + tok;
+  const int x = wk.x0 + y, tok = pg_div(x, G), head = wk.h * G + x - tok * G, lim = wk.sq.len - wk.sq.count + tok;
   float w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) w[j] = lim < 0 ? 0.0f : v[j] / sum;
@@ -1209,7 +1222,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh(
     }
     // from the first token that sees the wave's first position
     for (int x0 = max(p0 - new0, 0) * G / 16 * 16; x0 < R; x0 += 16) {
-      const int x = min(x0 + r, R - 1), tok = x / G, head = h * G + x % G;
+      const int x = min(x0 + r, R - 1), tok = pg_div(x, G), head = h * G + x - tok * G;
       const int lim = x0 + r < R ? new0 + tok : -1;
       const pg_q* qp = Q + (sq.first + tok) * qrow + head * qhead;
       PgQuery qf;
@@ -1315,8 +1328,8 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
 #pragma unroll
   for (int n = 0; n <= NL; ++n) {
     const int y = x0 + (n < NL ? r8 + RS * n : tid & 63);
-    tr[n] = y / G;
-    gr[n] = y % G;
+    tr[n] = pg_div(y, G);
+    gr[n] = y - tr[n] * G;
   }
   vh_u32x4 qr[NL];
   float zr = 0.0f;
@@ -1352,8 +1365,8 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
       put(buf ^ 1);
       if (x + 128 < x1) load();
     }
-    if (new0 + min(x + 63, R - 1) / G < p0) continue;              // no row sees the wave's positions
-    const bool part = p0 + 63 > new0 + x / G;                      // not all of them by every row
+    if (new0 + pg_div(min(x + 63, R - 1), G) < p0) continue;              // no row sees the wave's positions
+    const bool part = p0 + 63 > new0 + pg_div(x, G);                      // not all of them by every row
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float z = lz[buf][32 * u + r];
@@ -1369,7 +1382,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
         for (int i = 0; i < 2; ++i) s[i] = pg_mfma32(kf[i][k], qf, s[i]);
       }
       if (part) {
-        const int lim = new0 + min(x + 32 * u + r, R - 1) / G;
+        const int lim = new0 + pg_div(min(x + 32 * u + r, R - 1), G);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
