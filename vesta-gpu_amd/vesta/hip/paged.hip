@@ -712,8 +712,9 @@ PG_ATTN(pg_attn, 4)
 PG_ATTN(pg_attn8, 8)
 
 // Attention of many rows. A block makes 128 rows of one (sequence, key head),
-// 32 to a wave, over steps of 64 positions that its four waves share: key and value rows lie in LDS (double-buffered; the loads of the
-// step after next are in flight while one is used). Products in tiles of
+// 32 to a wave, over steps of 64 positions that its four waves share: key and
+// value rows lie in LDS (double-buffered; the loads of the step after next are
+// in flight while one is used). Products in tiles of
 // 32 x 32 x 16: lane 32 g + r holds row r, fold positions 8 g .. + 7 of an
 // operand; column r, rows 8 (i / 4) + 4 g + i % 4 of the result, i < 16. As in
 // pg_attn, scores are K Q^T, outputs V^T P^T, and the weights feed the second
@@ -1086,25 +1087,28 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 #endif
 
 // The parts of a tile of ROWS rows put together: a block of 512 threads makes
-// up to 16 rows of it, E / 4 lanes a row; where there are fewer rows their
-// parts are dealt to the lane groups left, whose results are added in order
-// (128 parts of four rows, one group a row: 60 us; dealt out: 4).
+// up to `each_rows` (1, 4 or 16) rows of it, E / 4 lanes a row; where there are
+// fewer rows their parts are dealt to the lane groups left, whose results are
+// added in order. What bounds it is the chain of loads (128 parts of four rows,
+// one group a row: 60 us; four rows a block, four groups a row: 11.7; a row a
+// block: 8.5).
 template <int ROWS, int STEP>
 __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, const int* __restrict__ lengths, int B,
                                              int cap, int M, int H, int G, int target, int least, int run, int limit,
-                                             const float* __restrict__ ws, pg_q* __restrict__ out, long orow,
+                                             int each_rows, const float* __restrict__ ws, pg_q* __restrict__ out, long orow,
                                              long ohead, float* __restrict__ lse) {
   constexpr int LR = PG_E / 4, NGR = 512 / LR;
   __shared__ float jm[NGR], js[NGR];
   __shared__ vh_f32x4 jv[512];
-  const int tid = threadIdx.x, c = tid % LR, grp = tid / LR, y0 = blockIdx.x % (ROWS / 16) * 16;
+  const int tid = threadIdx.x, c = tid % LR, grp = tid / LR, cut = ROWS / each_rows;
+  const int tile = pg_div(blockIdx.x, cut), y0 = ((int)blockIdx.x - tile * cut) * each_rows;
   PgWork wk;                                                       // grid: H (M G / ROWS + B) tiles or more
-  if (!pg_work<ROWS, STEP>(wk, blockIdx.x / (ROWS / 16), run, true, starts, lengths, B, M, cap, H, G, target, least, limit,
+  if (!pg_work<ROWS, STEP>(wk, tile, run, true, starts, lengths, B, M, cap, H, G, target, least, limit,
                            nullptr, 0))
     return;
   int last, steps, parts;
   pg_span<ROWS, STEP>(wk, G, last, steps, parts);
-  const int n = min(16, wk.R - wk.x0 - y0);                        // rows
+  const int n = min(each_rows, wk.R - wk.x0 - y0);                 // rows
   if (parts == 1 || n <= 0) return;
   const int n2 = n == 1 ? 1 : 1 << (32 - __builtin_clz(n - 1)), slices = NGR / n2;
   const int y = y0 + grp % n2, slice = grp / n2;
@@ -1178,9 +1182,10 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
 #define PG_JOIN(name, rows, step)                                                                                  \
   extern "C" __global__ __launch_bounds__(512) void name(                                                          \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int cap, int M, int H, int G,        \
-      int target, int least, int run, int limit, const float* __restrict__ ws, pg_q* __restrict__ out, long orow,  \
-      long ohead, float* __restrict__ lse) {                                                                       \
-    pg_join_body<rows, step>(starts, lengths, B, cap, M, H, G, target, least, run, limit, ws, out, orow, ohead, lse);        \
+      int target, int least, int run, int limit, int each_rows, const float* __restrict__ ws,                      \
+      pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse) {                                    \
+    pg_join_body<rows, step>(starts, lengths, B, cap, M, H, G, target, least, run, limit, each_rows, ws, out, orow, \
+                             ohead, lse);                                                                          \
   }
 PG_JOIN(pg_join, 16, PG_STEP)
 #if PG_KIND != PG_F32 || PG_E == 64

@@ -55,6 +55,7 @@ KINDS = ('f16', 'bf16', 'f32')         # kernels' queries: the cache's type, or 
 PAGE_MAX = 1 << 16
 STEP = {64: 64, 128: 32}               # positions of a wave's step in pg_attn, by width
 JOIN_BLOCK = 512
+JOIN_BLOCKS = 2048            # rows of a pg_join block: the fewest of 1, 4 and 16 with so many blocks
 
 # How a call's work is laid out; us a call (GPU time) on both sides of each rule.
 ROWS = 16                     # query rows of a pg_attn block; pg_wide's have 128
@@ -102,9 +103,9 @@ SIGNATURES = {
     'pg_attn': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllpp' + 'plp',
     'pg_attn2': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllpp' + 'plp',
     'pg_attn8': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllpp' + 'plp',
-    'pg_join': 'ppiiiiiiiiippllp',
+    'pg_join': 'ppiiiiiiiiiippllp',
     'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllppp',
-    'pg_wide_join': 'ppiiiiiiiiippllp',
+    'pg_wide_join': 'ppiiiiiiiiiippllp',
     'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiii',
     'pg_given': 'plppiiiippipii',
     'pg_weigh_wide': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiiiip',
@@ -418,9 +419,10 @@ class PagedCache:
                 else:
                     attn(*args, scores, pitch, self._err)
                 if target:
+                    cut = next((c for c in (1, 4) if tiles * rows // c <= JOIN_BLOCKS), 16)
                     (kn.pg_wide_join if wide else kn.pg_join)(
-                        tiles * (rows // 16), JOIN_BLOCK, stream, *seqs[4:], B, N * self.page, M, self.heads, G, target,
-                        least, run, blocks, base + ws, *to)
+                        tiles * (rows // cut), JOIN_BLOCK, stream, *seqs[4:], B, N * self.page, M, self.heads, G, target,
+                        least, run, blocks, cut, base + ws, *to)
             if weight is not None and B and So:
                 self._receive(kn, stream, (*qs, self._pools[0] + at), seqs, (B, M, G), most, wide, scale2, lse, scores,
                               pitch, (weight.data_ptr(), S, weight_out.data_ptr(), So))
