@@ -78,7 +78,9 @@ __device__ __forceinline__ vh_u32x4 pg_pack8(pg_f8 v) {
 // ---------------------------------------------------------------- append
 // New key and value rows into their pages, eight elements a thread (fp32 ones
 // rounded to the pool's type). Bound by memory: 12,900 rows of 8 heads of 128,
-// 106 MB read and written, 19.0 us (5.6 TB/s); eight rows 3.1 us, a launch.
+// 106 MB read and written, 18.8 us (5.6 TB/s); eight rows 2.8 us, a launch. The
+// stores pass by the cache: with other data in it the same call is 19.3 us, 23.7
+// with plain ones, and the attention that follows takes the same time.
 template <typename T>
 __device__ __forceinline__ vh_u32x4 pg_load8(const T* p);
 template <>
@@ -100,6 +102,9 @@ __device__ __forceinline__ void pg_append_body(const T* __restrict__ k, const T*
   const long at = (long)blockIdx.x * blockDim.x + threadIdx.x;
   const int i = (int)(at / per), c = (int)(at % per);
   if (i >= M) return;
+  const int h = c / (PG_E / 8), e = c % (PG_E / 8) * 8;
+  const vh_u32x4 kx = pg_load8(k + i * krow + h * khead + e), vx = pg_load8(v + i * vrow + h * vhead + e);
+  __builtin_amdgcn_sched_barrier(0);                    // in flight while the place is looked up
   // the last sequence whose first row is at or before i
   int lo = 0, hi = B;
   while (hi - lo > 1) {
@@ -112,11 +117,9 @@ __device__ __forceinline__ void pg_append_body(const T* __restrict__ k, const T*
   if (j >= 0 && j < s.count && pos >= 0) {
     const int page = table[(size_t)lo * N + (pos >> shift)];
     if ((unsigned)page < (unsigned)pages) {
-      const int h = c / (PG_E / 8), e = c % (PG_E / 8) * 8;
       const size_t to = ((((size_t)page << shift) + (pos & ((1 << shift) - 1))) * H + h) * PG_E + e;
-      const vh_u32x4 kx = pg_load8(k + i * krow + h * khead + e), vx = pg_load8(v + i * vrow + h * vhead + e);
-      *(vh_u32x4*)(kp + to) = kx;
-      *(vh_u32x4*)(vp + to) = vx;
+      __builtin_nontemporal_store(kx, (vh_u32x4*)(kp + to));
+      __builtin_nontemporal_store(vx, (vh_u32x4*)(vp + to));
     } else {
       bad |= PG_ERR_PAGE;
     }
@@ -1582,8 +1585,8 @@ extern "C" __global__ __launch_bounds__(1024) void pg_select(const float* __rest
 }
 
 // pg_move: the kept rows of all layers into the pages of the other table, 16
-// bytes of a key and of a value row a thread: 393 MB in 79 us (5.0 TB/s, a
-// copy's rate).
+// bytes of a key and of a value row a thread: 393 MB in 72 us (5.5 TB/s; 79 with
+// plain stores, which leave the rows in a cache that nothing reads them from).
 extern "C" __global__ __launch_bounds__(256) void pg_move(unsigned short* __restrict__ kp, unsigned short* __restrict__ vp,
                                                           int pages, int shift, const int* __restrict__ table, int N,
                                                           const int* __restrict__ to, int No,
@@ -1605,6 +1608,6 @@ extern "C" __global__ __launch_bounds__(256) void pg_move(unsigned short* __rest
   const size_t from = (pool + ((size_t)sp << shift) + (s & mask)) * per + c;
   const size_t into = (pool + ((size_t)dp << shift) + (d & mask)) * per + c;
   const vh_u32x4 kx = *((const vh_u32x4*)kp + from), vx = *((const vh_u32x4*)vp + from);
-  *((vh_u32x4*)kp + into) = kx;
-  *((vh_u32x4*)vp + into) = vx;
+  __builtin_nontemporal_store(kx, (vh_u32x4*)kp + into);
+  __builtin_nontemporal_store(vx, (vh_u32x4*)vp + into);
 }
