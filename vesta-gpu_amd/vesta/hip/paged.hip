@@ -737,7 +737,16 @@ PG_ATTN(pg_attn8, 8)
 // 27,001, 1.95 TFLOP in 2060-2110 us (925-945 TFLOP/s, 68% of a large library
 // product's rate). At width 64 the softmax on the vector units (about 1400
 // cycles a step against 512), and for short chunks the blocks' starts and ends
-// (10 us): six chunks of up to 512 tokens 27 us (200 TFLOP/s).
+// (4 us): six chunks of up to 512 tokens 25 us (220 TFLOP/s).
+// Waits for loads whose registers a loop reads: left to the first use inside it,
+// the wait is for all loads issued since as well, each time round (pg_wide, six
+// chunks of up to 512 tokens: 27.8 -> 25.8 us).
+template <int N>
+__device__ __forceinline__ void pg_here(vh_u32x4 (&f)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) asm volatile("" : "+v"(f[k]));
+}
+
 #if PG_KIND != PG_F32 || PG_E == 64
 #define PG_SLACK 8.0f
 #define PG_WROW (PG_E + 32)                // halves of a value row in LDS: 64 bytes past a multiple of all banks
@@ -875,6 +884,14 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     look(t0);
     load(t0);
     look(min(t0 + 1, t1 - 1));
+  }
+#if PG_KIND == PG_F32
+#pragma unroll
+  for (int k = 0; k < KS; ++k) pg_here(qf[k]);
+#else
+  pg_here(qf);
+#endif
+  if (t0 < t1) {
     put(t0);
     if (t0 + 1 < t1) {
       load(t0 + 1);
@@ -1362,8 +1379,10 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
     for (int n = 0; n < NL; ++n) lq[buf][(r8 + RS * n) * (CH + 1) + c8] = qr[n];
     if (tid < 64) lz[buf][tid] = zr;
   };
+  if (x0 < x1) load();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) pg_here(kf[i]);
   if (x0 < x1) {
-    load();
     put(0);
     if (x0 + 64 < x1) load();
   }

@@ -73,8 +73,8 @@ WIDE_FROM = {(64, False): (128, 64, 4096), (128, False): (64, 64, 1024), (64, Tr
 # 14.0, 16384 86.9 / 21.3; width 128 after 700 12.1 / 13.0, 1024 15.9 / 13.0, 16384 176 / 27.7; 64 sequences after up
 # to 900 (512 tiles, width 128) 31.5 / 36.1, 256 after up to 2000 (2048 tiles) 258 / 274, 64 after up to 4000 142 / 125.
 SPLIT = {64: 2048, 128: 1024}
-TARGET = 2048                 # parts in all, about (64 after up to 4000, 1024 / 1536 / 2048 / 3072: 131.0 / 128.5 / 125.3
-                              # / 126.3; 2 after 100003: 160.2 / 162.4 / 162.0 / 167.1) ...
+TARGET = 2048                 # parts in all, about (64 after up to 4000, 1024 / 1536 / 2048 / 4096: 132.2 / 127.4 / 125.5
+                              # / 131.1; 2 after 100003: 159.6 / 160.8 / 158.6 / 163.5) ...
 PART_STEPS = 8                # ... each of at least so many steps: two a wave
 # The same of pg_wide, where it has fewer tiles than fill the chip twice (two blocks a CU are resident).
 WIDE_SPLIT, WIDE_TARGET, WIDE_PART_STEPS = 1024, 512, 8
@@ -90,7 +90,7 @@ SCORES_MAX = 1 << 27          # scores (512 MB) that pg_attn keeps for the weigh
                               # made again by pg_weigh: 37)
 WEIGH = 128                   # positions of a pg_weigh block
 WEIGH_BLOCKS = 2048           # blocks of pg_weigh_wide, about, by slices of the rows (4 x 1999, 512 / 1024 / 1536 / 2048 /
-                              # 3072: 319 / 205 / 198 / 197 / 204)
+                              # 4096: 323 / 202 / 196 / 195 / 206)
 SELECT_FEW = 4096             # positions up to which pg_select has 256 threads, not 1024 (1152 times 1024: 13 / 38)
 ERRORS = {1: 'a page id outside the pool', 2: 'starts that do not ascend, or lie past the rows',
           4: 'a length past its table', 8: 'a sequence with more new tokens than `most`'}
