@@ -21,13 +21,17 @@ def _gpu():
         pytest.skip('no GPU')
 
 
-@pytest.fixture(params=('rule', 'rows of 16', 'rows of 128'))
+@pytest.fixture(params=('rule', 'rows of 16', 'rows of 128', 'rows of 256'))
 def blocks(request, monkeypatch):
     """Attention as the rule has it, or by the kernel for few or for many rows throughout."""
     from vesta import paged
     if request.param != 'rule':
-        monkeypatch.setattr(paged, 'FEW_ROWS', 0 if request.param == 'rows of 128' else 1 << 30)
+        monkeypatch.setattr(paged, 'FEW_ROWS', 1 << 30 if request.param == 'rows of 16' else 0)
         monkeypatch.setattr(paged, 'WIDE_FROM', WIDE)
+        monkeypatch.setattr(paged, 'TWICE', (1 << 30, 0, 0))
+    if request.param == 'rows of 256':               # of width 128, the others as 128
+        monkeypatch.setattr(paged, 'TWICE', (0, 0, 0))
+        monkeypatch.setattr(paged, 'WIDE_SPLIT', 1 << 30)
 
 
 def _gen(*seed):
@@ -559,16 +563,18 @@ def test_serving_run():
 @pytest.mark.parametrize('width', (64, 128))
 def test_every_variant(monkeypatch, dtype, query, width):
     """The same batch through every kernel that a rule may pick: two, four or eight waves, positions dealt to parts or not,
-    blocks of 16 or 128 rows, weights from kept scores or made again, in slices of the rows or not."""
+    blocks of 16, 128 or 256 rows, weights from kept scores or made again, in slices of the rows or not."""
     from vesta import paged
     b = Batch([1, 40, 1, 3], [700, 333, 2500, 3], 2, 2, width, 16, dtype, query)
     want, bound, got, gerr = b.want()
-    base = dict(EIGHT_WAVES=0, TWO_WAVES=0, WIDE_FROM=WIDE, SPLIT={64: 1 << 30, 128: 1 << 30}, WIDE_SPLIT=1 << 30, FEW_ROWS=1 << 20)
+    base = dict(EIGHT_WAVES=0, TWO_WAVES=0, WIDE_FROM=WIDE, TWICE=(1 << 30, 0, 0), SPLIT={64: 1 << 30, 128: 1 << 30},
+                WIDE_SPLIT=1 << 30, FEW_ROWS=1 << 20)
     parts = dict(SPLIT={64: 0, 128: 0}, WIDE_SPLIT=0)
     for kw in ({}, dict(EIGHT_WAVES=1 << 20), dict(TWO_WAVES=1 << 20), parts, {**parts, 'TARGET': 16, 'PART_STEPS': 1}, dict(SCORES_MAX=0),
                dict(FEW_ROWS=0), dict(FEW_ROWS=0, **parts), dict(FEW_ROWS=0, WEIGH_BLOCKS=1),
                dict(FEW_ROWS=0, WIDE_TARGET=1 << 12, WIDE_PART_STEPS=1, WEIGH_BLOCKS=1 << 20, **parts),
-               dict(RUN=1), dict(RUN=64, FEW_ROWS=0), dict(RUN_LONG=0, FEW_ROWS=0)):
+               dict(RUN=1), dict(RUN=64, FEW_ROWS=0), dict(RUN_LONG=0, FEW_ROWS=0), dict(TWICE=(0, 0, 0), FEW_ROWS=0),
+               dict(TWICE=(0, 0, 0), FEW_ROWS=0, WEIGH_BLOCKS=1 << 20)):
         for name, value in {**base, **kw}.items():
             monkeypatch.setattr(paged, name, value)
         out, w = b.attend(weight=torch.zeros_like(got, dtype=torch.float32))

@@ -54,7 +54,8 @@ def _rows(M, H, E=64, dtype=torch.float16):
 
 
 @pytest.mark.parametrize('bad', [dict(pages=0), dict(heads=0), dict(layers=0), dict(page=0), dict(page=48),
-                                 dict(page=1 << 17), dict(width=80), dict(dtype='f32'), dict(pages=1 << 25)])
+                                 dict(page=1 << 17), dict(width=80), dict(dtype='f32'), dict(pages=1 << 25),
+                                 dict(heads=1 << 25)])
 def test_shapes_refused(bad):
     with pytest.raises(ValueError):
         PagedCache(**{**dict(pages=4, heads=2), **bad})
@@ -118,6 +119,23 @@ def test_strides():
             c.attend(bad, table, starts, lengths)
         with pytest.raises(ValueError):
             c.attend(q, table, starts, lengths, out=bad)
+
+
+@pytest.mark.parametrize('width,rows,pages,kernel,threads', [
+    (64, 500, 20, 'pg_wide', 256), (128, 500, 20, 'pg_wide8', 512), (128, 500, 10, 'pg_wide', 256),
+    (128, 60, 40, 'pg_wide', 256)])
+def test_rows_of_a_block(width, rows, pages, kernel, threads):
+    """Many rows over many positions take blocks of 256 rows at width 128; each tile has a block of the grid."""
+    B, H, G = 32, 8, 4
+    c = _Dry(8, H, width=width)
+    table = torch.zeros(B, pages, dtype=torch.int32)
+    starts = torch.arange(B + 1, dtype=torch.int32) * rows
+    q = torch.zeros(B * rows, H * G, width, dtype=torch.float16)
+    c.attend(q, table, starts, _ints(*[64 * pages] * B), most=rows)
+    name, grid, block, vals = c.log[-1]
+    assert (name, block) == (kernel, threads)
+    tile = 64 * threads // 128
+    assert grid >= B * H * -(-rows * G // tile) and grid % 8 == 0
 
 
 def test_attend_refusals():

@@ -714,10 +714,19 @@ PG_ATTN(pg_attn2, 2)
 PG_ATTN(pg_attn, 4)
 PG_ATTN(pg_attn8, 8)
 
+// Waits for loads whose registers a loop reads: left to the first use inside it,
+// the wait is for all loads issued since as well, each time round (pg_wide, six
+// chunks of up to 512 tokens: 27.8 -> 25.8 us).
+template <int N>
+__device__ __forceinline__ void pg_here(vh_u32x4 (&f)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) asm volatile("" : "+v"(f[k]));
+}
+
 // Attention of many rows. A block makes 128 rows of one (sequence, key head),
-// 32 to a wave, over steps of 64 positions that its four waves share: key and
-// value rows lie in LDS (double-buffered; the loads of the step after next are
-// in flight while one is used). Products in tiles of
+// or 256 (W: its waves, 32 rows each), over steps of 64 positions that its
+// waves share: key and value rows lie in LDS (double-buffered; the loads of the
+// step after next are in flight while one is used). Products in tiles of
 // 32 x 32 x 16: lane 32 g + r holds row r, fold positions 8 g .. + 7 of an
 // operand; column r, rows 8 (i / 4) + 4 g + i % 4 of the result, i < 16. As in
 // pg_attn, scores are K Q^T, outputs V^T P^T, and the weights feed the second
@@ -731,22 +740,17 @@ PG_ATTN(pg_attn8, 8)
 // positions; they take this kernel at width 64 only (at 128 their planes leave
 // one block a CU, no faster than pg_attn: 32 x 768 1169 us against 1171).
 //
-// What bounds it: at width 128 the matrix cores (1024 cycles of a wave's step)
-// and LDS (each operand read serves 32 rows: 32 KB a wave's step, as many
-// cycles of the CU's LDS as of its matrix cores) about evenly: 4096 tokens after
-// 27,001, 1.95 TFLOP in 2060-2110 us (925-945 TFLOP/s, 68% of a large library
+// What bounds it at width 128: a wave's step takes 1024 cycles of the matrix
+// cores, 1000 to 1300 of the vector units (the softmax) and, as each operand
+// read from LDS serves 32 rows, 360 of the CU's LDS, 1440 for its four SIMDs.
+// Two blocks of four waves drift into step and do each in turn (4700 cycles for
+// a step of both; 4096 tokens after 27,001, 1.95 TFLOP in 2050-2100 us). In
+// blocks of eight, two groups of four waves, one of each on a SIMD, are kept
+// apart by barriers: while one has the matrix cores, the other has the vector
+// units. The same 4096 tokens in 1800 us (1085 TFLOP/s, 80% of a large library
 // product's rate). At width 64 the softmax on the vector units (about 1400
 // cycles a step against 512), and for short chunks the blocks' starts and ends
 // (4 us): six chunks of up to 512 tokens 25 us (220 TFLOP/s).
-// Waits for loads whose registers a loop reads: left to the first use inside it,
-// the wait is for all loads issued since as well, each time round (pg_wide, six
-// chunks of up to 512 tokens: 27.8 -> 25.8 us).
-template <int N>
-__device__ __forceinline__ void pg_here(vh_u32x4 (&f)[N]) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) asm volatile("" : "+v"(f[k]));
-}
-
 #if PG_KIND != PG_F32 || PG_E == 64
 #define PG_SLACK 8.0f
 #define PG_WROW (PG_E + 32)                // halves of a value row in LDS: 64 bytes past a multiple of all banks
@@ -759,25 +763,26 @@ __device__ __forceinline__ pg_f16v pg_mfma32(vh_u32x4 a, vh_u32x4 b, pg_f16v c) 
 #endif
 }
 
-extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
+template <int W>
+__device__ __forceinline__ void pg_wide_body(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,
     const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
     const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
     int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
     float* __restrict__ ws, unsigned* __restrict__ err) {
-  constexpr int KS = PG_E / 16, DT = PG_E / 32, CH = PG_E / 8, NL = 64 * CH / 256;   // k-steps, dim tiles, 16-byte
-  constexpr int RS = 256 / CH;                                     // pieces of a row; a thread's pieces and rows apart
+  constexpr int KS = PG_E / 16, DT = PG_E / 32, CH = PG_E / 8;     // k-steps, dim tiles, 16-byte pieces of a row
+  constexpr int TILE = 32 * W, RS = 64 * W / CH, NL = 64 / RS;     // rows; a thread's rows of a step apart, its pieces
   __shared__ __attribute__((aligned(16))) vh_u32x4 lk[2][64 * (CH + 1)];
   __shared__ __attribute__((aligned(16))) unsigned short lv[2][64 * PG_WROW];
   __shared__ int lwild[2];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
   PgWork wk;
-  if (!pg_work<128, 64>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, limit, err,
+  if (!pg_work<TILE, 64>(wk, blockIdx.x, run, false, starts, lengths, B, M, N << shift, H, G, target, least, limit, err,
                         most))
     return;
   int last, steps, parts;
-  pg_span<128, 64>(wk, G, last, steps, parts);
+  pg_span<TILE, 64>(wk, G, last, steps, parts);
   if (wk.part >= parts) return;
   const PgSeq sq = wk.sq;
   const int R = wk.R, x0 = wk.x0 + 32 * wave, h = wk.h, new0 = sq.len - sq.count;
@@ -832,23 +837,32 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     for (int n = 0; n < NL; ++n) page[n] = tb[min(64 * t + r8 + RS * n, last) >> shift];
   };
   vh_u32x4 kr[NL], vr[NL];
-  auto load = [&](int t) {
+  unsigned at[NL];
+  auto where = [&](int t) {
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
       const bool in = (unsigned)page[n] < (unsigned)pages;
       if (!in) bad = PG_ERR_PAGE;
-      const size_t at = (((unsigned)(in ? page[n] : 0) << shift)
-                         + (unsigned)(min(64 * t + r8 + RS * n, last) & ((1 << shift) - 1))) * rowlen;
-      kr[n] = ld16(kh + at);
-      vr[n] = ld16(vh + at);
+      at[n] = ((unsigned)(in ? page[n] : 0) << shift) + (unsigned)(min(64 * t + r8 + RS * n, last) & ((1 << shift) - 1));
     }
   };
+  auto load_k = [&]() {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) kr[n] = ld16(kh + (size_t)at[n] * (unsigned)rowlen);
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) vr[n] = ld16(vh + (size_t)at[n] * (unsigned)rowlen);
+  };
   // Key rows are 16 bytes past a multiple of all banks apart, so that a column
-  // of their pieces falls on all of them. Values past the last position are 0,
-  // and where some row sees a step in part so are those that are not finite
-  // (0 * inf); that there are such is noted.
-  auto put = [&](int t) {
-    const int buf = t & 1;
+  // of their pieces falls on all of them.
+  auto put_k = [&](int t) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) lk[t & 1][(r8 + RS * n) * (CH + 1) + c8] = kr[n];
+  };
+  // Values past the last position are 0, and where some row sees a step in part
+  // so are those that are not finite (0 * inf); that there are such is noted.
+  auto put_v = [&](int t) {
     if (64 * t + 63 > last) {
 #pragma unroll
       for (int n = 0; n < NL; ++n)
@@ -860,17 +874,13 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 #pragma unroll
       for (int n = 0; n < NL; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
       if (any) {
-        lwild[buf] = t + 1;
+        lwild[t & 1] = t + 1;
 #pragma unroll
         for (int n = 0; n < NL; ++n) vr[n] = pg_tame(vr[n]);
       }
     }
 #pragma unroll
-    for (int n = 0; n < NL; ++n) {
-      const int row = r8 + RS * n;
-      lk[buf][row * (CH + 1) + c8] = kr[n];
-      *(vh_u32x4*)(lv[buf] + row * PG_WROW + 8 * c8) = vr[n];
-    }
+    for (int n = 0; n < NL; ++n) *(vh_u32x4*)(lv[t & 1] + (r8 + RS * n) * PG_WROW + 8 * c8) = vr[n];
   };
   pg_f16v o[DT];
 #pragma unroll
@@ -880,54 +890,33 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
   float m2 = -INFINITY, sum = 0.0f;
   if (tid < 2) lwild[tid] = 0;
   vh_lds_sync();                                                   // noted as none before a step may be noted
-  if (t0 < t1) {
-    look(t0);
-    load(t0);
-    look(min(t0 + 1, t1 - 1));
-  }
-#if PG_KIND == PG_F32
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s4 lds4;
+  auto value = [&](int t, int i, int k, int d) {
+    const unsigned short* vb = lv[t & 1] + (32 * i + 16 * k + 4 * g + ((lane & 15) >> 2)) * PG_WROW + 32 * d
+                               + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vb);
+    const s4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vb + 8 * PG_WROW));
+    return __builtin_bit_cast(vh_u32x4, __builtin_shufflevector(a, e, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  auto sees = [&](int t) { return x0 < R && 64 * t <= wlast; };    // whether the wave has a row that sees step t
+  // the values of a step that are not finite, to the rows that see them
+  auto add_wild = [&](int t) {
+#pragma nounroll
+    for (int s = 64 * t; s <= min(64 * t + 63, last); ++s)
 #pragma unroll
-  for (int k = 0; k < KS; ++k) pg_here(qf[k]);
-#else
-  pg_here(qf);
-#endif
-  if (t0 < t1) {
-    put(t0);
-    if (t0 + 1 < t1) {
-      load(t0 + 1);
-      look(min(t0 + 2, t1 - 1));
-    }
-  }
-  for (int t = t0; t < t1; ++t) {
-    vh_lds_sync();                       // step t is staged; the other buffer's step is read
-    if (t + 1 < t1) {
-      put(t + 1);
-      if (t + 2 < t1) {
-        load(t + 2);
-        look(min(t + 3, t1 - 1));
-      }
-    }
-    const int p0 = 64 * t, buf = t & 1;
-    if (x0 >= R || p0 > wlast) continue;
-    const vh_u32x4* K = lk[buf];
-    const unsigned short* V = lv[buf];
-    const bool seen = p0 + 63 > wfirst;                            // not the whole step by every row
-    const bool wild = lwild[buf] == t + 1;                         // added back below
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s4 lds4;
-    auto value = [&](int i, int k, int d) {
-      const unsigned short* vb = V + (32 * i + 16 * k + 4 * g + ((lane & 15) >> 2)) * PG_WROW + 32 * d
-                                 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)vb);
-      const s4 e = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vb + 8 * PG_WROW));
-      return __builtin_shufflevector(a, e, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float v = pg_taken(vp + h * PG_E, rowlen, tb, pages, shift, s, 32 * d + 8 * (j >> 2) + 4 * g + (j & 3));
+          o[d][j] += s <= lim ? v : 0.0f;
+        }
+  };
 #if PG_KIND != PG_F32
-    // the matrix cores' share of a step goes before the other block's softmax
-    // (4096 tokens after 27001, width 128: 2147 -> 2050 us; width 64, where the
-    // softmax is most of a step, 27 -> 30)
-    if (PG_E == 128) __builtin_amdgcn_s_setprio(1);
-    pg_f16v s[2];
+  pg_f16v s[2];
+  vh_u32x4 pf[2][2];
+  auto scores = [&](int t) {
+    const vh_u32x4* K = lk[t & 1];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -936,8 +925,10 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
     for (int k = 0; k < KS; ++k)
 #pragma unroll
       for (int i = 0; i < 2; ++i) s[i] = pg_mfma32(K[(32 * i + r) * (CH + 1) + 2 * k + g], qf[k], s[i]);
-    if (PG_E == 128) __builtin_amdgcn_s_setprio(0);
-    if (seen) {
+  };
+  auto soften = [&](int t) {
+    const int p0 = 64 * t;
+    if (p0 + 63 > wfirst) {                                        // not the whole step by every row
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -950,7 +941,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const float a = s[0][j], e = s[1][j];                        // (a bit_cast of a vector's element takes its first)
-      bi = max(bi, max(__builtin_bit_cast(int, a), __builtin_bit_cast(int, e)));
+      bi = max(max(bi, __builtin_bit_cast(int, a)), __builtin_bit_cast(int, e));
     }
     float bm = __builtin_bit_cast(float, bi);
     if (__any(bi < 0)) {
@@ -971,7 +962,6 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
         for (int j = 0; j < 16; ++j) o[d][j] *= c;
     }
     const float ref = m2 == -INFINITY ? 0.0f : m2;                 // no score above -inf yet: all weights 0
-    vh_u32x4 pf[2][2];
     float ts[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -984,106 +974,217 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
         pf[i][k] = pg_pack8(pg_f8{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]});
       }
     sum += (ts[0] + ts[1]) + (ts[2] + ts[3]);
-    if (PG_E == 128) __builtin_amdgcn_s_setprio(1);
+  };
+  auto gather = [&](int t) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = pg_mfma32(__builtin_bit_cast(vh_u32x4, value(i, k, d)), pf[i][k], o[d]);
-    if (PG_E == 128) __builtin_amdgcn_s_setprio(0);
+        for (int d = 0; d < DT; ++d) o[d] = pg_mfma32(value(t, i, k, d), pf[i][k], o[d]);
+  };
+#endif
+  if (t0 < t1) {
+    look(t0);
+    where(t0);
+    load_k();
+    load_v();
+    look(min(t0 + 1, t1 - 1));
+  }
+#if PG_KIND == PG_F32
+#pragma unroll
+  for (int k = 0; k < KS; ++k) pg_here(qf[k]);
 #else
-#pragma nounroll
-    for (int i = 0; i < 2; ++i) {
-      pg_f16v hi, lo;
+  pg_here(qf);
+#endif
+#if PG_KIND != PG_F32
+  // Two groups of four waves take turns. In its turn at the products a wave
+  // also puts its share of the next step's keys and of this one's values into
+  // LDS, where nobody reads them before both groups have done so.
+  if constexpr (W == 8) {
+    unsigned av[NL];                     // rows of the values to be asked for next: the keys' of a step before
+    auto place = [&](int t) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) hi[j] = lo[j] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const vh_u32x4 kf = K[(32 * i + r) * (CH + 1) + 2 * k + g];
-        hi = pg_mfma32(kf, qf[k][0], hi);
-        lo = pg_mfma32(kf, qf[k][1], lo);
-        lo = pg_mfma32(kf, qf[k][2], lo);
+      for (int n = 0; n < NL; ++n) av[n] = at[n];
+      if (t < t1) {
+        where(t);
+        look(min(t + 1, t1 - 1));
       }
-      float s[16], fin = 0.0f;
+    };
+    auto ask = [&](int t) {              // the values of step t, the keys of the next
+      if (t >= t1) return;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        s[j] = vh_hilo(hi[j], lo[j]);
-        fin = fmaf(hi[j], 0.0f, fin);
-      }
-      if (__any(fin != fin)) {                                     // as in pg_scores
+      for (int n = 0; n < NL; ++n) vr[n] = ld16(vh + (size_t)av[n] * (unsigned)rowlen);
+      if (t + 1 < t1) load_k();
+    };
+    auto stage = [&](int t) {
+      if (t + 1 < t1) put_k(t + 1);
+      put_v(t);
+    };
+    if (t0 < t1) {
+      put_k(t0);
+      place(t0 + 1);
+      if (t0 + 1 < t1) load_k();         // (its values are there)
+      place(t0 + 2);
+    }
+    vh_lds_sync();
+    if (wave >= 4) vh_lds_sync();        // half a step behind
+    if (t0 < t1) {
+      stage(t0);
+      if (sees(t0)) scores(t0);
+      vh_lds_sync();
+    }
+    for (int t = t0; t < t1; ++t) {
+      ask(t + 1);
+      if (sees(t)) soften(t);
+      place(t + 3);
+      vh_lds_sync();
+      __builtin_amdgcn_s_setprio(1);     // (1935 us without)
+      if (t + 1 < t1) stage(t + 1);
+      const int noted = lwild[t & 1];
+      if (sees(t)) {
+        gather(t);
+        // LDS reads run ahead of the products that take them (1920 us as the compiler has it)
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float acc = 0.0f;
-#pragma nounroll
-          for (int c = 0; c < CH; ++c) {
-            float kv[8];
-            unpack8(K[(32 * i + 8 * (j >> 2) + 4 * g + (j & 3)) * (CH + 1) + c], kv);
-#pragma unroll
-            for (int d = 0; d < 8; ++d) acc = fmaf(qp[8 * c + d], kv[d], acc);
-          }
-          if (!(__builtin_fabsf(hi[j]) < INFINITY)) s[j] = acc;
+        for (int n = 0; n < 13; ++n) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+        if (noted == t + 1) add_wild(t);
       }
-      if (seen) {
+      if (t + 1 < t1 && sees(t + 1)) {
+        scores(t + 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = p0 + 32 * i + 8 * (j >> 2) + 4 * g + (j & 3) <= lim ? s[j] : -INFINITY;
-      }
-      float bm = s[0];
-#pragma unroll
-      for (int j = 1; j < 16; ++j) bm = fmaxf(bm, s[j]);
-      bm = vh_pair32(bm, op_max);
-      const float n2 = fmaxf(m2, bm * k2);
-      const float ref = n2 == -INFINITY ? 0.0f : n2;               // no score above -inf yet: all weights 0
-      const float c = __builtin_amdgcn_exp2f(m2 - ref);
-      m2 = n2;
-      vh_u32x4 pf[2][3];
-      float ts[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * k + j], k2, -ref));
-        ts[k] = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-        pg_split(w, pf[k]);
-      }
-      sum = fmaf(sum, c, ts[0] + ts[1]);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        pg_f16v th, tw;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) th[j] = tw[j] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const vh_u32x4 vf = __builtin_bit_cast(vh_u32x4, value(i, k, d));
-          th = pg_mfma32(vf, pf[k][0], th);
-          tw = pg_mfma32(vf, pf[k][1], tw);
-          tw = pg_mfma32(vf, pf[k][2], tw);
+        for (int n = 0; n < 12; ++n) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[d][j] = fmaf(o[d][j], c, vh_hilo(th[j], tw[j]));
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      if (t + 1 < t1) vh_lds_sync();
+    }
+    if (wave < 4) vh_lds_sync();         // as many barriers as the other group
+  }
+#endif
+  if constexpr (W == 4) {
+    if (t0 < t1) {
+      put_k(t0);
+      put_v(t0);
+      if (t0 + 1 < t1) {
+        where(t0 + 1);
+        load_k();
+        load_v();
+        look(min(t0 + 2, t1 - 1));
       }
     }
-#endif
-    if (wild) {
+    for (int t = t0; t < t1; ++t) {
+      vh_lds_sync();                       // step t is staged; the other buffer's step is read
+      if (t + 1 < t1) {
+        put_k(t + 1);
+        put_v(t + 1);
+        if (t + 2 < t1) {
+          where(t + 2);
+          load_k();
+          load_v();
+          look(min(t + 3, t1 - 1));
+        }
+      }
+      if (!sees(t)) continue;
+      const int noted = lwild[t & 1];
+#if PG_KIND != PG_F32
+      scores(t);
+      soften(t);
+      gather(t);
+#else
+      const int p0 = 64 * t;
+      const bool seen = p0 + 63 > wfirst;
+      const vh_u32x4* K = lk[t & 1];
 #pragma nounroll
-      for (int s = p0; s <= min(p0 + 63, last); ++s)
+      for (int i = 0; i < 2; ++i) {
+        pg_f16v hi, lo;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int j = 0; j < 16; ++j) hi[j] = lo[j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const vh_u32x4 kf = K[(32 * i + r) * (CH + 1) + 2 * k + g];
+          hi = pg_mfma32(kf, qf[k][0], hi);
+          lo = pg_mfma32(kf, qf[k][1], lo);
+          lo = pg_mfma32(kf, qf[k][2], lo);
+        }
+        float s[16], fin = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          s[j] = vh_hilo(hi[j], lo[j]);
+          fin = fmaf(hi[j], 0.0f, fin);
+        }
+        if (__any(fin != fin)) {                                     // as in pg_scores
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float v = pg_taken(vp + h * PG_E, rowlen, tb, pages, shift, s, 32 * d + 8 * (j >> 2) + 4 * g + (j & 3));
-            o[d][j] += s <= lim ? v : 0.0f;
+            float acc = 0.0f;
+#pragma nounroll
+            for (int c = 0; c < CH; ++c) {
+              float kv[8];
+              unpack8(K[(32 * i + 8 * (j >> 2) + 4 * g + (j & 3)) * (CH + 1) + c], kv);
+#pragma unroll
+              for (int d = 0; d < 8; ++d) acc = fmaf(qp[8 * c + d], kv[d], acc);
+            }
+            if (!(__builtin_fabsf(hi[j]) < INFINITY)) s[j] = acc;
           }
+        }
+        if (seen) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[j] = p0 + 32 * i + 8 * (j >> 2) + 4 * g + (j & 3) <= lim ? s[j] : -INFINITY;
+        }
+        float bm = s[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) bm = fmaxf(bm, s[j]);
+        bm = vh_pair32(bm, op_max);
+        const float n2 = fmaxf(m2, bm * k2);
+        const float ref = n2 == -INFINITY ? 0.0f : n2;               // no score above -inf yet: all weights 0
+        const float c = __builtin_amdgcn_exp2f(m2 - ref);
+        m2 = n2;
+        vh_u32x4 pf[2][3];
+        float ts[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * k + j], k2, -ref));
+          ts[k] = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+          pg_split(w, pf[k]);
+        }
+        sum = fmaf(sum, c, ts[0] + ts[1]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          pg_f16v th, tw;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) th[j] = tw[j] = 0.0f;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const vh_u32x4 vf = value(t, i, k, d);
+            th = pg_mfma32(vf, pf[k][0], th);
+            tw = pg_mfma32(vf, pf[k][1], tw);
+            tw = pg_mfma32(vf, pf[k][2], tw);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[d][j] = fmaf(o[d][j], c, vh_hilo(th[j], tw[j]));
+        }
+      }
+#endif
+      if (noted == t + 1) add_wild(t);
     }
   }
   if (__any(bad != 0) && lane == 0) pg_raise(err, PG_ERR_PAGE);
   if (!live) return;
   sum = vh_pair32(sum, op_sum);
-  const bool whole = parts == 1;
+  const bool whole = W == 8 || parts == 1;                         // (eight waves are not launched for parts)
   const float inv = 1.0f / sum;        // (exact enough for results of 16 bits: a division each was 0.5 us of a block's end)
   pg_q* op = out + (sq.first + tok) * orow + head * ohead;
-  float* wp = ws + (size_t)wk.at * PG_WS(128);
+  float* wp = ws + (size_t)wk.at * PG_WS(TILE);
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -1093,17 +1194,31 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_wide(
       for (int j = 0; j < 4; ++j)
         v[j] = !whole ? o[d][4 * i + j] : lim < 0 ? 0.0f : PG_KIND == PG_F32 ? o[d][4 * i + j] / sum : o[d][4 * i + j] * inv;
       if (whole) pg_store4(op + 32 * d + 8 * i + 4 * g, v);
-      else *(vh_f32x4*)(wp + 256 + (32 * wave + r) * PG_E + 32 * d + 8 * i + 4 * g) = vh_f32x4{v[0], v[1], v[2], v[3]};
+      else *(vh_f32x4*)(wp + 2 * TILE + (32 * wave + r) * PG_E + 32 * d + 8 * i + 4 * g) = vh_f32x4{v[0], v[1], v[2], v[3]};
     }
   if (g == 0) {
     if (!whole) {
       wp[32 * wave + r] = m2;
-      wp[128 + 32 * wave + r] = sum;
+      wp[TILE + 32 * wave + r] = sum;
     } else if (lse) {
       lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : m2 + __builtin_amdgcn_logf(sum);
     }
   }
 }
+#define PG_WIDE(name, waves)                                                                                       \
+  extern "C" __global__ __launch_bounds__(64 * waves, 2) void name(                                                \
+      const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,                    \
+      const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,           \
+      const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target,     \
+      int least, int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead,        \
+      float* __restrict__ lse, float* __restrict__ ws, unsigned* __restrict__ err) {                               \
+    pg_wide_body<waves>(Q, qrow, qhead, kp, vp, pages, shift, table, N, starts, lengths, B, M, H, G, target,       \
+                        least, run, limit, most, scale2, out, orow, ohead, lse, ws, err);                          \
+  }
+PG_WIDE(pg_wide, 4)
+#if PG_KIND != PG_F32 && PG_E == 128
+PG_WIDE(pg_wide8, 8)
+#endif
 #endif
 
 // The parts of a tile of ROWS rows put together: a block of 512 threads makes

@@ -61,12 +61,13 @@ JOIN_BLOCKS = 2048            # rows of a pg_join block: the fewest of 1, 4 and 
 ROWS = 16                     # query rows of a pg_attn block; pg_wide's have 128
 FEW_ROWS = 32                 # a sequence of up to so many rows (new tokens times heads of a group) is pg_attn's
 # More are pg_wide's, by (width, whether the queries are f32), from so many of its tiles on, or from so many rows a
-# sequence where the tables have more than so many positions. pg_attn / pg_wide, width 64, 16 bits: 8 x 128 after 900
-# (96 tiles) 25.7 / 28.9, 16 x 128 (192) 42.1 / 30.5, 1 x 64 after 8000 22.2 / 20.9, 1 x 256 52.2 / 28.1; width 128,
-# four heads a group: 1 x 128 (32 tiles) 7.0 / 12.0, 4 x 128 after 500 (128) 33.3 / 26.8, 2 x 16 after 30000 91 / 59;
-# f32, width 64: 16 x 128 after 900 53.7 / 55.3, 24 x 128 76.7 / 75.2, 32 x 768 321 / 178, 1 x 64 after 8000 25.7 /
+# sequence where the tables have more than so many positions. pg_attn / pg_wide, width 64, 16 bits: 8 x 64 after 900
+# (96 tiles) 16.7 / 24.8, 8 x 128 after 500 20.1 / 17.9, 16 x 128 after 500 (192) 30.7 / 18.6, 1 x 64 after 8000 28.6 /
+# 29.0, 1 x 256 56.4 / 31.5; width 128, four heads a group: 1 x 128 (32 tiles) 7.9 / 10.9, 2 x 128 after 500 (64) 20.9 /
+# 23.8, 4 x 128 (128) 34.5 / 24.5, 4 x 16 after 900 21.7 / 27.1, 1 x 64 after 2000 29.3 / 27.9, 2 x 16 after 30000 99.8 /
+# 56.5; f32, width 64: 16 x 128 after 900 53.7 / 55.3, 24 x 128 76.7 / 75.2, 32 x 768 321 / 178, 1 x 64 after 8000 25.7 /
 # 33.5, 1 x 256 63.3 / 48.6; f32, width 128: even at best, so it is not made.
-WIDE_FROM = {(64, False): (128, 64, 4096), (128, False): (64, 64, 1024), (64, True): (256, 256, 4096),
+WIDE_FROM = {(64, False): (128, 64, 4096), (128, False): (64, 64, 1536), (64, True): (256, 256, 4096),
              (128, True): (1 << 30, 1 << 30, 0)}
 # A tile's positions go to several blocks, and a second launch puts them together, where the tables have more than
 # SPLIT positions times tiles / 256. One token, 12 heads, whole / in parts: width 64 after 1024 9.6 / 14.0, 2048 15.4 /
@@ -78,6 +79,11 @@ TARGET = 2048                 # parts in all, about (64 after up to 4000, 1024 /
 PART_STEPS = 8                # ... each of at least so many steps: two a wave
 # The same of pg_wide, where it has fewer tiles than fill the chip twice (two blocks a CU are resident).
 WIDE_SPLIT, WIDE_TARGET, WIDE_PART_STEPS = 1024, 512, 8
+# Width 128, 16 bits, a tile's positions in one block: pg_wide8 (256 rows a block) from so many rows a sequence,
+# positions of the tables and tiles of 128 rows on (128 / 256 rows a block: 64 x 32 tokens of four heads after 900, 128
+# rows a sequence, 56.9 / 69.8; 4 x 600 34.1 / 38.3; 8 x 128 after 500, 256 tiles, 26.7 / 30.1; 32 x 700 266.8 / 249.6; 16
+# x 128 after 900, 512 tiles, 53.8 / 48.4; 2 x 8192 1254 / 1092; 4096 after 27001 2070 / 1810).
+TWICE = 256, 768, 512
 EIGHT_WAVES = 256             # pg_attn of up to so many tiles (a block a CU) in blocks of eight waves (one token after
                               # 700, four / eight waves: 11.1 / 10.4; 8 x 128, 864 tiles: 13.4 / 19.1) ...
 TWO_WAVES = 8                 # ... and of more, where the tables have up to so many steps, of two (f32, four / two waves:
@@ -105,6 +111,7 @@ SIGNATURES = {
     'pg_attn8': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllpp' + 'plp',
     'pg_join': 'ppiiiiiiiiiippllp',
     'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllppp',
+    'pg_wide8': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllppp',
     'pg_wide_join': 'ppiiiiiiiiiippllp',
     'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiii',
     'pg_given': 'plppiiiippipii',
@@ -118,9 +125,9 @@ SIGNATURES = {
 def kernels_of(width: int, kind: str) -> set:
     """The kernels of a module: attention of many rows and its weights are not made for f32 queries, but the former at
     width 64."""
-    without = set()
+    without = set() if (width, kind) in ((128, 'f16'), (128, 'bf16')) else {'pg_wide8'}
     if kind == 'f32':
-        without = {'pg_weigh_wide', 'pg_total'} | ({'pg_wide', 'pg_wide_join'} if width != 64 else set())
+        without |= {'pg_weigh_wide', 'pg_total'} | ({'pg_wide', 'pg_wide_join'} if width != 64 else set())
     return set(SIGNATURES) - without
 
 
@@ -231,6 +238,8 @@ class PagedCache:
             raise ValueError(f'pages of {page} rows: a power of two up to {PAGE_MAX}')
         if min(pages, heads, layers) < 1:
             raise ValueError(f'{pages} pages, {heads} heads, {layers} layers: one at least of each')
+        if heads * width >= 1 << 31:
+            raise ValueError(f'{heads} heads of {width}: rows of fewer than 2^31 values')
         if pages * page >= 1 << 31:
             raise ValueError(f'{pages} pages of {page} rows: fewer than 2^31 rows a layer')
         self.pages, self.heads, self.width, self.layers, self.page = pages, heads, width, layers, page
@@ -402,7 +411,7 @@ class PagedCache:
                     scores = 4 * floats
                     floats += M * Hq * pitch
             if M and B:
-                attn, block, rows, tiles, target, blocks, least, run = self._layout(kn, B, N, M, G, wide)
+                attn, block, rows, tiles, target, blocks, least, run = self._layout(kn, B, N, M, G, wide, most)
                 ws = 4 * floats
                 floats += blocks * rows * (self.width + 2) if target else 0
             if floats:
@@ -436,7 +445,7 @@ class PagedCache:
         return most * G > FEW_ROWS and (self.heads * max(B, M * G // 128) >= tiles
                                         or most * G >= rows and N * self.page > positions)
 
-    def _layout(self, kn, B, N, M, G, wide):
+    def _layout(self, kn, B, N, M, G, wide, most):
         """The kernel and threads of a block, its rows, the tiles of so many rows there can be, the parts asked for (0:
         one a tile) and those there can be, the least steps of one, the blocks to an XCD in turn."""
         positions = N * self.page
@@ -452,8 +461,12 @@ class PagedCache:
         run = RUN
         if wide:
             attn, block = kn.pg_wide, BLOCK
-            if M * G >= 128 * RUN_LONG * B:
-                run = M * G // (128 * B)
+            if self.width == 128 and target == 0 and all(n >= m for n, m in zip((most * G, positions, tiles), TWICE)):
+                attn, block, rows = kn.pg_wide8, 2 * BLOCK, 256
+                tiles = self.heads * (M * G // rows + B)
+                blocks = tiles + 64
+            if M * G >= rows * RUN_LONG * B:
+                run = M * G // (rows * B)
         elif target:
             attn, block = kn.pg_attn, BLOCK
         elif tiles <= EIGHT_WAVES:
