@@ -189,6 +189,21 @@ def test_attend(blocks, dtype, query, width, group, page, shape):
 
 
 @pytest.mark.parametrize('dtype,query', KINDS)
+@pytest.mark.parametrize('width', (64, 128))
+def test_sequences_of_many_tiles(blocks, dtype, query, width):
+    """Tiles of several sequences in the order of their steps: ragged ones, one that begins long before its rows, one
+    without any, one whose first rows are padding, one of padding alone."""
+    b = Batch([650, 0, 333, 701, 1, 290, 90], [650, 50, 1200, 500, 2000, 290, 0], 2, 2, width, 16, dtype, query)
+    want, bound, got, gerr = b.want()
+    for most in (None, 701):
+        out, w = b.attend(most=most, weight=torch.zeros_like(got, dtype=torch.float32))
+        _close(out, want, bound)
+        _close(w, got, gerr)
+        _close(b.attend(most=most), want, bound)
+    b.cache.check()
+
+
+@pytest.mark.parametrize('dtype,query', KINDS)
 def test_attend_long(blocks, dtype, query):
     """Contexts of some thousands, few and many sequences, and a scale of the caller's."""
     for counts, lengths, heads, group in (([1], [5000], 1, 1), ([1, 1], [3001, 64], 4, 4), ([7], [4100], 2, 2),

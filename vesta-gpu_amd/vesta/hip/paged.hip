@@ -423,6 +423,43 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
     if (at == B * H && threadIdx.x < 64) pg_faults(starts, lengths, B, M, cap, most, err);
     return false;
   }
+  // Where sequences have several tiles of many rows, all tiles longest first: a
+  // CU has few of them, and a long one that starts late is waited for (sequence
+  // by sequence / longest first: 16 x 1024 of 12 heads of 64 68 / 50 us, 32 x
+  // 700 63 / 57; four tiles a sequence: 6 x up to 512 26.0 / 28.0).
+  if (ROWS >= 128 && !joined && target == 0 && run < PG_RUN_LONG && B <= 64 && most * G >= 5 * ROWS) {
+    if (block == 0 && threadIdx.x < 64) pg_faults(starts, lengths, B, M, cap, most, err);
+    PgSeq s = {};
+    if (lane < B) s = pg_seq(starts, lengths, lane, M, cap);
+    const int R = s.count * G, T = (R + ROWS - 1) / ROWS, first = s.len - s.count;
+    const int at = pg_deal(block, run), x = pg_div(at, H);
+    if (x >= __builtin_amdgcn_readlane(pg_scan(T), 63) || at >= limit) return false;
+    auto longer = [&](int n) -> int {                              // the lane's tiles of n steps or more
+      const long y = ((long)(n - 1) * STEP - first) * G;           // their last row is y or later
+      return n <= 0 || y < 0 ? T : y >= R ? 0 : T - (int)y / ROWS;
+    };
+    int lo = 0, hi = cap / STEP + 2;                               // more than x tiles have lo steps, not so hi
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__builtin_amdgcn_readlane(pg_scan(longer(mid)), 63) > x) lo = mid; else hi = mid;
+    }
+    const int a = longer(hi), n = longer(lo) - a, sum = pg_scan(n);
+    const int rest = x - __builtin_amdgcn_readlane(pg_scan(a), 63);
+    const int l = __builtin_ctzll(__ballot(sum > rest));
+    o.b = l;
+    o.h = at - x * H;
+    o.sq.first = __builtin_amdgcn_readlane(s.first, l);
+    o.sq.count = __builtin_amdgcn_readlane(s.count, l);
+    o.sq.len = __builtin_amdgcn_readlane(s.len, l);
+    o.tiles = __builtin_amdgcn_readlane(T, l);
+    o.tile = o.tiles - 1 - __builtin_amdgcn_readlane(a, l) - (rest - __builtin_amdgcn_readlane(sum - n, l));
+    o.each = 0x7fffffff;
+    o.part = 0;
+    o.at = at;
+    o.R = o.sq.count * G;
+    o.x0 = o.tile * ROWS;
+    return true;
+  }
   o.each = pg_each<ROWS, STEP>(starts, lengths, B, M, cap, H, G, target, least);
   auto mine = [&](int b, PgSeq& s, int& tiles, int& parts) -> int {
     tiles = parts = 0;
