@@ -1595,15 +1595,20 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
         for (int j = 0; j < 16; ++j) acc[i][j] += __builtin_amdgcn_exp2f(fmaf(s[i][j], scale2, -z));
     }
   }
-  // over the rows: lane 32 g + r keeps position 32 (r / 16) + 8 (r % 16 / 4) + 4 g + r % 4
-  float w = 0.0f;
+  // Over the rows: lane 32 g + r keeps position 32 (r / 16) + 8 (r % 16 / 4) + 4 g + r % 4.
+  // Lanes that differ in a bit of r each take over the sums that differ in it
+  // alike, 31 exchanges (a sum at a time: 160).
+  float sums[32];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int k = 0; k < 32; ++k) sums[k] = acc[k >> 4][k & 15];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float v = group_red_sum(acc[i][j], 32);
-      if (r == 16 * i + j) w = v;
+  for (int m = 16; m > 0; m >>= 1)
+#pragma unroll
+    for (int k = 0; k < m; ++k) {
+      const float give = r & m ? sums[k] : sums[k + m], keep = r & m ? sums[k + m] : sums[k];
+      sums[k] = keep + __shfl_xor(give, m, 64);
     }
+  const float w = sums[0];
   const int s = p0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * g + (r & 3);
   if (s >= So) return;
   if (slices > 1) part[((size_t)slice * B * H + bh) * So + s] = w;
