@@ -138,6 +138,18 @@ def test_rows_of_a_block(width, rows, pages, kernel, threads):
     assert grid >= B * H * -(-rows * G // tile) and grid % 8 == 0
 
 
+@pytest.mark.parametrize('width,B,pages,parts', [(128, 1, 17, True), (128, 24, 17, False), (128, 24, 70, True),
+                                                 (64, 1, 31, False), (64, 1, 40, True), (64, 16, 70, False),
+                                                 (64, 16, 90, True), (64, 64, 60, False), (64, 64, 70, True)])
+def test_positions_in_parts(width, B, pages, parts):
+    """One token a sequence: in one block where there are tiles enough for the chip, in parts over long tables."""
+    c = _Dry(8, 8, width=width)
+    c.attend(torch.zeros(B, 8, width, dtype=torch.float16), torch.zeros(B, pages, dtype=torch.int32),
+             torch.arange(B + 1, dtype=torch.int32), _ints(*[64 * pages] * B), most=1)
+    assert (c.log[-1][0] == 'pg_join') == parts
+    assert c.log[0][1] > B * 8
+
+
 def test_attend_refusals():
     c = _Dry(8, 3)
     table, starts, lengths = _batch()

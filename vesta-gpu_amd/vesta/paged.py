@@ -55,7 +55,8 @@ KINDS = ('f16', 'bf16', 'f32')         # kernels' queries: the cache's type, or 
 PAGE_MAX = 1 << 16
 STEP = {64: 64, 128: 32}               # positions of a wave's step in pg_attn, by width
 JOIN_BLOCK = 512
-JOIN_BLOCKS = 2048            # rows of a pg_join block: the fewest of 1, 4 and 16 with so many blocks
+JOIN_BLOCKS = 512             # rows of a pg_join block: the fewest of 1, 4 and 16 with so many blocks (512 / 2048: 128
+                              # tiles after up to 5000 49 / 62, 512 after up to 4000 163 / 173, 16 the same)
 
 # How a call's work is laid out; us a call (GPU time) on both sides of each rule.
 ROWS = 16                     # query rows of a pg_attn block; pg_wide's have 128
@@ -69,11 +70,14 @@ FEW_ROWS = 32                 # a sequence of up to so many rows (new tokens tim
 # 33.5, 1 x 256 63.3 / 48.6; f32, width 128: even at best, so it is not made.
 WIDE_FROM = {(64, False): (128, 64, 4096), (128, False): (64, 64, 1536), (64, True): (256, 256, 4096),
              (128, True): (1 << 30, 1 << 30, 0)}
-# A tile's positions go to several blocks, and a second launch puts them together, where the tables have more than
-# SPLIT positions times tiles / 256. One token, 12 heads, whole / in parts: width 64 after 1024 9.6 / 14.0, 2048 15.4 /
-# 14.0, 16384 86.9 / 21.3; width 128 after 700 12.1 / 13.0, 1024 15.9 / 13.0, 16384 176 / 27.7; 64 sequences after up
-# to 900 (512 tiles, width 128) 31.5 / 36.1, 256 after up to 2000 (2048 tiles) 258 / 274, 64 after up to 4000 142 / 125.
-SPLIT = {64: 2048, 128: 1024}
+# A tile's positions go to several blocks, and a second launch puts them together, where the tables have more than so
+# many positions: SPLIT up to 48 tiles, as many times more as there are tiles up to SPLIT_MOST, from 256 tiles on SPLIT
+# for each 256. One token, whole / in parts, sequences of one length: width 64, 12 tiles after 1500 15.0 / 16.5, 2000
+# 17.8 / 17.0, 5000 33.7 / 17.0; 64 tiles after 2000 17.2 / 17.3, 3000 23.3 / 21.3; 128 after 3000 24.7 / 30.5, 5000 37.0
+# / 39.1; 288 after 2000 36.3 / 40.0, 3000 50.9 / 50.0, 5000 98.5 / 81.0; width 128, 8 tiles after 700 11.9 / 13.7, 1000
+# 14.8 / 13.9; 64 after 700 12.2 / 14.0, 2000 26.1 / 22.5; 128 after 2000 27.5 / 33.2, 3000 37.5 / 41.5, 5000 85.6 /
+# 70.9; 192 after 3000 54.0 / 60.7, 5000 101 / 105; 512 after up to 900 31.5 / 36.1, up to 4000 142 / 125.
+SPLIT, SPLIT_MOST = {64: 2048, 128: 1024}, {64: 5120, 128: 4096}
 TARGET = 2048                 # parts in all, about (64 after up to 4000, 1024 / 1536 / 2048 / 4096: 132.2 / 127.4 / 125.5
                               # / 131.1; 2 after 100003: 159.6 / 160.8 / 158.6 / 163.5) ...
 PART_STEPS = 8                # ... each of at least so many steps: two a wave
@@ -453,8 +457,12 @@ class PagedCache:
             rows, aim, most_tiles, least, split = 128, WIDE_TARGET, 2 * WIDE_TARGET, WIDE_PART_STEPS, WIDE_SPLIT
         else:
             rows, aim, most_tiles, least, split = ROWS, TARGET, 16 * TARGET, PART_STEPS, SPLIT[self.width]
-        tiles = self.heads * (M * G // rows + B)
-        target = aim if tiles < most_tiles and positions * 256 > split * max(tiles, 256) else 0
+        tiles = self.heads * (B if most * G <= rows else M * G // rows + B)
+        if tiles > 256:
+            split = split * tiles // 256
+        elif not wide:
+            split = max(split, min(split * tiles // 48, SPLIT_MOST[self.width]))
+        target = aim if tiles < most_tiles and positions > split else 0
         blocks = target + tiles + 64
         if blocks >= 1 << 28 or M * G >= 1 << 30:
             raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
