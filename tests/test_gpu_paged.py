@@ -583,9 +583,10 @@ def test_every_variant(monkeypatch, dtype, query, width):
     b = Batch([1, 40, 1, 3], [700, 333, 2500, 3], 2, 2, width, 16, dtype, query)
     want, bound, got, gerr = b.want()
     base = dict(EIGHT_WAVES=0, TWO_WAVES=0, WIDE_FROM=WIDE, TWICE=(1 << 30, 0, 0), SPLIT={64: 1 << 30, 128: 1 << 30},
-                WIDE_SPLIT=1 << 30, FEW_ROWS=1 << 20)
+                WIDE_SPLIT=1 << 30, FEW_ROWS=1 << 20, SCORES_ROWS=1 << 30)
     parts = dict(SPLIT={64: 0, 128: 0}, WIDE_SPLIT=0)
-    for kw in ({}, dict(EIGHT_WAVES=1 << 20), dict(TWO_WAVES=1 << 20), parts, {**parts, 'TARGET': 16, 'PART_STEPS': 1}, dict(SCORES_MAX=0),
+    for kw in ({}, dict(EIGHT_WAVES=1 << 20), dict(TWO_WAVES=1 << 20), parts, {**parts, 'TARGET': 16, 'PART_STEPS': 1},
+               dict(SCORES_MAX=0), dict(SCORES_ROWS=2), dict(EIGHT_WAVES=1 << 20, SCORES_ROWS=40),
                dict(FEW_ROWS=0), dict(FEW_ROWS=0, **parts), dict(FEW_ROWS=0, WEIGH_BLOCKS=1),
                dict(FEW_ROWS=0, WIDE_TARGET=1 << 12, WIDE_PART_STEPS=1, WEIGH_BLOCKS=1 << 20, **parts),
                dict(RUN=1), dict(RUN=64, FEW_ROWS=0), dict(RUN_LONG=0, FEW_ROWS=0), dict(TWICE=(0, 0, 0), FEW_ROWS=0),

@@ -98,6 +98,9 @@ RUN_LONG = 64                 # ... but all tiles of a head where they are so ma
                               # together (4096 tokens after 27001, 16 / 64 / all 128 tiles: 2369 / 2261 / 2114)
 SCORES_MAX = 1 << 27          # scores (512 MB) that pg_attn keeps for the weights' pass (32 tokens after up to 1000: 24;
                               # made again by pg_weigh: 37)
+SCORES_ROWS = 8               # rows of a sequence up to which it does (kept / made again, 12 heads of 64: 8 x 1 after 900 18.6
+                              # / 23.4, 8 x 8 26.4 / 23.5, 8 x 128 178 / 58, 64 x 8 after 1000 56 / 79; 8 x 4 of 128: 32 x 1
+                              # 34.3 / 47.0, 64 x 4, 16 rows, 77 / 83, 64 x 8 124 / 100)
 WEIGH = 128                   # positions of a pg_weigh block
 WEIGH_BLOCKS = 2048           # blocks of pg_weigh_wide, about, by slices of the rows (4 x 1999, 512 / 1024 / 1536 / 2048 /
                               # 4096: 323 / 202 / 196 / 195 / 206)
@@ -405,13 +408,13 @@ class PagedCache:
         stream, back = self._enter()
         try:
             f32 = q.dtype is self._f32
-            wide = self._wide(B, N, M, G, most, f32) and not (f32 and weight is not None)
+            wide = self._wide(B, N, M, G, most, f32)
             lse = scores = pitch = target = 0
             floats = 0                   # of the one workspace: lse, scores, parts
             if weight is not None:
                 pitch = -(-N * self.page // 64) * 64
                 floats = -(-M * Hq // 4) * 4
-                if not wide and 0 < M * Hq * pitch <= SCORES_MAX:
+                if not wide and most * G <= SCORES_ROWS and 0 < M * Hq * pitch <= SCORES_MAX:
                     scores = 4 * floats
                     floats += M * Hq * pitch
             if M and B:
@@ -496,7 +499,7 @@ class PagedCache:
         if scores:
             blocks = -(-So // 1024)
             kn.pg_given(bh * blocks, BLOCK, stream, scores, pitch, *seqs[4:], cap, M, self.heads, G, lse, *to, blocks)
-        elif not wide:
+        elif not wide or kn is self._kind.get(self._f32):
             blocks = -(-So // WEIGH)
             kn.pg_weigh(_dealt(bh * blocks, RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2, lse, *to,
                         blocks, RUN)
