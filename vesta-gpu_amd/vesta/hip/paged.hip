@@ -322,7 +322,7 @@ __device__ __forceinline__ float pg_taken(const unsigned short* __restrict__ vh,
 // maxima, sums and weighted values in `ws` for pg_join.
 //
 // What bounds it: over long contexts the cache's bytes: two tokens of 32 heads
-// after 100,003 positions of 8 heads of 128, 818 MB in 162 us (5.05 TB/s, a
+// after 100,003 positions of 8 heads of 128, 818 MB in 158 us (5.15 TB/s, a
 // copy's rate), 64 ragged sequences of up to 4000 603 MB in 125 (4.8 TB/s);
 // over short ones the chain of dependent loads (lengths, pages, rows: 5.5 us
 // with one position, 1.4 us for each further step of a wave). A wave's next
@@ -1487,8 +1487,8 @@ extern "C" __global__ __launch_bounds__(256) void pg_given(const float* __restri
 // the rows' lse), on tiles of 32 x 32 x 16 as in pg_wide. A wave's sums stay in
 // registers over all rows. Several slices (few positions, many rows) leave
 // their sums in `part` [slice][B H So] for pg_total. 4 x 1999 tokens of 32 heads
-// (8 of 128 keyed): 79 us, of which 45 the rows and 34 the blocks' starts and
-// ends; slices of one size for all positions instead: 99.
+// (8 of 128 keyed): 79.5 us, of which 45 the rows and the rest the blocks' starts
+// and ends; slices of one size for all positions instead: 99.
 #if PG_KIND != PG_F32
 extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
