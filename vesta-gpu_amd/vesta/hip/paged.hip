@@ -1393,8 +1393,8 @@ PG_JOIN(pg_wide_join, 128, 64)
 // head), 32 to a wave, their key rows in registers, and goes through the rows
 // that see them, 16 at a time, in order: no atomics, the same sums each time.
 // `out` may be `old`: a thread reads an element before it writes it.
-// Scores are made again (as in pg_attn), the weight is 2^(score - lse). For fp32
-// queries, and where the scores would be too many to keep.
+// Scores are made again (as in pg_attn), the weight is 2^(score - lse). Where
+// pg_attn made few rows, and for fp32 queries of width 128.
 extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
     const int* __restrict__ table, int N, const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
@@ -1481,23 +1481,24 @@ extern "C" __global__ __launch_bounds__(256) void pg_given(const float* __restri
     if (p0 + 256 * u < So) out[(size_t)bh * So + p0 + 256 * u] = acc[u];
 }
 
-// The same for many rows of 16-bit queries: a block takes 256 positions of one
+// The same for many rows (fp32: of width 64): a block takes 256 positions of one
 // (sequence, key head), 64 to a wave, their key rows in registers, and a slice
 // of the rows that see them, 64 at a time through LDS (double-buffered, with
-// the rows' lse), on tiles of 32 x 32 x 16 as in pg_wide. A wave's sums stay in
-// registers over all rows. Several slices (few positions, many rows) leave
+// the rows' lse, fp32 rows scaled and in three planes as in pg_query), on tiles
+// of 32 x 32 x 16 as in pg_wide. A wave's sums stay in registers over all rows. Several slices (few positions, many rows) leave
 // their sums in `part` [slice][B H So] for pg_total. 4 x 1999 tokens of 32 heads
 // (8 of 128 keyed): 79.5 us, of which 45 the rows and the rest the blocks' starts
-// and ends; slices of one size for all positions instead: 99.
-#if PG_KIND != PG_F32
+// and ends; slices of one size for all positions instead: 99. fp32: 32 x 768 of 12
+// heads of 64, with the attention, 333 us in pg_weigh, 240 here.
+#if PG_KIND != PG_F32 || PG_E == 64
 extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
     const int* __restrict__ table, int N, const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
     int H, int G, float scale2, const float* __restrict__ lse, const float* old, int S,
     float* out, int So, int blocks, int run, int slices, float* __restrict__ part) {
   constexpr int KS = PG_E / 16, CH = PG_E / 8, NL = 64 * CH / 256, RS = 256 / CH;
-  __shared__ __attribute__((aligned(16))) vh_u32x4 lq[2][64 * (CH + 1)];
-  __shared__ float lz[2][64];
+  __shared__ __attribute__((aligned(16))) vh_u32x4 lq[2][PG_PLANES][64 * (CH + 1)];
+  __shared__ float lz[2][64], lk2[2][64];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
   const int id = pg_deal(blockIdx.x, run);
@@ -1530,12 +1531,23 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
     tr[n] = pg_div(y, G);
     gr[n] = y - tr[n] * G;
   }
+#if PG_KIND == PG_F32
+  vh_f32x4 qr[NL][2];
+#else
   vh_u32x4 qr[NL];
+#endif
   float zr = 0.0f;
   auto load = [&]() {                                              // past the last row: the last token, without weight
 #pragma unroll
-    for (int n = 0; n < NL; ++n)
-      qr[n] = ld16(Q + (sq.first + min(tr[n], sq.count - 1)) * qrow + (h * G + gr[n]) * qhead + 8 * c8);
+    for (int n = 0; n < NL; ++n) {
+      const pg_q* qp = Q + (sq.first + min(tr[n], sq.count - 1)) * qrow + (h * G + gr[n]) * qhead + 8 * c8;
+#if PG_KIND == PG_F32
+      qr[n][0] = *(const vh_f32x4*)qp;
+      qr[n][1] = *(const vh_f32x4*)(qp + 4);
+#else
+      qr[n] = ld16(qp);
+#endif
+    }
     if (tid < 64)
       zr = tr[NL] < sq.count ? lse[(size_t)(sq.first + tr[NL]) * (H * G) + h * G + gr[NL]] : INFINITY;
 #pragma unroll
@@ -1550,7 +1562,30 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
   };
   auto put = [&](int buf) {
 #pragma unroll
-    for (int n = 0; n < NL; ++n) lq[buf][(r8 + RS * n) * (CH + 1) + c8] = qr[n];
+    for (int n = 0; n < NL; ++n) {
+      const int row = r8 + RS * n;
+#if PG_KIND == PG_F32
+      float v[8], mx = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = qr[n][j >> 2][j & 3];
+        mx = fmaxf(mx, __builtin_fabsf(v[j]));
+      }
+#pragma unroll
+      for (int m = 1; m < CH; m <<= 1) mx = fmaxf(mx, __shfl_xor(mx, m, 64));
+      int e = 0;
+      if (mx > 0.0f && mx < INFINITY) e = max(__builtin_amdgcn_frexp_expf(mx), -100);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __builtin_ldexpf(v[j], -e);
+      vh_u32x4 f[3];
+      pg_split(v, f);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) lq[buf][p][row * (CH + 1) + c8] = f[p];
+      if (c8 == 0) lk2[buf][row] = __builtin_ldexpf(scale2, e);
+#else
+      lq[buf][0][row * (CH + 1) + c8] = qr[n];
+#endif
+    }
     if (tid < 64) lz[buf][tid] = zr;
   };
   if (x0 < x1) load();
@@ -1568,7 +1603,11 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
     }
     if (new0 + pg_div(min(x + 63, R - 1), G) < p0) continue;              // no row sees the wave's positions
     const bool part = p0 + 63 > new0 + pg_div(x, G);                      // not all of them by every row
+#if PG_KIND == PG_F32
+#pragma nounroll
+#else
 #pragma unroll
+#endif
     for (int u = 0; u < 2; ++u) {
       const float z = lz[buf][32 * u + r];
       pg_f16v s[2];
@@ -1576,12 +1615,71 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
+#if PG_KIND == PG_F32
+      const float k2 = lk2[buf][32 * u + r];
+      pg_f16v lo[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) lo[i][j] = 0.0f;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        const vh_u32x4 qf = lq[buf][(32 * u + r) * (CH + 1) + 2 * k + g];
+        const int at = (32 * u + r) * (CH + 1) + 2 * k + g;
+        const vh_u32x4 q0 = lq[buf][0][at], q1 = lq[buf][1][at], q2 = lq[buf][2][at];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[i] = pg_mfma32(kf[i][k], q0, s[i]);
+          lo[i] = pg_mfma32(kf[i][k], q1, lo[i]);
+          lo[i] = pg_mfma32(kf[i][k], q2, lo[i]);
+        }
+      }
+      float fin = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) fin = fmaf(s[i][j], 0.0f, fin);
+      if (__any(fin != fin)) {                                     // as in pg_scores
+        const int y = min(x + 32 * u + r, R - 1), tok = pg_div(y, G);
+        const pg_q* qp = Q + (sq.first + tok) * qrow + (h * G + y - tok * G) * qhead;
+#pragma nounroll
+        for (int e = 0; e < 32; ++e) {
+          const int at = min(p0 + 32 * (e >> 4) + 8 * ((e & 15) >> 2) + 4 * g + (e & 3), sq.len - 1);
+          const int page = table[(size_t)b * N + (at >> shift)];
+          const unsigned short* kq = kp + ((((size_t)((unsigned)page < (unsigned)pages ? page : 0) << shift)
+                                            + (at & ((1 << shift) - 1))) * H + h) * PG_E;
+          float whole = 0.0f;
+#pragma nounroll
+          for (int c = 0; c < CH; ++c) {
+            float kv[8];
+            unpack8(ld16(kq + 8 * c), kv);
+#pragma unroll
+            for (int d = 0; d < 8; ++d) whole = fmaf(qp[8 * c + d], kv[d], whole);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float hi = s[i][j];
+              if (e == 16 * i + j && !(__builtin_fabsf(hi) < INFINITY)) {
+                s[i][j] = whole;
+                lo[i][j] = 0.0f;
+              }
+            }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[i][j] = vh_hilo(s[i][j], lo[i][j]);
+#else
+      const float k2 = scale2;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const vh_u32x4 qf = lq[buf][0][(32 * u + r) * (CH + 1) + 2 * k + g];
 #pragma unroll
         for (int i = 0; i < 2; ++i) s[i] = pg_mfma32(kf[i][k], qf, s[i]);
       }
+#endif
       if (part) {
         const int lim = new0 + pg_div(min(x + 32 * u + r, R - 1), G);
 #pragma unroll
@@ -1592,7 +1690,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[i][j] += __builtin_amdgcn_exp2f(fmaf(s[i][j], scale2, -z));
+        for (int j = 0; j < 16; ++j) acc[i][j] += __builtin_amdgcn_exp2f(fmaf(s[i][j], k2, -z));
     }
   }
   // Over the rows: lane 32 g + r keeps position 32 (r / 16) + 8 (r % 16 / 4) + 4 g + r % 4.

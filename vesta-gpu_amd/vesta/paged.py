@@ -130,11 +130,10 @@ SIGNATURES = {
 
 
 def kernels_of(width: int, kind: str) -> set:
-    """The kernels of a module: attention of many rows and its weights are not made for f32 queries, but the former at
-    width 64."""
+    """The kernels of a module: those of many rows are not made for f32 queries of width 128."""
     without = set() if (width, kind) in ((128, 'f16'), (128, 'bf16')) else {'pg_wide8'}
-    if kind == 'f32':
-        without |= {'pg_weigh_wide', 'pg_total'} | ({'pg_wide', 'pg_wide_join'} if width != 64 else set())
+    if (width, kind) == (128, 'f32'):
+        without |= {'pg_weigh_wide', 'pg_total', 'pg_wide', 'pg_wide_join'}
     return set(SIGNATURES) - without
 
 
@@ -499,7 +498,7 @@ class PagedCache:
         if scores:
             blocks = -(-So // 1024)
             kn.pg_given(bh * blocks, BLOCK, stream, scores, pitch, *seqs[4:], cap, M, self.heads, G, lse, *to, blocks)
-        elif not wide or kn is self._kind.get(self._f32):
+        elif not wide:
             blocks = -(-So // WEIGH)
             kn.pg_weigh(_dealt(bh * blocks, RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2, lse, *to,
                         blocks, RUN)
