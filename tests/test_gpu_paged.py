@@ -589,8 +589,8 @@ def test_every_variant(monkeypatch, dtype, query, width):
                dict(SCORES_MAX=0), dict(SCORES_ROWS=2), dict(EIGHT_WAVES=1 << 20, SCORES_ROWS=40),
                dict(FEW_ROWS=0), dict(FEW_ROWS=0, **parts), dict(FEW_ROWS=0, WEIGH_BLOCKS=1),
                dict(FEW_ROWS=0, WIDE_TARGET=1 << 12, WIDE_PART_STEPS=1, WEIGH_BLOCKS=1 << 20, **parts),
-               dict(RUN=1), dict(RUN=64, FEW_ROWS=0), dict(RUN_LONG=0, FEW_ROWS=0), dict(TWICE=(0, 0, 0), FEW_ROWS=0),
-               dict(TWICE=(0, 0, 0), FEW_ROWS=0, WEIGH_BLOCKS=1 << 20)):
+               dict(RUN=1), dict(WIDE_RUN=64, FEW_ROWS=0), dict(WIDE_RUN=3, FEW_ROWS=0),
+               dict(TWICE=(0, 0, 0), FEW_ROWS=0), dict(TWICE=(0, 0, 0), FEW_ROWS=0, WEIGH_BLOCKS=1 << 20)):
         for name, value in {**base, **kw}.items():
             monkeypatch.setattr(paged, name, value)
         out, w = b.attend(weight=torch.zeros_like(got, dtype=torch.float32))

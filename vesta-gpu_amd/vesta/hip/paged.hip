@@ -352,7 +352,6 @@ __device__ __forceinline__ int pg_deal(int block, int run) {       // the block'
   const int n = pg_div(j, run);
   return (n * 8 + (block & 7)) * run + j - n * run;
 }
-#define PG_RUN_LONG 64
 template <int ROWS, int STEP>
 __device__ __forceinline__ void pg_count(const PgSeq& s, int G, int& tiles, int& steps) {
   tiles = (s.count * G + ROWS - 1) / ROWS;
@@ -426,8 +425,10 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
   // Where sequences have several tiles of many rows, all tiles longest first: a
   // CU has few of them, and a long one that starts late is waited for (sequence
   // by sequence / longest first: 16 x 1024 of 12 heads of 64 68 / 50 us, 32 x
-  // 700 63 / 57; four tiles a sequence: 6 x up to 512 26.0 / 28.0).
-  if (ROWS >= 128 && !joined && target == 0 && run < PG_RUN_LONG && B <= 64 && most * G >= 5 * ROWS) {
+  // 700 63 / 57; four tiles a sequence: 6 x up to 512 26.0 / 28.0; 1 x 9000 of 12
+  // heads a head's tiles to an XCD 269 / 208, of two of 128 keyed, 4096 after
+  // 20,000, 3050 / 900, of eight 1885 / 1850 after 27,001).
+  if (ROWS >= 128 && !joined && target == 0 && B <= 64 && most * G >= 5 * ROWS) {
     if (block == 0 && threadIdx.x < 64) pg_faults(starts, lengths, B, M, cap, most, err);
     PgSeq s = {};
     if (lane < B) s = pg_seq(starts, lengths, lane, M, cap);
@@ -496,7 +497,7 @@ __device__ __forceinline__ bool pg_work(PgWork& o, int block, int run, bool join
       o.sq.len = __builtin_amdgcn_readlane(s.len, l);
       o.tiles = __builtin_amdgcn_readlane(tiles, l);
       const int rest = at - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
-      const bool by_head = run >= PG_RUN_LONG || o.tiles <= 8;
+      const bool by_head = o.tiles <= 8;
       o.part = target ? pg_div(rest, o.tiles * H) : 0;
       const int ht = rest - o.part * (o.tiles * H), inner = by_head ? o.tiles : H;
       const int major = pg_div(ht, inner), minor = ht - major * inner;

@@ -93,14 +93,16 @@ EIGHT_WAVES = 256             # pg_attn of up to so many tiles (a block a CU) in
 TWO_WAVES = 8                 # ... and of more, where the tables have up to so many steps, of two (f32, four / two waves:
                               # 8 x 128 13.2 / 8.4, 64 tokens after 256 18.6 / 16.0, after 512 24.6 / 24.6; 64 after
                               # 600 of width 128, 19 steps, 22.4 / 23.5)
-RUN = 8                       # neighbouring blocks that go to one XCD (4 x 1999 in 4 / 16 / 64: 234 / 246 / 269) ...
-RUN_LONG = 64                 # ... but all tiles of a head where they are so many or more, which read the head's rows
-                              # together (4096 tokens after 27001, 16 / 64 / all 128 tiles: 2369 / 2261 / 2114)
+# Neighbouring blocks that go to one XCD, of pg_attn and of the kernels for many rows (64 x 1 after up to 4000, 16 heads
+# of 64, in 4 / 8: 145 / 135; in 1 / 4 / 8 / 16: 4 x 1999 with weights 179 / 181 / 194 / 189, 8 x 128 after 500 21.7 /
+# 17.5 / 17.4 / 17.2).
+RUN, WIDE_RUN = 8, 4
 SCORES_MAX = 1 << 27          # scores (512 MB) that pg_attn keeps for the weights' pass (32 tokens after up to 1000: 24;
                               # made again by pg_weigh: 37)
-SCORES_ROWS = 8               # rows of a sequence up to which it does (kept / made again, 12 heads of 64: 8 x 1 after 900 18.6
-                              # / 23.4, 8 x 8 26.4 / 23.5, 8 x 128 178 / 58, 64 x 8 after 1000 56 / 79; 8 x 4 of 128: 32 x 1
-                              # 34.3 / 47.0, 64 x 4, 16 rows, 77 / 83, 64 x 8 124 / 100)
+# Rows of a sequence up to which it does (kept / made again, 12 heads of 64: 8 x 1 after 900 18.6 / 23.4, 8 x 8 26.4 /
+# 23.5, 8 x 128 178 / 58, 64 x 8 after 1000 56 / 79; 8 x 4 of 128: 32 x 1 34.3 / 47.0, 64 x 4, 16 rows, 77 / 83, 64 x 8
+# 124 / 100).
+SCORES_ROWS = 8
 WEIGH = 128                   # positions of a pg_weigh block
 WEIGH_BLOCKS = 2048           # blocks of pg_weigh_wide, about, by slices of the rows (4 x 1999, 512 / 1024 / 1536 / 2048 /
                               # 4096: 323 / 202 / 196 / 195 / 206)
@@ -468,15 +470,13 @@ class PagedCache:
         blocks = target + tiles + 64
         if blocks >= 1 << 28 or M * G >= 1 << 30:
             raise ValueError(f'q: {M} rows of {B} sequences are too many for one call')
-        run = RUN
+        run = WIDE_RUN if wide else RUN
         if wide:
             attn, block = kn.pg_wide, BLOCK
             if self.width == 128 and target == 0 and all(n >= m for n, m in zip((most * G, positions, tiles), TWICE)):
                 attn, block, rows = kn.pg_wide8, 2 * BLOCK, 256
                 tiles = self.heads * (M * G // rows + B)
                 blocks = tiles + 64
-            if M * G >= rows * RUN_LONG * B:
-                run = M * G // (rows * B)
         elif target:
             attn, block = kn.pg_attn, BLOCK
         elif tiles <= EIGHT_WAVES:
@@ -485,7 +485,7 @@ class PagedCache:
             attn, block = kn.pg_attn2, BLOCK // 2
         else:
             attn, block = kn.pg_attn, BLOCK
-        return attn, block, rows, tiles, target, blocks, least, max(run, 1)
+        return attn, block, rows, tiles, target, blocks, least, run
 
     def _floats(self, n):
         """A workspace of a call."""
@@ -506,8 +506,8 @@ class PagedCache:
             blocks = -(-So // 256)
             slices = max(1, min(WEIGH_BLOCKS // (bh * blocks), most * G // 256))
             part = None if slices == 1 else self._floats(slices * bh * So)
-            kn.pg_weigh_wide(_dealt(bh * blocks * slices, RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2,
-                             lse, *to, blocks, RUN, slices, _at(part))
+            kn.pg_weigh_wide(_dealt(bh * blocks * slices, WIDE_RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G,
+                             scale2, lse, *to, blocks, WIDE_RUN, slices, _at(part))
             if slices > 1:
                 kn.pg_total(bh * blocks, BLOCK, stream, part.data_ptr(), slices, *seqs[4:], cap, B, M, self.heads, *to,
                             blocks)
