@@ -1392,7 +1392,8 @@ PG_JOIN(pg_wide_join, 128, 64)
 // the sequence's rows (tokens and the group's heads) of the softmax weight at
 // s; 0 past the length. A block takes 128 positions of one (sequence, key
 // head), 32 to a wave, their key rows in registers, and goes through the rows
-// that see them, 16 at a time, in order: no atomics, the same sums each time.
+// that see them, 16 at a time, in order: no atomics, the same sums each time. In
+// slices of the rows, where there are few blocks, as pg_weigh_wide.
 // `out` may be `old`: a thread reads an element before it writes it.
 // Scores are made again (as in pg_attn), the weight is 2^(score - lse). Where
 // pg_attn made few rows, and for fp32 queries of width 128.
@@ -1400,13 +1401,14 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh(
     const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, int pages, int shift,
     const int* __restrict__ table, int N, const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
     int H, int G, float scale2, const float* __restrict__ lse, const float* old, int S, float* out, int So,
-    int blocks, int run) {
+    int blocks, int run, int slices, float* __restrict__ part) {
   constexpr int KS = PG_E / 32;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, q = lane >> 4;
   const int id = pg_deal(blockIdx.x, run);
-  if (id >= B * H * blocks) return;
-  const int h = id / blocks % H, b = id / blocks / H, p0 = id % blocks * 128 + 32 * wave;
+  if (id >= B * H * blocks * slices) return;
+  const int slice = id % slices, task = id / slices;
+  const int h = task / blocks % H, b = task / blocks / H, b0 = task % blocks * 128, p0 = b0 + 32 * wave;
   if (p0 >= So) return;
   const PgSeq sq = pg_seq(starts, lengths, b, M, N << shift);
   const int new0 = sq.len - sq.count, R = sq.count * G;
@@ -1420,8 +1422,11 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh(
 #pragma unroll
       for (int k = 0; k < KS; ++k) kf[i][k] = ld16(kp + (at * H + h) * PG_E + 32 * k + 8 * q);
     }
-    // from the first token that sees the wave's first position
-    for (int x0 = max(p0 - new0, 0) * G / 16 * 16; x0 < R; x0 += 16) {
+    // the slice's share of the rows from the first token that sees the block's
+    // first position, from the first that sees the wave's
+    const int tile0 = max(b0 - new0, 0) * G / 16, share = (max((R + 15) / 16 - tile0, 0) + slices - 1) / slices;
+    const int end = min((tile0 + (slice + 1) * share) * 16, R);
+    for (int x0 = max((tile0 + slice * share) * 16, max(p0 - new0, 0) * G / 16 * 16); x0 < end; x0 += 16) {
       const int x = min(x0 + r, R - 1), tok = pg_div(x, G), head = h * G + x - tok * G;
       const int lim = x0 + r < R ? new0 + tok : -1;
       const pg_q* qp = Q + (sq.first + tok) * qrow + head * qhead;
@@ -1449,7 +1454,9 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh(
       w += __shfl_xor(w, 4, 64);
       w += __shfl_xor(w, 8, 64);
       const int s = p0 + 16 * i + 4 * q + j;
-      if (r == 0 && s < So) out[bh * So + s] = w + (s < new0 ? old[bh * S + s] : 0.0f);
+      if (r != 0 || s >= So) continue;
+      if (slices > 1) part[((size_t)slice * B * H + bh) * So + s] = w;
+      else out[bh * So + s] = w + (s < new0 ? old[bh * S + s] : 0.0f);
     }
 }
 
@@ -1713,6 +1720,7 @@ extern "C" __global__ __launch_bounds__(256, 2) void pg_weigh_wide(
   if (slices > 1) part[((size_t)slice * B * H + bh) * So + s] = w;
   else out[(size_t)bh * So + s] = w + (s < new0 ? old[(size_t)bh * S + s] : 0.0f);
 }
+#endif
 
 // The slices' sums added to the old ones, in order.
 extern "C" __global__ __launch_bounds__(256) void pg_total(const float* __restrict__ part, int slices,
@@ -1726,7 +1734,6 @@ extern "C" __global__ __launch_bounds__(256) void pg_total(const float* __restri
   for (int k = 0; k < slices; ++k) w += part[((size_t)k * B * H + bh) * So + s];
   out[(size_t)bh * So + s] = w + (s < sq.len - sq.count ? old[(size_t)bh * S + s] : 0.0f);
 }
-#endif
 
 // ---------------------------------------------------------------- eviction
 // pg_select: a block per (layer, sequence, head) finds which positions stay:

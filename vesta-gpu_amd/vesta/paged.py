@@ -103,9 +103,10 @@ SCORES_MAX = 1 << 27          # scores (512 MB) that pg_attn keeps for the weigh
 # 23.5, 8 x 128 178 / 58, 64 x 8 after 1000 56 / 79; 8 x 4 of 128: 32 x 1 34.3 / 47.0, 64 x 4, 16 rows, 77 / 83, 64 x 8
 # 124 / 100).
 SCORES_ROWS = 8
-WEIGH = 128                   # positions of a pg_weigh block
-WEIGH_BLOCKS = 2048           # blocks of pg_weigh_wide, about, by slices of the rows (4 x 1999, 512 / 1024 / 1536 / 2048 /
-                              # 4096: 323 / 202 / 196 / 195 / 206)
+# Blocks of the kernels that make scores again, about, by slices of the rows (pg_weigh_wide, 4 x 1999, 512 / 1024 / 1536 /
+# 2048 / 4096: 323 / 202 / 196 / 195 / 206; pg_weigh, fp32 of width 128, whole / in slices: 1 x 909 of six heads, two
+# keyed, 228 / 51, 8 x 128 of 32/8 65 / 43).
+WEIGH_BLOCKS = 2048
 SELECT_FEW = 4096             # positions up to which pg_select has 256 threads, not 1024 (1152 times 1024: 13 / 38)
 ERRORS = {1: 'a page id outside the pool', 2: 'starts that do not ascend, or lie past the rows',
           4: 'a length past its table', 8: 'a sequence with more new tokens than `most`'}
@@ -122,7 +123,7 @@ SIGNATURES = {
     'pg_wide': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllppp',
     'pg_wide8': 'pll' + 'pp' + _SEQS + 'iiii' + 'iiiiif' + 'pllppp',
     'pg_wide_join': 'ppiiiiiiiiiippllp',
-    'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiii',
+    'pg_weigh': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiiiip',
     'pg_given': 'plppiiiippipii',
     'pg_weigh_wide': 'pll' + 'p' + _SEQS + 'iiii' + 'fppipiiiip',
     'pg_total': 'pippiiiipipii',
@@ -135,7 +136,7 @@ def kernels_of(width: int, kind: str) -> set:
     """The kernels of a module: those of many rows are not made for f32 queries of width 128."""
     without = set() if (width, kind) in ((128, 'f16'), (128, 'bf16')) else {'pg_wide8'}
     if (width, kind) == (128, 'f32'):
-        without |= {'pg_weigh_wide', 'pg_total', 'pg_wide', 'pg_wide_join'}
+        without |= {'pg_weigh_wide', 'pg_wide', 'pg_wide_join'}
     return set(SIGNATURES) - without
 
 
@@ -498,19 +499,16 @@ class PagedCache:
         if scores:
             blocks = -(-So // 1024)
             kn.pg_given(bh * blocks, BLOCK, stream, scores, pitch, *seqs[4:], cap, M, self.heads, G, lse, *to, blocks)
-        elif not wide:
-            blocks = -(-So // WEIGH)
-            kn.pg_weigh(_dealt(bh * blocks, RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2, lse, *to,
-                        blocks, RUN)
-        else:
+            return
+        weigh, width, run = (kn.pg_weigh_wide, 256, WIDE_RUN) if wide else (kn.pg_weigh, 128, RUN)
+        blocks = -(-So // width)
+        slices = max(1, min(WEIGH_BLOCKS // (bh * blocks), most * G // width))
+        part = None if slices == 1 else self._floats(slices * bh * So)
+        weigh(_dealt(bh * blocks * slices, run), BLOCK, stream, *keys, *seqs, B, M, self.heads, G, scale2, lse, *to, blocks,
+              run, slices, _at(part))
+        if slices > 1:
             blocks = -(-So // 256)
-            slices = max(1, min(WEIGH_BLOCKS // (bh * blocks), most * G // 256))
-            part = None if slices == 1 else self._floats(slices * bh * So)
-            kn.pg_weigh_wide(_dealt(bh * blocks * slices, WIDE_RUN), BLOCK, stream, *keys, *seqs, B, M, self.heads, G,
-                             scale2, lse, *to, blocks, WIDE_RUN, slices, _at(part))
-            if slices > 1:
-                kn.pg_total(bh * blocks, BLOCK, stream, part.data_ptr(), slices, *seqs[4:], cap, B, M, self.heads, *to,
-                            blocks)
+            kn.pg_total(bh * blocks, BLOCK, stream, part.data_ptr(), slices, *seqs[4:], cap, B, M, self.heads, *to, blocks)
 
     def _weights(self, name, w, lead, least):
         try:
