@@ -637,3 +637,60 @@ def test_evict_long(n):
             assert torch.equal(b.cache.keys[0, b.to[i].long()[dst // 64], dst % 64],
                                b.cache.keys[0, b.table[i].long()[src // 64], src % 64])
     b.cache.check()
+
+
+@pytest.mark.parametrize('dtype,query', KINDS)
+@pytest.mark.parametrize('width', (64, 128))
+@pytest.mark.parametrize('below', (16.5, 24.5, 25.5, 29.5))
+def test_a_long_tail_keeps_its_mass(blocks, dtype, query, width, below):
+    """One position in 32 takes nearly all of the softmax and has value 0, all others weigh 2^-below of it and have a
+    value of 4096: the output is theirs alone, in whatever part, step and wave they come.
+
+    A tail weight is off by its rounding to 16 bits, half a step of itself, or half of fp16's fixed step where it is
+    small: the largest weight is 2^11 at least, so that is 2^-36 of the largest (bf16 has none; fp32 queries' planes
+    carry 24 bits of it); by 2^-22 and 4 half steps of the largest score's fp32 exponent (below half steps of 32 at
+    most) otherwise, as is the sum; the sums of up to 3000 positions by a half step each."""
+    counts, lengths = [1, 140, 3], [3000, 700, 96]
+    b = Batch(counts, lengths, 2, 2, width, 16, dtype, query)
+    for i, n in enumerate(lengths):
+        p = torch.arange(n, device='cuda')
+        at = b.table[i].long()[p // 16], p % 16
+        b.cache.keys[0][at] = 0.0
+        b.cache.vals[0][at] = 4096.0
+        top = p % 32 == 0
+        b.cache.keys[0, at[0][top], at[1][top], :, 5] = 1.0
+        b.cache.vals[0, at[0][top], at[1][top]] = 0.0
+    b.q.zero_()
+    b.q[:, :, 5] = 1.0
+    scale = below * math.log(2)
+    want, *_ = b.want(scale=scale)
+    w = 2.0 ** -below
+    u = 2.0 ** -24
+    rounded = 0.0 if query == 'f32' else max(torch.finfo(DT[dtype]).eps / 2, 2.0 ** -36 / w if dtype == 'f16' else 0.0)
+    rel = rounded + 2 * (2.0 ** -22 + 4 * 32 * u) + 3000 * u
+    ur = u if query == 'f32' else torch.finfo(DT[query]).eps / 2
+    bound = want * (rel + ur) * 1.01 + (2.0 ** -25 if query == 'f16' else 0.0)
+    assert (want[0] > 0).all()
+    _close(b.attend(scale=scale), want, bound)
+    _close(b.attend(scale=scale, most=140), want, bound)
+
+
+@pytest.mark.parametrize('dtype,query', KINDS)
+def test_scores_of_many_millions(blocks, dtype, query):
+    """Scores whose fp32 steps are whole numbers, two of them equal: their weights stay in their types' range, equal, and
+    each is rounded once (fp32 queries: sums, the exponential's 2^-22 aside, which both have alike, and a division)."""
+    b = Batch([1, 40], [70, 200], 2, 1, 64, 16, dtype, query)
+    for pool in (b.cache.keys, b.cache.vals):
+        pool.nan_to_num_(0.0).zero_()
+    for i in range(2):
+        for s, v in ((3, 2.0), (50, 4.0)):
+            b.cache.keys[0, b.table[i, s // 16], s % 16] = 1000.0
+            b.cache.vals[0, b.table[i, s // 16], s % 16] = v
+    b.q.fill_(1000.0)
+    # log2(e) 6.4e7 times the scale: between 2^24 and 2^27
+    for scale in (0.1, 0.21, 0.33, 0.57, 0.77, 1.0, 1.13):
+        out = b.attend(scale=scale)
+        want = torch.full(out.shape, 3.0, dtype=torch.float64, device='cuda')
+        rounded = 8 * 2.0 ** -24 if query == 'f32' else torch.finfo(DT[dtype]).eps
+        _close(out, want, want * rounded * 1.01)
+    b.cache.check()

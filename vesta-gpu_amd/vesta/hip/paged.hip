@@ -277,6 +277,34 @@ __device__ __forceinline__ void pg_scores(const vh_u32x4* kf, const PgQuery& qf,
 #endif
 }
 
+// Weights are 2^(score - reference), the reference a running one PG_BIAS below
+// the row's largest score: fp16, which holds the second product's operand, has
+// full precision down to 2^-14 only and nothing below 2^-25, so the largest
+// weight is 2^15 and a long tail of small ones keeps its mass down to 2^-40 of
+// it (with a largest of 1, positions 2^-25.5 below one lost all of theirs, while
+// the sum counted it). fp32's three planes want 2^14 (their second is 2^11 times
+// what the first leaves), pg_wide's largest may be 2^PG_SLACK more. bf16 has the
+// range. Sums, weighted values and the parts' maxima are all against the
+// reference, so that it cancels.
+#define PG_SLACK (PG_KIND == PG_BF16 ? 8 : 4)
+#define PG_ATTN_BIAS (PG_KIND == PG_BF16 ? 0 : PG_KIND == PG_F32 ? 14 : 15)
+#define PG_WIDE_BIAS (PG_KIND == PG_BF16 ? 0 : PG_KIND == PG_F32 ? 14 : 15 - PG_SLACK)
+// The reference of a largest score bm k2: rounded up where the nearest would
+// give a weight above 2^BIAS (scores of 2^24 and more).
+template <int BIAS>
+__device__ __forceinline__ float pg_reference(float bm, float k2) {
+  if constexpr (BIAS == 0) return bm * k2;
+  float n = fmaf(bm, k2, -(float)BIAS);
+  if (fmaf(bm, k2, -n) > (float)BIAS) n = fmaf(__builtin_fabsf(n), 0x1p-23f, n);
+  return n;
+}
+// log2 of a row's sum of 2^score, from its sum against reference m. (The bias is
+// taken out of both first: log2 of a small number has more bits behind the point.)
+template <int BIAS>
+__device__ __forceinline__ float pg_lse(float m, float sum) {
+  return (m + (float)BIAS) + __builtin_amdgcn_logf(__builtin_ldexpf(sum, -BIAS));
+}
+
 // Whether a 16-bit value is an infinity or a NaN (its exponent bits all set),
 // and the same of a word's two: a unit added to the exponents carries into the
 // halves' top bits.
@@ -647,7 +675,7 @@ __device__ __forceinline__ void pg_attn_body(
 #pragma unroll
     for (int n = 1; n < 4 * NG; ++n) bm = fmaxf(bm, s[n >> 2][n & 3]);
     bm = vh_pair32(vh_pair16(bm, op_max), op_max);
-    const float n2 = fmaxf(m2, bm * qf.k2);
+    const float n2 = fmaxf(m2, pg_reference<PG_ATTN_BIAS>(bm, qf.k2));
     const float ref = n2 == -INFINITY ? 0.0f : n2;                 // no score above -inf yet: all weights 0
     const float c = __builtin_amdgcn_exp2f(m2 - ref);
     m2 = n2;
@@ -755,7 +783,7 @@ __device__ __forceinline__ void pg_attn_body(
     } else if (lse) {
       // log2 of the row's sum of 2^score: +inf for a row that sees nothing, so
       // that all its weights are 0
-      lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : m + __builtin_amdgcn_logf(sum);
+      lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : pg_lse<PG_ATTN_BIAS>(m, sum);
     }
   }
 }
@@ -793,8 +821,8 @@ __device__ __forceinline__ void pg_here(vh_u32x4 (&f)[N]) {
 // product from the registers they are in: fold position 8 g + e stands for
 // position 4 g + e (e < 4) or 8 + 4 g + e - 4 of 16. The weighted values
 // accumulate in the matrix cores' own registers; they are rescaled only when a
-// row's maximum has grown by more than 2^PG_SLACK since (weights up to that
-// are exact in the sums and rounded as finely). fp32 queries and weights go in
+// row's reference has grown by more than PG_SLACK since (weights up to 2^PG_SLACK
+// times the largest are exact in the sums and rounded as finely). fp32 queries and weights go in
 // three planes, 32 positions at a time, and each 32 positions' weighted values
 // are summed on their own and added in fp32, so that no sum is a chain over all
 // positions; they take this kernel at width 64 only (at 128 their planes leave
@@ -812,7 +840,6 @@ __device__ __forceinline__ void pg_here(vh_u32x4 (&f)[N]) {
 // cycles a step against 512), and for short chunks the blocks' starts and ends
 // (4 us): six chunks of up to 512 tokens 25 us (220 TFLOP/s).
 #if PG_KIND != PG_F32 || PG_E == 64
-#define PG_SLACK 8.0f
 #define PG_WROW (PG_E + 32)                // halves of a value row in LDS: 64 bytes past a multiple of all banks
 typedef float pg_f16v __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ pg_f16v pg_mfma32(vh_u32x4 a, vh_u32x4 b, pg_f16v c) {
@@ -1010,8 +1037,8 @@ __device__ __forceinline__ void pg_wide_body(
       for (int j = 1; j < 16; ++j) bm = fmaxf(bm, fmaxf(s[0][j], s[1][j]));
     }
     bm = vh_pair32(bm, op_max);
-    const float n2 = bm * scale2;
-    if (__any(n2 > m2 + PG_SLACK || (n2 > m2 && m2 == -INFINITY))) {
+    const float n2 = pg_reference<PG_WIDE_BIAS>(bm, scale2);
+    if (__any(n2 - m2 > (float)PG_SLACK)) {                        // (a first one too: m2 is -inf)
       const float m = fmaxf(m2, n2);
       const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - m);
       m2 = m;
@@ -1203,7 +1230,7 @@ __device__ __forceinline__ void pg_wide_body(
 #pragma unroll
         for (int j = 1; j < 16; ++j) bm = fmaxf(bm, s[j]);
         bm = vh_pair32(bm, op_max);
-        const float n2 = fmaxf(m2, bm * k2);
+        const float n2 = fmaxf(m2, pg_reference<PG_WIDE_BIAS>(bm, k2));
         const float ref = n2 == -INFINITY ? 0.0f : n2;               // no score above -inf yet: all weights 0
         const float c = __builtin_amdgcn_exp2f(m2 - ref);
         m2 = n2;
@@ -1261,7 +1288,7 @@ __device__ __forceinline__ void pg_wide_body(
       wp[32 * wave + r] = m2;
       wp[TILE + 32 * wave + r] = sum;
     } else if (lse) {
-      lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : m2 + __builtin_amdgcn_logf(sum);
+      lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : pg_lse<PG_WIDE_BIAS>(m2, sum);
     }
   }
 }
@@ -1372,7 +1399,8 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
 #pragma unroll
   for (int j = 0; j < 4; ++j) w[j] = lim < 0 ? 0.0f : v[j] / sum;
   pg_store4(out + (wk.sq.first + tok) * orow + head * ohead + 4 * c, w);
-  if (lse && c == 0) lse[(size_t)(wk.sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : m + __builtin_amdgcn_logf(sum);
+  constexpr int BIAS = ROWS == 16 ? PG_ATTN_BIAS : PG_WIDE_BIAS;
+  if (lse && c == 0) lse[(size_t)(wk.sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : pg_lse<BIAS>(m, sum);
 }
 #define PG_JOIN(name, rows, step)                                                                                  \
   extern "C" __global__ __launch_bounds__(512) void name(                                                          \
