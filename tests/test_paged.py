@@ -235,3 +235,27 @@ def test_kernels_compile(width, kind):
     key = b'.vgpr_spill_count'                        # of every kernel: a MessagePack number after the key
     spills = [code[i + len(key)] for i in range(len(code)) if code.startswith(key, i)]
     assert len(spills) == len(paged.kernels_of(width, kind)) and not any(spills)
+
+
+def test_starts_are_needed():
+    """Only eviction does without them: the kernels of the others read them."""
+    c = _Dry(8, 3)
+    table, _, lengths = _batch()
+    k = _rows(5, 3)
+    for call in (lambda: c.append(k, k, table, None, lengths), lambda: c.attend(k, table, None, lengths),
+                 lambda: c.attend(k, table, None, lengths, weight=torch.zeros(2, 3, 192))):
+        with pytest.raises(TypeError, match='starts'):
+            call()
+    assert not c.log
+
+
+def test_extend_needs_starts():
+    from vesta.gpt2 import VestaGPT2
+    c = _Dry(8, 3)
+    m = object.__new__(VestaGPT2)
+    m.L, m.H, m.E, m.D, m.W = 1, 3, 64, 192, dict(wte=torch.zeros(5, 192, dtype=torch.float16),
+                                                  fcw=torch.zeros(1, 192, 768, dtype=torch.float16))
+    m._pf = m._paged = None
+    table, _, lengths = _batch()
+    with pytest.raises(TypeError, match='starts'):
+        m.extend(c, _ints(*[0] * 5), _ints(*[0] * 5), table, None, lengths)

@@ -351,7 +351,7 @@ class VestaGPT2:
                 raise TypeError(f'{name}: need a contiguous int32 tensor on {cache.device}')
         if tokens.dim() != 1 or tokens.shape[0] < 1 or positions.shape != tokens.shape:
             raise ValueError(f'tokens {tuple(tokens.shape)}, positions {tuple(positions.shape)}: need two of [M], M >= 1')
-        B, N, _ = cache._batch(table, starts, lengths)
+        B, N, _ = cache._batch(table, lengths, starts)
         if B < 1 or N < 1:
             raise ValueError(f'table {tuple(table.shape)}: one sequence and one page at least')
         if weight is not None:

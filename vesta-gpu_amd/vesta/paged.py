@@ -286,13 +286,13 @@ class PagedCache:
             raise ValueError(f'{name}: shape {tuple(got)}, need {tuple("any" if w is None else w for w in shape)}')
         return t.data_ptr()
 
-    def _batch(self, table, starts, lengths):
-        """B, N and the kernels' arguments for a batch."""
+    def _batch(self, table, lengths, starts=None, new=True):
+        """B, N and the kernels' arguments for a batch (``new``: of new tokens, whose ``starts`` they need)."""
         at = self._ints('table', table, _ANY2)
         B, N = table.shape
         if N * self.page >= 1 << 31:
             raise ValueError(f'table: {N} pages of {self.page} rows a sequence, fewer than 2^31 rows are possible')
-        return B, N, (self.pages, self._shift, at, N, 0 if starts is None else self._ints('starts', starts, (B + 1,)),
+        return B, N, (self.pages, self._shift, at, N, self._ints('starts', starts, (B + 1,)) if new else 0,
                       self._ints('lengths', lengths, (B,)))
 
     def _rows(self, name, t, dtypes, heads=None, like=None):
@@ -341,7 +341,7 @@ class PagedCache:
         into their pages of ``layer``. They are of the cache's type or f32
         (rounded to nearest). Rows of other sequences' slots stay as they are;
         a page that two of the new rows' sequences share gets either's."""
-        B, N, seqs = self._batch(table, starts, lengths)
+        B, N, seqs = self._batch(table, lengths, starts)
         at = self._layer(layer)
         k_at, *ks = self._rows('k', k, self._new, self.heads)
         v_at, *vs = self._rows('v', v, (k.dtype,), like=k.shape)
@@ -377,7 +377,7 @@ class PagedCache:
 
         ``most``: a bound of the new tokens of a sequence that the program
         knows (1 for a decode step); the work is laid out by it."""
-        B, N, seqs = self._batch(table, starts, lengths)
+        B, N, seqs = self._batch(table, lengths, starts)
         at = self._layer(layer)
         qs = self._rows('q', q, self._queries)
         M, Hq, _ = q.shape
@@ -535,7 +535,7 @@ class PagedCache:
         Returns (lengths [B], weight_out [layers, B, heads, S'], kept [layers,
         B, heads, keep]): the new lengths, the kept positions' weights (0
         behind them) and which positions they were (-1 behind them)."""
-        B, N, seqs = self._batch(table, None, lengths)
+        B, N, seqs = self._batch(table, lengths, new=False)
         to_at = self._ints('to', to, (B, None))
         No = to.shape[1]
         if to_at == seqs[2] and B and N:
