@@ -259,3 +259,40 @@ def test_extend_needs_starts():
     table, _, lengths = _batch()
     with pytest.raises(TypeError, match='starts'):
         m.extend(c, _ints(*[0] * 5), _ints(*[0] * 5), table, None, lengths)
+
+
+def test_whole_numbers_of_any_type():
+    """A NumPy number of few bits, as comes out of an array, does not overflow in the addresses and sizes made of it."""
+    import numpy as np
+    c = _Dry(np.int32(64), np.int8(3), layers=np.int8(40), page=np.int16(64))
+    for n in (c.pages, c.heads, c.layers, c.page, c.width):
+        assert type(n) is int
+    table, starts, lengths = _batch()
+    k = _rows(5, 3)
+    c.append(k, k, table, starts, lengths, layer=np.int8(39))
+    assert c.log[-1][3][6] - c.keys.data_ptr() == 39 * 64 * 64 * 3 * 64 * 2
+    c.attend(k, table, starts, lengths, layer=np.int16(39))
+    assert c.log[-1][3][3] - c.keys.data_ptr() == 39 * 64 * 64 * 3 * 64 * 2
+    q = _rows(2 * 100, 3 * 32)
+    starts, lengths = _ints(0, 100, 200), _ints(100, 100)
+    c.attend(q, table, starts, lengths, most=100)
+    want = c.log[-1]
+    c.attend(q, table, starts, lengths, most=np.int8(100))
+    assert c.log[-1][:3] == want[:3] and c.log[-1][3][11:21] == want[3][11:21]
+    w = torch.zeros(40, 2, 3, 192)
+    to = torch.zeros(2, 2, dtype=torch.int32)
+    c.evict(w, table, lengths, 120, to, 9)
+    want = [e[1:3] for e in c.log[-2:]]
+    c.evict(w, table, lengths, np.int8(120), to, np.int8(9))
+    assert [e[1:3] for e in c.log[-2:]] == want
+
+
+def test_evict_numbers_past_32_bits():
+    """More recent positions than there can be are all of them; more kept ones than a kernel can count are refused."""
+    c = _Dry(8, 1, page=1 << 16)
+    w, table, lengths = torch.zeros(1, 1, 1, 1 << 16), torch.zeros(1, 1, dtype=torch.int32), _ints(9)
+    c.evict(w, table, lengths, 5, torch.ones(1, 1, dtype=torch.int32), recent=1 << 40)
+    assert [e[0] for e in c.log] == ['pg_select', 'pg_move'] and c.log[0][3][7] == 5
+    for keep in (5, 1 << 31):
+        with pytest.raises(ValueError, match='2.31'):
+            c.evict(w, table, lengths, keep, torch.ones(1, 1 << 15, dtype=torch.int32))

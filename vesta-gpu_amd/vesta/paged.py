@@ -239,6 +239,7 @@ class PagedCache:
             self._kind[torch.float32] = _kernels(self.device.index, width, 'f32')
 
     def _shape(self, pages, heads, width, layers, page, dtype):
+        pages, heads, width, layers, page = map(operator.index, (pages, heads, width, layers, page))
         if dtype not in ('f16', 'bf16'):
             raise ValueError(f"dtype {dtype!r}: the cache is 'f16' or 'bf16'")
         if width not in WIDTHS:
@@ -290,10 +291,13 @@ class PagedCache:
         """B, N and the kernels' arguments for a batch (``new``: of new tokens, whose ``starts`` they need)."""
         at = self._ints('table', table, _ANY2)
         B, N = table.shape
-        if N * self.page >= 1 << 31:
-            raise ValueError(f'table: {N} pages of {self.page} rows a sequence, fewer than 2^31 rows are possible')
+        self._few('table', N)
         return B, N, (self.pages, self._shift, at, N, self._ints('starts', starts, (B + 1,)) if new else 0,
                       self._ints('lengths', lengths, (B,)))
+
+    def _few(self, name, n):
+        if n * self.page >= 1 << 31:
+            raise ValueError(f'{name}: {n} pages of {self.page} rows a sequence, fewer than 2^31 rows are possible')
 
     def _rows(self, name, t, dtypes, heads=None, like=None):
         """New tokens' rows [M, heads, width]: any strides but the last, 16-byte aligned. Returns their address and
@@ -316,7 +320,8 @@ class PagedCache:
         return at, row, head
 
     def _layer(self, layer):
-        if not 0 <= operator.index(layer) < self.layers:
+        layer = operator.index(layer)
+        if not 0 <= layer < self.layers:
             raise ValueError(f'layer {layer} of {self.layers}')
         return layer * self._layer_bytes
 
@@ -387,7 +392,7 @@ class PagedCache:
         scale2 = 1.4426950408889634 * (self._scale if scale is None else float(scale))
         if not 2.0 ** -126 <= scale2 < 2.0 ** 127:
             raise ValueError(f'scale {scale}: positive and finite in 32 bits')
-        if most is not None and operator.index(most) < 1:
+        if most is not None and (most := operator.index(most)) < 1:
             raise ValueError(f'most {most}: at least 1')
         if out is None:
             out = q.new_empty((M, Hq, self.width))
@@ -518,7 +523,7 @@ class PagedCache:
             fits = False
         if not fits:
             raise TypeError(f'{name}: need a contiguous float32 tensor on {self.device}')
-        if tuple(shape[:-1]) != lead or shape[-1] < least:
+        if tuple(shape[:-1]) != lead or not least <= shape[-1] < 1 << 31:
             raise ValueError(f'{name}: shape {tuple(shape)}, need {lead} and {least} positions at least')
         return shape[-1]
 
@@ -540,7 +545,9 @@ class PagedCache:
         No = to.shape[1]
         if to_at == seqs[2] and B and N:
             raise ValueError('to: pages other than those that are read')
-        if operator.index(keep) < 1 or operator.index(recent) < 0:
+        self._few('to', No)
+        keep, recent = operator.index(keep), operator.index(recent)
+        if keep < 1 or recent < 0:
             raise ValueError(f'keep {keep} of at least 1 position, recent {recent} of at least 0')
         if No * self.page < keep:
             raise ValueError(f'to: {No} pages of {self.page} rows cannot hold {keep} positions')
@@ -562,8 +569,8 @@ class PagedCache:
         stream, back = self._enter()
         try:
             kn.pg_select(self.layers * B * self.heads, 256 if N * self.page <= SELECT_FEW else 1024, stream,
-                         weight.data_ptr(), S, seqs[5], N * self.page, B, self.heads, keep, recent, kept.data_ptr(),
-                         weight_out.data_ptr(), So, new.data_ptr(), self._err)
+                         weight.data_ptr(), S, seqs[5], N * self.page, B, self.heads, keep, min(recent, keep),
+                         kept.data_ptr(), weight_out.data_ptr(), So, new.data_ptr(), self._err)
             kn.pg_move(self.layers * B * blocks, BLOCK, stream, *self._pools, *seqs[:4], to_at, No, kept.data_ptr(), keep,
                        B, self.heads, blocks, self._err)
         finally:
