@@ -694,3 +694,26 @@ def test_scores_of_many_millions(blocks, dtype, query):
         rounded = 8 * 2.0 ** -24 if query == 'f32' else torch.finfo(DT[dtype]).eps
         _close(out, want, want * rounded * 1.01)
     b.cache.check()
+
+
+@pytest.mark.parametrize('new', ('f16', 'f32'))
+def test_an_impossible_sequence_appends_nothing(new):
+    """A length past the table or starts that cannot be: the cache's rows stay, those of the other sequences come."""
+    b = Batch([2, 3, 1], [16, 48, 16], 2, 1, 64, 16, spare=0)
+    b.table[0, 1:], b.table[2, 1:] = b.table[1, 1], b.table[1, 2]      # stale entries behind their own page
+    rows = torch.randn(6, 2, 64, generator=b.gen, device='cuda').to(DT[new])
+    good = b.starts, b.lengths
+    # (starts, lengths, the sequences that are stored)
+    for starts, lengths, stored in ((good[0], _ints([49, 48, 16]), (1, 2)), (good[0], _ints([16, 1 << 30, 16]), (0, 2)),
+                                    (good[0], _ints([16, -1, 99]), (0,)), (_ints([-1, 2, 5, 6]), good[1], (1, 2)),
+                                    (_ints([0, 2, 5, 7]), good[1], (0, 1)), (_ints([0, 2, 5, 4]), good[1], (0, 1))):
+        before = b.cache.keys.clone(), b.cache.vals.clone()
+        b.cache.append(rows, -rows, b.table, starts, lengths)
+        for sign, pool, want in zip((1, -1), (b.cache.keys, b.cache.vals), before):
+            for i in stored:
+                for j, s in enumerate(range(b.lens[i] - b.counts[i], b.lens[i])):
+                    want[0, b.table[i, s // 16], s % 16] = sign * rows[int(good[0][i]) + j].half()
+            assert torch.equal(pool.view(torch.int16), want.view(torch.int16))
+        with pytest.raises(RuntimeError, match='length|starts'):
+            b.cache.check()
+        rows = rows + 1

@@ -15,7 +15,8 @@
 //
 // Everything that comes from the device (page ids, starts, lengths) is checked
 // where it is used: an impossible one raises the error word and is replaced
-// by a possible one, so that no access leaves its tensor.
+// by a possible one, so that no access leaves its tensor; nothing is appended
+// for a sequence that has one.
 
 #define PG_F16 0
 #define PG_BF16 1
@@ -114,7 +115,7 @@ __device__ __forceinline__ void pg_append_body(const T* __restrict__ k, const T*
   const PgSeq s = pg_seq(starts, lengths, lo, M, N << shift);
   unsigned bad = s.bad;
   const int j = i - s.first, pos = s.len - s.count + j;
-  if (j >= 0 && j < s.count && pos >= 0) {
+  if (!s.bad && j >= 0 && j < s.count && pos >= 0) {   // (a place made possible would be another row's)
     const int page = table[(size_t)lo * N + (pos >> shift)];
     if ((unsigned)page < (unsigned)pages) {
       const size_t to = ((((size_t)page << shift) + (pos & ((1 << shift) - 1))) * H + h) * PG_E + e;

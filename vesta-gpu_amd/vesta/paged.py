@@ -26,9 +26,11 @@ Everything stays on the device and on torch's current stream, so a call can be
 captured in a HIP graph and replayed with other contents of its tensors.
 Calls allocate their workspaces from torch's allocator, none is shared between
 two calls, which may come from several threads and streams. Tensors are checked
-on the host (``TypeError``, ``ValueError``); what lies in ``table``, ``starts`` and ``lengths`` is checked on the device,
-where an impossible value is replaced by a possible one and raises an error
-word that ``check()`` reads.
+on the host (``TypeError``, ``ValueError``); what lies in ``table``, ``starts``
+and ``lengths`` is checked on the device, where an impossible value is replaced
+by a possible one and raises an error word that ``check()`` reads: results, a
+weight updated in place among them, are then invalid. Nothing is appended for a
+sequence whose starts or length are impossible, so the cache's rows stay right.
 
 The decode cache of ``VestaGPT2`` [B, L, tmax, H, 64] (reference
 ``vesta/gpt2.py:31-33``) holds one position for all its rows; this one is for
