@@ -296,3 +296,73 @@ def test_evict_numbers_past_32_bits():
     for keep in (5, 1 << 31):
         with pytest.raises(ValueError, match='2.31'):
             c.evict(w, table, lengths, keep, torch.ones(1, 1 << 15, dtype=torch.int32))
+
+
+def _view(base, at, shape, strides):
+    return torch.as_strided(base, shape, strides, at)
+
+
+def test_outputs_apart_from_queries():
+    """out shares no memory with q, by whatever offset, and its rows none with one another; parts of one projection's
+    rows do not."""
+    c = _Dry(8, 3)
+    table, starts, lengths = _batch()
+    for dtype in (torch.float16, torch.float32):
+        flat = torch.zeros(20000, dtype=dtype)
+        q = flat[:5 * 384].view(5, 6, 64)
+        n = len(c.log)
+        for out in (flat[384:6 * 384].view(5, 6, 64),                           # a row on
+                    flat[64:5 * 384 + 64].view(5, 6, 64),                       # a head on
+                    flat[4 * 384:9 * 384].view(5, 6, 64),                       # the last row
+                    _view(flat, 384, (5, 6, 64), (768, 64, 1)),                 # between rows that lie apart, and on others
+                    _view(flat, 0, (5, 6, 64), (64, 320, 1)),                   # heads first
+                    _view(flat, 10000, (5, 6, 64), (64, 64, 1)),                # rows on heads
+                    _view(flat, 10000, (5, 6, 64), (320, 64, 1)), _view(flat, 10000, (5, 6, 64), (64, 256, 1)),
+                    _view(flat, 10000, (5, 6, 64), (384, 32, 1)), _view(flat, 10000, (5, 6, 64), (0, 64, 1))):
+            with pytest.raises(ValueError, match='out'):
+                c.attend(q, table, starts, lengths, out=out)
+        assert len(c.log) == n
+        for out in (flat[5 * 384:10 * 384].view(5, 6, 64), _view(flat, 5 * 384, (5, 6, 64), (64, 320, 1))):
+            assert c.attend(q, table, starts, lengths, out=out) is out
+        wide = torch.zeros(5, 18, 64, dtype=dtype)
+        for a, b in ((0, 6), (6, 0), (0, 12), (12, 0), (6, 12), (3, 10)):
+            c.attend(wide[:, a:a + 6], table, starts, lengths, out=wide[:, b:b + 6])
+            heads_first = torch.zeros(18, 5, 64, dtype=dtype).transpose(0, 1)
+            c.attend(heads_first[:, a:a + 6], table, starts, lengths, out=heads_first[:, b:b + 6])
+            by_head = torch.zeros(6, 18, 64, dtype=dtype).transpose(0, 1)       # 5 of 18 rows a head
+            c.attend(by_head[a:a + 5], table, starts, lengths, out=by_head[b:b + 5])
+        for a, b in ((0, 5), (5, 0), (3, 8), (6, 6)):
+            with pytest.raises(ValueError, match='out'):
+                c.attend(wide[:, a:a + 6], table, starts, lengths, out=wide[:, b:b + 6])
+        one = torch.zeros(1, 12, 64, dtype=dtype)
+        args = table, _ints(0, 0, 1), lengths
+        c.attend(one[:, :6], *args, out=one[:, 6:])
+        with pytest.raises(ValueError, match='out'):
+            c.attend(one[:, :6], *args, out=one[:, 5:11])
+
+
+def test_weights_apart():
+    """The new weights are the old ones' own memory, place by place, or none of it; an eviction's none of it."""
+    c = _Dry(8, 3)
+    table, starts, lengths = _batch()
+    q = _rows(5, 6)
+    flat = torch.zeros(8000)
+    w = flat[:6 * 200].view(2, 3, 200)
+    for at, S in ((4, 200), (1000, 200), (1199, 192), (0, 192), (0, 201)):
+        with pytest.raises(ValueError, match='weight_out'):
+            c.attend(q, table, starts, lengths, weight=w, weight_out=flat[at:at + 6 * S].view(2, 3, S))
+        with pytest.raises(ValueError, match='weight_out'):
+            c.attend(q, table, starts, lengths, weight=flat[at:at + 6 * S].view(2, 3, S), weight_out=w)
+    assert not c.log
+    for at, S in ((0, 200), (1200, 200), (1300, 192)):
+        c.attend(q, table, starts, lengths, weight=w, weight_out=flat[at:at + 6 * S].view(2, 3, S))
+    one = _Dry(8, 1)
+    one.attend(_rows(2, 2), table[:1], _ints(0, 2), lengths[:1], weight=flat[:200].view(1, 1, 200),
+               weight_out=flat[:192].view(1, 1, 192))
+    to = torch.ones(2, 1, dtype=torch.int32)
+    n = len(c.log)
+    for at in (0, 64, 1199):
+        with pytest.raises(ValueError, match='weight_out'):
+            c.evict(w[None], table, lengths, 5, to, weight_out=flat[at:at + 6 * 64].view(1, 2, 3, 64))
+    assert len(c.log) == n
+    c.evict(w[None], table, lengths, 5, to, weight_out=flat[1200:1200 + 6 * 64].view(1, 2, 3, 64))

@@ -212,6 +212,34 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
+def _grid2(shape, strides):
+    """(size, stride) of a [rows, heads, width] tensor's two outer axes, the one of shorter stride first; an axis of one
+    has no stride."""
+    return sorted(((n, s if n > 1 else 0) for n, s in zip(shape[:2], strides)), key=lambda a: a[1])
+
+
+def _collides(shape, strides):
+    """Whether rows of a [rows, heads, width] tensor may lie on one another."""
+    (n0, s0), (n1, s1) = _grid2(shape, strides)
+    return n0 > 1 and s0 < shape[2] or n1 > 1 and s1 < (n0 - 1) * s0 + shape[2]
+
+
+def _overlap(shape, size, a, b):
+    """Whether two tensors of one shape and item size, (address, row stride, head stride) each, may share memory. They do
+    not where one ends before the other, or where they are parts of one row (one head of heads-first rows), as the
+    queries of a fused projection and its other columns."""
+    ga, gb = _grid2(shape, a[1:]), _grid2(shape, b[1:])
+    last = [sum((n - 1) * s for n, s in g) + shape[2] for g in (ga, gb)]
+    apart = (b[0] - a[0]) // size
+    if apart >= last[0] or -apart >= last[1] or not shape[0] * shape[1]:
+        return False
+    pitch = ga[1][1]
+    if pitch == 0 or gb[1] != ga[1]:
+        return True
+    (f0, f1), apart = ((g[0][0] - 1) * g[0][1] + shape[2] for g in (ga, gb)), apart % pitch
+    return apart < f0 or apart + f1 > pitch
+
+
 def _dealt(n, run):
     """Blocks of a grid whose kernel deals n tasks to the device's eight XCDs in runs."""
     return 8 * run * -(-n // (8 * run))
@@ -373,14 +401,16 @@ class PagedCache:
         positions in ``layer``: softmax(``scale`` q . k), 1 / sqrt(width) by
         default, times the values. ``q`` is of the cache's type or, over an f16
         cache, f32; the result is of q's type: ``out`` [M, G * heads, width],
-        made if not given. A token that sees no position gets zeros.
+        made if not given (its memory none of q's, its rows apart from one
+        another). A token that sees no position gets zeros.
 
         ``weight`` [B, heads, S] (f32, contiguous, S at least the table's
         positions): the softmax weight that each position has received so far.
         Then the call returns (out, weight_out), where weight_out [B, heads, S'] is
         weight plus what the new tokens give, over the query heads of the key
         head; the new positions start at 0, and past the lengths it is 0.
-        ``weight_out`` may be given, ``weight`` itself is updated if it is not.
+        ``weight_out`` may be given (memory of its own), ``weight`` itself is
+        updated if it is not.
 
         ``most``: a bound of the new tokens of a sequence that the program
         knows (1 for a decode step); the work is laid out by it."""
@@ -401,15 +431,18 @@ class PagedCache:
             to = out.data_ptr(), Hq * self.width, self.width
         else:
             to = self._rows('out', out, (q.dtype,), like=q.shape)
-            if M > 1 and to[1] == 0 or Hq > 1 and to[2] == 0:
+            if _collides(q.shape, to[1:]):
                 raise ValueError(f'out: rows that lie on one another (strides {out.stride()})')
-            if to[0] == qs[0] and M:
-                raise ValueError('out: a tensor other than q (which a second pass may read again)')
+            if _overlap(q.shape, 4 if q.dtype is self._f32 else 2, qs, to):
+                raise ValueError('out: memory other than that of q (which a second pass may read again)')
         S = So = 0
         if weight is not None:
             weight_out = weight if weight_out is None else weight_out
             S, So = (self._weights(n, w, (B, self.heads), N * self.page)
                      for n, w in (('weight', weight), ('weight_out', weight_out)))
+            if weight_out is not weight and self._shared(weight, weight_out) and (
+                    weight_out.data_ptr() != weight.data_ptr() or So != S and B * self.heads > 1):
+                raise ValueError('weight_out: weight itself or other memory')
         elif weight_out is not None:
             raise ValueError('weight_out: no weight given')
         most = M if most is None else min(most, M)
@@ -529,6 +562,12 @@ class PagedCache:
             raise ValueError(f'{name}: shape {tuple(shape)}, need {lead} and {least} positions at least')
         return shape[-1]
 
+    @staticmethod
+    def _shared(a, b):
+        """Whether two contiguous tensors of 4-byte items share memory."""
+        at, to = a.data_ptr(), b.data_ptr()
+        return at < to + 4 * b.numel() and to < at + 4 * a.numel()
+
     def evict(self, weight, table, lengths, keep, to, recent=0, weight_out=None):
         """Keep ``keep`` positions of each sequence (all where it has no more):
         its ``recent`` last ones and, of the others, those of largest
@@ -558,8 +597,8 @@ class PagedCache:
         if weight_out is None:
             weight_out = self._empty(lead + (No * self.page,), dtype=self._f32, device=self.device)
         So = self._weights('weight_out', weight_out, lead, No * self.page)
-        if B and weight_out.data_ptr() == weight.data_ptr():
-            raise ValueError('weight_out: a tensor other than weight')
+        if self._shared(weight, weight_out):
+            raise ValueError('weight_out: memory other than that of weight')
         kept = self._empty(lead + (keep,), dtype=self._i32, device=self.device)
         new = self._empty(B, dtype=self._i32, device=self.device)
         if B == 0:
