@@ -231,7 +231,7 @@ def _overlap(shape, size, a, b):
     ga, gb = _grid2(shape, a[1:]), _grid2(shape, b[1:])
     last = [sum((n - 1) * s for n, s in g) + shape[2] for g in (ga, gb)]
     apart = (b[0] - a[0]) // size
-    if apart >= last[0] or -apart >= last[1] or not shape[0] * shape[1]:
+    if apart >= last[0] or -apart >= last[1] or not shape[0]:
         return False
     pitch = ga[1][1]
     if pitch == 0 or gb[1] != ga[1]:
@@ -431,9 +431,15 @@ class PagedCache:
             to = out.data_ptr(), Hq * self.width, self.width
         else:
             to = self._rows('out', out, (q.dtype,), like=q.shape)
-            if _collides(q.shape, to[1:]):
+            q_at, q_row, q_head = qs
+            o_at, o_row, o_head = to
+            E, size = self.width, 4 if q.dtype is self._f32 else 2
+            # (what most calls are is told by a line each: the whole rules take 3 us more)
+            if not (o_head >= E and o_row >= (Hq - 1) * o_head + E) and _collides(q.shape, (o_row, o_head)):
                 raise ValueError(f'out: rows that lie on one another (strides {out.stride()})')
-            if _overlap(q.shape, 4 if q.dtype is self._f32 else 2, qs, to):
+            if q_at < o_at + size * ((M - 1) * o_row + (Hq - 1) * o_head + E) \
+                    and o_at < q_at + size * ((M - 1) * q_row + (Hq - 1) * q_head + E) \
+                    and _overlap(q.shape, size, qs, to):
                 raise ValueError('out: memory other than that of q (which a second pass may read again)')
         S = So = 0
         if weight is not None:
