@@ -717,3 +717,18 @@ def test_an_impossible_sequence_appends_nothing(new):
         with pytest.raises(RuntimeError, match='length|starts'):
             b.cache.check()
         rows = rows + 1
+
+
+def test_check_waits_for_other_streams():
+    """An error of a call that another stream has not reached yet is found, and only once."""
+    b = Batch([2], [40], 2, 1, 64, 16)
+    x = torch.randn(8192, 8192, device='cuda').bfloat16()
+    bad = _ints([1 << 20])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for _ in range(20):
+            x @ x                                        # some 15 ms
+        b.cache.append(b.q, b.q, b.table, b.starts, bad)
+    with pytest.raises(RuntimeError, match='length'):
+        b.cache.check()
+    b.cache.check()

@@ -366,3 +366,31 @@ def test_weights_apart():
             c.evict(w[None], table, lengths, 5, to, weight_out=flat[at:at + 6 * 64].view(1, 2, 3, 64))
     assert len(c.log) == n
     c.evict(w[None], table, lengths, 5, to, weight_out=flat[1200:1200 + 6 * 64].view(1, 2, 3, 64))
+
+
+def test_an_error_during_check_is_kept():
+    """check() reads and clears the word in one step: what a call of another thread raises next is the next check's."""
+    import ctypes
+    c = _Dry(8, 3)
+    c._wait = lambda: None
+
+    class Device(_Recorder):
+        def __getattr__(self, name):
+            record = super().__getattr__(name)
+
+            def launch(grid, block, stream, err, took):
+                record(grid, block, stream, err, took)
+                word = ctypes.c_int.from_address(err)
+                ctypes.c_int.from_address(took).value = word.value
+                word.value = next_word
+            return launch
+    c._kind = {c.dtype: Device(c.log)}
+    c.err.fill_(1)
+    next_word = 4
+    with pytest.raises(RuntimeError, match='page id'):
+        c.check()
+    next_word = 0
+    with pytest.raises(RuntimeError, match='length'):
+        c.check()
+    c.check()
+    assert [e[0] for e in c.log] == ['pg_take'] * 3

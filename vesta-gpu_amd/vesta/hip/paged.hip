@@ -33,6 +33,11 @@ __device__ __forceinline__ void pg_raise(unsigned* err, unsigned bits) {
   __hip_atomic_fetch_or(err, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// The error word, read and cleared at once.
+extern "C" __global__ __launch_bounds__(64) void pg_take(unsigned* __restrict__ err, unsigned* __restrict__ took) {
+  if (threadIdx.x == 0) *took = __hip_atomic_exchange(err, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // x / d of whole numbers, x >= 0 and d > 0: the compiler's 32-bit division is
 // some 35 dependent operations, and a small call waits for half a dozen. Below
 // 2^22 the reciprocal's quotient is off by one at most.

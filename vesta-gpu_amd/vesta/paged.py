@@ -131,6 +131,7 @@ SIGNATURES = {
     'pg_total': 'pippiiiipipii',
     'pg_select': 'pipiiiiippipp',
     'pg_move': 'ppiipipipiiiip',
+    'pg_take': 'pp',
 }
 
 
@@ -624,12 +625,24 @@ class PagedCache:
             self._leave(back)
         return new, weight_out, kept
 
+    def _wait(self):
+        """For all the device's streams."""
+        import torch
+        torch.cuda.synchronize(self.device)
+
     def check(self):
-        """Raise if an earlier call met a page, a length or starts that cannot
-        be (one synchronisation); the word is cleared first."""
-        word = int(self.err.item())
+        """Raise if an earlier call, on any stream, met a page, a length or
+        starts that cannot be (waits for the device); the word is cleared in
+        the same step, so that none raised meanwhile is lost."""
+        self._wait()
+        took = self._empty(1, dtype=self._i32, device=self.device)
+        stream, back = self._enter()
+        try:
+            self._kind[self.dtype].pg_take(1, 64, stream, self._err, took.data_ptr())
+        finally:
+            self._leave(back)
+        word = int(took.item())
         if word:
-            self.err.zero_()
             why = ', '.join(text for bit, text in ERRORS.items() if word & bit)
             raise RuntimeError(f'paged cache: {why}; the results are invalid')
 
