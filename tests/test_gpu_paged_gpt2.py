@@ -254,3 +254,38 @@ def test_refusals(hf):
     a = a.clone()
     b, _ = m.extend(**{**ok, 'tokens': _ints([V - 1, 0]), 'positions': _ints([1023, 0])})
     assert torch.equal(a, b)
+
+
+def test_positions_and_ids_outside_their_tables(hf):
+    """A conversation past the learned positions and an id past the vocabulary are errors; what padded rows hold is not:
+    a sequence of length 0 in a batch of fixed size, a row before a sequence's first, rows behind the last sequence."""
+    from vesta.gpt2 import VestaGPT2
+    from vesta.paged import PagedCache
+    m = VestaGPT2(hf, batch=1, tmax=32, engine='layered')
+    cache = PagedCache(8, H, 64, layers=L, page=16)
+    table = _ints([[0], [1], [2]])
+    ok = dict(tokens=[1, 2, 3, 4, 5, 6], positions=[0, 1023, 0, 0, 1, 0])
+    batch = (table, _ints([0, 2, 3, 5]), _ints([2, 0, 1]))         # the second is padding, the third's first row too
+    rows = (0, 1, 4)
+
+    def call(tokens, positions):
+        out, _ = m.extend(cache, _ints(tokens), _ints(positions), *batch)
+        return out.clone()
+
+    want = call(**ok)
+    cache.check()
+    for what, low, high, text in (('positions', 0, 1023, 'position'), ('tokens', 0, V - 1, 'token id')):
+        for value in (-1, high + 1, -1 << 31, (1 << 31) - 1):
+            for i in range(6):
+                a = {**ok, what: list(ok[what])}
+                a[what][i] = value
+                got = call(**a)
+                if i in rows:
+                    with pytest.raises(RuntimeError, match=text):
+                        cache.check()
+                    a[what][i] = low if value < 0 else high
+                    assert torch.equal(got[0::2], call(**a)[0::2])
+                else:
+                    assert torch.equal(got[0::2], want[0::2])
+                cache.check()
+    m.check()

@@ -320,8 +320,9 @@ class VestaGPT2:
         rows lie in ``cache``, a ``vesta.paged.PagedCache`` of this model's
         layers and heads (f16), instead of this object's own: ``tokens`` and
         ``positions`` (int32 device tensors [M]; which learned position each
-        has, its count in the conversation whatever has been evicted) are the
-        rows of the batch that ``table``, ``starts`` and ``lengths`` describe
+        has, its count in the conversation whatever has been evicted: as many
+        as ``wpe`` has rows, so a conversation ends there or starts its count
+        anew) are the rows of the batch that ``table``, ``starts`` and ``lengths`` describe
         (``vesta.paged``). Chunks of prompts and single tokens may be mixed.
         Returns (logits [B, vocabulary], next [B]) of each sequence's last new
         token (of no meaning for a sequence without one), which the next call
@@ -333,7 +334,9 @@ class VestaGPT2:
         Nothing is read back, so a call can be captured in a HIP graph, after
         one call of as many tokens and sequences. Calls share this object's
         activation buffers, those of two streams must not overlap.
-        ``check()`` and ``cache.check()`` report what went wrong."""
+        ``check()`` and ``cache.check()`` report what went wrong: a position
+        or id outside its table is clamped into it, and an error of the
+        cache's if its row is a sequence's."""
         import torch
         from .paged import PagedCache, PagedPass
         from .prefill import Prefill, supported

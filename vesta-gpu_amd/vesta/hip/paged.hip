@@ -25,6 +25,8 @@
 #define PG_ERR_STARTS 2u        // starts not ascending, or past the rows
 #define PG_ERR_LENGTH 4u        // a length past the table
 #define PG_ERR_MOST 8u          // a sequence with more new tokens than `most`
+#define PG_ERR_POSITION 16u     // a position past the model's learned ones
+#define PG_ERR_TOKEN 32u        // a token id outside the vocabulary
 
 typedef __bf16 pg_b8 __attribute__((ext_vector_type(8)));
 typedef float pg_f8 __attribute__((ext_vector_type(8)));
@@ -62,6 +64,16 @@ __device__ __forceinline__ PgSeq pg_seq(const int* __restrict__ starts, const in
   s.len = min(max(n, 0), cap);
   s.bad = (s.first != a || end != e ? PG_ERR_STARTS : 0u) | (s.len != n ? PG_ERR_LENGTH : 0u);
   return s;
+}
+
+// Row i's sequence: the last whose first row is at or before it.
+__device__ __forceinline__ int pg_owner(const int* __restrict__ starts, int B, int i) {
+  int lo = 0, hi = B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= i) lo = mid; else hi = mid;
+  }
+  return lo;
 }
 
 // One element of a 16-bit word pair as fp32, and eight floats as 16-bit values
@@ -111,12 +123,7 @@ __device__ __forceinline__ void pg_append_body(const T* __restrict__ k, const T*
   const int h = c / (PG_E / 8), e = c % (PG_E / 8) * 8;
   const vh_u32x4 kx = pg_load8(k + i * krow + h * khead + e), vx = pg_load8(v + i * vrow + h * vhead + e);
   __builtin_amdgcn_sched_barrier(0);                    // in flight while the place is looked up
-  // the last sequence whose first row is at or before i
-  int lo = 0, hi = B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= i) lo = mid; else hi = mid;
-  }
+  const int lo = pg_owner(starts, B, i);
   const PgSeq s = pg_seq(starts, lengths, lo, M, N << shift);
   unsigned bad = s.bad;
   const int j = i - s.first, pos = s.len - s.count + j;
@@ -143,6 +150,35 @@ __device__ __forceinline__ void pg_append_body(const T* __restrict__ k, const T*
   }
 PG_APPEND(pg_append16, unsigned short)
 PG_APPEND(pg_append32, float)
+
+// What a model's pass over the cache begins with: the tokens' ids, and the rows
+// of their learned positions (ids and positions outside their tables clamped
+// into them, the ids by the embedding), eight elements a thread. An error where
+// a row that is a sequence's has such a one; padded rows may hold anything.
+extern "C" __global__ __launch_bounds__(256) void pg_input(const int* __restrict__ tokens,
+                                                           const int* __restrict__ positions,
+                                                           const unsigned short* __restrict__ wpe, int npos, int D, int V,
+                                                           const int* __restrict__ starts,
+                                                           const int* __restrict__ lengths, int B, int M, int cap,
+                                                           int* __restrict__ tok, unsigned short* __restrict__ rows,
+                                                           unsigned* __restrict__ err) {
+  const int per = D / 8;
+  const long at = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  const int i = (int)(at / per), c = (int)(at % per);
+  if (i >= M) return;
+  const int p = positions[i];
+  *(vh_u32x4*)(rows + (size_t)i * D + 8 * c) = ld16(wpe + (size_t)min(max(p, 0), npos - 1) * D + 8 * c);
+  if (c) return;
+  const int id = tokens[i];
+  tok[i] = id;
+  const unsigned bad = ((unsigned)p >= (unsigned)npos ? PG_ERR_POSITION : 0u)
+                       | ((unsigned)id >= (unsigned)V ? PG_ERR_TOKEN : 0u);
+  if (!bad) return;
+  const int b = pg_owner(starts, B, i);
+  const PgSeq s = pg_seq(starts, lengths, b, M, cap);
+  const int j = i - s.first;
+  if (j >= 0 && j < s.count && s.len - s.count + j >= 0) pg_raise(err, bad);
+}
 
 // ---------------------------------------------------------------- attention
 // Matrix-core products over 16-bit operands: lane l = 16 q + r holds row r,

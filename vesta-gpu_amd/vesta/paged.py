@@ -111,7 +111,8 @@ SCORES_ROWS = 8
 WEIGH_BLOCKS = 2048
 SELECT_FEW = 4096             # positions up to which pg_select has 256 threads, not 1024 (1152 times 1024: 13 / 38)
 ERRORS = {1: 'a page id outside the pool', 2: 'starts that do not ascend, or lie past the rows',
-          4: 'a length past its table', 8: 'a sequence with more new tokens than `most`'}
+          4: 'a length past its table', 8: 'a sequence with more new tokens than `most`',
+          16: "a position past the model's learned ones", 32: 'a token id outside the vocabulary'}
 
 # parameters of the kernels: p a pointer, l a 64-bit, i a 32-bit whole number, f an fp32
 _SEQS = 'iipipp'                       # pages, shift, table, its columns, starts, lengths
@@ -132,6 +133,7 @@ SIGNATURES = {
     'pg_select': 'pipiiiiippipp',
     'pg_move': 'ppiipipipiiiip',
     'pg_take': 'pp',
+    'pg_input': 'pppiiippiiippp',
 }
 
 
@@ -765,8 +767,14 @@ class PagedPass(Prefill):
         embed, qkv, rest, head = self._launches(M, B)
         b = self._buf
         wpe = self.m.W['wpe']
-        b.tok[:M].copy_(tokens)
-        torch.index_select(wpe, 0, positions.clamp(0, wpe.shape[0] - 1), out=b.wpe[:M])
+        stream, back = cache._enter()
+        try:
+            cache._kind[cache.dtype].pg_input(
+                -(-M * (self.m.D // 8) // BLOCK), BLOCK, stream, tokens.data_ptr(), positions.data_ptr(), wpe.data_ptr(),
+                wpe.shape[0], self.m.D, self.m.W['wte'].shape[0], starts.data_ptr(), lengths.data_ptr(), B, M,
+                table.shape[1] * cache.page, b.tok.data_ptr(), b.wpe.data_ptr(), cache._err)
+        finally:
+            cache._leave(back)
         q, o, k, v = (t[:M].view(M, H, -1) for t in (b.Q, b.O, b.K, b.V))
         self._replay(embed)
         for layer in range(self.layers):
