@@ -394,3 +394,25 @@ def test_an_error_during_check_is_kept():
         c.check()
     c.check()
     assert [e[0] for e in c.log] == ['pg_take'] * 3
+
+
+def test_gradients_are_refused():
+    """Nothing here has a backward pass: a tensor whose gradient is being recorded is refused, not answered without."""
+    c = _Dry(8, 3)
+    table, starts, lengths = _batch()
+    q, g = _rows(5, 3), _rows(5, 3).requires_grad_()
+    w, gw = torch.zeros(2, 3, 192), torch.zeros(2, 3, 192).requires_grad_()
+    to = torch.ones(2, 1, dtype=torch.int32)
+    calls = (lambda: c.append(g, q, table, starts, lengths), lambda: c.append(q, g, table, starts, lengths),
+             lambda: c.attend(g, table, starts, lengths), lambda: c.attend(q, table, starts, lengths, out=g),
+             lambda: c.attend(g * 2, table, starts, lengths), lambda: c.attend(q, table, starts, lengths, weight=gw),
+             lambda: c.attend(q, table, starts, lengths, weight=w, weight_out=gw),
+             lambda: c.evict(gw[None], table, lengths, 5, to))
+    for call in calls:
+        with pytest.raises(ValueError, match='gradient'):
+            call()
+    assert not c.log
+    with torch.no_grad():
+        for call in calls:
+            call()
+    c.attend(g.detach(), table, starts, lengths)

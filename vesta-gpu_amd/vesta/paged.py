@@ -31,6 +31,8 @@ and ``lengths`` is checked on the device, where an impossible value is replaced
 by a possible one and raises an error word that ``check()`` reads: results, a
 weight updated in place among them, are then invalid. Nothing is appended for a
 sequence whose starts or length are impossible, so the cache's rows stay right.
+Nothing here has a backward pass: a tensor whose gradient is being recorded is
+refused (``ValueError``).
 
 The decode cache of ``VestaGPT2`` [B, L, tmax, H, 64] (reference
 ``vesta/gpt2.py:31-33``) holds one position for all its rows; this one is for
@@ -302,6 +304,7 @@ class PagedCache:
         self._pools = self.keys.data_ptr(), self.vals.data_ptr()
         self._index = self.keys.get_device()
         self._i32, self._f32, self._empty = torch.int32, torch.float32, torch.empty
+        self._recording = torch.is_grad_enabled
         self._new = self.dtype, self._f32                          # types of new rows, and of queries
         self._queries = self._new if self._dt == 'f16' else (self.dtype,)
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -346,11 +349,17 @@ class PagedCache:
                 or (like is not None and shape != like):
             raise ValueError(f'{name}: shape {tuple(shape)}, need '
                              f'{tuple(like) if like is not None else ("rows", heads or "heads", self.width)}')
+        if t.requires_grad and self._recording():
+            self._no_gradient(name)
         row, head, one = t.stride()
         at = t.data_ptr()
         if (one != 1 or (row | head) & (3 if t.dtype is self._f32 else 7) or at & 15) and t.numel():
             raise ValueError(f'{name}: rows of consecutive, 16-byte aligned values needed (strides {t.stride()})')
         return at, row, head
+
+    @staticmethod
+    def _no_gradient(name):
+        raise ValueError(f'{name}: no gradient is made of it; detach it, or call under torch.no_grad()')
 
     def _layer(self, layer):
         layer = operator.index(layer)
@@ -567,6 +576,8 @@ class PagedCache:
             fits = False
         if not fits:
             raise TypeError(f'{name}: need a contiguous float32 tensor on {self.device}')
+        if w.requires_grad and self._recording():
+            self._no_gradient(name)
         if tuple(shape[:-1]) != lead or not least <= shape[-1] < 1 << 31:
             raise ValueError(f'{name}: shape {tuple(shape)}, need {lead} and {least} positions at least')
         return shape[-1]
