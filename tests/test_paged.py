@@ -416,3 +416,27 @@ def test_gradients_are_refused():
         for call in calls:
             call()
     c.attend(g.detach(), table, starts, lengths)
+
+
+def test_extend_on_the_models_device():
+    """A cache of another device is refused; the model's launches are made with its device the current one."""
+    from vesta.gpt2 import VestaGPT2
+    c = _Dry(8, 3)
+    within = []
+    c._enter = lambda: (within.append(1), (0, 'back'))[1]
+    c._leave = lambda back: within.append(back)
+
+    class Pass:
+        def run(self, *a):
+            return list(within)
+    m = object.__new__(VestaGPT2)
+    m.L, m.H, m.E, m.D, m._pf, m._paged = 1, 3, 64, 192, Pass(), Pass()
+    table, starts, lengths = _batch()
+    batch = _ints(*[0] * 5), _ints(*[0] * 5), table, starts, lengths
+    weights = dict(fcw=torch.zeros(1, 192, 768, dtype=torch.float16))
+    m.W = dict(wte=torch.zeros(5, 192, dtype=torch.float16, device='meta'), **weights)
+    with pytest.raises(ValueError, match='device'):
+        m.extend(c, *batch)
+    assert not within
+    m.W = dict(wte=torch.zeros(5, 192, dtype=torch.float16), **weights)
+    assert m.extend(c, *batch) == [1] and within == [1, 'back']

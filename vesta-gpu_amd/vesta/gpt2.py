@@ -346,6 +346,8 @@ class VestaGPT2:
         have = (cache.layers, cache.heads, cache.width, cache.dtype)
         if have != want:
             raise ValueError(f'cache of (layers, heads, width, type) {have}, the model has {want}')
+        if cache.device != self.W['wte'].device:
+            raise ValueError(f"cache on device {cache.device}, the model on {self.W['wte'].device}")
         if not supported(self.D, self.H, self.W['fcw'].shape[2]):
             raise ValueError('extend needs 64-wide heads and widths that are multiples of 64')
         for name, t in (('tokens', tokens), ('positions', positions)):
@@ -359,13 +361,17 @@ class VestaGPT2:
             raise ValueError(f'table {tuple(table.shape)}: one sequence and one page at least')
         if weight is not None:
             cache._weights('weight', weight, (self.L, B, self.H), N * cache.page)
-        if self._paged is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError('extend: call once before capturing such a call')
-            if self._pf is None:
-                self._pf = Prefill(self)
-            self._paged = PagedPass(self, self._pf)
-        return self._paged.run(cache, tokens, positions, table, starts, lengths, weight, most)
+        _, back = cache._enter()             # (the layers' launches go to the current device's stream)
+        try:
+            if self._paged is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError('extend: call once before capturing such a call')
+                if self._pf is None:
+                    self._pf = Prefill(self)
+                self._paged = PagedPass(self, self._pf)
+            return self._paged.run(cache, tokens, positions, table, starts, lengths, weight, most)
+        finally:
+            cache._leave(back)
 
     def warm(self, n):
         """n decode steps through the prefill kernel (untimed warm-up)."""
