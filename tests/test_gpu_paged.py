@@ -732,3 +732,42 @@ def test_check_waits_for_other_streams():
     with pytest.raises(RuntimeError, match='length'):
         b.cache.check()
     b.cache.check()
+
+
+@pytest.mark.parametrize('width', (64, 128))
+@pytest.mark.parametrize('parts', (False, True))
+@pytest.mark.parametrize('kept', (False, True))
+def test_every_bit_of_fp32_queries(blocks, monkeypatch, width, parts, kept):
+    """Outputs and received weights to the last bits of 24, by every kernel (what is lost without a plane, and the bounds:
+    paged_planes.py, whose own test plants that on the CPU)."""
+    import paged_planes as pp
+    from vesta import paged
+    if parts:
+        for name, value in dict(SPLIT={64: 0, 128: 0}, WIDE_SPLIT=0, PART_STEPS=1, WIDE_PART_STEPS=1, TARGET=16).items():
+            monkeypatch.setattr(paged, name, value)
+    monkeypatch.setattr(paged, 'SCORES_ROWS', 1 << 30 if kept else 0)
+    G = 2
+    b = Batch([1, 200, 3], [2, 300, 140], 2, G, width, 16, 'f16', 'f32')
+    for pool in (b.cache.keys, b.cache.vals):
+        pool.nan_to_num_(0.0).zero_()
+    for i in range(3):
+        for s, v in ((0, 1.0), (1, -1.0)):
+            b.cache.keys[0, b.table[i, 0], s, :, s] = 1.0
+            b.cache.vals[0, b.table[i, 0], s] = v
+    x = pp.gaps(204 * 2 * G, width).view(204, 2 * G)
+    b.q.zero_()
+    b.q[:, :, 0] = 512.0
+    b.q[:, :, 1] = (512.0 - x).to(b.q)
+    assert torch.equal(b.q[:, :, 1].double().cpu(), 512.0 - x)
+    out, bound, w0, w1, rel = pp.answer(x)
+    got, w = b.attend(scale=pp.SCALE, weight=torch.zeros(3, 2, b.table.shape[1] * 16, device='cuda'))
+    wide = [t.cuda()[..., None].expand(204, 2 * G, width) for t in (out, bound)]
+    _close(got, *wide)
+    _close(b.attend(scale=pp.SCALE), *wide)
+    rows = [0, 1, 201, 204]
+    for i in range(3):
+        for s, one in ((0, w0), (1, w1)):
+            want = one[rows[i]:rows[i + 1]].reshape(-1, 2, G).sum((0, 2)).cuda()
+            _close(w[i, :, s], want, want * (rel + G * b.counts[i] * 2.0 ** -24))
+    assert not w[:, :, 2:].any()
+    b.cache.check()
