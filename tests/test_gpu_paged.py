@@ -647,7 +647,7 @@ def test_a_long_tail_keeps_its_mass(blocks, dtype, query, width, below):
     value of 4096: the output is theirs alone, in whatever part, step and wave they come.
 
     A tail weight is off by its rounding to 16 bits, half a step of itself, or half of fp16's fixed step where it is
-    small: the largest weight is 2^11 at least, so that is 2^-36 of the largest (bf16 has none; fp32 queries' planes
+    small: 2^-25, of a largest weight of 2^9 at least, so 2^-34 of the largest (bf16 has none; fp32 queries' planes
     carry 24 bits of it); by 2^-22 and 4 half steps of the largest score's fp32 exponent (below half steps of 32 at
     most) otherwise, as is the sum; the sums of up to 3000 positions by a half step each."""
     counts, lengths = [1, 140, 3], [3000, 700, 96]
@@ -666,7 +666,7 @@ def test_a_long_tail_keeps_its_mass(blocks, dtype, query, width, below):
     want, *_ = b.want(scale=scale)
     w = 2.0 ** -below
     u = 2.0 ** -24
-    rounded = 0.0 if query == 'f32' else max(torch.finfo(DT[dtype]).eps / 2, 2.0 ** -36 / w if dtype == 'f16' else 0.0)
+    rounded = 0.0 if query == 'f32' else max(torch.finfo(DT[dtype]).eps / 2, 2.0 ** -34 / w if dtype == 'f16' else 0.0)
     rel = rounded + 2 * (2.0 ** -22 + 4 * 32 * u) + 3000 * u
     ur = u if query == 'f32' else torch.finfo(DT[query]).eps / 2
     bound = want * (rel + ur) * 1.01 + (2.0 ** -25 if query == 'f16' else 0.0)

@@ -319,16 +319,18 @@ __device__ __forceinline__ void pg_scores(const vh_u32x4* kf, const PgQuery& qf,
 #endif
 }
 
-// Weights are 2^(score - reference), the reference a running one PG_BIAS below
-// the row's largest score: fp16, which holds the second product's operand, has
-// full precision down to 2^-14 only and nothing below 2^-25, so the largest
-// weight is 2^15 and a long tail of small ones keeps its mass down to 2^-40 of
-// it (with a largest of 1, positions 2^-25.5 below one lost all of theirs, while
-// the sum counted it). fp32's three planes want 2^14 (their second is 2^11 times
-// what the first leaves), pg_wide's largest may be 2^PG_SLACK more. bf16 has the
-// range. Sums, weighted values and the parts' maxima are all against the
-// reference, so that it cancels.
-#define PG_SLACK (PG_KIND == PG_BF16 ? 8 : 4)
+// Weights are 2^(score - reference), the reference a running one below the row's
+// largest score: fp16, which holds the second product's operand, has full
+// precision down to 2^-14 only and nothing below 2^-25, so the largest weight is
+// 2^15 and a long tail of small ones keeps its mass down to 2^-40 of it (with a
+// largest of 1, positions 2^-25.5 below one lost all of theirs, while the sum
+// counted it). pg_wide's may grow by 2^PG_SLACK before it rescales (fp16, 4 x 600
+// after 500 of width 128, slack 4 / 6 / 8: 58.0 / 56.7 / 56.7 us), so its largest
+// is 2^9 at first and its tail reaches to 2^-34. fp32's three planes want 2^14
+// (their second is 2^11 times what the first leaves); bf16 has the range. Sums,
+// weighted values and the parts' maxima are all against the reference, so that it
+// cancels.
+#define PG_SLACK (PG_KIND == PG_BF16 ? 8 : 6)
 #define PG_ATTN_BIAS (PG_KIND == PG_BF16 ? 0 : PG_KIND == PG_F32 ? 14 : 15)
 #define PG_WIDE_BIAS (PG_KIND == PG_BF16 ? 0 : PG_KIND == PG_F32 ? 14 : 15 - PG_SLACK)
 // The reference of a largest score bm k2: rounded up where the nearest would
@@ -1079,9 +1081,10 @@ __device__ __forceinline__ void pg_wide_body(
       for (int j = 1; j < 16; ++j) bm = fmaxf(bm, fmaxf(s[0][j], s[1][j]));
     }
     bm = vh_pair32(bm, op_max);
-    const float n2 = pg_reference<PG_WIDE_BIAS>(bm, scale2);
-    if (__any(n2 - m2 > (float)PG_SLACK)) {                        // (a first one too: m2 is -inf)
-      const float m = fmaxf(m2, n2);
+    // (a first one too: m2 is -inf; what pg_reference may add to it counts, and is added where it is taken)
+    const float n2 = fmaf(bm, scale2, -(float)PG_WIDE_BIAS);
+    if (__any(fmaf(__builtin_fabsf(n2), 0x1p-23f, n2 - m2) > (float)PG_SLACK)) {
+      const float m = fmaxf(m2, pg_reference<PG_WIDE_BIAS>(bm, scale2));
       const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - m);
       m2 = m;
       sum *= c;
