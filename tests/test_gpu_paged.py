@@ -771,3 +771,42 @@ def test_every_bit_of_fp32_queries(blocks, monkeypatch, width, parts, kept):
             _close(w[i, :, s], want, want * (rel + G * b.counts[i] * 2.0 ** -24))
     assert not w[:, :, 2:].any()
     b.cache.check()
+
+
+@pytest.mark.parametrize('dtype,query', KINDS)
+@pytest.mark.parametrize('width', (64, 128))
+@pytest.mark.parametrize('parts', (False, True))
+def test_a_nan_far_below_the_largest_score(blocks, monkeypatch, dtype, query, width, parts):
+    """A visible NaN reaches the output whatever its position's weight, also one that fp32 has as 0: 0 * NaN."""
+    from vesta import paged
+    if parts:
+        for name, value in dict(SPLIT={64: 0, 128: 0}, WIDE_SPLIT=0, PART_STEPS=1, WIDE_PART_STEPS=1, TARGET=64).items():
+            monkeypatch.setattr(paged, name, value)
+    for counts, lengths in (([1, 3], [3000, 200]), ([140], [1500])):
+        b = Batch(counts, lengths, 2, 1, width, 16, dtype, query)
+        b.q.zero_()
+        b.q[:, :, 0] = 1.0
+        for i in range(len(counts)):
+            for s in range(112):
+                b.cache.keys[0, b.table[i, s // 16], s % 16, :, 0] = -400.0
+        b.cache.vals[0, b.table[:, 0].long(), 10, 0, 3] = math.nan
+        want, bound, *_ = b.want(scale=1.0)
+        assert want[:, 0, 3].isnan().all() and want.isnan().sum() == len(want)
+        _close(b.attend(scale=1.0), want, bound)
+        b.cache.keys[0, b.table[:, 0].long(), 12, 1, 5] = math.nan
+        got, w = b.attend(scale=1.0, weight=torch.zeros(len(counts), 2, b.table.shape[1] * 16, device='cuda'))
+        assert got[:, 1].isnan().all() and got[:, 0].isnan().sum() == len(want)
+        assert w[:, 1, :100].isnan().all() and not w[:, 0].isnan().any()
+
+
+def test_an_empty_table():
+    """Sequences that can hold nothing: their tokens see nothing, as padded rows do."""
+    from vesta.paged import PagedCache
+    for dtype, query in KINDS:
+        c = PagedCache(2, 2, 64, page=16, dtype=dtype)
+        q = torch.ones(5, 4, 64, device='cuda', dtype=DT[query])
+        out, w = c.attend(q, torch.empty(2, 0, dtype=torch.int32, device='cuda'), _ints([0, 2, 5]), _ints([0, 0]),
+                          weight=torch.ones(2, 2, 7, device='cuda'))
+        assert not out.any() and not w.any()
+        c.append(q[:, :2], q[:, :2], torch.empty(2, 0, dtype=torch.int32, device='cuda'), _ints([0, 2, 5]), _ints([0, 0]))
+        c.check()

@@ -1388,7 +1388,7 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
       float pm[8], ps[8];
       vh_f32x4 pv[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {                                // past the last: the last again, without weight
+      for (int u = 0; u < 8; ++u) {                                // past the last: the last again, not counted
         const int p = p0 + u * slices;
         const float* w = wp + min(p, parts - 1) * next;
         pm[u] = p < parts ? w[y] : -INFINITY;
@@ -1404,10 +1404,9 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
       v *= old;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        // a part without a score has no weight, unless its sum is a NaN, which it keeps
-        const float f = p0 + u * slices >= parts ? 0.0f : pm[u] == -INFINITY ? (ps[u] == ps[u] ? 0.0f : 1.0f)
-                                                                             : __builtin_amdgcn_exp2f(pm[u] - mm);
-        if (f != 0.0f) {
+        // a part without a score, or far below the largest, has no weight; a NaN in it stays one (0 * NaN)
+        const float f = pm[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[u] - mm);
+        if (p0 + u * slices < parts) {
           sum = fmaf(ps[u], f, sum);
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] = fmaf(pv[u][j], f, v[j]);
@@ -1425,13 +1424,12 @@ __device__ __forceinline__ void pg_join_body(const int* __restrict__ starts, con
     if (slice > 0) return;
     float mm = m;
     for (int k = 1; k < slices; ++k) mm = fmaxf(mm, jm[grp + k * n2]);
-    const float old = m == -INFINITY ? (sum == sum ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - mm);
+    const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
     sum *= old;
     v *= old;
     for (int k = 1; k < slices; ++k) {
       const float km = jm[grp + k * n2], ks = js[grp + k * n2];
-      const float f = km == -INFINITY ? (ks == ks ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(km - mm);
-      if (f == 0.0f) continue;
+      const float f = km == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(km - mm);
       sum = fmaf(ks, f, sum);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = fmaf(jv[tid + k * n2 * LR][j], f, v[j]);
