@@ -737,7 +737,8 @@ def test_check_waits_for_other_streams():
 @pytest.mark.parametrize('width', (64, 128))
 @pytest.mark.parametrize('parts', (False, True))
 @pytest.mark.parametrize('kept', (False, True))
-def test_every_bit_of_fp32_queries(blocks, monkeypatch, width, parts, kept):
+@pytest.mark.parametrize('base', (512.0, 0.75))
+def test_every_bit_of_fp32_queries(blocks, monkeypatch, width, parts, kept, base):
     """Outputs and received weights to the last bits of 24, by every kernel (what is lost without a plane, and the bounds:
     paged_planes.py, whose own test plants that on the CPU)."""
     import paged_planes as pp
@@ -750,16 +751,18 @@ def test_every_bit_of_fp32_queries(blocks, monkeypatch, width, parts, kept):
     b = Batch([1, 200, 3], [2, 300, 140], 2, G, width, 16, 'f16', 'f32')
     for pool in (b.cache.keys, b.cache.vals):
         pool.nan_to_num_(0.0).zero_()
+    b.cache.keys[..., 2] = -1000.0
     for i in range(3):
+        b.cache.keys[0, b.table[i, 0], :2] = 0.0
         for s, v in ((0, 1.0), (1, -1.0)):
             b.cache.keys[0, b.table[i, 0], s, :, s] = 1.0
             b.cache.vals[0, b.table[i, 0], s] = v
-    x = pp.gaps(204 * 2 * G, width).view(204, 2 * G)
+    x = pp.gaps(204 * 2 * G, width, base).view(204, 2 * G)
     b.q.zero_()
-    b.q[:, :, 0] = 512.0
-    b.q[:, :, 1] = (512.0 - x).to(b.q)
-    assert torch.equal(b.q[:, :, 1].double().cpu(), 512.0 - x)
-    out, bound, w0, w1, rel = pp.answer(x)
+    b.q[:, :, 0], b.q[:, :, 2] = base, 1.0
+    b.q[:, :, 1] = (base - x).to(b.q)
+    assert torch.equal(b.q[:, :, 1].double().cpu(), base - x)
+    out, bound, w0, w1, rel = pp.answer(x, base)
     got, w = b.attend(scale=pp.SCALE, weight=torch.zeros(3, 2, b.table.shape[1] * 16, device='cuda'))
     wide = [t.cuda()[..., None].expand(204, 2 * G, width) for t in (out, bound)]
     _close(got, *wide)

@@ -443,14 +443,18 @@ def test_extend_on_the_models_device():
 
 
 def test_a_lost_plane_shows():
-    """The GPU tests' rows of fp32 queries: right with three planes of queries and weights, off with fewer of either."""
+    """The GPU tests' rows of fp32 queries: right with three planes of queries and weights, off with fewer of either, or
+    with weights that are made larger by their exponents."""
     import paged_planes as pp
-    x = pp.gaps(400, 1)
-    out, bound, *_ = pp.answer(x)
-    for queries, weights in ((3, 3), (2, 3), (3, 2), (1, 3), (3, 1)):
-        off = ((pp.emulate(x, queries, weights) - out).abs() > bound).sum()
-        assert off == 0 if (queries, weights) == (3, 3) else off > 40, (queries, weights, int(off))
+    for base in pp.BASES:
+        x = pp.gaps(400, 1, base)
+        out, bound, *_ = pp.answer(x, base)
+        wrong = ((3, 2), (1, 3), (3, 1)) + (((2, 3),) if base == 512.0 else ((3, 3, 14),))
+        for planes in ((3, 3), *wrong):
+            off = ((pp.emulate(x, base, *planes) - out).abs() > bound).sum()
+            assert off == 0 if planes == (3, 3) else off > 40, (base, planes, int(off))
     # weights received: the exponent without the query's third plane is 2^-14 less
-    _, _, _, w, rel = pp.answer(x)
-    less = torch.exp2(-(512.0 - pp.cut((512.0 - x) / 1024.0, 2) * 1024.0)) / (1 + torch.exp2(-x))
+    x = pp.gaps(400, 1, 512.0)
+    _, _, _, w, rel = pp.answer(x, 512.0)
+    less = torch.exp2(-(512.0 - pp.cut(512.0 - x, 2))) / (1 + torch.exp2(-x))
     assert ((less - w).abs() > 1.5 * rel * w).all()

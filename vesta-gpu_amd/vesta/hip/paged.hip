@@ -193,8 +193,11 @@ __device__ __forceinline__ vh_f32x4 pg_mfma(vh_u32x4 a, vh_u32x4 b, vh_f32x4 c) 
 }
 
 // fp32 values go through the matrix cores in three fp16 planes v = hi + (lo +
-// tail) / 2^11, each what is left cut off after 11 bits: 24 bits. The two lower
-// planes share an accumulator.
+// tail) / 2^LO, each what is left cut off after 11 bits: 24 bits. The two lower
+// planes share an accumulator. LO is 11, as the second plane begins there; 25 for
+// weights, of which there may be many small ones: a largest of 1, or just above,
+// leaves less than 2^15 to the second plane, and those below 2^-14, where the
+// first has fp16's fixed step, have bits down to 2^-49 (LO 11: 2^-35).
 #if PG_KIND == PG_F32
 #define PG_PLANES 3
 typedef float pg_q;
@@ -202,14 +205,17 @@ typedef float pg_q;
 #define PG_PLANES 1
 typedef unsigned short pg_q;
 #endif
+#define PG_WEIGHT_LO 25
+template <int LO = 11>
 __device__ __forceinline__ void pg_split(const float* v, vh_u32x4* f) {
 #if PG_KIND == PG_F32
   typedef __fp16 h2 __attribute__((ext_vector_type(2)));
+  constexpr float S = (float)(1 << LO);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const h2 h = __builtin_amdgcn_cvt_pkrtz(v[2 * j], v[2 * j + 1]);
-    const float r0 = fmaf((float)h[0], -VH_LO_SCALE, v[2 * j] * VH_LO_SCALE);
-    const float r1 = fmaf((float)h[1], -VH_LO_SCALE, v[2 * j + 1] * VH_LO_SCALE);
+    const float r0 = fmaf((float)h[0], -S, v[2 * j] * S);
+    const float r1 = fmaf((float)h[1], -S, v[2 * j + 1] * S);
     const h2 l = __builtin_amdgcn_cvt_pkrtz(r0, r1);
     const h2 t = __builtin_amdgcn_cvt_pkrtz(r0 - (float)l[0], r1 - (float)l[1]);
     f[0][j] = __builtin_bit_cast(unsigned, h);
@@ -220,6 +226,9 @@ __device__ __forceinline__ void pg_split(const float* v, vh_u32x4* f) {
   f[0] = pg_pack8(pg_f8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]});
 #endif
 }
+
+// A weighted value from its products with the weights' planes.
+__device__ __forceinline__ float pg_weighted(float h, float l) { return fmaf(l, 1.0f / (1 << PG_WEIGHT_LO), h); }
 
 // A wave's lanes hand each other values through LDS, whose operations a wave
 // executes in order: this keeps the compiler to that order too.
@@ -319,27 +328,28 @@ __device__ __forceinline__ void pg_scores(const vh_u32x4* kf, const PgQuery& qf,
 #endif
 }
 
-// Weights are 2^(score - reference), the reference a running one below the row's
-// largest score: fp16, which holds the second product's operand, has full
+// Weights are 2^(score - reference), the reference a running one at or below the
+// row's largest score: fp16, which holds the second product's operand, has full
 // precision down to 2^-14 only and nothing below 2^-25, so the largest weight is
-// 2^15 and a long tail of small ones keeps its mass down to 2^-40 of it (with a
-// largest of 1, positions 2^-25.5 below one lost all of theirs, while the sum
-// counted it). pg_wide's may grow by 2^PG_SLACK before it rescales (fp16, 4 x 600
-// after 500 of width 128, slack 4 / 6 / 8: 58.0 / 56.7 / 56.7 us), so its largest
-// is 2^9 at first and its tail reaches to 2^-34. fp32's three planes want 2^14
-// (their second is 2^11 times what the first leaves); bf16 has the range. Sums,
-// weighted values and the parts' maxima are all against the reference, so that it
-// cancels.
+// 2^PG_ATTN_BIAS and a long tail of small ones keeps its mass down to 2^-40 of it
+// (with a largest of 1, positions 2^-25.5 below one lost all of theirs, while the
+// sum counted it). pg_wide's may grow by 2^PG_SLACK before it rescales (fp16, 4 x
+// 600 after 500 of width 128, slack 4 / 6 / 8: 58.0 / 56.7 / 56.7 us), so its
+// largest is 2^9 at first and its tail reaches to 2^-34. bf16 has the range, and
+// fp32's planes (pg_split): their weights' exponents stay near 0, where they have
+// most bits (with a largest weight of 2^14, 8 x 128 was off by 1.9e-7, not 1.5e-7).
+// Sums, weighted values and the parts' maxima are all against the reference, so
+// that it cancels.
 #define PG_SLACK (PG_KIND == PG_BF16 ? 8 : 6)
-#define PG_ATTN_BIAS (PG_KIND == PG_BF16 ? 0 : PG_KIND == PG_F32 ? 14 : 15)
-#define PG_WIDE_BIAS (PG_KIND == PG_BF16 ? 0 : PG_KIND == PG_F32 ? 14 : 15 - PG_SLACK)
+#define PG_ATTN_BIAS (PG_KIND == PG_F16 ? 15 : 0)
+#define PG_WIDE_BIAS (PG_KIND == PG_F16 ? 15 - PG_SLACK : 0)
 // The reference of a largest score bm k2: rounded up where the nearest would
-// give a weight above 2^BIAS (scores of 2^24 and more).
+// give a weight that its type cannot hold (scores of 2^24 and more).
 template <int BIAS>
 __device__ __forceinline__ float pg_reference(float bm, float k2) {
-  if constexpr (BIAS == 0) return bm * k2;
-  float n = fmaf(bm, k2, -(float)BIAS);
-  if (fmaf(bm, k2, -n) > (float)BIAS) n = fmaf(__builtin_fabsf(n), 0x1p-23f, n);
+  if constexpr (PG_KIND == PG_BF16) return bm * k2;
+  float n = BIAS ? fmaf(bm, k2, -(float)BIAS) : bm * k2;
+  if (fmaf(bm, k2, -n) > (PG_KIND == PG_F32 ? 1.0f : (float)BIAS)) n = fmaf(__builtin_fabsf(n), 0x1p-23f, n);
   return n;
 }
 // log2 of a row's sum of 2^score, from its sum against reference m. (The bias is
@@ -731,7 +741,7 @@ __device__ __forceinline__ void pg_attn_body(
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(s[2 * k + (j >> 2)][j & 3], qf.k2, -ref));
       ts += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-      pg_split(w, pf[k]);
+      pg_split<PG_WEIGHT_LO>(w, pf[k]);
     }
     sum = fmaf(sum, c, ts);
     typedef short s4 __attribute__((ext_vector_type(4)));
@@ -757,7 +767,7 @@ __device__ __forceinline__ void pg_attn_body(
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #if PG_KIND == PG_F32
-        o[d][j] = fmaf(o[d][j], c, vh_hilo(th[j], tw[j]));
+        o[d][j] = fmaf(o[d][j], c, pg_weighted(th[j], tw[j]));
 #else
         o[d][j] = fmaf(o[d][j], c, th[j]);
 #endif
@@ -1287,7 +1297,7 @@ __device__ __forceinline__ void pg_wide_body(
 #pragma unroll
           for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * k + j], k2, -ref));
           ts[k] = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-          pg_split(w, pf[k]);
+          pg_split<PG_WEIGHT_LO>(w, pf[k]);
         }
         sum = fmaf(sum, c, ts[0] + ts[1]);
 #pragma unroll
@@ -1303,7 +1313,7 @@ __device__ __forceinline__ void pg_wide_body(
             tw = pg_mfma32(vf, pf[k][2], tw);
           }
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[d][j] = fmaf(o[d][j], c, vh_hilo(th[j], tw[j]));
+          for (int j = 0; j < 16; ++j) o[d][j] = fmaf(o[d][j], c, pg_weighted(th[j], tw[j]));
         }
       }
 #endif
