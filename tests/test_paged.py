@@ -331,6 +331,12 @@ def test_outputs_apart_from_queries():
             c.attend(heads_first[:, a:a + 6], table, starts, lengths, out=heads_first[:, b:b + 6])
             by_head = torch.zeros(6, 18, 64, dtype=dtype).transpose(0, 1)       # 5 of 18 rows a head
             c.attend(by_head[a:a + 5], table, starts, lengths, out=by_head[b:b + 5])
+        halves = torch.zeros(5, 6, 128, dtype=dtype)
+        for t in (halves, halves.reshape(6, 5, 128).transpose(0, 1)):
+            c.attend(t[..., :64], table, starts, lengths, out=t[..., 64:])
+            c.attend(t[..., 64:], table, starts, lengths, out=t[..., :64])
+            with pytest.raises(ValueError, match='out'):
+                c.attend(t[..., :64], table, starts, lengths, out=t[..., 32:96])
         for a, b in ((0, 5), (5, 0), (3, 8), (6, 6)):
             with pytest.raises(ValueError, match='out'):
                 c.attend(wide[:, a:a + 6], table, starts, lengths, out=wide[:, b:b + 6])

@@ -232,17 +232,19 @@ def _collides(shape, strides):
 def _overlap(shape, size, a, b):
     """Whether two tensors of one shape and item size, (address, row stride, head stride) each, may share memory. They do
     not where one ends before the other, or where they are parts of one row (one head of heads-first rows), as the
-    queries of a fused projection and its other columns."""
+    queries of a fused projection and its other columns, or of one head's."""
     ga, gb = _grid2(shape, a[1:]), _grid2(shape, b[1:])
     last = [sum((n - 1) * s for n, s in g) + shape[2] for g in (ga, gb)]
     apart = (b[0] - a[0]) // size
     if apart >= last[0] or -apart >= last[1] or not shape[0]:
         return False
-    pitch = ga[1][1]
-    if pitch == 0 or gb[1] != ga[1]:
-        return True
-    (f0, f1), apart = ((g[0][0] - 1) * g[0][1] + shape[2] for g in (ga, gb)), apart % pitch
-    return apart < f0 or apart + f1 > pitch
+    (inner, outer), E = (s for _, s in ga), shape[2]
+
+    def between(pitch, fa, fb):          # what a and b cover of each `pitch`: fa from 0 on, fb from where b begins
+        return fa <= apart % pitch <= pitch - fb
+    if outer and gb[1][1] == outer and between(outer, *((g[0][0] - 1) * g[0][1] + E for g in (ga, gb))):
+        return False
+    return not (inner and ga == gb and outer % inner == 0 and between(inner, E, E))
 
 
 def _dealt(n, run):
@@ -646,7 +648,8 @@ class PagedCache:
     def check(self):
         """Raise if an earlier call, on any stream, met a page, a length or
         starts that cannot be (waits for the device); the word is cleared in
-        the same step, so that none raised meanwhile is lost."""
+        the same step, so that none raised meanwhile is lost. Not while a
+        graph is captured."""
         self._wait()
         took = self._empty(1, dtype=self._i32, device=self.device)
         stream, back = self._enter()
