@@ -892,7 +892,7 @@ __device__ __forceinline__ void pg_here(vh_u32x4 (&f)[N]) {
 // units. The same 4096 tokens in 1800 us (1085 TFLOP/s, 80% of a large library
 // product's rate). At width 64 the softmax on the vector units (about 1400
 // cycles a step against 512), and for short chunks the blocks' starts and ends
-// (4 us): six chunks of up to 512 tokens 25 us (220 TFLOP/s).
+// (4 us): six chunks of up to 512 tokens 23 us (240 TFLOP/s).
 #if PG_KIND != PG_F32 || PG_E == 64
 #define PG_WROW (PG_E + 32)                // halves of a value row in LDS: 64 bytes past a multiple of all banks
 typedef float pg_f16v __attribute__((ext_vector_type(16)));
