@@ -29,7 +29,7 @@ _DTYPES = {'f32': torch.float32, 'f16': torch.float16, 'bf16': torch.bfloat16}
 _BLOCK = 32
 # the least and largest power of two of a block's elements, for rows that are read as f16 or bf16: every value is one
 # of theirs
-_POWERS = {('i8', 'f16'): (-24, 9), ('i8', 'bf16'): (-126, 121), ('e4m3', 'f16'): (-15, 7), ('e4m3', 'bf16'): (-117, 119)}
+_POWERS = {('i8', 'f16'): (-24, 9), ('i8', 'bf16'): (-126, 119), ('e4m3', 'f16'): (-15, 7), ('e4m3', 'bf16'): (-117, 119)}
 _BIAS = {'i8': 133, 'e4m3': 127}      # what is held is the power and this (an i8 element counts 64ths)
 
 
