@@ -5,8 +5,12 @@
 // (64, 128) and kind PG_KIND:
 //   0  fp16 cache, fp16 queries       1  bf16 cache, bf16 queries
 //   2  fp16 cache, fp32 queries (results in fp32)
+// With PG_FORM 1 or 2 (hip/form8.h) the pool holds rows in 8 bits, which are
+// operands of 16 once loaded; append, read-back are then hip/paged8.hip's, and
+// weights and eviction not made.
 //
-// One layer's pool is [pages, page, H, E]; row s of sequence b lies in page
+// One layer's pool is [pages, page, H, E] ([pages, H, page, E] in 8 bits: rows
+// of 64 bytes, of which a head's lie together); row s of sequence b lies in page
 // table[b, s / page], slot s % page (page = 2^shift). starts[b] .. starts[b + 1]
 // are the rows of sequence b's new tokens in the call's [M, ..] tensors,
 // lengths[b] its positions with them: new token j is at position
@@ -27,6 +31,17 @@
 #define PG_ERR_MOST 8u          // a sequence with more new tokens than `most`
 #define PG_ERR_POSITION 16u     // a position past the model's learned ones
 #define PG_ERR_TOKEN 32u        // a token id outside the vocabulary
+
+#ifndef PG_FORM
+#define PG_FORM 0
+#define PG_POOL const unsigned short* __restrict__ kp, const unsigned short* __restrict__ vp
+#define PG_POOL_ARGS kp, vp
+#else
+#define PG_POOL                                                                                   \
+  const unsigned char *__restrict__ kp, const unsigned char *__restrict__ vp,                     \
+      const unsigned char *__restrict__ ks, const unsigned char *__restrict__ vs
+#define PG_POOL_ARGS kp, vp, ks, vs
+#endif
 
 typedef __bf16 pg_b8 __attribute__((ext_vector_type(8)));
 typedef float pg_f8 __attribute__((ext_vector_type(8)));
@@ -93,6 +108,7 @@ __device__ __forceinline__ vh_u32x4 pg_pack8(pg_f8 v) {
 #endif
 }
 
+#if !PG_FORM
 // ---------------------------------------------------------------- append
 // New key and value rows into their pages, eight elements a thread (fp32 ones
 // rounded to the pool's type). Bound by memory: 12,900 rows of 8 heads of 128,
@@ -150,6 +166,7 @@ __device__ __forceinline__ void pg_append_body(const T* __restrict__ k, const T*
   }
 PG_APPEND(pg_append16, unsigned short)
 PG_APPEND(pg_append32, float)
+#endif
 
 // What a model's pass over the cache begins with: the tokens' ids, and the rows
 // of their learned positions (ids and positions outside their tables clamped
@@ -238,9 +255,13 @@ __device__ __forceinline__ void pg_wave_sync() {
 }
 
 // 16 query rows as the products' column operand: lane 16 q + r holds row r's
-// dims 32 k + 8 q .. + 7, k < E / 32. fp32 rows are scaled by a power of two
+// dims pg_dim(k, q) .. + 7, k < E / 32: 32 k + 8 q, or, with keys in 8 bits, of
+// each 64 dims 16 from 16 q on, as a lane has them by one load. fp32 rows are scaled by a power of two
 // to below 1, so that any magnitude splits; k2 is the factor that makes scores
 // powers of two: scale log2(e), times that power.
+__device__ __forceinline__ constexpr int pg_dim(int k, int q) {
+  return PG_FORM ? 64 * (k >> 1) + 16 * q + 8 * (k & 1) : 32 * k + 8 * q;
+}
 struct PgQuery {
   vh_u32x4 f[PG_E / 32][PG_PLANES];
   float k2;
@@ -251,7 +272,7 @@ __device__ __forceinline__ void pg_query(PgQuery& o, const pg_q* __restrict__ qp
   float mx = 0.0f;
 #pragma unroll
   for (int k = 0; k < PG_E / 32; ++k) {
-    const vh_f32x4 a = *(const vh_f32x4*)(qp + 32 * k + 8 * q), c = *(const vh_f32x4*)(qp + 32 * k + 8 * q + 4);
+    const vh_f32x4 a = *(const vh_f32x4*)(qp + pg_dim(k, q)), c = *(const vh_f32x4*)(qp + pg_dim(k, q) + 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       v[k][j] = a[j];
@@ -273,7 +294,7 @@ __device__ __forceinline__ void pg_query(PgQuery& o, const pg_q* __restrict__ qp
   o.k2 = __builtin_ldexpf(scale2, e);
 #else
 #pragma unroll
-  for (int k = 0; k < PG_E / 32; ++k) o.f[k][0] = ld16(qp + 32 * k + 8 * q);
+  for (int k = 0; k < PG_E / 32; ++k) o.f[k][0] = ld16(qp + pg_dim(k, q));
   o.k2 = scale2;
 #endif
 }
@@ -314,8 +335,8 @@ __device__ __forceinline__ void pg_scores(const vh_u32x4* kf, const PgQuery& qf,
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const unsigned x = (unsigned)__shfl((int)kf[k][w], 16 * c + pr, 64);
-            acc = fmaf(qp[32 * k + 8 * c + 2 * w], h2f_lo(x), acc);
-            acc = fmaf(qp[32 * k + 8 * c + 2 * w + 1], h2f_hi(x), acc);
+            acc = fmaf(qp[pg_dim(k, c) + 2 * w], h2f_lo(x), acc);
+            acc = fmaf(qp[pg_dim(k, c) + 2 * w + 1], h2f_hi(x), acc);
           }
       if (!(__builtin_fabsf(h[j]) < INFINITY)) s[j] = acc;
     }
@@ -377,14 +398,20 @@ __device__ __forceinline__ vh_u32x4 pg_tame(vh_u32x4 v) {
   }
   return v;
 }
-// What pg_tame took out of row s of a head's values (rows of `rowlen`, the
-// table's and the pool's as the kernels have them), added to a row's outputs
-// that see it: dim `dim` of it.
-__device__ __forceinline__ float pg_taken(const unsigned short* __restrict__ vh, size_t rowlen,
-                                          const int* __restrict__ tb, int pages, int shift, int s, int dim) {
+// What pg_tame took out of row s of head h's values (the table's row and the
+// pool as the kernels have them), added to a row's outputs that see it: dim
+// `dim` of it.
+__device__ __forceinline__ float pg_taken(PG_POOL, int H, int h, const int* __restrict__ tb, int pages, int shift, int s,
+                                          int dim) {
   const int page = tb[s >> shift];
+#if PG_FORM
+  const size_t row = (((size_t)((unsigned)page < (unsigned)pages ? page : 0) * H + h) << shift) + (s & ((1 << shift) - 1));
+  const unsigned x = vp[row * PG_E + dim];
+  const unsigned short v = (unsigned short)pg_open(x, 0u, pg_power(vs[row * (PG_E / 32) + dim / 32]))[0];
+#else
   const size_t at = (((size_t)((unsigned)page < (unsigned)pages ? page : 0)) << shift) + (s & ((1 << shift) - 1));
-  const unsigned short v = vh[at * rowlen + dim];
+  const unsigned short v = (vp + h * PG_E)[at * ((size_t)H * PG_E) + dim];
+#endif
   return pg_wild(v) ? pg_to_f(v) : 0.0f;
 }
 
@@ -620,13 +647,13 @@ __device__ __forceinline__ void pg_store4(pg_q* p, const float* v) {
 
 template <int W>
 __device__ __forceinline__ void pg_attn_body(
-    const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,
-    const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
+    const pg_q* __restrict__ Q, long qrow, long qhead, PG_POOL, int pages, int shift, const int* __restrict__ table, int N,
     const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
     int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
     float* __restrict__ ws, float* __restrict__ sc, long pitch, unsigned* __restrict__ err) {
   constexpr int KS = PG_E / 32, NG = PG_STEP / 16, NV = PG_STEP * PG_E / 512, DT = PG_E / 16;
-  constexpr int VL = PG_E / 8, VR = 64 / VL;                       // lanes of a value row; rows of a wave's load
+  constexpr int VC = PG_FORM ? 2 : 1;                              // pieces of 8 values that a lane loads at once
+  constexpr int VL = PG_E / 8 / VC, VR = 64 / VL;                  // lanes of a value row; rows of a wave's load
   __shared__ __attribute__((aligned(16))) unsigned short lv[W][PG_STEP * PG_VROW];
   __shared__ float om[W][2][16];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -647,13 +674,36 @@ __device__ __forceinline__ void pg_attn_body(
   const int lim = sq.len - sq.count + tok;                         // this lane's last position
   const int first = sq.len - sq.count + pg_div(x0, G);                    // the first row's
   const pg_q* qp = Q + (sq.first + tok) * qrow + head * qhead;
-  const size_t rowlen = (size_t)H * PG_E;
   const int* tb = table + (size_t)wk.b * N;
-  const unsigned short *kh = kp + h * PG_E + 8 * q, *vh = vp + h * PG_E + lane % VL * 8;
   // the page of a step's positions, one a lane: looked up a step ahead of its
   // rows, and looked at only then (a wait for it would be one for the rows
   // asked for before it)
   auto look = [&](int t) { return tb[min(t * PG_STEP + lane % PG_STEP, last) >> shift]; };
+#if PG_FORM
+  // A lane's loads are 16 elements each, its position's powers one more; what
+  // it needs of others' it gets when it opens the elements.
+  vh_u32x4 kr[NG][KS / 2], vr[NV / 2];
+  pg_powers kw, vw;
+  auto load = [&](int t, int page) {
+    const bool in = (unsigned)page < (unsigned)pages;
+    if (!in) bad = PG_ERR_PAGE;
+    const unsigned rw = (((unsigned)(in ? page : 0) * H + h) << shift)
+                        + (unsigned)(min(t * PG_STEP + lane % PG_STEP, last) & ((1 << shift) - 1));
+    kw = ((const pg_powers*)ks)[rw];
+    vw = ((const pg_powers*)vs)[rw];
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const unsigned char* p = kp + 16 * q + (size_t)(unsigned)__shfl((int)rw, 16 * i + r, 64) * PG_E;
+#pragma unroll
+      for (int k = 0; k < KS / 2; ++k) kr[i][k] = ld16(p + 64 * k);
+    }
+#pragma unroll
+    for (int n = 0; n < NV / 2; ++n)
+      vr[n] = ld16(vp + 16 * (lane % VL) + (size_t)(unsigned)__shfl((int)rw, n * VR + lane / VL, 64) * PG_E);
+  };
+#else
+  const size_t rowlen = (size_t)H * PG_E;
+  const unsigned short *kh = kp + h * PG_E + 8 * q, *vh = vp + h * PG_E + lane % VL * 8;
   vh_u32x4 kr[NG][KS], vr[NV];
   auto load = [&](int t, int page) {
     const bool in = (unsigned)page < (unsigned)pages;
@@ -669,6 +719,7 @@ __device__ __forceinline__ void pg_attn_body(
 #pragma unroll
     for (int n = 0; n < NV; ++n) vr[n] = ld16(vh + (unsigned)__shfl((int)rw, n * VR + lane / VL, 64) * rowlen);
   };
+#endif
   float o[DT][4] = {};
   float m2 = -INFINITY, sum = 0.0f;
   unsigned short* V = lv[wave];
@@ -683,8 +734,32 @@ __device__ __forceinline__ void pg_attn_body(
   for (int t = t0 + wave; t < t1; t += W) {
     const int p0 = t * PG_STEP;
     float s[NG][4];
+#if PG_FORM
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const unsigned w = (unsigned)__shfl((int)kw, 16 * i + r, 64) >> (q & 2 ? 8 : 0);
+      vh_u32x4 kf[KS];
+#pragma unroll
+      for (int k = 0; k < KS; k += 2) {
+        const pg_factor p = pg_power(w >> 8 * k & 255u);
+        kf[k] = pg_open(kr[i][k / 2][0], kr[i][k / 2][1], p);
+        kf[k + 1] = pg_open(kr[i][k / 2][2], kr[i][k / 2][3], p);
+      }
+      pg_scores(kf, qf, qp, lane, s[i]);
+    }
+    vh_u32x4 v8[NV];
+#pragma unroll
+    for (int n = 0; n < NV; n += 2) {
+      const unsigned w = (unsigned)__shfl((int)vw, n / 2 * VR + lane / VL, 64);
+      const pg_factor p = pg_power(w >> 8 * (lane % VL / 2) & 255u);
+      v8[n] = pg_open(vr[n / 2][0], vr[n / 2][1], p);
+      v8[n + 1] = pg_open(vr[n / 2][2], vr[n / 2][3], p);
+    }
+#else
 #pragma unroll
     for (int i = 0; i < NG; ++i) pg_scores(kr[i], qf, qp, lane, s[i]);
+    vh_u32x4 (&v8)[NV] = vr;
+#endif
     const bool seen = p0 + PG_STEP - 1 > first;                    // not the whole step by every row
     // values past the last position are 0; ones that are not finite are left
     // out of the product where a row may not see their position, or a plane of
@@ -693,21 +768,21 @@ __device__ __forceinline__ void pg_attn_body(
     if (p0 + PG_STEP - 1 > last) {
 #pragma unroll
       for (int n = 0; n < NV; ++n)
-        if (p0 + n * VR + lane / VL > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
+        if (p0 + n / VC * VR + lane / VL > last) v8[n] = vh_u32x4{0u, 0u, 0u, 0u};
     }
     if (seen || PG_KIND == PG_F32) {
       unsigned any = 0u;
 #pragma unroll
-      for (int n = 0; n < NV; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
+      for (int n = 0; n < NV; ++n) any |= pg_wild2(v8[n][0]) | pg_wild2(v8[n][1]) | pg_wild2(v8[n][2]) | pg_wild2(v8[n][3]);
       wild = __any(any != 0u);
       if (wild) {
 #pragma unroll
-        for (int n = 0; n < NV; ++n) vr[n] = pg_tame(vr[n]);
+        for (int n = 0; n < NV; ++n) v8[n] = pg_tame(v8[n]);
       }
     }
     pg_wave_sync();                                                // the step before is read
 #pragma unroll
-    for (int n = 0; n < NV; ++n) *(vh_u32x4*)(V + (n * VR + lane / VL) * PG_VROW + lane % VL * 8) = vr[n];
+    for (int n = 0; n < NV; ++n) *(vh_u32x4*)(V + (n / VC * VR + lane / VL) * PG_VROW + (lane % VL * VC + n % VC) * 8) = v8[n];
     pg_wave_sync();
     if (t + W < t1) {
       load(t + W, page);
@@ -780,7 +855,7 @@ __device__ __forceinline__ void pg_attn_body(
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float v = pg_taken(vp + h * PG_E, rowlen, tb, pages, shift, s, 16 * d + 4 * q + j);
+            const float v = pg_taken(PG_POOL_ARGS, H, h, tb, pages, shift, s, 16 * d + 4 * q + j);
             o[d][j] += s <= lim ? v : 0.0f;
           }
     }
@@ -844,12 +919,11 @@ __device__ __forceinline__ void pg_attn_body(
 
 #define PG_ATTN(name, waves) \
   extern "C" __global__ __launch_bounds__(64 * waves, 2) void name( \
-      const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp, \
-      const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N, \
+      const pg_q* __restrict__ Q, long qrow, long qhead, PG_POOL, int pages, int shift, const int* __restrict__ table, int N, \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least, \
       int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse, \
       float* __restrict__ ws, float* __restrict__ sc, long pitch, unsigned* __restrict__ err) { \
-    pg_attn_body<waves>(Q, qrow, qhead, kp, vp, pages, shift, table, N, starts, lengths, B, M, H, \
+    pg_attn_body<waves>(Q, qrow, qhead, PG_POOL_ARGS, pages, shift, table, N, starts, lengths, B, M, H, \
                         G, target, least, run, limit, most, scale2, out, orow, ohead, lse, ws, sc, pitch, err); \
   }
 PG_ATTN(pg_attn2, 2)
@@ -906,13 +980,13 @@ __device__ __forceinline__ pg_f16v pg_mfma32(vh_u32x4 a, vh_u32x4 b, pg_f16v c) 
 
 template <int W>
 __device__ __forceinline__ void pg_wide_body(
-    const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,
-    const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,
+    const pg_q* __restrict__ Q, long qrow, long qhead, PG_POOL, int pages, int shift, const int* __restrict__ table, int N,
     const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
     int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse,
     float* __restrict__ ws, unsigned* __restrict__ err) {
   constexpr int KS = PG_E / 16, DT = PG_E / 32, CH = PG_E / 8;     // k-steps, dim tiles, 16-byte pieces of a row
-  constexpr int TILE = 32 * W, RS = 64 * W / CH, NL = 64 / RS;     // rows; a thread's rows of a step apart, its pieces
+  constexpr int VC = PG_FORM ? 2 : 1;                              // pieces that a thread loads at once
+  constexpr int TILE = 32 * W, RS = 64 * W * VC / CH, NL = 64 / RS;   // rows; a thread's rows of a step apart, its loads
   __shared__ __attribute__((aligned(16))) vh_u32x4 lk[2][64 * (CH + 1)];
   __shared__ __attribute__((aligned(16))) unsigned short lv[2][64 * PG_WROW];
   __shared__ int lwild[2];
@@ -967,61 +1041,100 @@ __device__ __forceinline__ void pg_wide_body(
 #pragma unroll
   for (int k = 0; k < KS; ++k) qf[k] = ld16(qp + 16 * k + 8 * g);
 #endif
-  // staging: thread t takes piece t % CH of rows t / CH + RS n
-  const size_t rowlen = (size_t)H * PG_E;
+  // staging: thread t takes piece t % CH (two, in 8 bits) of rows t / CH + RS n
   const int* tb = table + (size_t)wk.b * N;
-  const int c8 = tid % CH, r8 = tid / CH;
+  const int c8 = tid % (CH / VC), r8 = tid / (CH / VC);
+#if !PG_FORM
+  const size_t rowlen = (size_t)H * PG_E;
   const unsigned short *kh = kp + h * PG_E + 8 * c8, *vh = vp + h * PG_E + 8 * c8;
+#endif
   int page[NL];
   auto look = [&](int t) {                                         // as in pg_attn
 #pragma unroll
     for (int n = 0; n < NL; ++n) page[n] = tb[min(64 * t + r8 + RS * n, last) >> shift];
   };
   vh_u32x4 kr[NL], vr[NL];
+#if PG_FORM
+  unsigned kw[NL], vw[NL];                                         // their blocks' powers
+#endif
   unsigned at[NL];
   auto where = [&](int t) {
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
       const bool in = (unsigned)page[n] < (unsigned)pages;
       if (!in) bad = PG_ERR_PAGE;
-      at[n] = ((unsigned)(in ? page[n] : 0) << shift) + (unsigned)(min(64 * t + r8 + RS * n, last) & ((1 << shift) - 1));
+      const unsigned first = PG_FORM ? (unsigned)(in ? page[n] : 0) * H + h : (unsigned)(in ? page[n] : 0);
+      at[n] = (first << shift) + (unsigned)(min(64 * t + r8 + RS * n, last) & ((1 << shift) - 1));
     }
   };
+#if PG_FORM
+  auto row_k = [&](int n, unsigned a) {
+    kr[n] = ld16(kp + (size_t)a * PG_E + 16 * c8);
+    kw[n] = ks[(size_t)a * (PG_E / 32) + c8 / 2];
+  };
+  auto row_v = [&](int n, unsigned a) {
+    vr[n] = ld16(vp + (size_t)a * PG_E + 16 * c8);
+    vw[n] = vs[(size_t)a * (PG_E / 32) + c8 / 2];
+  };
+#else
+  auto row_k = [&](int n, unsigned a) { kr[n] = ld16(kh + (size_t)a * (unsigned)rowlen); };
+  auto row_v = [&](int n, unsigned a) { vr[n] = ld16(vh + (size_t)a * (unsigned)rowlen); };
+#endif
   auto load_k = [&]() {
 #pragma unroll
-    for (int n = 0; n < NL; ++n) kr[n] = ld16(kh + (size_t)at[n] * (unsigned)rowlen);
+    for (int n = 0; n < NL; ++n) row_k(n, at[n]);
   };
   auto load_v = [&]() {
 #pragma unroll
-    for (int n = 0; n < NL; ++n) vr[n] = ld16(vh + (size_t)at[n] * (unsigned)rowlen);
+    for (int n = 0; n < NL; ++n) row_v(n, at[n]);
   };
   // Key rows are 16 bytes past a multiple of all banks apart, so that a column
   // of their pieces falls on all of them.
   auto put_k = [&](int t) {
 #pragma unroll
-    for (int n = 0; n < NL; ++n) lk[t & 1][(r8 + RS * n) * (CH + 1) + c8] = kr[n];
+    for (int n = 0; n < NL; ++n) {
+#if PG_FORM
+      const pg_factor p = pg_power(kw[n]);
+      vh_u32x4* to = lk[t & 1] + (r8 + RS * n) * (CH + 1) + 2 * c8;
+      to[0] = pg_open(kr[n][0], kr[n][1], p);
+      to[1] = pg_open(kr[n][2], kr[n][3], p);
+#else
+      lk[t & 1][(r8 + RS * n) * (CH + 1) + c8] = kr[n];
+#endif
+    }
   };
   // Values past the last position are 0, and where some row sees a step in part
   // so are those that are not finite (0 * inf); that there are such is noted.
   auto put_v = [&](int t) {
+#if PG_FORM
+    vh_u32x4 v8[VC * NL];
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const pg_factor p = pg_power(vw[n]);
+      v8[2 * n] = pg_open(vr[n][0], vr[n][1], p);
+      v8[2 * n + 1] = pg_open(vr[n][2], vr[n][3], p);
+    }
+#else
+    vh_u32x4 (&v8)[NL] = vr;
+#endif
     if (64 * t + 63 > last) {
 #pragma unroll
-      for (int n = 0; n < NL; ++n)
-        if (64 * t + r8 + RS * n > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
+      for (int n = 0; n < VC * NL; ++n)
+        if (64 * t + r8 + RS * (n / VC) > last) v8[n] = vh_u32x4{0u, 0u, 0u, 0u};
       asm volatile("" ::: "memory");                               // kept a branch
     }
     if (PG_KIND == PG_F32 || 64 * t + 63 > bfirst) {               // (fp32: a plane of a weight may be 0)
       unsigned any = 0u;
 #pragma unroll
-      for (int n = 0; n < NL; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
+      for (int n = 0; n < VC * NL; ++n) any |= pg_wild2(v8[n][0]) | pg_wild2(v8[n][1]) | pg_wild2(v8[n][2]) | pg_wild2(v8[n][3]);
       if (any) {
         lwild[t & 1] = t + 1;
 #pragma unroll
-        for (int n = 0; n < NL; ++n) vr[n] = pg_tame(vr[n]);
+        for (int n = 0; n < VC * NL; ++n) v8[n] = pg_tame(v8[n]);
       }
     }
 #pragma unroll
-    for (int n = 0; n < NL; ++n) *(vh_u32x4*)(lv[t & 1] + (r8 + RS * n) * PG_WROW + 8 * c8) = vr[n];
+    for (int n = 0; n < VC * NL; ++n) *(vh_u32x4*)(lv[t & 1] + (r8 + RS * (n / VC)) * PG_WROW + 8 * (VC * c8 + n % VC)) = v8[n];
   };
   pg_f16v o[DT];
 #pragma unroll
@@ -1049,7 +1162,7 @@ __device__ __forceinline__ void pg_wide_body(
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float v = pg_taken(vp + h * PG_E, rowlen, tb, pages, shift, s, 32 * d + 8 * (j >> 2) + 4 * g + (j & 3));
+          const float v = pg_taken(PG_POOL_ARGS, H, h, tb, pages, shift, s, 32 * d + 8 * (j >> 2) + 4 * g + (j & 3));
           o[d][j] += s <= lim ? v : 0.0f;
         }
   };
@@ -1156,7 +1269,7 @@ __device__ __forceinline__ void pg_wide_body(
     auto ask = [&](int t) {              // the values of step t, the keys of the next
       if (t >= t1) return;
 #pragma unroll
-      for (int n = 0; n < NL; ++n) vr[n] = ld16(vh + (size_t)av[n] * (unsigned)rowlen);
+      for (int n = 0; n < NL; ++n) row_v(n, av[n]);
       if (t + 1 < t1) load_k();
     };
     auto stage = [&](int t) {
@@ -1349,12 +1462,12 @@ __device__ __forceinline__ void pg_wide_body(
 }
 #define PG_WIDE(name, waves)                                                                                       \
   extern "C" __global__ __launch_bounds__(64 * waves, 2) void name(                                                \
-      const pg_q* __restrict__ Q, long qrow, long qhead, const unsigned short* __restrict__ kp,                    \
-      const unsigned short* __restrict__ vp, int pages, int shift, const int* __restrict__ table, int N,           \
+      const pg_q* __restrict__ Q, long qrow, long qhead, PG_POOL, int pages, int shift,                            \
+      const int* __restrict__ table, int N,                                                                        \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target,     \
       int least, int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead,        \
       float* __restrict__ lse, float* __restrict__ ws, unsigned* __restrict__ err) {                               \
-    pg_wide_body<waves>(Q, qrow, qhead, kp, vp, pages, shift, table, N, starts, lengths, B, M, H, G, target,       \
+    pg_wide_body<waves>(Q, qrow, qhead, PG_POOL_ARGS, pages, shift, table, N, starts, lengths, B, M, H, G, target,       \
                         least, run, limit, most, scale2, out, orow, ohead, lse, ws, err);                          \
   }
 PG_WIDE(pg_wide, 4)
@@ -1468,6 +1581,7 @@ PG_JOIN(pg_join, 16, PG_STEP)
 PG_JOIN(pg_wide_join, 128, 64)
 #endif
 
+#if !PG_FORM
 // ---------------------------------------------------------------- weights
 // out[b, h, s] = old[b, h, s] (0 for the chunk's own positions) + the sum over
 // the sequence's rows (tokens and the group's heads) of the softmax weight at
@@ -1996,3 +2110,4 @@ extern "C" __global__ __launch_bounds__(256) void pg_move(unsigned short* __rest
   __builtin_nontemporal_store(kx, (vh_u32x4*)kp + into);
   __builtin_nontemporal_store(vx, (vh_u32x4*)vp + into);
 }
+#endif

@@ -159,10 +159,10 @@ class _Launcher:
     """One kernel with a buffer for its arguments: filled and read by one call
     at a time."""
 
-    def __init__(self, fn, name):
+    def __init__(self, fn, name, signature):
         self.fn, self.name = fn, name
         self.lock = threading.Lock()
-        codes = '@' + ''.join(_CODES[c] for c in SIGNATURES[name])
+        codes = '@' + ''.join(_CODES[c] for c in signature)
         self.pack = struct.Struct(codes)
         self.buf = ctypes.create_string_buffer(self.pack.size)
         base = ctypes.addressof(self.buf)
@@ -179,19 +179,18 @@ class _Launcher:
 
 
 class _Kernels:
-    """The kernels of one head width and kind, loaded on one device."""
+    """A module's kernels, those of ``signatures``, loaded on one device."""
 
-    def __init__(self, device, width, kind):
+    def __init__(self, device, source, signatures):
         import torch
         self.mod = ctypes.c_void_p()
         with torch.cuda.device(device):
-            ok(lib().vh_module_load(compile_code(paged_source(width, kind)), ctypes.byref(self.mod)),
-               'paged cache module load')
+            ok(lib().vh_module_load(compile_code(source), ctypes.byref(self.mod)), 'module load')
             track(self)
-            for name in kernels_of(width, kind):
+            for name, signature in signatures.items():
                 fn = ctypes.c_void_p()
                 ok(lib().vh_module_get_function(self.mod, name.encode(), ctypes.byref(fn)), name)
-                setattr(self, name, _Launcher(fn, name))
+                setattr(self, name, _Launcher(fn, name, signature))
 
     def close(self):
         if self.mod is not None and self.mod.value:
@@ -204,12 +203,12 @@ _loaded = {}
 _loaded_lock = threading.Lock()
 
 
-def _kernels(device, width, kind):
+def loaded(device, key, source, signatures):
+    """The kernels known as ``key`` on a device, loaded where they are first asked for."""
     with _loaded_lock:
-        key = (device, width, kind)
-        if key not in _loaded:
-            _loaded[key] = _Kernels(device, width, kind)
-        return _loaded[key]
+        if (device, key) not in _loaded:
+            _loaded[device, key] = _Kernels(device, source(), signatures)
+        return _loaded[device, key]
 
 
 def _at(t):
@@ -271,9 +270,13 @@ class PagedCache:
         # torch.cuda's own, without the stream object around the handle
         self._current = torch._C._cuda_getDevice
         self._raw_stream = torch._C._cuda_getCurrentRawStream
-        self._kind = {self.dtype: _kernels(self.device.index, width, dtype)}
+        self._kind = {self.dtype: self._load(dtype)}
         if dtype == 'f16':
-            self._kind[torch.float32] = _kernels(self.device.index, width, 'f32')
+            self._kind[torch.float32] = self._load('f32')
+
+    def _load(self, kind):
+        return loaded(self.device.index, (self.width, kind), lambda: paged_source(self.width, kind),
+                      {name: SIGNATURES[name] for name in kernels_of(self.width, kind)})
 
     def _shape(self, pages, heads, width, layers, page, dtype):
         pages, heads, width, layers, page = map(operator.index, (pages, heads, width, layers, page))
@@ -301,9 +304,12 @@ class PagedCache:
         shape = (self.layers, self.pages, self.page, self.heads, self.width)
         self.keys = torch.zeros(shape, dtype=self.dtype, device=self.device)
         self.vals = torch.zeros(shape, dtype=self.dtype, device=self.device)
-        self._layer_bytes = self.keys[0].numel() * 2
-        # what every call needs (a call's checks cost about as much as its launch)
-        self._pools = self.keys.data_ptr(), self.vals.data_ptr()
+        self._ready(self.keys, self.vals)
+
+    def _ready(self, *pools):
+        """What every call needs (a call's checks cost about as much as its launch)."""
+        import torch
+        self._pools = [tuple(p[n].data_ptr() for p in pools) for n in range(self.layers)]      # each layer's
         self._index = self.keys.get_device()
         self._i32, self._f32, self._empty = torch.int32, torch.float32, torch.empty
         self._recording = torch.is_grad_enabled
@@ -367,7 +373,7 @@ class PagedCache:
         layer = operator.index(layer)
         if not 0 <= layer < self.layers:
             raise ValueError(f'layer {layer} of {self.layers}')
-        return layer * self._layer_bytes
+        return self._pools[layer]
 
     def _enter(self):
         """The stream to launch on, with the cache's device the current one; and the device to go back to, or None."""
@@ -404,8 +410,7 @@ class PagedCache:
             raise ValueError(f'k: {M} rows are too many for one call')
         stream, back = self._enter()
         try:
-            launch(grid, BLOCK, stream, k_at, v_at, *ks, *vs, self._pools[0] + at, self._pools[1] + at, *seqs, B,
-                   M, self.heads, self._err)
+            launch(grid, BLOCK, stream, k_at, v_at, *ks, *vs, *at, *seqs, B, M, self.heads, self._err)
         finally:
             self._leave(back)
 
@@ -490,8 +495,8 @@ class PagedCache:
                 scores = scores and base + scores
             if M and B:
                 to = (*to, lse)
-                args = (_dealt(blocks, run), block, stream, *qs, self._pools[0] + at, self._pools[1] + at, *seqs, B, M,
-                        self.heads, G, target, least, run, blocks, most, scale2, *to, base + ws if target else 0)
+                args = (_dealt(blocks, run), block, stream, *qs, *at, *seqs, B, M, self.heads, G, target, least, run,
+                        blocks, most, scale2, *to, base + ws if target else 0)
                 if wide:
                     attn(*args, self._err)
                 else:
@@ -502,7 +507,7 @@ class PagedCache:
                         tiles * (rows // cut), JOIN_BLOCK, stream, *seqs[4:], B, N * self.page, M, self.heads, G, target,
                         least, run, blocks, cut, base + ws, *to)
             if weight is not None and B and So:
-                self._receive(kn, stream, (*qs, self._pools[0] + at), seqs, (B, M, G), most, wide, scale2, lse, scores,
+                self._receive(kn, stream, (*qs, at[0]), seqs, (B, M, G), most, wide, scale2, lse, scores,
                               pitch, (weight.data_ptr(), S, weight_out.data_ptr(), So))
         finally:
             self._leave(back)
@@ -634,7 +639,7 @@ class PagedCache:
             kn.pg_select(self.layers * B * self.heads, 256 if N * self.page <= SELECT_FEW else 1024, stream,
                          weight.data_ptr(), S, seqs[5], N * self.page, B, self.heads, keep, min(recent, keep),
                          kept.data_ptr(), weight_out.data_ptr(), So, new.data_ptr(), self._err)
-            kn.pg_move(self.layers * B * blocks, BLOCK, stream, *self._pools, *seqs[:4], to_at, No, kept.data_ptr(), keep,
+            kn.pg_move(self.layers * B * blocks, BLOCK, stream, *self._pools[0], *seqs[:4], to_at, No, kept.data_ptr(), keep,
                        B, self.heads, blocks, self._err)
         finally:
             self._leave(back)
@@ -795,7 +800,7 @@ class PagedPass(Prefill):
             self._replay(qkv[layer])
             cache.append(k, v, table, starts, lengths, layer)
             cache.attend(q, table, starts, lengths, layer, out=o, most=most,
-                         weight=None if weight is None else weight[layer])
+                         **({} if weight is None else dict(weight=weight[layer])))
             self._replay(rest[layer])
         torch.index_select(b.Z, 0, (starts[1:] - 1).clamp(0, M - 1), out=b.ZL[:B])
         self._replay(head)

@@ -1,0 +1,133 @@
+"""A key/value cache in pages that holds its rows in 8 bits.
+
+    cache = PagedCache8(pages=512, heads=12, width=64, layers=12, page=64, dtype='f16', form='i8')
+    cache.append(k, v, table, starts, lengths, layer)             # new tokens' rows, rounded to what is held
+    out = cache.attend(q, table, starts, lengths, layer)          # their attention over all positions
+    cache.read(k, v, table, starts, lengths, layer)               # the new tokens' rows as they are held
+    cache.check()                                                 # raises if a call met a bad page (syncs)
+
+Batches, pages, streams, errors and refusals are ``vesta.paged.PagedCache``'s, and
+``VestaGPT2.extend`` takes either; long decodes, which are bound by the cache's
+bytes, read half as many here.
+
+Each 32 values of a row are 8-bit elements and one power of two, the byte layout
+of the OCP microscaling formats. A block's power is the least with which its
+largest value rounds to an element; values are rounded to nearest, a tie to even.
+
+* ``form='i8'``: whole numbers of +-127; a value is off by at most 1/127 of its
+  block's largest (1/255 where the largest is just below a power of two). A block
+  with an infinity or a NaN is held as NaNs.
+* ``form='e4m3'``: floats of 4 bits exponent and 3 bits fraction; a value is off by
+  at most 1/16 of itself, or by 2^-17.8 of its block's largest where that is more. An
+  infinity or NaN is held as a NaN.
+
+Powers are limited such that every value is one of ``dtype``'s: over 'f16' steps
+of 2^-24 at least, sizes of 65024 ('i8') or 57344 ('e4m3') at most, larger ones
+held as these. So nothing is rounded after the cache: attention multiplies what
+it holds, in 16 bits ('f16': f16 or f32 queries; 'bf16': bf16).
+
+No weights are counted and nothing is evicted here.
+"""
+from __future__ import annotations
+
+from pathlib import Path
+
+from .paged import BLOCK, KINDS, PAGED_SRC, SIGNATURES as SIGNATURES16, PagedCache, _collides, _overlap, kernels_of, loaded
+from .prefill import PRELUDE_SRC
+
+FORM_SRC = Path(__file__).resolve().parent / 'hip' / 'form8.h'
+PAGED8_SRC = Path(__file__).resolve().parent / 'hip' / 'paged8.hip'
+FORMS = ('i8', 'e4m3')
+SCALED = 32                            # values of a power
+LEAST = {('i8', 'f16'): 109, ('i8', 'bf16'): 7, ('e4m3', 'f16'): 112, ('e4m3', 'bf16'): 10}    # bytes of the least powers
+
+_ATTENTION = ('pg_attn', 'pg_attn2', 'pg_attn8', 'pg_wide', 'pg_wide8')
+_POOLS = slice(3, 5)                   # where the pools are in their parameters: two more here, the powers'
+SIGNATURES = {name: SIGNATURES16[name] for name in ('pg_join', 'pg_wide_join', 'pg_take', 'pg_input')}
+SIGNATURES.update({name: SIGNATURES16[name][:5] + 'pp' + SIGNATURES16[name][5:] for name in _ATTENTION})
+SIGNATURES.update({name: 'ppllll' + 'pppp' + SIGNATURES16['pg_append16'][8:]
+                   for name in ('pg_append16', 'pg_append32', 'pg_read16', 'pg_read32')})
+
+
+def paged8_source(width: int, kind: str, form: str) -> str:
+    return (f'#define VBLOCK {BLOCK}\n#define PG_E {width}\n#define PG_KIND {KINDS.index(kind)}\n'
+            f'#define PG_FORM {1 + FORMS.index(form)}\n'
+            + '\n'.join(src.read_text() for src in (PRELUDE_SRC, FORM_SRC, PAGED_SRC, PAGED8_SRC)))
+
+
+class PagedCache8(PagedCache):
+    """As ``PagedCache``, with rows of ``form`` 'i8' or 'e4m3' that stand for
+    values of ``dtype``. ``keys`` and ``vals`` are [layers, pages, heads, page,
+    width] tensors of elements (int8 or float8_e4m3fn), ``kscales`` and
+    ``vscales`` [layers, pages, heads, page, width / 32] bytes: a value is its
+    element times 2^(byte - 127), 'i8' elements counting 64ths."""
+
+    def __init__(self, pages, heads, width=64, layers=1, page=64, dtype='f16', form='i8', device=None):
+        if form not in FORMS:
+            raise ValueError(f'form {form!r}: one of {FORMS}')
+        self.form = form
+        super().__init__(pages, heads, width, layers, page, dtype, device)
+
+    def _load(self, kind):
+        return loaded(self.device.index, (self.width, kind, self.form),
+                      lambda: paged8_source(self.width, kind, self.form),
+                      {name: SIGNATURES[name] for name in kernels_of(self.width, kind) | {'pg_read16', 'pg_read32'}
+                       if name in SIGNATURES})
+
+    def _shape(self, pages, heads, width, layers, page, dtype):
+        super()._shape(pages, heads, width, layers, page, dtype)
+        if self.pages * self.page * self.heads >= 1 << 31:
+            raise ValueError(f'{pages} pages of {page} rows of {heads} heads: fewer than 2^31 a layer')
+
+    def _allocate(self, device):
+        import torch
+        self.device = device
+        self.dtype = torch.float16 if self._dt == 'f16' else torch.bfloat16
+        shape = (self.layers, self.pages, self.heads, self.page)
+        held = torch.int8 if self.form == 'i8' else torch.float8_e4m3fn
+        self.keys, self.vals = (torch.zeros(shape + (self.width,), dtype=torch.uint8, device=device).view(held)
+                                for _ in range(2))
+        self.kscales, self.vscales = (torch.full(shape + (self.width // SCALED,), LEAST[self.form, self._dt],
+                                                 dtype=torch.uint8, device=device) for _ in range(2))
+        self._ready(self.keys, self.vals, self.kscales, self.vscales)
+
+    def attend(self, q, table, starts, lengths, layer=0, scale=None, out=None, most=None):
+        """As ``PagedCache.attend``, without weights: attention of the new
+        tokens' queries ``q`` [M, G * heads, width] over what ``layer`` holds
+        of their sequences."""
+        return super().attend(q, table, starts, lengths, layer, scale, out, most=most)
+
+    def read(self, k, v, table, starts, lengths, layer=0):
+        """What ``layer`` holds of the new tokens' key and value rows (of
+        whole sequences, where their starts count all their positions), as
+        values into ``k``, ``v`` [M, heads, width]: of the cache's type or f32,
+        in either exactly. A row of a position that a sequence does not have (a
+        padded row's) becomes 0, rows behind the last sequence stay as they are.
+        Returns (k, v)."""
+        B, N, seqs = self._batch(table, lengths, starts)
+        at = self._layer(layer)
+        ks = self._rows('k', k, self._new, self.heads)
+        vs = self._rows('v', v, (k.dtype,), like=k.shape)
+        size = 4 if k.dtype is self._f32 else 2
+        for name, t, (_, *strides) in (('k', k, ks), ('v', v, vs)):
+            if _collides(t.shape, strides):
+                raise ValueError(f'{name}: rows that lie on one another (strides {t.stride()})')
+        if _overlap(k.shape, size, ks, vs):
+            raise ValueError('v: memory other than that of k')
+        M = k.shape[0]
+        if M == 0 or B == 0:
+            return k, v
+        kn = self._kind[self.dtype]
+        grid = -(-M * self.heads * (self.width // 8) // BLOCK)
+        if grid >= 1 << 31:
+            raise ValueError(f'k: {M} rows are too many for one call')
+        stream, back = self._enter()
+        try:
+            (kn.pg_read32 if size == 4 else kn.pg_read16)(grid, BLOCK, stream, ks[0], vs[0], *ks[1:], *vs[1:], *at, *seqs,
+                                                          B, M, self.heads, self._err)
+        finally:
+            self._leave(back)
+        return k, v
+
+    def evict(self, *args, **kwargs):
+        raise ValueError('a cache in 8 bits counts no weights and evicts nothing')
