@@ -1,0 +1,249 @@
+"""Log probabilities on the GPU (vesta/logprobs.py) against plain PyTorch in 64 bits: odd vocabularies and pitches, bans,
+ties, NaNs, one row and many, parts of rows and whole ones."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {'f32': torch.float32, 'f16': torch.float16, 'bf16': torch.bfloat16}
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip('no GPU')
+
+
+@pytest.fixture(params=('rule', '256 whole', '512 whole', '1024 whole', '256 in 3', '1024 in 64'))
+def layout(request, monkeypatch):
+    """Rows as the rule has them, or by one kernel, whole or in parts."""
+    from vesta import logprobs as lp
+    if request.param != 'rule':
+        threads, *_, parts = request.param.split()
+
+        def fixed(M, V, size):
+            each = V if parts == 'whole' else -(-V // int(parts))
+            return int(threads), -(-V // each), each
+
+        monkeypatch.setattr(lp, '_layout', fixed)
+
+
+def _gen(*seed):
+    return torch.Generator(device='cuda').manual_seed(sum(1009 ** i * int(s) for i, s in enumerate(seed)) % (1 << 31))
+
+
+def _check(x, given, top):
+    """The call's results for rows x.
+
+    A term e^(x - m) is off by 2^-22 of itself from the exponential and by the rounding of x - m times log2 e, two half
+    steps of |x - m| log2 e: its share of S by that times itself, of which the sum is bounded with the terms; a chain of
+    additions is V / 256 (a thread's) and 32 of lanes, waves and parts; log S and the differences are rounded once each."""
+    from vesta.logprobs import logprobs
+    got = logprobs(x, given, top=top)
+    M, V = x.shape
+    x = x.double()
+    m = x.amax(1, keepdim=True)
+    d = x - torch.where(m == -math.inf, 0.0, m)
+    e = torch.where(x == -math.inf, 0.0, torch.exp(d))
+    S = e.sum(1, keepdim=True)
+    none = S == 0
+    u = 2.0 ** -24
+    log_s = torch.where(none, 0.0, torch.log(S))
+    fin = torch.where(x == -math.inf, 0.0, d)
+    T = (e * fin).sum(1, keepdim=True)
+    H = torch.where(none, 0.0, log_s - T / S)
+    chain = (V / 256 + 32) * u
+    ds = ((e * (4 * u + 4 * u * fin.abs())).sum(1, keepdim=True) / S).nan_to_num(0) + chain          # relative, of S
+    dt = ((e * (4 * u + 4 * u * fin.abs()) * fin.abs()).sum(1, keepdim=True) / S).nan_to_num(0) \
+        + (T / S).abs().nan_to_num(0) * (chain + ds + 4 * u)
+    err = ds + 4 * u * (log_s.abs() + 1)
+    lp = d - log_s
+
+    def close(a, want, bound):
+        a = a.double()
+        same = (a == want) | (a.isnan() & want.isnan())
+        bad = ~(torch.where(same, 0.0, (a - want).abs() - bound) <= 0)
+        assert not bad.any(), (int(bad.sum()), a[bad][0].item(), want[bad][0].item(), bound.expand_as(want)[bad][0].item())
+
+    close(got.entropy, H.squeeze(1), (err + dt).squeeze(1))
+    if given is None:
+        assert got.given is None
+    else:
+        g = given.view(M, -1).long()
+        inside = (g >= 0) & (g < V)
+        want = torch.where(inside, lp.gather(1, g.clamp(0, V - 1)), math.nan).view(given.shape)
+        bound = err + 4 * u * want.view(M, -1).abs().nan_to_num(0, 0, 0)
+        assert got.given.shape == given.shape
+        close(got.given, want, bound.view(given.shape))
+    if top == 0:
+        assert got.top is None and got.ids is None
+        return got
+    order = torch.sort(torch.where(x.isnan(), math.inf, x), dim=1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(got.ids.long(), order)
+    want = lp.gather(1, order)
+    close(got.top, want, err + 4 * u * want.abs().nan_to_num(0, 0, 0))
+    return got
+
+
+VOCABS = (1, 2, 3, 7, 64, 65, 255, 1000, 1023, 4097, 50257)
+
+
+@pytest.mark.parametrize('kind', DT)
+@pytest.mark.parametrize('V', VOCABS)
+def test_rows(layout, kind, V):
+    gen = _gen(V, len(kind))
+    x = torch.randn(5, V, generator=gen, device='cuda').mul_(3)
+    x[1] *= 8
+    x[2] /= 100
+    x = x.to(DT[kind])
+    given = torch.randint(V, (5,), generator=gen, device='cuda')
+    for top in sorted({0, 1, min(V, 5), min(V, 20), min(V, 64)}):
+        _check(x, given, top)
+    _check(x, torch.randint(-1, V + 2, (5, 3), generator=gen, device='cuda', dtype=torch.int32), 1)
+    _check(x, None, 1)
+
+
+@pytest.mark.parametrize('kind', DT)
+@pytest.mark.parametrize('V', (3, 100, 1000, 4097, 50257))
+@pytest.mark.parametrize('share', (0.0, 0.0005, 0.2))
+def test_bans(layout, kind, V, share):
+    """Rows of which little or nothing is allowed: the rest follows by id."""
+    gen = _gen(V, 7)
+    x = torch.randn(6, V, generator=gen, device='cuda').mul_(2).to(DT[kind])
+    x.masked_fill_(torch.rand(6, V, generator=gen, device='cuda') >= share, -math.inf)
+    x[0, V // 2] = 1.0                                     # one allowed
+    x[1, 0] = -3.0
+    x[2] = -math.inf
+    x[3, V - 1] = torch.finfo(DT[kind]).min                # the type's lowest value beside -inf
+    x[4] = torch.finfo(DT[kind]).min
+    x[4, V // 3] = 0.0
+    given = torch.stack((torch.full((6,), V // 2, device='cuda'), torch.zeros(6, dtype=torch.long, device='cuda')), 1)
+    got = _check(x, given, min(V, 20))
+    assert got.entropy[2] == 0 and (got.given[2] == -math.inf).all() and (got.top[2] == -math.inf).all()
+
+
+@pytest.mark.parametrize('kind', DT)
+@pytest.mark.parametrize('V', (5, 300, 50257))
+def test_ties(layout, kind, V):
+    """Equal logits, signed zeros among them: the lowest ids first, however many."""
+    x = torch.zeros(5, V, device='cuda', dtype=DT[kind])
+    x[0, ::2] = -0.0
+    x[1] = torch.arange(V, device='cuda').remainder(3).to(x.dtype)
+    x[2, :V // 2] = 1.0
+    x[3] = -torch.arange(V, device='cuda').div(200, rounding_mode='floor').to(x.dtype)
+    x[4] = torch.arange(V, device='cuda').div(2000, rounding_mode='floor').to(x.dtype)
+    _check(x, torch.zeros(5, dtype=torch.long, device='cuda'), min(V, 64))
+    _check(x, None, 1)
+
+
+@pytest.mark.parametrize('kind', DT)
+@pytest.mark.parametrize('V', (4, 1000, 50257))
+def test_not_finite(layout, kind, V):
+    """A NaN or +inf makes its own row NaN and no other, its ids are in order."""
+    from vesta.logprobs import logprobs
+    x = torch.randn(5, V, generator=_gen(V), device='cuda').to(DT[kind])
+    x[1, V // 2] = math.nan
+    x[2, V - 1] = math.inf
+    x[3, 1] = math.nan
+    x[3, 2] = math.inf
+    x[3, 3] = -math.inf
+    given = torch.zeros(5, dtype=torch.int32, device='cuda')
+    got = logprobs(x, given, top=3)
+    for t in (got.given, got.entropy, got.top):
+        assert t[1:4].isnan().all() and t[[0, 4]].isfinite().all()
+    assert got.ids[1, 0] == V // 2 and got.ids[2, 0] == V - 1 and got.ids[3, :2].tolist() == [1, 2]
+    rest = torch.sort(x[1].nan_to_num(math.inf), descending=True, stable=True).indices[:3]
+    assert got.ids[1].tolist() == rest.tolist()
+    _check(x[[0, 4]], given[:2], 3)
+
+
+def test_pitches_and_offsets(layout):
+    """Rows inside a wider tensor, at any alignment, of which nothing beside them is read as theirs."""
+    for kind in DT:
+        wide = torch.full((6, 1100), math.nan, device='cuda', dtype=DT[kind])
+        for at in range(9):
+            x = wide[:, at:at + 1003]
+            x.copy_(torch.randn(6, 1003, generator=_gen(at), device='cuda'))
+            _check(x, torch.arange(6, device='cuda') * 200, 7)
+            wide.fill_(math.nan)
+        x = torch.randn(1, 700, generator=_gen(1), device='cuda').to(DT[kind])
+        _check(x.expand(4, 700), torch.arange(4, device='cuda'), 3)
+
+
+@pytest.mark.parametrize('kind', DT)
+@pytest.mark.parametrize('M,V', [(1, 200001), (3, 1 << 20), (300, 9001), (2000, 513)])
+def test_sizes(kind, M, V):
+    gen = _gen(M, V)
+    x = torch.randn(M, V, generator=gen, device='cuda').mul_(4).to(DT[kind])
+    given = torch.randint(V, (M, 2), generator=gen, device='cuda')
+    for top in (0, 10):
+        _check(x, given, top)
+
+
+def test_nearly_certain():
+    """Rows of one token far above the rest: log probabilities near 0 and small entropies."""
+    x = torch.zeros(40, 3001, device='cuda')
+    x[:, 77] = torch.arange(40, device='cuda') * 1.0
+    _check(x, torch.full((40,), 77, device='cuda'), 2)
+
+
+def test_a_large_offset():
+    """Rows past 2^31 elements."""
+    V = 300007
+    x = torch.zeros(7300, V, device='cuda', dtype=torch.float16)                    # 2.19e9 elements
+    x[-3:] = torch.randn(3, V, generator=_gen(9), device='cuda').half()
+    from vesta.logprobs import logprobs
+    given = torch.arange(7300, device='cuda')
+    got = logprobs(x, given, top=5)
+    last = _check(x[-3:], given[-3:], 5)
+    assert torch.equal(got.ids[-3:], last.ids)
+    assert (got.top[-3:] - last.top).abs().max() < 1e-5
+    assert (got.given[0] + math.log(V)).abs() < 1e-4 and got.ids[0].tolist() == [0, 1, 2, 3, 4]
+
+
+def test_empty():
+    from vesta.logprobs import logprobs
+    got = logprobs(torch.zeros(0, 9, device='cuda'), torch.zeros(0, dtype=torch.int32, device='cuda'), top=2)
+    assert got.given.shape == (0,) and got.entropy.shape == (0,) and got.top.shape == (0, 2)
+    got = logprobs(torch.zeros(4, 9, device='cuda'), torch.zeros(4, 0, dtype=torch.int64, device='cuda'))
+    assert got.given.shape == (4, 0) and got.entropy.shape == (4,)
+
+
+def test_gradients_refused():
+    from vesta.logprobs import logprobs
+    x = torch.zeros(2, 9, device='cuda', requires_grad=True)
+    with pytest.raises(ValueError, match='gradient'):
+        logprobs(x)
+    with torch.no_grad():
+        logprobs(x)
+
+
+def test_streams_and_graphs(layout):
+    """Two captured calls replay on new contents, eager calls of another stream beside them."""
+    from vesta.logprobs import logprobs
+    x = torch.randn(3, 5001, device='cuda')
+    given = torch.zeros(3, dtype=torch.int32, device='cuda')
+    logprobs(x, given, top=4)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = logprobs(x, given, top=4)
+        graphs.append((g, got))
+    side = torch.cuda.Stream()
+    for n in range(4):
+        x.normal_()
+        given.random_(0, 5001)
+        want = logprobs(x, given, top=4)
+        torch.cuda.synchronize()
+        for g, _ in graphs:
+            g.replay()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            eager = logprobs(x, given, top=4)
+        torch.cuda.synchronize()
+        for got in (eager, *(got for _, got in graphs)):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
