@@ -16,16 +16,27 @@ def _gpu():
         pytest.skip('no GPU')
 
 
-@pytest.fixture(params=('rule', '256 whole', '512 whole', '1024 whole', '256 in 3', '1024 in 64'))
+LAYOUTS = {                                                # kernel, threads, parts of a row
+    'rule': None, 'a wave': ('lp_rows64', 64, 1), 'a block of 256': ('lp_rows256', 256, 1),
+    'a block of 512': ('lp_rows512', 512, 1), 'a block of 1024': ('lp_rows1024', 1024, 1),
+    '3 blocks': ('lp_rows256', 256, 3), '64 blocks': ('lp_rows1024', 1024, 64), 'parts of 2': ('lp_part2', 256, 0),
+    'parts of 4': ('lp_part4', 256, 0), 'parts of 8': ('lp_part8', 256, 0)}
+
+
+@pytest.fixture(params=LAYOUTS)
 def layout(request, monkeypatch):
     """Rows as the rule has them, or by one kernel, whole or in parts."""
     from vesta import logprobs as lp
     if request.param != 'rule':
-        threads, *_, parts = request.param.split()
+        name, threads, parts = LAYOUTS[request.param]
 
-        def fixed(M, V, size):
-            each = V if parts == 'whole' else -(-V // int(parts))
-            return int(threads), -(-V // each), each
+        def fixed(M, V, size, top):
+            if parts == 0 and V < 16 // size:              # less than a load
+                return 'lp_rows64', 64, 1, V
+            each = -(-V // parts) if parts else 256 * int(name[-1]) * 16 // size
+            if parts == 0 and V > each:                    # (parts of the same size, of whole loads)
+                each = -(-V // -(-V // each) // (16 // size)) * (16 // size)
+            return name, threads, -(-V // each), each
 
         monkeypatch.setattr(lp, '_layout', fixed)
 

@@ -44,9 +44,15 @@ def test_other_arguments():
 
 
 @pytest.mark.parametrize('size', (2, 4))
-@pytest.mark.parametrize('M,V', [(1, 1), (1, 50257), (8, 50257), (1, 1 << 20), (3, 200000), (4096, 50257), (100000, 3), (64, 128001)])
-def test_layout(M, V, size):
-    """The parts of a row cover it, none is empty, and the joining kernel's limit holds."""
-    threads, parts, each = lp._layout(M, V, size)
-    assert threads in (256, 512, 1024) and 1 <= parts <= 64
+@pytest.mark.parametrize('top', (0, 5, 20, 64))
+@pytest.mark.parametrize('M', (1, 8, 64, 65, 256, 300, 4096, 100000))
+@pytest.mark.parametrize('V', (1, 3, 1000, 5001, 32768, 32769, 50257, 128001, 200000, 1 << 19, (1 << 19) + 1, (1 << 30) - 1))
+def test_layout(M, V, size, top):
+    """The parts of a row cover it, none is empty, and the kernels' limits hold."""
+    name, threads, parts, each = lp._layout(M, V, size, top)
+    assert name in lp.SIGNATURES and 1 <= parts <= 64
     assert parts * each >= V > (parts - 1) * each
+    if name.startswith('lp_part'):
+        assert threads == 256 and each <= 256 * int(name[7:]) * (16 // size) and V >= 16 // size and each % (16 // size) == 0
+    else:
+        assert name == f'lp_rows{threads}'

@@ -3,6 +3,7 @@
     m = VestaGPT2(hf, dtype='f16', batch=8, tmax=1024)
     m.reset(); m.x.copy_(tok); m.t.fill_(p); m.step()     # one decode step
     m.logits(), m.next()                                    # views, no sync
+    m.logprobs(given=ids, top=5)                            # log probabilities, entropies, alternatives; no sync
     m.check()                                               # raises if a launch failed (syncs)
 
 The object keeps a host copy of the position to refuse steps past the last
@@ -315,10 +316,11 @@ class VestaGPT2:
         self._prefill_kernel().launch(P, tokens, ins)
         self._take_outputs()
 
-    def extend(self, cache, tokens, positions, table, starts, lengths, weight=None, most=None):
+    def extend(self, cache, tokens, positions, table, starts, lengths, weight=None, most=None, given=None, top=0):
         """New tokens of sequences of different lengths whose key and value
-        rows lie in ``cache``, a ``vesta.paged.PagedCache`` of this model's
-        layers and heads (f16), instead of this object's own: ``tokens`` and
+        rows lie in ``cache``, a ``vesta.paged.PagedCache`` or
+        ``vesta.paged8.PagedCache8`` of this model's layers and heads (f16),
+        instead of this object's own: ``tokens`` and
         ``positions`` (int32 device tensors [M]; which learned position each
         has, its count in the conversation whatever has been evicted: as many
         as ``wpe`` has rows, so a conversation ends there or starts its count
@@ -331,6 +333,12 @@ class VestaGPT2:
         ``cache.evict``; ``most`` bounds the new tokens of a sequence (1 for a
         decode step).
 
+        ``given`` (int32 or int64 ids [M] or [M, C]), ``top``: a third result,
+        ``vesta.logprobs.LogProbs`` of all M rows: the log probabilities of
+        given[i] after row i (of a text, its own next tokens: how well the
+        model, or one whose cache holds 8 bits, foretells it), the entropies
+        and the ``top`` most likely tokens.
+
         Nothing is read back, so a call can be captured in a HIP graph, after
         one call of as many tokens and sequences. Calls share this object's
         activation buffers, those of two streams must not overlap.
@@ -338,10 +346,12 @@ class VestaGPT2:
         or id outside its table is clamped into it, and an error of the
         cache's if its row is a sequence's."""
         import torch
+        from . import logprobs
         from .paged import PagedCache, PagedPass
+        from .paged8 import PagedCache8
         from .prefill import Prefill, supported
         if not isinstance(cache, PagedCache):
-            raise TypeError('cache: need a vesta.paged.PagedCache')
+            raise TypeError('cache: need a vesta.paged.PagedCache or a vesta.paged8.PagedCache8')
         want = (self.L, self.H, self.E, self.W['wte'].dtype)
         have = (cache.layers, cache.heads, cache.width, cache.dtype)
         if have != want:
@@ -360,7 +370,10 @@ class VestaGPT2:
         if B < 1 or N < 1:
             raise ValueError(f'table {tuple(table.shape)}: one sequence and one page at least')
         if weight is not None:
+            if isinstance(cache, PagedCache8):
+                raise ValueError('weight: a cache in 8 bits counts none')
             cache._weights('weight', weight, (self.L, B, self.H), N * cache.page)
+        top = logprobs.check(given, top, tokens.shape[0], self.W['wte'].shape[0], cache.device)
         _, back = cache._enter()             # (the layers' launches go to the current device's stream)
         try:
             if self._paged is None:
@@ -369,7 +382,7 @@ class VestaGPT2:
                 if self._pf is None:
                     self._pf = Prefill(self)
                 self._paged = PagedPass(self, self._pf)
-            return self._paged.run(cache, tokens, positions, table, starts, lengths, weight, most)
+            return self._paged.run(cache, tokens, positions, table, starts, lengths, weight, most, given, top)
         finally:
             cache._leave(back)
 
@@ -390,6 +403,13 @@ class VestaGPT2:
         kp = self._prefill_kernel()
         for name in ('logit', 'next'):
             self.k.view(name).copy_(kp.view(name))
+
+    def logprobs(self, given=None, top=0):
+        """``vesta.logprobs.LogProbs`` of the last step's rows: the log
+        probabilities of ``given`` tokens (int32 or int64 ids [B] or [B, C]),
+        the entropies and the ``top`` most likely tokens. No synchronisation."""
+        from .logprobs import logprobs
+        return logprobs(self.logits(), given, top)
 
     def logits(self):
         return self._logit if self.k is None else self.k.view('logit')

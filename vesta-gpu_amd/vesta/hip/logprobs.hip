@@ -9,8 +9,8 @@
 // is read once; they are brought to a common maximum and added at the end. Sums
 // are fp32, of a thread's elements in order, then over lanes and waves in order.
 //
-// The k most likely: of 64 disjoint groups of threads, the kth largest of their
-// maxima is a bound that k elements reach. The few threads whose maximum does
+// The k most likely: of 64 disjoint groups of threads (a lane of each wave), the
+// kth largest of their maxima is a bound that k elements reach. The few threads whose maximum does
 // look at their elements again and list those that reach it; an element's rank
 // is the number of listed ones before it. Elements are compared as a key of their
 // value's order and, in the same word, their id's from the lowest.
@@ -60,11 +60,11 @@ __device__ __forceinline__ void lp_unpack(vh_u32x4 w, float* v) {
 }
 
 // An element's key, above 0; a value back from it.
-__device__ __forceinline__ lp_key lp_key_of(float v, int id) {
+__device__ __forceinline__ unsigned lp_word(float v) {
   const unsigned b = __builtin_bit_cast(unsigned, v + 0.0f);       // (-0 is 0)
-  const unsigned o = v != v ? 0xffffffffu : b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
-  return (lp_key)o << 32 | (unsigned)~id;
+  return v != v ? 0xffffffffu : b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ lp_key lp_key_of(float v, int id) { return (lp_key)lp_word(v) << 32 | (unsigned)~id; }
 __device__ __forceinline__ float lp_value(lp_key k) {
   const unsigned o = (unsigned)(k >> 32);
   return __builtin_bit_cast(float, o ^ (o >> 31 ? 0x80000000u : 0xffffffffu));
@@ -85,7 +85,7 @@ __device__ __forceinline__ void lp_move(LpSums& a, float m) {
   a.m = m;
 }
 template <int N>
-__device__ __forceinline__ void lp_add(LpSums& a, const float* v) {
+__device__ __forceinline__ float lp_add(LpSums& a, const float* v) {      // (the elements' largest)
   float m = v[0];
 #pragma unroll
   for (int j = 1; j < N; ++j) m = fmaxf(m, v[j]);
@@ -97,26 +97,38 @@ __device__ __forceinline__ void lp_add(LpSums& a, const float* v) {
     a.s += e;
     a.t = fmaf(e, fmaxf(d, -1e4f), a.t);
   }
+  return m;
+}
+// The waves' together.
+template <int NW>
+__device__ __forceinline__ LpSums lp_all(const LpSums* sums) {
+  const int lane = threadIdx.x & 63;
+  LpSums a = {-INFINITY, 0.0f, 0.0f};
+  if (lane < NW) a = sums[lane];
+  lp_move(a, wave_red_max(a.m));
+  a.s = wave_red_sum(a.s);
+  a.t = wave_red_sum(a.t);
+  return a;
 }
 
-// A thread's elements of x[0 .. n): up to the first 16-byte boundary and behind
-// the last whole load one each, between them every NT-th load of 16 bytes. `see`
-// gets U loads' elements, the first's id (a load's first is NT loads after the
-// one's before) and how many of them there are: the others are -inf.
-template <int NT, int U, typename F>
-__device__ __forceinline__ void lp_visit(const lp_t* __restrict__ x, int n, F see) {
-  const int tid = threadIdx.x;
-  const int head = min(n, (int)((16 - ((size_t)x & 15)) & 15) / (int)sizeof(lp_t));
-  const int loads = (n - head) / LP_VEC, tail = head + loads * LP_VEC;
-  const vh_u32x4* body = (const vh_u32x4*)(x + head);
-  vh_u32x4 w[U];
-  auto get = [&](int i) {
+// A thread's elements of x[0 .. n), in chunks of U loads of 16 bytes, NT loads
+// apart; one more chunk is an element before the first 16-byte boundary or behind
+// the last whole load.
+template <int NT, int U>
+struct LpSpan {
+  static constexpr int N = U * LP_VEC;
+  const lp_t* x;
+  int n, head, loads;
+  __device__ __forceinline__ LpSpan(const lp_t* from, int count) : x(from), n(count) {
+    head = min(n, (int)((16 - ((size_t)x & 15)) & 15) / (int)sizeof(lp_t));
+    loads = (n - head) / LP_VEC;
+  }
+  __device__ __forceinline__ void get(int i, vh_u32x4* w) const {  // the chunk that begins with load i
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = body[min(i + u * NT, loads - 1)];
-  };
-  if (tid < loads) get(tid);
-  for (int i = tid; i < loads; i += U * NT) {
-    float v[U * LP_VEC];
+    for (int u = 0; u < U; ++u) w[u] = ((const vh_u32x4*)(x + head))[min(i + u * NT, loads - 1)];
+  }
+  // How many elements a chunk has; the others, behind them, are made -inf.
+  __device__ __forceinline__ int open(int i, const vh_u32x4* w, float* v) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       lp_unpack(w[u], v + u * LP_VEC);
@@ -125,19 +137,39 @@ __device__ __forceinline__ void lp_visit(const lp_t* __restrict__ x, int n, F se
         for (int j = 0; j < LP_VEC; ++j) v[u * LP_VEC + j] = -INFINITY;
       }
     }
-    if (i + U * NT < loads) get(i + U * NT);
-    see(v, head + i * LP_VEC, min(U, (loads - i + NT - 1) / NT) * LP_VEC);
+    return min(U, (loads - i + NT - 1) / NT) * LP_VEC;
   }
-  const int rest = head + n - tail;                                // fewer than 16
-  if (tid < rest) {
-    const int id = tid < head ? tid : tail + tid - head;
-    float v[U * LP_VEC];
+  __device__ __forceinline__ int id(int i, int j) const { return head + (i + j / LP_VEC * NT) * LP_VEC + j % LP_VEC; }
+  // The element beside the loads: its id, or -1 for none.
+  __device__ __forceinline__ int beside() const {
+    const int t = threadIdx.x, behind = head + loads * LP_VEC + t - head;
+    return t < head ? t : behind < n ? behind : -1;
+  }
+  __device__ __forceinline__ void one(int id, float* v) const {
     v[0] = lp_f(x[id]);
 #pragma unroll
-    for (int j = 1; j < U * LP_VEC; ++j) v[j] = -INFINITY;
-    see(v, id, 1);
+    for (int j = 1; j < N; ++j) v[j] = -INFINITY;
   }
-}
+  // All chunks: see(first load (-1: the element beside), elements, how many, the id of one). The next chunk's loads are
+  // in flight while one is seen.
+  template <typename F>
+  __device__ __forceinline__ void visit(F see) const {
+    vh_u32x4 w[U];
+    float v[N];
+    const int extra = beside();
+    if ((int)threadIdx.x < loads) get(threadIdx.x, w);
+    for (int i = threadIdx.x; i < loads; i += U * NT) {
+      const int have = open(i, w, v);
+      if (i + U * NT < loads) get(i + U * NT, w);
+      see(i, v, have);
+    }
+    if (extra >= 0) {
+      one(extra, v);
+      see(-1, v, 1);
+    }
+  }
+  __device__ __forceinline__ int id_of(int i, int j) const { return i < 0 ? beside() : id(i, j); }
+};
 
 // A row's results. `x` is the row.
 struct LpRow {
@@ -155,6 +187,113 @@ __device__ __forceinline__ void lp_given(const LpRow& r, int V, const int* __res
   out[at] = id >= 0 && id < V ? lp_prob(r, lp_f(r.x[id])) : __builtin_nanf("");
 }
 
+// The code from here on runs once a block, and most of what it would take as
+// straight lines is fetching them (64 comparisons as such 2500 cycles, 1400 the
+// second time): short loops, few instructions.
+//
+// The kth largest of a wave's values, each lane with one, or a bound below it that
+// few more reach: of 16 lanes' maxima each fourth for k up to 8, 32 up to 20.
+__device__ __forceinline__ float lp_kth(float g, int k) {
+  int lanes = 64;
+  if (k <= 20) {
+    lanes = 32;
+    g = vh_pair32(g, op_max);
+  }
+  if (k <= 8) {
+    lanes = 16;
+    g = vh_pair16(g, op_max);
+  }
+  int above = 0;
+#pragma nounroll
+  for (int i = 0; i < lanes; i += 16)
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      above += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, g), i + j)) > g ? 1 : 0;
+  return wave_red_min(above < k ? g : INFINITY);                   // the least of those that fewer than k are above
+}
+// A group's largest, of its waves'.
+template <int NW>
+__device__ __forceinline__ float lp_group(const float (*owns)[64], int lane) {
+  float g = owns[0][lane];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) g = fmaxf(g, owns[w][lane]);
+  return g;
+}
+// -inf as a bound: fewer groups than k have anything else, and what else there is is listed.
+__device__ __forceinline__ float lp_least(float bound) { return fmaxf(bound, -3.402823466e38f); }
+// N of each lane's elements that reach the bound into the list, one of each lane
+// at a time; the lanes in this branch take places together. (Values are read
+// again: choosing a register takes more.)
+template <int N, typename F>
+__device__ __forceinline__ void lp_list(const lp_t* __restrict__ x, const float* v, float least, lp_key* list, int* listed,
+                                        F id_of) {
+  lp_key in = 0;                                                   // bit N - 1 - j: element j
+#pragma unroll
+  for (int j = 0; j < N; ++j) in = in + in + (v[j] >= least ? 1 : 0);
+#pragma nounroll
+  while (in) {
+    const int bit = 63 - __builtin_clzl(in), id = id_of(N - 1 - bit);
+    in &= ~((lp_key)1 << bit);
+    const lp_t value = x[id];
+    const lp_key lanes = __ballot(1);
+    const int before = __builtin_popcountl(lanes & (((lp_key)1 << (threadIdx.x & 63)) - 1));
+    int at = 0;
+    if (before == 0)
+      at = __hip_atomic_fetch_add(listed, __builtin_popcountl(lanes), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    at = __builtin_amdgcn_readfirstlane(at) + before;
+    if (at < LP_LIST) list[at] = lp_key_of(lp_f(value), id);
+  }
+}
+// The listed ones' ranks, of which `found` gets those below k.
+template <int NT, typename F>
+__device__ __forceinline__ void lp_order(const lp_key* list, int count, int k, F found) {
+  for (int i = threadIdx.x; i < count; i += NT) {
+    const lp_key key = list[i];
+    int rank = 0;
+#pragma nounroll
+    for (int j = 0; j < count; j += 4) {                           // (reads past the last are its own again)
+      lp_key o[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o[u] = list[min(j + u, count - 1)];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) rank += j + u < count && o[u] > key ? 1 : 0;
+    }
+    if (rank < k) found(rank, key);
+  }
+}
+// The places behind `count` listed elements, by one wave: the rest of x[0 .. n),
+// whose ids begin at `first`, is -inf, and follows by its ids (of the lowest
+// count + k ids k are at least, if there are as many); 0 where nothing does.
+template <typename F>
+__device__ __forceinline__ void lp_none(const lp_t* __restrict__ x, int n, int first, int count, int k, F found) {
+  const int lane = threadIdx.x & 63;
+  int at = count;
+  for (int i = 0; at < k && i < n; i += 64) {
+    const bool none = i + lane < n && lp_f(x[i + lane]) == -INFINITY;
+    const lp_key all = __ballot(none);
+    const int rank = at + __builtin_popcountl(all & (((lp_key)1 << lane) - 1));
+    if (none && rank < k) found(rank, lp_key_of(-INFINITY, first + i + lane));
+    at += __builtin_popcountl(all);
+  }
+  for (int i = at + lane; i < k; i += 64) found(i, 0);
+}
+// The block's largest key.
+template <int NW>
+__device__ __forceinline__ lp_key lp_block_best(lp_key top, lp_key* best) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const lp_key other = (lp_key)__shfl_xor((long)top, o, 64);
+    top = other > top ? other : top;
+  }
+  vh_lds_sync();
+  if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = top;
+  vh_lds_sync();
+  top = best[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) top = best[w] > top ? best[w] : top;
+  return top;
+}
+
 // A block makes one of `parts` parts of a row, of `each` elements: its results,
 // or with several parts its sums and most likely, in `ws`, for lp_join.
 template <int NT>
@@ -163,40 +302,34 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
                                              float* __restrict__ out_entropy, float* __restrict__ out_top,
                                              int* __restrict__ out_ids, lp_key* __restrict__ ws) {
   constexpr int NW = NT / 64, U = 4;
+  typedef LpSpan<NT, U> Span;
   __shared__ LpSums sums[NW];
-  __shared__ float groups[LP_TOP];
-  __shared__ float bound;
+  __shared__ float owns[NW][64];
   __shared__ int listed;
-  __shared__ __attribute__((aligned(16))) lp_key list[LP_LIST];
+  __shared__ lp_key list[LP_LIST];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long row = blockIdx.x / parts;
   const int part = (int)(blockIdx.x % parts), first = part * each, n = min(each, V - first);
   const lp_t* x = X + row * pitch;
+  const Span span(x + first, n);
   LpSums a = {-INFINITY, 0.0f, 0.0f};
-  lp_visit<NT, U>(x + first, n, [&](const float* v, int, int) { lp_add<U * LP_VEC>(a, v); });
-  const float own = a.m;                                           // the thread's largest
+  // Of the thread's chunks: which has its largest element, and the largest of the others.
+  int chunk = -1;
+  float other = -INFINITY;
+  span.visit([&](int i, const float* v, int) {
+    const float old = a.m, m = lp_add<Span::N>(a, v);
+    other = fmaxf(other, fminf(m, old));
+    chunk = m > old ? i : chunk;
+  });
+  const float own = a.m;
   lp_move(a, wave_red_max(a.m));
   a.s = wave_red_sum(a.s);
   a.t = wave_red_sum(a.t);
   if (lane == 0) sums[wave] = a;
-  if (k) {
-    const float g = group_red_max(own, NT / LP_TOP);
-    if (tid % (NT / LP_TOP) == 0) groups[tid / (NT / LP_TOP)] = g;
-    if (tid == 0) listed = 0;
-  }
+  owns[wave][lane] = own;
+  if (tid == 0) listed = 0;
   vh_lds_sync();
-  a = sums[0];
-  float m = a.m;
-#pragma unroll
-  for (int w = 1; w < NW; ++w) m = fmaxf(m, sums[w].m);
-  lp_move(a, m);
-#pragma unroll
-  for (int w = 1; w < NW; ++w) {
-    LpSums b = sums[w];
-    lp_move(b, m);
-    a.s += b.s;
-    a.t += b.t;
-  }
+  a = lp_all<NW>(sums);
   const LpRow r = lp_row(x, a);
   lp_key* mine = ws + (row * parts + part) * (2 + k);
   if (parts == 1) {
@@ -215,52 +348,31 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
       out_ids[row * k + rank] = lp_id(key);
     }
   };
-  if (wave == 0) {
-    const float g = groups[lane];
-    int rank = 0;
-#pragma unroll
-    for (int j = 0; j < LP_TOP; j += 4) {
-      const vh_f32x4 o = *(const vh_f32x4*)(groups + j);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) rank += o[e] > g || (o[e] == g && j + e < lane) ? 1 : 0;
-    }
-    if (rank == k - 1) bound = g;
-  }
-  vh_lds_sync();
-  // -inf as a bound: fewer groups than k have anything else, and what else there is is listed
-  const float least = bound == -INFINITY ? -3.402823466e38f : bound;
+  const float least = lp_least(lp_kth(lp_group<NW>(owns, lane), k));             // (each wave by itself)
   const bool odd = a.s != a.s;                                     // a NaN or +inf: found one by one
   if (!odd && own >= least) {
-    lp_visit<NT, U>(x + first, n, [&](const float* v, int id, int) {
-#pragma unroll
-      for (int j = 0; j < U * LP_VEC; ++j)
-        if (v[j] >= least) {
-          const int at = atomicAdd(&listed, 1);
-          if (at < LP_LIST) list[at] = lp_key_of(v[j], first + id + j / LP_VEC * (NT * LP_VEC) + j % LP_VEC);
-        }
-    });
+    auto look = [&](int i, const float* v, int) {
+      lp_list<Span::N>(x, v, least, list, &listed, [&](int j) { return first + span.id_of(i, j); });
+    };
+    if (other >= least) {
+      span.visit(look);
+    } else {
+      float v[Span::N];
+      if (chunk < 0) {
+        span.one(span.beside(), v);
+      } else {
+        vh_u32x4 w[U];
+        span.get(chunk, w);
+        span.open(chunk, w, v);
+      }
+      look(chunk, v, 0);
+    }
   }
   vh_lds_sync();
   const int count = listed;
   if (!odd && count <= LP_LIST) {
-    for (int i = tid; i < count; i += NT) {
-      const lp_key key = list[i];
-      int rank = 0;
-      for (int j = 0; j < count; ++j) rank += list[j] > key ? 1 : 0;
-      if (rank < k) found(rank, key);
-    }
-    // The rest are -inf, by their ids: of the lowest count + k ids k are at least, if the part has as many.
-    if (wave == 0) {
-      int at = count;
-      for (int i = 0; at < k && i < n; i += 64) {
-        const bool none = i + lane < n && lp_f(x[first + i + lane]) == -INFINITY;
-        const lp_key all = __ballot(none);
-        const int rank = at + __builtin_popcountl(all & (((lp_key)1 << lane) - 1));
-        if (none && rank < k) found(rank, lp_key_of(-INFINITY, first + i + lane));
-        at += __builtin_popcountl(all);
-      }
-      for (int i = at + lane; i < k; i += 64) found(i, 0);         // fewer than k elements in the part
-    }
+    lp_order<NT>(list, count, k, found);
+    if (wave == 0) lp_none(x + first, n, first, count, k, found);
     return;
   }
   // More reach the bound than are listed (many ties), or there are NaNs: the
@@ -269,24 +381,14 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
   lp_key last = ~(lp_key)0;
   for (int rank = 0; rank < k; ++rank) {
     lp_key top = 0;
-    lp_visit<NT, U>(x + first, n, [&](const float* v, int id, int have) {
+    span.visit([&](int i, const float* v, int have) {
 #pragma unroll
-      for (int j = 0; j < U * LP_VEC; ++j) {
-        const lp_key key = j < have ? lp_key_of(v[j], first + id + j / LP_VEC * (NT * LP_VEC) + j % LP_VEC) : 0;
+      for (int j = 0; j < Span::N; ++j) {
+        const lp_key key = j < have ? lp_key_of(v[j], first + span.id_of(i, j)) : 0;
         if (key < last && key > top) top = key;
       }
     });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const lp_key other = (lp_key)__shfl_xor((long)top, o, 64);
-      top = other > top ? other : top;
-    }
-    vh_lds_sync();
-    if (lane == 0) best[wave] = top;
-    vh_lds_sync();
-    last = best[0];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) last = best[w] > last ? best[w] : last;
+    last = lp_block_best<NW>(top, best);
     if (tid == 0) found(rank, last);
     if (last == 0) last = 1;                                       // none left: none after it either
   }
@@ -298,21 +400,123 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
       int* __restrict__ out_ids, lp_key* __restrict__ ws) {                                                        \
     lp_rows_body<threads>(X, pitch, V, given, wide, C, k, parts, each, out_given, out_entropy, out_top, out_ids, ws); \
   }
+LP_ROWS(lp_rows64, 64)
 LP_ROWS(lp_rows256, 256)
 LP_ROWS(lp_rows512, 512)
 LP_ROWS(lp_rows1024, 1024)
 
-// The parts of a row (64 at most) put together, a block a row.
-extern "C" __global__ __launch_bounds__(256) void lp_join(const lp_t* __restrict__ X, long pitch, int V,
-                                                          const int* __restrict__ given, int wide, int C, int k, int parts,
-                                                          float* __restrict__ out_given, float* __restrict__ out_entropy,
-                                                          float* __restrict__ out_top, int* __restrict__ out_ids,
-                                                          const lp_key* __restrict__ ws) {
-  __shared__ lp_key list[64 * LP_TOP];
-  const int tid = threadIdx.x, lane = tid & 63;
+// A part of NT L loads of 16 bytes of a row, which stay in registers: nothing is
+// looked at again. Loads are where they fall, at any alignment; the row's last
+// one begins early enough to end with it, and the elements that it has in common
+// with the one before count as -inf.
+typedef unsigned lp_u4 __attribute__((ext_vector_type(4), aligned(sizeof(lp_t))));
+template <int L>
+__device__ __forceinline__ void lp_part_body(const lp_t* __restrict__ X, long pitch, int V, int k, int parts, int each,
+                                             lp_key* __restrict__ ws) {
+  constexpr int NT = 256, NW = NT / 64;
+  __shared__ LpSums sums[NW];
+  __shared__ float owns[NW][64];
+  __shared__ int listed;
+  __shared__ lp_key list[LP_LIST];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long row = blockIdx.x / parts;
+  const int part = (int)(blockIdx.x % parts), first = part * each, end = min(first + each, V);
+  const lp_t* x = X + row * pitch;
+  vh_u32x4 w[L];
+#pragma unroll
+  for (int l = 0; l < L; ++l) w[l] = *(const lp_u4*)(x + min(first + (l * NT + tid) * LP_VEC, V - LP_VEC));
+  float v[L * LP_VEC];
+#pragma unroll
+  for (int l = 0; l < L; ++l) {
+    lp_unpack(w[l], v + l * LP_VEC);
+    const int e = first + (l * NT + tid) * LP_VEC, early = e < end ? e - (V - LP_VEC) : LP_VEC;     // elements not its own
+    if (early > 0) {
+#pragma unroll
+      for (int j = 0; j < LP_VEC; ++j) v[l * LP_VEC + j] = j >= early ? v[l * LP_VEC + j] : -INFINITY;
+    }
+  }
+  auto id_of = [&](int j) { return min(first + (j / LP_VEC * NT + tid) * LP_VEC, V - LP_VEC) + j % LP_VEC; };
+  float own = v[0];
+#pragma unroll
+  for (int j = 1; j < L * LP_VEC; ++j) own = fmaxf(own, v[j]);
+  own = fmaxf(own, -INFINITY);                                     // (a NaN where all are)
+  owns[wave][lane] = own;
+  if (tid == 0) listed = 0;
+  vh_lds_sync();
+  const float g = lp_group<NW>(owns, lane);
+  LpSums a = {wave_red_max(g), 0.0f, 0.0f};
+  if (k) {
+    const float least = lp_least(lp_kth(g, k));                    // (each wave by itself)
+    if (own >= least) lp_list<L * LP_VEC>(x, v, least, list, &listed, id_of);
+  }
+  const float ref = lp_ref(a.m);
+#pragma unroll
+  for (int j = 0; j < L * LP_VEC; ++j) {
+    const float d = v[j] - ref, e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+    a.s += e;
+    a.t = fmaf(e, fmaxf(d, -1e4f), a.t);
+  }
+  a.s = wave_red_sum(a.s);
+  a.t = wave_red_sum(a.t);
+  if (lane == 0) sums[wave] = a;
+  vh_lds_sync();
+  a = lp_all<NW>(sums);
+  lp_key* mine = ws + (row * parts + part) * (2 + k);
+  if (tid == 0) {
+    mine[0] = (lp_key)__builtin_bit_cast(unsigned, a.m) << 32 | __builtin_bit_cast(unsigned, a.s);
+    mine[1] = __builtin_bit_cast(unsigned, a.t);
+  }
+  if (k == 0) return;
+  const int count = listed;
+  if (a.s == a.s && count <= LP_LIST) {
+    auto found = [&](int rank, lp_key key) { mine[2 + rank] = key; };
+    lp_order<NT>(list, count, k, found);
+    if (wave == 0) lp_none(x + first, end - first, first, count, k, found);
+    return;
+  }
+  __shared__ lp_key best[NW];
+  lp_key last = ~(lp_key)0;
+  for (int rank = 0; rank < k; ++rank) {
+    lp_key top = 0;
+#pragma unroll
+    for (int j = 0; j < L * LP_VEC; ++j) {
+      const int e = first + (j / LP_VEC * NT + tid) * LP_VEC, early = e - (V - LP_VEC);
+      const lp_key key = e < end && j % LP_VEC >= early ? lp_key_of(v[j], id_of(j)) : 0;
+      if (key < last && key > top) top = key;
+    }
+    last = lp_block_best<NW>(top, best);
+    if (tid == 0) mine[2 + rank] = last;
+    if (last == 0) last = 1;                                       // none left: none after it either
+  }
+}
+#define LP_PART(name, loads)                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void name(const lp_t* __restrict__ X, long pitch, int V, int k, int parts, \
+                                                         int each, lp_key* __restrict__ ws) {                      \
+    lp_part_body<loads>(X, pitch, V, k, parts, each, ws);                                                          \
+  }
+LP_PART(lp_part2, 2)
+LP_PART(lp_part4, 4)
+LP_PART(lp_part8, 8)
+
+// The parts of a row (64 at most, of k listed elements each, MOST in all) put
+// together by a wave, as a part is by its block.
+template <int MOST>
+__device__ __forceinline__ void lp_join_body(const lp_t* __restrict__ X, long pitch, int V, const int* __restrict__ given,
+                                             int wide, int C, int k, int parts, float* __restrict__ out_given,
+                                             float* __restrict__ out_entropy, float* __restrict__ out_top,
+                                             int* __restrict__ out_ids, const lp_key* __restrict__ ws) {
+  __shared__ lp_key list[MOST];
+  const int lane = threadIdx.x, n = parts * k;
   const long row = blockIdx.x;
   const lp_key* from = ws + row * parts * (2 + k);
-  for (int i = tid; i < parts * k; i += 256) list[i] = from[i / k * (2 + k) + 2 + i % k];
+  auto entry = [&](int i) {
+    const int p = i / k;
+    return from[p * (2 + k) + 2 + i - p * k];
+  };
+  constexpr int E = 4;                                             // a lane's first entries
+  lp_key own[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) own[e] = lane + 64 * e < n ? entry(lane + 64 * e) : 0;
   LpSums a = {-INFINITY, 0.0f, 0.0f};
   if (lane < parts) {
     const lp_key w = from[lane * (2 + k)];
@@ -324,25 +528,41 @@ extern "C" __global__ __launch_bounds__(256) void lp_join(const lp_t* __restrict
   a.s = wave_red_sum(a.s);
   a.t = wave_red_sum(a.t);
   const LpRow r = lp_row(X + row * pitch, a);
-  for (int c = tid; c < C; c += 256) lp_given(r, V, given, wide, C, row, c, out_given);
-  if (tid == 0) out_entropy[row] = a.s == 0.0f ? 0.0f : r.log_s - a.t / a.s;
-  vh_lds_sync();
-  for (int i = tid; i < parts * k; i += 256) {
-    const lp_key key = list[i];
-    if (key == 0) continue;
-    int rank = i % k;                                              // its own part's are in order, and so are the others'
-    for (int p = 0; p < parts && rank < k; ++p) {
-      if (p == i / k) continue;
-      int lo = 0, hi = k;                                          // larger ones: lo at least, fewer than hi + 1
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (list[p * k + mid] > key) lo = mid + 1; else hi = mid;
-      }
-      rank += lo;
-    }
-    if (rank < k) {
-      out_top[row * k + rank] = lp_prob(r, lp_value(key));
-      out_ids[row * k + rank] = lp_id(key);
-    }
+  for (int c = lane; c < C; c += 64) lp_given(r, V, given, wide, C, row, c, out_given);
+  if (lane == 0) out_entropy[row] = a.s == 0.0f ? 0.0f : r.log_s - a.t / a.s;
+  if (k == 0) return;
+  // entries that reach the kth largest of the lanes' largest ones
+  lp_key top = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) top = own[e] > top ? own[e] : top;
+  for (int i = lane + 64 * E; i < n; i += 64) {
+    const lp_key o = entry(i);
+    top = o > top ? o : top;
   }
+  const float g = top == 0 ? -INFINITY : lp_value(top);             // (a NaN counts as the largest)
+  const unsigned least = lp_word(lp_kth(g != g ? INFINITY : g, k));
+  int count = 0;
+  auto pick = [&](lp_key key) {
+    const bool in = key != 0 && (unsigned)(key >> 32) >= least;
+    const lp_key all = __ballot(in);
+    if (in) list[count + __builtin_popcountl(all & (((lp_key)1 << lane) - 1))] = key;
+    count += __builtin_popcountl(all);
+  };
+#pragma unroll
+  for (int e = 0; e < E; ++e) pick(own[e]);
+  for (int i = 64 * E; i < n; i += 64) pick(i + lane < n ? entry(i + lane) : 0);
+  vh_lds_sync();
+  lp_order<64>(list, count, k, [&](int rank, lp_key key) {
+    out_top[row * k + rank] = lp_prob(r, lp_value(key));
+    out_ids[row * k + rank] = lp_id(key);
+  });
 }
+#define LP_JOIN(name, most)                                                                                        \
+  extern "C" __global__ __launch_bounds__(64) void name(                                                           \
+      const lp_t* __restrict__ X, long pitch, int V, const int* __restrict__ given, int wide, int C, int k, int parts, \
+      float* __restrict__ out_given, float* __restrict__ out_entropy, float* __restrict__ out_top,                 \
+      int* __restrict__ out_ids, const lp_key* __restrict__ ws) {                                                  \
+    lp_join_body<most>(X, pitch, V, given, wide, C, k, parts, out_given, out_entropy, out_top, out_ids, ws);       \
+  }
+LP_JOIN(lp_join, 256)
+LP_JOIN(lp_join_many, 64 * LP_TOP)

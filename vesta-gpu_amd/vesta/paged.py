@@ -669,6 +669,8 @@ class PagedCache:
 
 
 PLANS = 8                              # row counts whose launches a PagedPass keeps recorded
+SCORED = 512                           # rows whose logits it makes at a time where all rows' log probabilities are asked
+                                       # for: 103 MB of GPT-2's, which stay in the memory-side cache
 
 
 class PagedPass(Prefill):
@@ -689,6 +691,7 @@ class PagedPass(Prefill):
                                        t=torch.zeros(1, dtype=torch.int32, device=self.err.device))
         self._ws, self._ws_at, self._graph, self._plan, self.mod = None, ctypes.c_void_p(), None, [], None
         self._held, self._buf, self._plans = (0, 0), None, {}
+        self._scores, self._score_plans = None, {}
         self._outgrown = []              # buffers that a captured graph may hold
 
     def _room(self, M, B):
@@ -712,7 +715,7 @@ class PagedPass(Prefill):
             ZL=torch.empty(B, m.D, **f32), CF=torch.zeros(2 * last * m.D, **f16), logit=torch.empty(B, V, **f32),
             x=torch.zeros(B, **i32), next=torch.zeros(B, **f32), apv=torch.empty(B * ARGMAX_SPLIT, **f32),
             api=torch.empty(B * ARGMAX_SPLIT, **i32))
-        self._plans = {}
+        self._plans, self._score_plans = {}, {}
 
     def _workspace(self, n):
         if self._ws is None or self._ws.numel() < n:
@@ -777,12 +780,60 @@ class PagedPass(Prefill):
                             [self._record(lambda n=n: rest(n)) for n in range(self.layers)], self._record(head))
         return self._plans[key]
 
-    def run(self, cache, tokens, positions, table, starts, lengths, weight=None, most=None):
+    def _score_room(self, M):
+        """Buffers for the logits of M rows, SCORED at a time."""
+        import torch
+        from . import logprobs
+        rows = min(SCORED, M)
+        if self._scores is not None and self._scores[1].shape[0] >= rows:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f'extend: call once with the log probabilities of {M} tokens before capturing such a call')
+        W, dev = self.m.W['wte'], self.err.device
+        logprobs.load(dev.index, torch.float32)
+        rows = min(SCORED, 1 << (rows - 1).bit_length())
+        self._outgrown.append(self._scores)
+        self._scores = (torch.zeros(2 * 16 * _mtiles(rows) * self.m.D, dtype=torch.float16, device=dev),
+                        torch.empty(rows, W.shape[0], dtype=torch.float32, device=dev))
+        self._score_plans = {}
+
+    def _score(self, M, given, top):
+        """The log probabilities of all M rows (``vesta.logprobs``), their logits made SCORED rows at a time."""
+        from . import logprobs
+        m, b, W = self.m, self._buf, self.m.W
+        D, V, dev = m.D, W['wte'].shape[0], self.err.device
+        frag, logits = self._scores
+        if M not in self._score_plans:
+            while len(self._score_plans) >= PLANS:
+                del self._score_plans[next(iter(self._score_plans))]
+
+            def product(first, n):
+                self._norm(b.Z[first:first + n], W['lnfw'], W['lnfb'], frag, n)
+                if n <= MHEAD_ROWS:
+                    self._mhead(frag, D, V, logits, n)
+                else:
+                    self._pgemm(frag, D, 'wte', None, V, MODE_PLAIN, out=logits, ldo=V, M=n)
+
+            self._score_plans[M] = [(first, n, self._record(lambda first=first, n=n: product(first, n)))
+                                    for first in range(0, M, SCORED) for n in (min(SCORED, M - first),)]
+        got = logprobs.empty(given, top, M, dev)
+        for first, n, plan in self._score_plans[M]:
+            self._replay(plan)
+            part = slice(first, first + n)
+            logprobs.fill(logprobs.LogProbs(*(None if t is None else t[part] for t in got)), logits[:n],
+                          None if given is None else given[part], top)
+        return got
+
+    def run(self, cache, tokens, positions, table, starts, lengths, weight=None, most=None, given=None, top=0):
         """The new tokens' pass; returns the logits of each sequence's last
-        row and the largest's id, which the next call overwrites."""
+        row and the largest's id, which the next call overwrites, and, of
+        ``given`` tokens or ``top`` alternatives, all rows' log probabilities."""
         import torch
         M, B, H = tokens.shape[0], table.shape[0], self.m.H
+        scored = given is not None or top
         self._room(M, B)
+        if scored:
+            self._score_room(M)
         embed, qkv, rest, head = self._launches(M, B)
         b = self._buf
         wpe = self.m.W['wpe']
@@ -804,4 +855,5 @@ class PagedPass(Prefill):
             self._replay(rest[layer])
         torch.index_select(b.Z, 0, (starts[1:] - 1).clamp(0, M - 1), out=b.ZL[:B])
         self._replay(head)
-        return b.logit[:B], b.x[:B]
+        out = b.logit[:B], b.x[:B]
+        return (*out, self._score(M, given, top)) if scored else out
