@@ -51,6 +51,23 @@ __device__ __forceinline__ pg_factor pg_power(unsigned s) {
 }
 #endif
 
+// Whether any of 16 elements, or of a row's powers, stands for a NaN.
+__device__ __forceinline__ unsigned pg_odd(vh_u32x4 w) {
+  unsigned any = 0u;
+#if PG_FORM == 2
+#pragma unroll
+  for (int j = 0; j < 4; ++j) any |= (w[j] & 0x7f7f7f7fu) + 0x01010101u;
+#endif
+  return any & 0x80808080u;
+}
+__device__ __forceinline__ unsigned pg_odd_powers(pg_powers s) {
+#if PG_FORM == 1
+  return ((s & 0x7f7f7f7fu) + 0x01010101u) & s & 0x80808080u;
+#else
+  return 0u;
+#endif
+}
+
 // Four elements as two words of 16-bit values, exactly.
 // Whole numbers: fp16: q + 128 is put behind the exponent of 1024, and 1152 taken
 // off again (1 + 2 + 2 operations and a quarter more for the sign); bf16: through

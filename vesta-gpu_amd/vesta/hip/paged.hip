@@ -747,42 +747,55 @@ __device__ __forceinline__ void pg_attn_body(
       }
       pg_scores(kf, qf, qp, lane, s[i]);
     }
-    vh_u32x4 v8[NV];
-#pragma unroll
-    for (int n = 0; n < NV; n += 2) {
-      const unsigned w = (unsigned)__shfl((int)vw, n / 2 * VR + lane / VL, 64);
-      const pg_factor p = pg_power(w >> 8 * (lane % VL / 2) & 255u);
-      v8[n] = pg_open(vr[n / 2][0], vr[n / 2][1], p);
-      v8[n + 1] = pg_open(vr[n / 2][2], vr[n / 2][3], p);
-    }
 #else
 #pragma unroll
     for (int i = 0; i < NG; ++i) pg_scores(kr[i], qf, qp, lane, s[i]);
-    vh_u32x4 (&v8)[NV] = vr;
 #endif
     const bool seen = p0 + PG_STEP - 1 > first;                    // not the whole step by every row
     // values past the last position are 0; ones that are not finite are left
     // out of the product where a row may not see their position, or a plane of
     // its weight may be 0: 0 * inf ...
     bool wild = false;
+#if PG_FORM
+    if (seen || PG_KIND == PG_F32) {
+      unsigned any = pg_odd_powers(vw);
+#pragma unroll
+      for (int n = 0; n < NV / 2; ++n) any |= pg_odd(vr[n]);
+      wild = __any(any != 0u);
+    }
+    pg_wave_sync();                                                // the step before is read
+#pragma unroll
+    for (int n = 0; n < NV / 2; ++n) {                             // (opened one by one: all at once take 64 registers)
+      const int row = n * VR + lane / VL;
+      const pg_factor p = pg_power((unsigned)__shfl((int)vw, row, 64) >> 8 * (lane % VL / 2) & 255u);
+      vh_u32x4* to = (vh_u32x4*)(V + row * PG_VROW + lane % VL * 16);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        vh_u32x4 v = pg_open(vr[n][2 * c], vr[n][2 * c + 1], p);
+        if (p0 + PG_STEP - 1 > last && p0 + row > last) v = vh_u32x4{0u, 0u, 0u, 0u};
+        to[c] = wild ? pg_tame(v) : v;
+      }
+    }
+#else
     if (p0 + PG_STEP - 1 > last) {
 #pragma unroll
       for (int n = 0; n < NV; ++n)
-        if (p0 + n / VC * VR + lane / VL > last) v8[n] = vh_u32x4{0u, 0u, 0u, 0u};
+        if (p0 + n * VR + lane / VL > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
     }
     if (seen || PG_KIND == PG_F32) {
       unsigned any = 0u;
 #pragma unroll
-      for (int n = 0; n < NV; ++n) any |= pg_wild2(v8[n][0]) | pg_wild2(v8[n][1]) | pg_wild2(v8[n][2]) | pg_wild2(v8[n][3]);
+      for (int n = 0; n < NV; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
       wild = __any(any != 0u);
       if (wild) {
 #pragma unroll
-        for (int n = 0; n < NV; ++n) v8[n] = pg_tame(v8[n]);
+        for (int n = 0; n < NV; ++n) vr[n] = pg_tame(vr[n]);
       }
     }
     pg_wave_sync();                                                // the step before is read
 #pragma unroll
-    for (int n = 0; n < NV; ++n) *(vh_u32x4*)(V + (n / VC * VR + lane / VL) * PG_VROW + (lane % VL * VC + n % VC) * 8) = v8[n];
+    for (int n = 0; n < NV; ++n) *(vh_u32x4*)(V + (n * VR + lane / VL) * PG_VROW + lane % VL * 8) = vr[n];
+#endif
     pg_wave_sync();
     if (t + W < t1) {
       load(t + W, page);
@@ -1107,34 +1120,45 @@ __device__ __forceinline__ void pg_wide_body(
   // so are those that are not finite (0 * inf); that there are such is noted.
   auto put_v = [&](int t) {
 #if PG_FORM
-    vh_u32x4 v8[VC * NL];
+    bool wild = false;
+    if (PG_KIND == PG_F32 || 64 * t + 63 > bfirst) {               // (fp32: a plane of a weight may be 0)
+      unsigned any = 0u;
+#pragma unroll
+      for (int n = 0; n < NL; ++n) any |= pg_odd(vr[n]) | pg_odd_powers((pg_powers)vw[n]);
+      wild = any != 0u;
+      if (wild) lwild[t & 1] = t + 1;
+    }
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
       const pg_factor p = pg_power(vw[n]);
-      v8[2 * n] = pg_open(vr[n][0], vr[n][1], p);
-      v8[2 * n + 1] = pg_open(vr[n][2], vr[n][3], p);
+      vh_u32x4* to = (vh_u32x4*)(lv[t & 1] + (r8 + RS * n) * PG_WROW + 16 * c8);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        vh_u32x4 v = pg_open(vr[n][2 * c], vr[n][2 * c + 1], p);
+        if (64 * t + 63 > last && 64 * t + r8 + RS * n > last) v = vh_u32x4{0u, 0u, 0u, 0u};
+        to[c] = wild ? pg_tame(v) : v;
+      }
     }
 #else
-    vh_u32x4 (&v8)[NL] = vr;
-#endif
     if (64 * t + 63 > last) {
 #pragma unroll
-      for (int n = 0; n < VC * NL; ++n)
-        if (64 * t + r8 + RS * (n / VC) > last) v8[n] = vh_u32x4{0u, 0u, 0u, 0u};
+      for (int n = 0; n < NL; ++n)
+        if (64 * t + r8 + RS * n > last) vr[n] = vh_u32x4{0u, 0u, 0u, 0u};
       asm volatile("" ::: "memory");                               // kept a branch
     }
     if (PG_KIND == PG_F32 || 64 * t + 63 > bfirst) {               // (fp32: a plane of a weight may be 0)
       unsigned any = 0u;
 #pragma unroll
-      for (int n = 0; n < VC * NL; ++n) any |= pg_wild2(v8[n][0]) | pg_wild2(v8[n][1]) | pg_wild2(v8[n][2]) | pg_wild2(v8[n][3]);
+      for (int n = 0; n < NL; ++n) any |= pg_wild2(vr[n][0]) | pg_wild2(vr[n][1]) | pg_wild2(vr[n][2]) | pg_wild2(vr[n][3]);
       if (any) {
         lwild[t & 1] = t + 1;
 #pragma unroll
-        for (int n = 0; n < VC * NL; ++n) v8[n] = pg_tame(v8[n]);
+        for (int n = 0; n < NL; ++n) vr[n] = pg_tame(vr[n]);
       }
     }
 #pragma unroll
-    for (int n = 0; n < VC * NL; ++n) *(vh_u32x4*)(lv[t & 1] + (r8 + RS * (n / VC)) * PG_WROW + 8 * (VC * c8 + n % VC)) = v8[n];
+    for (int n = 0; n < NL; ++n) *(vh_u32x4*)(lv[t & 1] + (r8 + RS * n) * PG_WROW + 8 * c8) = vr[n];
+#endif
   };
   pg_f16v o[DT];
 #pragma unroll

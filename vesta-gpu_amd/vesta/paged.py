@@ -390,6 +390,13 @@ class PagedCache:
             import torch
             torch.cuda.set_device(back)
 
+    def _blocks(self, M):
+        """Blocks that take M rows' eight values a thread."""
+        grid = -(-M * self.heads * (self.width // 8) // BLOCK)
+        if grid >= 1 << 31:
+            raise ValueError(f'k: {M} rows are too many for one call')
+        return grid
+
     # ------------------------------------------------------------ operators
     def append(self, k, v, table, starts, lengths, layer=0):
         """The new tokens' key and value rows ``k``, ``v`` [M, heads, width]
@@ -405,9 +412,7 @@ class PagedCache:
             return
         kn = self._kind[self.dtype]
         launch = kn.pg_append32 if k.dtype is self._f32 else kn.pg_append16
-        grid = -(-M * self.heads * (self.width // 8) // BLOCK)
-        if grid >= 1 << 31:
-            raise ValueError(f'k: {M} rows are too many for one call')
+        grid = self._blocks(M)
         stream, back = self._enter()
         try:
             launch(grid, BLOCK, stream, k_at, v_at, *ks, *vs, *at, *seqs, B, M, self.heads, self._err)
@@ -526,7 +531,7 @@ class PagedCache:
         if wide:
             rows, aim, most_tiles, least, split = 128, WIDE_TARGET, 2 * WIDE_TARGET, WIDE_PART_STEPS, WIDE_SPLIT
         else:
-            rows, aim, most_tiles, least, split = ROWS, TARGET, 16 * TARGET, PART_STEPS, SPLIT[self.width]
+            rows, aim, most_tiles, least, split = ROWS, self._parts(), 16 * TARGET, PART_STEPS, SPLIT[self.width]
         tiles = self.heads * (B if most * G <= rows else M * G // rows + B)
         if tiles > 256:
             split = split * tiles // 256
@@ -552,6 +557,10 @@ class PagedCache:
         else:
             attn, block = kn.pg_attn, BLOCK
         return attn, block, rows, tiles, target, blocks, least, run
+
+    def _parts(self):
+        """About how many parts of long positions pg_attn makes."""
+        return TARGET
 
     def _floats(self, n):
         """A workspace of a call."""

@@ -41,8 +41,12 @@ FORMS = ('i8', 'e4m3')
 SCALED = 32                            # values of a power
 LEAST = {('i8', 'f16'): 109, ('i8', 'bf16'): 7, ('e4m3', 'f16'): 112, ('e4m3', 'bf16'): 10}    # bytes of the least powers
 
+# Parts of long positions, about: twice what the chip holds at once (1024 / 1536 / 2048, 2 sequences after 120,001 of width
+# 128 99 / 104 / 109, 96 after up to 6000 148 / 149 / 152, 4 after 20,000 of width 64 59 / 54 / 55).
+PARTS = {64: 1536, 128: 1024}
+
 _ATTENTION = ('pg_attn', 'pg_attn2', 'pg_attn8', 'pg_wide', 'pg_wide8')
-_POOLS = slice(3, 5)                   # where the pools are in their parameters: two more here, the powers'
+# the pools' two parameters are four here, with the powers'
 SIGNATURES = {name: SIGNATURES16[name] for name in ('pg_join', 'pg_wide_join', 'pg_take', 'pg_input')}
 SIGNATURES.update({name: SIGNATURES16[name][:5] + 'pp' + SIGNATURES16[name][5:] for name in _ATTENTION})
 SIGNATURES.update({name: 'ppllll' + 'pppp' + SIGNATURES16['pg_append16'][8:]
@@ -91,6 +95,16 @@ class PagedCache8(PagedCache):
                                                  dtype=torch.uint8, device=device) for _ in range(2))
         self._ready(self.keys, self.vals, self.kscales, self.vscales)
 
+    def _parts(self):
+        return PARTS[self.width]
+
+    def _blocks(self, M):
+        """Blocks whose waves take 1024 values of a head each, of 16 rows or 8."""
+        waves = -(-M * self.width // 1024) * self.heads
+        if waves >= 1 << 31:
+            raise ValueError(f'k: {M} rows are too many for one call')
+        return -(-waves // (BLOCK // 64))
+
     def attend(self, q, table, starts, lengths, layer=0, scale=None, out=None, most=None):
         """As ``PagedCache.attend``, without weights: attention of the new
         tokens' queries ``q`` [M, G * heads, width] over what ``layer`` holds
@@ -108,19 +122,19 @@ class PagedCache8(PagedCache):
         at = self._layer(layer)
         ks = self._rows('k', k, self._new, self.heads)
         vs = self._rows('v', v, (k.dtype,), like=k.shape)
-        size = 4 if k.dtype is self._f32 else 2
-        for name, t, (_, *strides) in (('k', k, ks), ('v', v, vs)):
-            if _collides(t.shape, strides):
+        size, E, last = 4 if k.dtype is self._f32 else 2, self.width, [0, 0]
+        for n, (name, t, (_, row, head)) in enumerate((('k', k, ks), ('v', v, vs))):
+            last[n] = (k.shape[0] - 1) * row + (self.heads - 1) * head + E
+            # (what most calls are is told by a line: the whole rules take 3 us more)
+            if not (head >= E and row >= (self.heads - 1) * head + E) and _collides(t.shape, (row, head)):
                 raise ValueError(f'{name}: rows that lie on one another (strides {t.stride()})')
-        if _overlap(k.shape, size, ks, vs):
+        if ks[0] < vs[0] + size * last[1] and vs[0] < ks[0] + size * last[0] and _overlap(k.shape, size, ks, vs):
             raise ValueError('v: memory other than that of k')
         M = k.shape[0]
         if M == 0 or B == 0:
             return k, v
         kn = self._kind[self.dtype]
-        grid = -(-M * self.heads * (self.width // 8) // BLOCK)
-        if grid >= 1 << 31:
-            raise ValueError(f'k: {M} rows are too many for one call')
+        grid = self._blocks(M)
         stream, back = self._enter()
         try:
             (kn.pg_read32 if size == 4 else kn.pg_read16)(grid, BLOCK, stream, ks[0], vs[0], *ks[1:], *vs[1:], *at, *seqs,
