@@ -214,6 +214,20 @@ def test_a_large_offset():
     assert (got.given[0] + math.log(V)).abs() < 1e-4 and got.ids[0].tolist() == [0, 1, 2, 3, 4]
 
 
+def test_very_many_rows():
+    """More rows than a launch has waves: in several launches."""
+    from vesta.logprobs import logprobs
+    M = (1 << 26) + 7
+    x = torch.zeros(M, 2, device='cuda', dtype=torch.float16)
+    x[-1, 1] = 3.0
+    given = torch.ones(M, dtype=torch.int32, device='cuda')
+    got = logprobs(x, given, top=1)
+    assert (got.given[:-1] + math.log(2)).abs().max() < 1e-6 and (got.entropy[:-1] - math.log(2)).abs().max() < 1e-6
+    assert not got.ids[:-1].any() and got.ids[-1, 0] == 1
+    _check(x[-9:], given[-9:], 1)
+    assert (got.given[-1] + math.log1p(math.exp(-3))).abs() < 1e-6
+
+
 def test_empty():
     from vesta.logprobs import logprobs
     got = logprobs(torch.zeros(0, 9, device='cuda'), torch.zeros(0, dtype=torch.int32, device='cuda'), top=2)

@@ -121,6 +121,11 @@ def test_the_models_own_steps(hf):  # noqa: F811
         assert got.given[1:, 1].isnan().all() and got.given[0, 1].isfinite()
         assert torch.equal(got.ids.long(), torch.sort(m.logits(), descending=True, stable=True).indices[:, :4])
         assert torch.equal(got.ids[:, 0], m.x)
+        m = VestaGPT2(hf, batch=1, tmax=32, engine=engine)
+        m.reset()
+        m.prefill(_ints([[5, 6, 7]]))
+        got = m.logprobs(top=1)
+        assert got.given is None and got.entropy.shape == (1,) and torch.equal(got.ids[0], m.x)
 
 
 @pytest.mark.parametrize('form', ('i8', 'e4m3'))

@@ -174,8 +174,11 @@ def fill(got, logits, given, top):
     index = logits.get_device()
     C = 0 if given is None else given.numel() // M
     name, threads, parts, each = _layout(M, V, logits.element_size(), top)
-    if M * parts >= 1 << 31:
-        raise ValueError(f'logits: {M} rows are too many for one call')
+    if M * parts * threads >= 1 << 32:       # more threads than a launch can have: half the rows at a time
+        for rows in (slice(0, M // 2), slice(M // 2, M)):
+            fill(LogProbs(*(None if t is None else t[rows] for t in got)), logits[rows],
+                 None if given is None else given[rows], top)
+        return
     kn = _known.get((index, logits.dtype)) or load(index, logits.dtype)
     row = (logits.data_ptr(), logits.stride(0) if M > 1 else V, V, given.data_ptr() if C else 0,
            int(C > 0 and given.dtype is torch.int64), C, top, parts)

@@ -101,7 +101,7 @@ class PagedCache8(PagedCache):
     def _blocks(self, M):
         """Blocks whose waves take 1024 values of a head each, of 16 rows or 8."""
         waves = -(-M * self.width // 1024) * self.heads
-        if waves >= 1 << 31:
+        if waves >= 1 << 26:                 # (a launch has fewer than 2^32 threads)
             raise ValueError(f'k: {M} rows are too many for one call')
         return -(-waves // (BLOCK // 64))
 
