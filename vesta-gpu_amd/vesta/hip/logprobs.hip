@@ -244,22 +244,38 @@ __device__ __forceinline__ void lp_list(const lp_t* __restrict__ x, const float*
     if (at < LP_LIST) list[at] = lp_key_of(lp_f(value), id);
   }
 }
-// The listed ones' ranks, of which `found` gets those below k.
+// The listed ones' ranks, of which `found` gets those below k, 64 at a time. Of
+// few the first wave counts the larger ones; of more each wave a share of them,
+// in `ranks`, which is zeroed (2000 rows of 50257 in bf16, 64 of some 300 listed:
+// 143 -> 130 us; of a few it would be a barrier more).
 template <int NT, typename F>
-__device__ __forceinline__ void lp_order(const lp_key* list, int count, int k, F found) {
-  for (int i = threadIdx.x; i < count; i += NT) {
+__device__ __forceinline__ void lp_order(const lp_key* list, int* ranks, int count, int k, F found) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool alone = NT == 64 || count <= 16;
+  const int waves = alone ? 1 : NT / 64;
+  if (wave >= waves) return;
+  for (int c = 0; c < count; c += 64) {
+    const int i = min(c + lane, count - 1);
     const lp_key key = list[i];
     int rank = 0;
 #pragma nounroll
-    for (int j = 0; j < count; j += 4) {                           // (reads past the last are its own again)
+    for (int j = wave; j < count; j += 4 * waves) {                // (reads past the last are its own again)
       lp_key o[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) o[u] = list[min(j + u, count - 1)];
+      for (int u = 0; u < 4; ++u) o[u] = list[min(j + u * waves, count - 1)];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) rank += j + u < count && o[u] > key ? 1 : 0;
+      for (int u = 0; u < 4; ++u) rank += j + u * waves < count && o[u] > key ? 1 : 0;
     }
-    if (rank < k) found(rank, key);
+    if (alone) {
+      if (c + lane < count && rank < k) found(rank, key);
+    } else if (c + lane < count && rank) {
+      __hip_atomic_fetch_add(ranks + i, rank, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
   }
+  if (alone) return;
+  vh_lds_sync();
+  for (int i = threadIdx.x; i < count; i += NT)
+    if (ranks[i] < k) found(ranks[i], list[i]);
 }
 // The places behind `count` listed elements, by one wave: the rest of x[0 .. n),
 // whose ids begin at `first`, is -inf, and follows by its ids (of the lowest
@@ -305,7 +321,8 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
   typedef LpSpan<NT, U> Span;
   __shared__ LpSums sums[NW];
   __shared__ float owns[NW][64];
-  __shared__ int listed;
+  __shared__ int listed, ranks[NW > 1 ? LP_LIST : 1];
+  __shared__ float bound;
   __shared__ lp_key list[LP_LIST];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long row = blockIdx.x / parts;
@@ -328,6 +345,8 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
   if (lane == 0) sums[wave] = a;
   owns[wave][lane] = own;
   if (tid == 0) listed = 0;
+  if (NW > 1 && k)
+    for (int i = tid; i < LP_LIST; i += NT) ranks[i] = 0;
   vh_lds_sync();
   a = lp_all<NW>(sums);
   const LpRow r = lp_row(x, a);
@@ -348,7 +367,17 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
       out_ids[row * k + rank] = lp_id(key);
     }
   };
-  const float least = lp_least(lp_kth(lp_group<NW>(owns, lane), k));             // (each wave by itself)
+  float least;
+  if (NW <= 4 || k <= 8) {                                         // little for a SIMD's waves: each by itself
+    least = lp_least(lp_kth(lp_group<NW>(owns, lane), k));
+  } else {
+    if (wave == 0) {
+      const float b = lp_kth(lp_group<NW>(owns, lane), k);
+      if (lane == 0) bound = b;
+    }
+    vh_lds_sync();
+    least = lp_least(bound);
+  }
   const bool odd = a.s != a.s;                                     // a NaN or +inf: found one by one
   if (!odd && own >= least) {
     auto look = [&](int i, const float* v, int) {
@@ -371,7 +400,7 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
   vh_lds_sync();
   const int count = listed;
   if (!odd && count <= LP_LIST) {
-    lp_order<NT>(list, count, k, found);
+    lp_order<NT>(list, ranks, count, k, found);
     if (wave == 0) lp_none(x + first, n, first, count, k, found);
     return;
   }
@@ -416,7 +445,7 @@ __device__ __forceinline__ void lp_part_body(const lp_t* __restrict__ X, long pi
   constexpr int NT = 256, NW = NT / 64;
   __shared__ LpSums sums[NW];
   __shared__ float owns[NW][64];
-  __shared__ int listed;
+  __shared__ int listed, ranks[LP_LIST];
   __shared__ lp_key list[LP_LIST];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long row = blockIdx.x / parts;
@@ -442,6 +471,8 @@ __device__ __forceinline__ void lp_part_body(const lp_t* __restrict__ X, long pi
   own = fmaxf(own, -INFINITY);                                     // (a NaN where all are)
   owns[wave][lane] = own;
   if (tid == 0) listed = 0;
+  if (k)
+    for (int i = tid; i < LP_LIST; i += NT) ranks[i] = 0;
   vh_lds_sync();
   const float g = lp_group<NW>(owns, lane);
   LpSums a = {wave_red_max(g), 0.0f, 0.0f};
@@ -470,7 +501,7 @@ __device__ __forceinline__ void lp_part_body(const lp_t* __restrict__ X, long pi
   const int count = listed;
   if (a.s == a.s && count <= LP_LIST) {
     auto found = [&](int rank, lp_key key) { mine[2 + rank] = key; };
-    lp_order<NT>(list, count, k, found);
+    lp_order<NT>(list, ranks, count, k, found);
     if (wave == 0) lp_none(x + first, end - first, first, count, k, found);
     return;
   }
@@ -552,7 +583,7 @@ __device__ __forceinline__ void lp_join_body(const lp_t* __restrict__ X, long pi
   for (int e = 0; e < E; ++e) pick(own[e]);
   for (int i = 64 * E; i < n; i += 64) pick(i + lane < n ? entry(i + lane) : 0);
   vh_lds_sync();
-  lp_order<64>(list, count, k, [&](int rank, lp_key key) {
+  lp_order<64>(list, nullptr, count, k, [&](int rank, lp_key key) {
     out_top[row * k + rank] = lp_prob(r, lp_value(key));
     out_ids[row * k + rank] = lp_id(key);
   });
