@@ -161,45 +161,63 @@ PG8_APPEND(pg_append32, float)
 // The rows of the new tokens' positions back as values. A row of a token at a
 // negative position, or of a sequence that cannot be, becomes 0; rows that are
 // no sequence's stay.
-// Stores of 16 bytes leave as many out: the caches put lines together (28,800 rows
-// of 25 heads of 64 into fp16 76.4 us; past the caches 95.6, and 100 in pieces that
-// two lanes have exchanged such that a store leaves nothing out).
-template <typename T>
-__device__ __forceinline__ void pg8_put(T* p, vh_u32x4 w, pg_factor f) {
+// A lane's 16 values. In 16 bits its stores of 16 bytes leave as many out: the
+// caches put the lines together (28,800 rows of 25 heads of 64 76.4 us; past the
+// caches 95.6, and 100 in pieces that two lanes have exchanged such that a store
+// leaves nothing out).
+__device__ __forceinline__ void pg8_put(unsigned short* p, vh_u32x4 w, pg_factor f) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const vh_u32x4 v = pg_open(w[2 * j], w[2 * j + 1], f);
-    if constexpr (sizeof(T) == 2) {
-      *(vh_u32x4*)(p + 8 * j) = v;
-    } else {
+  for (int j = 0; j < 2; ++j) *(vh_u32x4*)(p + 8 * j) = pg_open(w[2 * j], w[2 * j + 1], f);
+}
+// In 32 bits a store would leave out 48 bytes of 64: four lanes, whose 64 values
+// are one row's, store the first's together, then the second's.
+template <int FROM>
+__device__ __forceinline__ void pg8_put4(float* p, vh_u32x4 w, pg_factor f) {
+  constexpr int CTRL = FROM * 0x55;                                // of each four lanes the FROM-th
+  const int q = threadIdx.x & 3;
+  unsigned t[4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const unsigned a = v[2 * n], b = v[2 * n + 1];
-        *(vh_f32x4*)(p + 8 * j + 4 * n) = vh_f32x4{pg_to_f((unsigned short)(a & 0xffffu)), pg_to_f((unsigned short)(a >> 16)),
-                                                   pg_to_f((unsigned short)(b & 0xffffu)), pg_to_f((unsigned short)(b >> 16))};
-      }
-    }
-  }
+  for (int j = 0; j < 4; ++j) t[j] = (unsigned)__builtin_amdgcn_mov_dpp((int)w[j], CTRL, 0xF, 0xF, true);
+  const pg_factor g =
+      __builtin_bit_cast(pg_factor, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, f), CTRL, 0xF, 0xF, true));
+  const vh_u32x2 v = pg_open4(q & 2 ? (q & 1 ? t[3] : t[2]) : (q & 1 ? t[1] : t[0]), g);
+  *(vh_f32x4*)(p + 16 * (FROM - q) + 4 * q) =
+      vh_f32x4{pg_to_f((unsigned short)(v[0] & 0xffffu)), pg_to_f((unsigned short)(v[0] >> 16)),
+               pg_to_f((unsigned short)(v[1] & 0xffffu)), pg_to_f((unsigned short)(v[1] >> 16))};
+}
+__device__ __forceinline__ void pg8_put(float* p, vh_u32x4 w, pg_factor f) {
+  pg8_put4<0>(p, w, f);
+  pg8_put4<1>(p, w, f);
+  pg8_put4<2>(p, w, f);
+  pg8_put4<3>(p, w, f);
 }
 template <typename T>
 __device__ __forceinline__ void pg8_read_body(T* __restrict__ k, T* __restrict__ v, long krow, long khead, long vrow,
                                               long vhead, PG_POOL, int pages, int shift, const int* __restrict__ table,
                                               int N, const int* __restrict__ starts, const int* __restrict__ lengths,
-                                              int B, int M, int H, unsigned* __restrict__ err) {
+                                              int B, int M, int H, int past, unsigned* __restrict__ err) {
   Pg8At at;
   if (!pg8_task(at, M, H)) return;
   pg8_place(at, pages, shift, table, N, starts, lengths, B, M, H);
   vh_u32x4 kw = {0u, 0u, 0u, 0u}, vw = kw;
   unsigned sk = PG8_LOW, sv = PG8_LOW;
   if (at.there) {
-    kw = ld16(kp + at.row * PG_E + at.e);
-    vw = ld16(vp + at.row * PG_E + at.e);
+    const vh_u32x4 *ka = (const vh_u32x4*)(kp + at.row * PG_E + at.e), *va = (const vh_u32x4*)(vp + at.row * PG_E + at.e);
+    if (past) {                                                    // (the asm keeps this a branch of its own)
+      asm volatile("" ::: "memory");
+      kw = __builtin_nontemporal_load(ka);
+      vw = __builtin_nontemporal_load(va);
+      asm volatile("" ::: "memory");
+    } else {
+      kw = *ka;
+      vw = *va;
+    }
     sk = ks[at.row * (PG_E / 32) + at.e / 32];
     sv = vs[at.row * (PG_E / 32) + at.e / 32];
   }
   if (at.ours) {
-    pg8_put<T>(k + at.i * krow + at.h * khead + at.e, kw, pg_power(sk));
-    pg8_put<T>(v + at.i * vrow + at.h * vhead + at.e, vw, pg_power(sv));
+    pg8_put(k + at.i * krow + at.h * khead + at.e, kw, pg_power(sk));
+    pg8_put(v + at.i * vrow + at.h * vhead + at.e, vw, pg_power(sv));
   }
   if (at.bad) pg_raise(err, at.bad);
 }
@@ -207,9 +225,9 @@ __device__ __forceinline__ void pg8_read_body(T* __restrict__ k, T* __restrict__
   extern "C" __global__ __launch_bounds__(256) void name(                                                          \
       type* __restrict__ k, type* __restrict__ v, long krow, long khead, long vrow, long vhead, PG_POOL, int pages, \
       int shift, const int* __restrict__ table, int N, const int* __restrict__ starts,                             \
-      const int* __restrict__ lengths, int B, int M, int H, unsigned* __restrict__ err) {                          \
+      const int* __restrict__ lengths, int B, int M, int H, int past, unsigned* __restrict__ err) {                \
     pg8_read_body<type>(k, v, krow, khead, vrow, vhead, PG_POOL_ARGS, pages, shift, table, N, starts, lengths, B,  \
-                        M, H, err);                                                                                \
+                        M, H, past, err);                                                                          \
   }
 PG8_READ(pg_read16, unsigned short)
 PG8_READ(pg_read32, float)

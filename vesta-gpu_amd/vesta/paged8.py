@@ -33,7 +33,7 @@ from __future__ import annotations
 from pathlib import Path
 
 from .paged import BLOCK, KINDS, PAGED_SRC, SIGNATURES as SIGNATURES16, PagedCache, _collides, _overlap, kernels_of, loaded
-from .prefill import PRELUDE_SRC
+from .prefill import MEM_CACHE_BYTES, PRELUDE_SRC
 
 FORM_SRC = Path(__file__).resolve().parent / 'hip' / 'form8.h'
 PAGED8_SRC = Path(__file__).resolve().parent / 'hip' / 'paged8.hip'
@@ -45,12 +45,18 @@ LEAST = {('i8', 'f16'): 109, ('i8', 'bf16'): 7, ('e4m3', 'f16'): 112, ('e4m3', '
 # 128 99 / 104 / 109, 96 after up to 6000 148 / 149 / 152, 4 after 20,000 of width 64 59 / 54 / 55).
 PARTS = {64: 1536, 128: 1024}
 
+# Bytes read and written from which the pool is read past the memory-side cache (through it / past it: 28,800 rows of 25
+# heads of 64, 332 MB, 78 / 65 us; 12 heads into fp32, 265 MB, 58 / 54; 25 heads into fp32, 553 MB, 131 / 125; the same call
+# again and again, 8 heads of 128, 212 MB, 36 / 41).
+READ_PAST = MEM_CACHE_BYTES * 7 // 8
+
 _ATTENTION = ('pg_attn', 'pg_attn2', 'pg_attn8', 'pg_wide', 'pg_wide8')
 # the pools' two parameters are four here, with the powers'
 SIGNATURES = {name: SIGNATURES16[name] for name in ('pg_join', 'pg_wide_join', 'pg_take', 'pg_input')}
 SIGNATURES.update({name: SIGNATURES16[name][:5] + 'pp' + SIGNATURES16[name][5:] for name in _ATTENTION})
 SIGNATURES.update({name: 'ppllll' + 'pppp' + SIGNATURES16['pg_append16'][8:]
-                   for name in ('pg_append16', 'pg_append32', 'pg_read16', 'pg_read32')})
+                   for name in ('pg_append16', 'pg_append32')})
+SIGNATURES.update({name: SIGNATURES['pg_append16'][:-1] + 'ip' for name in ('pg_read16', 'pg_read32')})
 
 
 def paged8_source(width: int, kind: str, form: str) -> str:
@@ -135,10 +141,11 @@ class PagedCache8(PagedCache):
             return k, v
         kn = self._kind[self.dtype]
         grid = self._blocks(M)
+        past = 2 * M * self.heads * (size * E + E + E // SCALED) > READ_PAST
         stream, back = self._enter()
         try:
             (kn.pg_read32 if size == 4 else kn.pg_read16)(grid, BLOCK, stream, ks[0], vs[0], *ks[1:], *vs[1:], *at, *seqs,
-                                                          B, M, self.heads, self._err)
+                                                          B, M, self.heads, past, self._err)
         finally:
             self._leave(back)
         return k, v
