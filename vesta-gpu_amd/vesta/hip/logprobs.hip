@@ -15,6 +15,12 @@
 // is the number of listed ones before it. Elements are compared as a key of their
 // value's order and, in the same word, their id's from the lowest.
 //
+// What bounds it: many rows, memory (8192 rows of 50257 in fp32 267 us, 6.2 TB/s; with
+// five alternatives 279); few, a CU's share of the bandwidth (200 rows of 128001 in
+// bf16, a row a CU: 13.4 us, then 7 for 20 alternatives), the chain from launch to
+// loads to reductions (8 rows of 50257 7.0 us, with five 9.0), half of it fetching
+// instructions that run once.
+//
 // A NaN or +inf in a row makes its results NaN (its order: NaN is the largest); a
 // row of -inf alone allows nothing: all its log probabilities are -inf, its
 // entropy 0.

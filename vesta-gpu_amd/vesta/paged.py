@@ -34,6 +34,8 @@ sequence whose starts or length are impossible, so the cache's rows stay right.
 Nothing here has a backward pass: a tensor whose gradient is being recorded is
 refused (``ValueError``).
 
+``vesta.paged8.PagedCache8`` is the same with rows held in 8 bits.
+
 The decode cache of ``VestaGPT2`` [B, L, tmax, H, 64] (reference
 ``vesta/gpt2.py:31-33``) holds one position for all its rows; this one is for
 programs whose rows come and go.
@@ -679,7 +681,8 @@ class PagedCache:
 
 PLANS = 8                              # row counts whose launches a PagedPass keeps recorded
 SCORED = 512                           # rows whose logits it makes at a time where all rows' log probabilities are asked
-                                       # for: 103 MB of GPT-2's, which stay in the memory-side cache
+                                       # for: 103 MB of GPT-2's, which stay in the memory-side cache (24,576 rows, 256 /
+                                       # 512 / 1024 / 4096 at a time: 7.8 / 6.7 / 7.1 / 6.9 ms)
 
 
 class PagedPass(Prefill):
