@@ -231,7 +231,7 @@ def test_attend_long(blocks, dtype, query, form):  # noqa: F811
 def test_every_variant(monkeypatch, dtype, query, form, width):
     """The same batch through every kernel that a rule may pick: two, four or eight waves, positions dealt to parts or
     not, blocks of 16, 128 or 256 rows."""
-    from vesta import paged, paged8
+    from vesta import paged
     b = Batch8([1, 40, 1, 3], [700, 333, 2500, 3], 2, 2, width, 16, dtype, form, query)
     want, bound, *_ = b.want()
     base = dict(EIGHT_WAVES=0, TWO_WAVES=0, WIDE_FROM=WIDE, TWICE=(1 << 30, 0, 0), SPLIT={64: 1 << 30, 128: 1 << 30},
@@ -242,8 +242,6 @@ def test_every_variant(monkeypatch, dtype, query, form, width):
                dict(RUN=1), dict(WIDE_RUN=64, FEW_ROWS=0), dict(TWICE=(0, 0, 0), FEW_ROWS=0)):
         for name, value in {**base, **kw}.items():
             monkeypatch.setattr(paged, name, value)
-        if 'TARGET' in kw:
-            monkeypatch.setattr(paged8, 'PARTS', {64: kw['TARGET'], 128: kw['TARGET']})
         _close(b.attend(), want, bound)
         monkeypatch.undo()
 

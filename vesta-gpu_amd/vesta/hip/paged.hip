@@ -807,7 +807,7 @@ __device__ __forceinline__ void pg_attn_body(
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = p0 + 16 * i + 4 * q + j <= lim ? s[i][j] : -INFINITY;
     }
-    if (sc && live) {                                              // for pg_given, in powers of 2
+    if (!PG_FORM && sc && live) {                                  // for pg_given, in powers of 2
       float* to = sc + ((long)(sq.first + tok) * (H * G) + head) * pitch + p0 + 4 * q;
 #pragma unroll
       for (int i = 0; i < NG; ++i)
@@ -900,8 +900,16 @@ __device__ __forceinline__ void pg_attn_body(
     sum = fmaf(om[w][1][r], f[w], sum);
   }
   if (!live) return;
+#if PG_FORM
+  // (found again: three waves a SIMD have no registers to keep them over the loop)
+  int again = r;
+  asm volatile("" : "+v"(again));
+  const int x1 = min(x0 + again, R - 1), tok1 = pg_div(x1, G), head1 = h * G + x1 - tok1 * G;
+#else
+  const int tok1 = tok, head1 = head;
+#endif
   const bool whole = parts == 1;
-  pg_q* op = out + (sq.first + tok) * orow + head * ohead;
+  pg_q* op = out + (sq.first + tok1) * orow + head1 * ohead;
   float* wp = ws + (size_t)wk.at * PG_WS(16);
 #pragma unroll
   for (int d = wave; d < DT; d += W) {
@@ -922,16 +930,18 @@ __device__ __forceinline__ void pg_attn_body(
     if (!whole) {
       wp[r] = m;
       wp[16 + r] = sum;
-    } else if (lse) {
+    } else if (!PG_FORM && lse) {
       // log2 of the row's sum of 2^score: +inf for a row that sees nothing, so
       // that all its weights are 0
-      lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : pg_lse<PG_ATTN_BIAS>(m, sum);
+      lse[(size_t)(sq.first + tok1) * (H * G) + head1] = lim < 0 ? INFINITY : pg_lse<PG_ATTN_BIAS>(m, sum);
     }
   }
 }
 
+// Waves a SIMD: rows in 8 bits take few enough registers for three (two: eight
+// sequences after 30,000 of width 128 107 us, three: 98).
 #define PG_ATTN(name, waves) \
-  extern "C" __global__ __launch_bounds__(64 * waves, 2) void name( \
+  extern "C" __global__ __launch_bounds__(64 * waves, PG_FORM && PG_KIND != PG_F32 && waves < 8 ? 3 : 2) void name( \
       const pg_q* __restrict__ Q, long qrow, long qhead, PG_POOL, int pages, int shift, const int* __restrict__ table, int N, \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least, \
       int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse, \
@@ -1479,7 +1489,7 @@ __device__ __forceinline__ void pg_wide_body(
     if (!whole) {
       wp[32 * wave + r] = m2;
       wp[TILE + 32 * wave + r] = sum;
-    } else if (lse) {
+    } else if (!PG_FORM && lse) {
       lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : pg_lse<PG_WIDE_BIAS>(m2, sum);
     }
   }

@@ -41,10 +41,6 @@ FORMS = ('i8', 'e4m3')
 SCALED = 32                            # values of a power
 LEAST = {('i8', 'f16'): 109, ('i8', 'bf16'): 7, ('e4m3', 'f16'): 112, ('e4m3', 'bf16'): 10}    # bytes of the least powers
 
-# Parts of long positions, about: twice what the chip holds at once (1024 / 1536 / 2048, 2 sequences after 120,001 of width
-# 128 99 / 104 / 109, 96 after up to 6000 148 / 149 / 152, 4 after 20,000 of width 64 59 / 54 / 55).
-PARTS = {64: 1536, 128: 1024}
-
 # Bytes read and written from which the pool is read past the memory-side cache (through it / past it: 28,800 rows of 25
 # heads of 64, 332 MB, 78 / 65 us; 12 heads into fp32, 265 MB, 58 / 54; 25 heads into fp32, 553 MB, 131 / 125; the same call
 # again and again, 8 heads of 128, 212 MB, 36 / 41).
@@ -100,9 +96,6 @@ class PagedCache8(PagedCache):
         self.kscales, self.vscales = (torch.full(shape + (self.width // SCALED,), LEAST[self.form, self._dt],
                                                  dtype=torch.uint8, device=device) for _ in range(2))
         self._ready(self.keys, self.vals, self.kscales, self.vscales)
-
-    def _parts(self):
-        return PARTS[self.width]
 
     def _blocks(self, M):
         """Blocks whose waves take 1024 values of a head each, of 16 rows or 8."""
