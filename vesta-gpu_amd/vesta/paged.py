@@ -85,8 +85,8 @@ WIDE_FROM = {(64, False): (128, 64, 4096), (128, False): (64, 64, 1536), (64, Tr
 # 70.9; 192 after 3000 54.0 / 60.7, 5000 101 / 105; 512 after up to 900 31.5 / 36.1, up to 4000 142 / 125.
 SPLIT, SPLIT_MOST = {64: 2048, 128: 1024}, {64: 5120, 128: 4096}
 TARGET = 2048                 # parts in all, about (64 after up to 4000, 1024 / 1536 / 2048 / 4096: 132.2 / 127.4 / 125.5
-                              # / 131.1; 2 after 100003: 159.6 / 160.8 / 158.6 / 163.5; in 8 bits, 1024 / 1536 / 2048 /
-                              # 3072: 8 after 30,000 103 / 105 / 98 / 102, 2 after 120,001 106 / 100 / 101 / 104) ...
+                              # / 131.1; 2 after 100003: 159.6 / 160.8 / 158.6 / 163.5; in 8 bits, 1024 / 1536 / 2048:
+                              # 8 after 30,000 103 / 105 / 98, 2 after 120,001 106 / 100 / 101) ...
 PART_STEPS = 8                # ... each of at least so many steps: two a wave
 # The same of pg_wide, where it has fewer tiles than fill the chip twice (two blocks a CU are resident).
 WIDE_SPLIT, WIDE_TARGET, WIDE_PART_STEPS = 1024, 512, 8
