@@ -344,6 +344,56 @@ def test_bad_contents_raise_after(blocks):  # noqa: F811
                 assert {tuple(at) for at in changed.nonzero().tolist()} <= rows
 
 
+@pytest.mark.parametrize('form,dtype', [('i8', 'f16'), ('e4m3', 'bf16')])
+@pytest.mark.parametrize('heads,page', [(8, 16), (16, 1), (24, 64), (12, 8)])
+def test_heads_taken_together(form, dtype, heads, page):
+    """Rows of 128 whose heads a wave of append may take eight of: what it leaves is the held form of each row, in its
+    own place alone, from any strides; nothing of a sequence that cannot be."""
+    counts, lengths = [1, 5, 0, 17, 3, 1, 2], [1, 70, 33, 17, 2, 400, 65]
+    b = Batch8(counts, lengths, heads, 1, 128, page, dtype, form)
+    wide = torch.randn(sum(counts) + 1, 2 * heads + 1, 128, generator=b.gen, device='cuda').to(DT[dtype])
+    k, v = wide[:, :heads], wide[:, heads + 1:]
+    for starts, lost in ((b.starts, ()), (torch.cat((b.starts[:-1], _ints([900]))), (6,))):
+        want = [[_bytes(t).clone() for t in pool] for pool in b.pools]
+        i0 = 0
+        for i, (c, n) in enumerate(zip(counts, lengths)):
+            for j in range(c):
+                s = n - c + j
+                if s >= 0 and i not in lost:
+                    for (pool, powers), rows in zip(want, (k, v)):
+                        code, byte = held8.hold(rows[i0 + j], form, dtype)
+                        pool[0, b.table[i, s // page], :, s % page] = code
+                        powers[0, b.table[i, s // page], :, s % page] = byte
+            i0 += c
+        b.cache.append(k, v, b.table, starts, b.lengths)
+        for pool, w in zip(b.pools, want):
+            for t, x in zip(pool, w):
+                assert torch.equal(_bytes(t), x)
+        if lost:
+            with pytest.raises(RuntimeError, match='starts'):
+                b.cache.check()
+        wide.neg_()
+    b.cache.check()
+
+
+@pytest.mark.parametrize('form', FORMS)
+@pytest.mark.parametrize('width,new', [(64, 'f16'), (64, 'f32'), (128, 'f16'), (128, 'f32')])
+def test_read_past_the_cache(form, width, new, monkeypatch):
+    """Large reads load the pool another way: the same values."""
+    from vesta import paged8
+    b = Batch8([40, 1, 33], [300, 65, 33], 5, 1, width, 16, 'f16', form)
+    got = []
+    for most in (1 << 60, 0):
+        monkeypatch.setattr(paged8, 'READ_PAST', most)
+        out = torch.full((76, 11, width), 7.0, dtype=DT[new], device='cuda')
+        b.cache.read(out[:, :5], out[:, 6:], b.table, b.starts, b.lengths)
+        got.append(out)
+    assert torch.equal(*got) and (got[0][74:] == 7).all() and (got[0][:, 5] == 7).all()
+    first = torch.cat([b.rows(i, b.cache.keys)[:, -c:] for i, c in enumerate(b.counts)], 1).transpose(0, 1)
+    _same(got[0][:74, :5], first)
+    b.cache.check()
+
+
 def test_other_stream_and_graph():
     """Captured calls replay on new contents; two graphs and eager calls in between share nothing."""
     b = Batch8([1, 1, 1], [50, 700, 3], 2, 2, 64, 16, spare=2)

@@ -1,12 +1,12 @@
 // Rows into and out of a paged cache in 8 bits (hip/form8.h), after hip/paged.hip.
 //
-// A wave takes 1024 values of one head: 16 values a lane, of 16 rows of 64 or 8 of
-// 128, so that what it stores lies together (a head's rows of a page do), the
-// powers too: as eight values of all heads a lane, whose powers reach memory two
-// or four bytes at a time, 12,900 rows of 8 heads of 128 took 22.8 us to append.
-// Bound by memory: these rows 16.3 us (80 MB, 4.9 TB/s), 28,800 rows of 25 heads of
-// 64 read back in 65.5 us (332 MB, 5.05 TB/s); eight rows 3.6 us, a launch and the
-// loads that wait for one another.
+// A wave takes rows of one head, so that what it reads or stores of the pool lies
+// together (a head's rows of a page do), the powers too: with rows of all heads,
+// whose powers reach memory two or four bytes at a time, 12,900 rows of 8 heads of
+// 128 took 22.8 us to append. Bound by memory: these rows 15.0 us (80 MB, 5.3 TB/s),
+// 28,800 rows of 25 heads of 64 appended in 67 and read back in 69.8 us (332 MB, 4.75
+// TB/s), of 8 heads of 128, whose pools the memory-side cache keeps, in 33.4 (6.4);
+// eight rows 3.6 us, a launch and the loads that wait for one another.
 
 // A lane's neighbour in its two.
 __device__ __forceinline__ float pg8_other(float v) {
@@ -75,47 +75,51 @@ struct Pg8Row {
   }
 };
 
-// A lane's row i of the call's, its head's piece of 16 values, and where the pool
-// has them.
-#define PG8_ROWS (1024 / PG_E)             // of a wave
+// A lane's row i of the call's, its head's piece of PER values, and where the pool
+// has them. A wave takes HEADS heads of ROWS rows.
+template <int PER, int HEADS>
 struct Pg8At {
+  static constexpr int LANES = PG_E / PER, ROWS = 64 / LANES / HEADS;
   int i, h, e;                             // e: the piece's first dim
   size_t row;                              // of the pool
   bool ours, there;                        // a sequence's row, or what may be one; one that the pool has a place for
   unsigned bad;
+  __device__ __forceinline__ bool task(int M, int H) {
+    const int lane = threadIdx.x & 63;
+    const unsigned groups = (unsigned)H / HEADS;                   // (HEADS 1, or H a multiple)
+    const unsigned w = __builtin_amdgcn_readfirstlane(blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6)), g = w / groups;
+    h = (int)(w - g * groups) * HEADS + lane / LANES % HEADS;
+    e = lane % LANES * PER;
+    i = (int)g * ROWS + lane / LANES / HEADS;
+    return (size_t)g * ROWS < (size_t)M;
+  }
+  __device__ __forceinline__ void place(int pages, int shift, const int* __restrict__ table, int N,
+                                        const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
+                                        int H) {
+    // the wave's first row's sequence; most often that of its last row too
+    const int first = __builtin_amdgcn_readfirstlane(i);
+    int b = pg_owner(starts, B, first);
+    if (ROWS > 1 && b + 1 < B && starts[b + 1] < first + ROWS) b = pg_owner(starts, B, i);
+    const PgSeq s = pg_seq(starts, lengths, b, M, N << shift);
+    const int j = i - s.first, pos = s.len - s.count + j;
+    ours = i < M && (s.bad != 0 || (j >= 0 && j < s.count));
+    bad = i < M ? s.bad : 0u;
+    there = ours && s.bad == 0 && pos >= 0;
+    row = 0;
+    if (!there) return;
+    const int page = table[(size_t)b * N + (pos >> shift)];
+    there = (unsigned)page < (unsigned)pages;
+    if (!there) bad |= PG_ERR_PAGE;
+    row = (((size_t)(there ? page : 0) * H + h) << shift) + (pos & ((1 << shift) - 1));
+  }
 };
-__device__ __forceinline__ bool pg8_task(Pg8At& o, int M, int H) {
-  const int lane = threadIdx.x & 63;
-  const unsigned w = __builtin_amdgcn_readfirstlane(blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6)), g = w / (unsigned)H;
-  o.h = (int)(w - g * (unsigned)H);
-  o.e = lane % (PG_E / 16) * 16;
-  if ((size_t)g * PG8_ROWS >= (size_t)M) return false;
-  o.i = (int)g * PG8_ROWS + lane / (PG_E / 16);
-  return true;
-}
-__device__ __forceinline__ void pg8_place(Pg8At& o, int pages, int shift, const int* __restrict__ table, int N,
-                                          const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M,
-                                          int H) {
-  // the wave's first row's sequence; most often that of its last row too
-  const int first = __builtin_amdgcn_readfirstlane(o.i);
-  int b = pg_owner(starts, B, first);
-  if (b + 1 < B && starts[b + 1] < first + PG8_ROWS) b = pg_owner(starts, B, o.i);
-  const PgSeq s = pg_seq(starts, lengths, b, M, N << shift);
-  const int j = o.i - s.first, pos = s.len - s.count + j;
-  o.ours = o.i < M && (s.bad != 0 || (j >= 0 && j < s.count));
-  o.bad = o.i < M ? s.bad : 0u;
-  o.there = o.ours && s.bad == 0 && pos >= 0;
-  o.row = 0;
-  if (!o.there) return;
-  const int page = table[(size_t)b * N + (pos >> shift)];
-  o.there = (unsigned)page < (unsigned)pages;
-  if (!o.there) o.bad |= PG_ERR_PAGE;
-  o.row = (((size_t)(o.there ? page : 0) * H + o.h) << shift) + (pos & ((1 << shift) - 1));
-}
 
 // ---------------------------------------------------------------- append
-// As the 16-bit cache's: nothing is stored for a sequence that cannot be.
-template <typename T>
+// As the 16-bit cache's: nothing is stored for a sequence that cannot be. 16 values
+// a lane, 1024 a wave, of 16 rows of 64 or 8 of 128 (8 values a lane, whose loads
+// leave nothing out: 75 us for the 67 above), or of HEADS heads of one row of 128.
+// Stores go past the caches (19.2 -> 17.3 us before the heads of a row were together).
+template <typename T, int HEADS>
 __device__ __forceinline__ void pg8_append_body(const T* __restrict__ k, const T* __restrict__ v, long krow, long khead,
                                                 long vrow, long vhead, unsigned char* __restrict__ kp,
                                                 unsigned char* __restrict__ vp, unsigned char* __restrict__ ks,
@@ -123,14 +127,14 @@ __device__ __forceinline__ void pg8_append_body(const T* __restrict__ k, const T
                                                 const int* __restrict__ table, int N, const int* __restrict__ starts,
                                                 const int* __restrict__ lengths, int B, int M, int H,
                                                 unsigned* __restrict__ err) {
-  Pg8At at;
-  if (!pg8_task(at, M, H)) return;
+  Pg8At<16, HEADS> at;
+  if (!at.task(M, H)) return;
   const long i = min(at.i, M - 1);
   Pg8Row<T> kw, vw;
   kw.get(k + i * krow + at.h * khead + at.e);
   vw.get(v + i * vrow + at.h * vhead + at.e);
   __builtin_amdgcn_sched_barrier(0);                               // in flight while the place is looked up
-  pg8_place(at, pages, shift, table, N, starts, lengths, B, M, H);
+  at.place(pages, shift, table, N, starts, lengths, B, M, H);
   float x[16];
   unsigned sk, sv;
   kw.open(x);
@@ -147,65 +151,67 @@ __device__ __forceinline__ void pg8_append_body(const T* __restrict__ k, const T
   }
   if (at.bad) pg_raise(err, at.bad);
 }
-#define PG8_APPEND(name, type)                                                                                     \
+#define PG8_APPEND(name, type, heads)                                                                              \
   extern "C" __global__ __launch_bounds__(256) void name(                                                          \
       const type* __restrict__ k, const type* __restrict__ v, long krow, long khead, long vrow, long vhead,        \
       unsigned char* __restrict__ kp, unsigned char* __restrict__ vp, unsigned char* __restrict__ ks,              \
       unsigned char* __restrict__ vs, int pages, int shift, const int* __restrict__ table, int N,                  \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H,                        \
       unsigned* __restrict__ err) {                                                                                \
-    pg8_append_body<type>(k, v, krow, khead, vrow, vhead, kp, vp, ks, vs, pages, shift, table, N, starts, lengths, \
-                          B, M, H, err);                                                                           \
+    pg8_append_body<type, heads>(k, v, krow, khead, vrow, vhead, kp, vp, ks, vs, pages, shift, table, N, starts,  \
+                                 lengths, B, M, H, err);                                                           \
   }
-PG8_APPEND(pg_append16, unsigned short)
-PG8_APPEND(pg_append32, float)
+PG8_APPEND(pg_append16, unsigned short, 1)
+PG8_APPEND(pg_append32, float, 1)
+#if PG_E == 128
+PG8_APPEND(pg_append16x8, unsigned short, 8)
+#endif
 
 // ---------------------------------------------------------------- read
 // The rows of the new tokens' positions back as values. A row of a token at a
 // negative position, or of a sequence that cannot be, becomes 0; rows that are
 // no sequence's stay.
-// A lane's 16 values. In 16 bits its stores of 16 bytes leave as many out: the
-// caches put the lines together (28,800 rows of 25 heads of 64 76.4 us; past the
-// caches 95.6, and 100 in pieces that two lanes have exchanged such that a store
-// leaves nothing out).
-__device__ __forceinline__ void pg8_put(unsigned short* p, vh_u32x4 w, pg_factor f) {
+//
+// A lane stores 16 bytes beside its neighbours', whole lines, past the caches, so
+// that the pool may stay in them; as 16 values a lane, two or four stores that leave
+// bytes out, they need the caches to put lines together, and push it out (28,800
+// rows, 25 heads of 64: 72.5 -> 69.8 us; 12 heads 39.3 -> 28.2, in fp32 62.5 -> 42.2; 8
+// heads of 128 50 -> 33.4; past the caches with what is left out 106).
+
+// A lane's elements, which are 16 bytes of values.
+template <typename T>
+struct Pg8Piece {
+  typedef vh_u32x2 held;
+  static __device__ __forceinline__ vh_u32x4 open(held w, pg_factor f) { return pg_open(w[0], w[1], f); }
+};
+template <>
+struct Pg8Piece<float> {
+  typedef unsigned held;
+  static __device__ __forceinline__ vh_u32x4 open(held w, pg_factor f) {
+    const vh_u32x2 v = pg_open4(w, f);
+    vh_u32x4 o;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) *(vh_u32x4*)(p + 8 * j) = pg_open(w[2 * j], w[2 * j + 1], f);
-}
-// In 32 bits a store would leave out 48 bytes of 64: four lanes, whose 64 values
-// are one row's, store the first's together, then the second's.
-template <int FROM>
-__device__ __forceinline__ void pg8_put4(float* p, vh_u32x4 w, pg_factor f) {
-  constexpr int CTRL = FROM * 0x55;                                // of each four lanes the FROM-th
-  const int q = threadIdx.x & 3;
-  unsigned t[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) t[j] = (unsigned)__builtin_amdgcn_mov_dpp((int)w[j], CTRL, 0xF, 0xF, true);
-  const pg_factor g =
-      __builtin_bit_cast(pg_factor, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, f), CTRL, 0xF, 0xF, true));
-  const vh_u32x2 v = pg_open4(q & 2 ? (q & 1 ? t[3] : t[2]) : (q & 1 ? t[1] : t[0]), g);
-  *(vh_f32x4*)(p + 16 * (FROM - q) + 4 * q) =
-      vh_f32x4{pg_to_f((unsigned short)(v[0] & 0xffffu)), pg_to_f((unsigned short)(v[0] >> 16)),
-               pg_to_f((unsigned short)(v[1] & 0xffffu)), pg_to_f((unsigned short)(v[1] >> 16))};
-}
-__device__ __forceinline__ void pg8_put(float* p, vh_u32x4 w, pg_factor f) {
-  pg8_put4<0>(p, w, f);
-  pg8_put4<1>(p, w, f);
-  pg8_put4<2>(p, w, f);
-  pg8_put4<3>(p, w, f);
-}
+    for (int j = 0; j < 2; ++j) {
+      o[2 * j] = __builtin_bit_cast(unsigned, pg_to_f((unsigned short)(v[j] & 0xffffu)));
+      o[2 * j + 1] = __builtin_bit_cast(unsigned, pg_to_f((unsigned short)(v[j] >> 16)));
+    }
+    return o;
+  }
+};
 template <typename T>
 __device__ __forceinline__ void pg8_read_body(T* __restrict__ k, T* __restrict__ v, long krow, long khead, long vrow,
                                               long vhead, PG_POOL, int pages, int shift, const int* __restrict__ table,
                                               int N, const int* __restrict__ starts, const int* __restrict__ lengths,
                                               int B, int M, int H, int past, unsigned* __restrict__ err) {
-  Pg8At at;
-  if (!pg8_task(at, M, H)) return;
-  pg8_place(at, pages, shift, table, N, starts, lengths, B, M, H);
-  vh_u32x4 kw = {0u, 0u, 0u, 0u}, vw = kw;
+  typedef Pg8Piece<T> P;
+  Pg8At<16 / (int)sizeof(T), 1> at;
+  if (!at.task(M, H)) return;
+  at.place(pages, shift, table, N, starts, lengths, B, M, H);
+  typename P::held kw = {}, vw = {};
   unsigned sk = PG8_LOW, sv = PG8_LOW;
   if (at.there) {
-    const vh_u32x4 *ka = (const vh_u32x4*)(kp + at.row * PG_E + at.e), *va = (const vh_u32x4*)(vp + at.row * PG_E + at.e);
+    const typename P::held *ka = (const typename P::held*)(kp + at.row * PG_E + at.e),
+                           *va = (const typename P::held*)(vp + at.row * PG_E + at.e);
     if (past) {                                                    // (the asm keeps this a branch of its own)
       asm volatile("" ::: "memory");
       kw = __builtin_nontemporal_load(ka);
@@ -219,8 +225,10 @@ __device__ __forceinline__ void pg8_read_body(T* __restrict__ k, T* __restrict__
     sv = vs[at.row * (PG_E / 32) + at.e / 32];
   }
   if (at.ours) {
-    pg8_put(k + at.i * krow + at.h * khead + at.e, kw, pg_power(sk));
-    pg8_put(v + at.i * vrow + at.h * vhead + at.e, vw, pg_power(sv));
+    const vh_u32x4 kx = P::open(kw, pg_power(sk)), vx = P::open(vw, pg_power(sv));
+    vh_u32x4 *ko = (vh_u32x4*)(k + at.i * krow + at.h * khead + at.e), *vo = (vh_u32x4*)(v + at.i * vrow + at.h * vhead + at.e);
+    __builtin_nontemporal_store(kx, ko);
+    __builtin_nontemporal_store(vx, vo);
   }
   if (at.bad) pg_raise(err, at.bad);
 }

@@ -393,12 +393,12 @@ class PagedCache:
             import torch
             torch.cuda.set_device(back)
 
-    def _blocks(self, M):
-        """Blocks that take M rows' eight values a thread."""
+    def _appending(self, kn, M, f32):
+        """The kernel that appends M rows and its blocks, of eight values a thread."""
         grid = -(-M * self.heads * (self.width // 8) // BLOCK)
         if grid >= 1 << 31:
             raise ValueError(f'k: {M} rows are too many for one call')
-        return grid
+        return kn.pg_append32 if f32 else kn.pg_append16, grid
 
     # ------------------------------------------------------------ operators
     def append(self, k, v, table, starts, lengths, layer=0):
@@ -413,9 +413,7 @@ class PagedCache:
         M = k.shape[0]
         if M == 0 or B == 0 or N == 0:
             return
-        kn = self._kind[self.dtype]
-        launch = kn.pg_append32 if k.dtype is self._f32 else kn.pg_append16
-        grid = self._blocks(M)
+        launch, grid = self._appending(self._kind[self.dtype], M, k.dtype is self._f32)
         stream, back = self._enter()
         try:
             launch(grid, BLOCK, stream, k_at, v_at, *ks, *vs, *at, *seqs, B, M, self.heads, self._err)

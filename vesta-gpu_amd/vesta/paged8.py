@@ -41,18 +41,24 @@ FORMS = ('i8', 'e4m3')
 SCALED = 32                            # values of a power
 LEAST = {('i8', 'f16'): 109, ('i8', 'bf16'): 7, ('e4m3', 'f16'): 112, ('e4m3', 'bf16'): 10}    # bytes of the least powers
 
-# Bytes read and written from which the pool is read past the memory-side cache (through it / past it: 28,800 rows of 25
-# heads of 64, 332 MB, 78 / 65 us; 12 heads into fp32, 265 MB, 58 / 54; 25 heads into fp32, 553 MB, 131 / 125; the same call
-# again and again, 8 heads of 128, 212 MB, 36 / 41).
-READ_PAST = MEM_CACHE_BYTES * 7 // 8
+# Bytes of elements from which a call reads the pool past the memory-side cache, which holds what later calls and layers
+# may read again (three pools in turn, through it / past it: 28,800 rows of 25 heads of 64, 92 MB each, 71.5 / 69.7 us; 8
+# heads of 128, 59 MB, 34.0 / 46.2; 12 heads of 64, 44 MB, 28.0 / 36.0).
+READ_PAST = MEM_CACHE_BYTES * 5 // 16
+# Heads of 128 whose 16-bit rows a wave of append takes together, one position's, where it has a multiple of them: its
+# place is found once, by scalar operations (12,900 rows of 8 heads, a head of eight rows / eight heads of one: 17.1 /
+# 15.5 us, 28,800: 44.4 / 41.3; in fp32 67.5 / 67.1).
+TOGETHER = 8
 
 _ATTENTION = ('pg_attn', 'pg_attn2', 'pg_attn8', 'pg_wide', 'pg_wide8')
 # the pools' two parameters are four here, with the powers'
 SIGNATURES = {name: SIGNATURES16[name] for name in ('pg_join', 'pg_wide_join', 'pg_take', 'pg_input')}
 SIGNATURES.update({name: SIGNATURES16[name][:5] + 'pp' + SIGNATURES16[name][5:] for name in _ATTENTION})
 SIGNATURES.update({name: 'ppllll' + 'pppp' + SIGNATURES16['pg_append16'][8:]
-                   for name in ('pg_append16', 'pg_append32')})
+                   for name in ('pg_append16', 'pg_append32', 'pg_append16x8')})
 SIGNATURES.update({name: SIGNATURES['pg_append16'][:-1] + 'ip' for name in ('pg_read16', 'pg_read32')})
+
+_OWN = {64: {'pg_read16', 'pg_read32'}, 128: {'pg_read16', 'pg_read32', 'pg_append16x8'}}      # beside kernels_of's
 
 
 def paged8_source(width: int, kind: str, form: str) -> str:
@@ -77,7 +83,7 @@ class PagedCache8(PagedCache):
     def _load(self, kind):
         return loaded(self.device.index, (self.width, kind, self.form),
                       lambda: paged8_source(self.width, kind, self.form),
-                      {name: SIGNATURES[name] for name in kernels_of(self.width, kind) | {'pg_read16', 'pg_read32'}
+                      {name: SIGNATURES[name] for name in kernels_of(self.width, kind) | _OWN[self.width]
                        if name in SIGNATURES})
 
     def _shape(self, pages, heads, width, layers, page, dtype):
@@ -97,12 +103,17 @@ class PagedCache8(PagedCache):
                                                  dtype=torch.uint8, device=device) for _ in range(2))
         self._ready(self.keys, self.vals, self.kscales, self.vscales)
 
-    def _blocks(self, M):
-        """Blocks whose waves take 1024 values of a head each, of 16 rows or 8."""
-        waves = -(-M * self.width // 1024) * self.heads
+    def _blocks(self, M, rows, heads):
+        """Blocks whose waves take so many of M rows of so many heads each."""
+        waves = -(-M // rows) * (self.heads // heads)
         if waves >= 1 << 26:                 # (a launch has fewer than 2^32 threads)
             raise ValueError(f'k: {M} rows are too many for one call')
         return -(-waves // (BLOCK // 64))
+
+    def _appending(self, kn, M, f32):
+        heads = TOGETHER if self.width == 128 and not f32 and self.heads % TOGETHER == 0 else 1
+        grid = self._blocks(M, 1024 // (self.width * heads), heads)
+        return kn.pg_append32 if f32 else kn.pg_append16 if heads == 1 else kn.pg_append16x8, grid
 
     def attend(self, q, table, starts, lengths, layer=0, scale=None, out=None, most=None):
         """As ``PagedCache.attend``, without weights: attention of the new
@@ -133,8 +144,8 @@ class PagedCache8(PagedCache):
         if M == 0 or B == 0:
             return k, v
         kn = self._kind[self.dtype]
-        grid = self._blocks(M)
-        past = 2 * M * self.heads * (size * E + E + E // SCALED) > READ_PAST
+        grid = self._blocks(M, 1024 // (E * size), 1)
+        past = 2 * M * self.heads * E > READ_PAST
         stream, back = self._enter()
         try:
             (kn.pg_read32 if size == 4 else kn.pg_read16)(grid, BLOCK, stream, ks[0], vs[0], *ks[1:], *vs[1:], *at, *seqs,
