@@ -377,20 +377,22 @@ def test_heads_taken_together(form, dtype, heads, page):
 
 
 @pytest.mark.parametrize('form', FORMS)
-@pytest.mark.parametrize('width,new', [(64, 'f16'), (64, 'f32'), (128, 'f16'), (128, 'f32')])
-def test_read_past_the_cache(form, width, new, monkeypatch):
-    """Large reads load the pool another way: the same values."""
-    from vesta import paged8
-    b = Batch8([40, 1, 33], [300, 65, 33], 5, 1, width, 16, 'f16', form)
-    got = []
-    for most in (1 << 60, 0):
-        monkeypatch.setattr(paged8, 'READ_PAST', most)
-        out = torch.full((76, 11, width), 7.0, dtype=DT[new], device='cuda')
-        b.cache.read(out[:, :5], out[:, 6:], b.table, b.starts, b.lengths)
-        got.append(out)
-    assert torch.equal(*got) and (got[0][74:] == 7).all() and (got[0][:, 5] == 7).all()
-    first = torch.cat([b.rows(i, b.cache.keys)[:, -c:] for i, c in enumerate(b.counts)], 1).transpose(0, 1)
-    _same(got[0][:74, :5], first)
+@pytest.mark.parametrize('dtype,query', KINDS)
+@pytest.mark.parametrize('width,group', [(64, 1), (128, 4)])
+def test_rows_loaded_past_the_cache(form, dtype, query, width, group, monkeypatch):
+    """The pools of a long decode are loaded another way: the same results."""
+    from vesta import paged, paged8
+    b = Batch8([1, 1, 2, 0, 1], [900, 1, 333, 70, 2500], 3, group, width, 16, dtype, form, query)
+    want, bound, *_ = b.want()
+    monkeypatch.setattr(paged, 'EIGHT_WAVES', 0)
+    for split in (1 << 30, 0):
+        monkeypatch.setattr(paged, 'SPLIT', {64: split, 128: split})
+        got = []
+        for most in (1 << 60, 0):
+            monkeypatch.setattr(paged8, 'ATTEND_PAST', most)
+            got.append(b.cache.attend(b.q, b.table, b.starts, b.lengths, most=2))
+        _close(got[0], want, bound)
+        assert torch.equal(*got)
     b.cache.check()
 
 

@@ -645,7 +645,14 @@ __device__ __forceinline__ void pg_store4(pg_q* p, const float* v) {
 #endif
 }
 
-template <int W>
+#if PG_FORM
+// 16 elements; PAST: past the caches.
+template <bool PAST>
+__device__ __forceinline__ vh_u32x4 pg_row16(const unsigned char* p) {
+  return PAST ? __builtin_nontemporal_load((const vh_u32x4*)p) : ld16(p);
+}
+#endif
+template <int W, bool PAST = false>
 __device__ __forceinline__ void pg_attn_body(
     const pg_q* __restrict__ Q, long qrow, long qhead, PG_POOL, int pages, int shift, const int* __restrict__ table, int N,
     const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least,
@@ -695,11 +702,11 @@ __device__ __forceinline__ void pg_attn_body(
     for (int i = 0; i < NG; ++i) {
       const unsigned char* p = kp + 16 * q + (size_t)(unsigned)__shfl((int)rw, 16 * i + r, 64) * PG_E;
 #pragma unroll
-      for (int k = 0; k < KS / 2; ++k) kr[i][k] = ld16(p + 64 * k);
+      for (int k = 0; k < KS / 2; ++k) kr[i][k] = pg_row16<PAST>(p + 64 * k);
     }
 #pragma unroll
     for (int n = 0; n < NV / 2; ++n)
-      vr[n] = ld16(vp + 16 * (lane % VL) + (size_t)(unsigned)__shfl((int)rw, n * VR + lane / VL, 64) * PG_E);
+      vr[n] = pg_row16<PAST>(vp + 16 * (lane % VL) + (size_t)(unsigned)__shfl((int)rw, n * VR + lane / VL, 64) * PG_E);
   };
 #else
   const size_t rowlen = (size_t)H * PG_E;
@@ -940,18 +947,21 @@ __device__ __forceinline__ void pg_attn_body(
 
 // Waves a SIMD: rows in 8 bits take few enough registers for three (two: eight
 // sequences after 30,000 of width 128 107 us, three: 98).
-#define PG_ATTN(name, waves) \
+#define PG_ATTN(name, waves, ...) \
   extern "C" __global__ __launch_bounds__(64 * waves, PG_FORM && PG_KIND != PG_F32 && waves < 8 ? 3 : 2) void name( \
       const pg_q* __restrict__ Q, long qrow, long qhead, PG_POOL, int pages, int shift, const int* __restrict__ table, int N, \
       const int* __restrict__ starts, const int* __restrict__ lengths, int B, int M, int H, int G, int target, int least, \
       int run, int limit, int most, float scale2, pg_q* __restrict__ out, long orow, long ohead, float* __restrict__ lse, \
       float* __restrict__ ws, float* __restrict__ sc, long pitch, unsigned* __restrict__ err) { \
-    pg_attn_body<waves>(Q, qrow, qhead, PG_POOL_ARGS, pages, shift, table, N, starts, lengths, B, M, H, \
+    pg_attn_body<waves, ##__VA_ARGS__>(Q, qrow, qhead, PG_POOL_ARGS, pages, shift, table, N, starts, lengths, B, M, H, \
                         G, target, least, run, limit, most, scale2, out, orow, ohead, lse, ws, sc, pitch, err); \
   }
 PG_ATTN(pg_attn2, 2)
 PG_ATTN(pg_attn, 4)
 PG_ATTN(pg_attn8, 8)
+#if PG_FORM
+PG_ATTN(pg_attn_past, 4, true)
+#endif
 
 // Waits for loads whose registers a loop reads: left to the first use inside it,
 // the wait is for all loads issued since as well, each time round (pg_wide, six
@@ -1489,7 +1499,7 @@ __device__ __forceinline__ void pg_wide_body(
     if (!whole) {
       wp[32 * wave + r] = m2;
       wp[TILE + 32 * wave + r] = sum;
-    } else if (!PG_FORM && lse) {
+    } else if (lse) {
       lse[(size_t)(sq.first + tok) * (H * G) + head] = lim < 0 ? INFINITY : pg_lse<PG_WIDE_BIAS>(m2, sum);
     }
   }

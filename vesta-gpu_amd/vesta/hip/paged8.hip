@@ -202,7 +202,7 @@ template <typename T>
 __device__ __forceinline__ void pg8_read_body(T* __restrict__ k, T* __restrict__ v, long krow, long khead, long vrow,
                                               long vhead, PG_POOL, int pages, int shift, const int* __restrict__ table,
                                               int N, const int* __restrict__ starts, const int* __restrict__ lengths,
-                                              int B, int M, int H, int past, unsigned* __restrict__ err) {
+                                              int B, int M, int H, unsigned* __restrict__ err) {
   typedef Pg8Piece<T> P;
   Pg8At<16 / (int)sizeof(T), 1> at;
   if (!at.task(M, H)) return;
@@ -210,17 +210,8 @@ __device__ __forceinline__ void pg8_read_body(T* __restrict__ k, T* __restrict__
   typename P::held kw = {}, vw = {};
   unsigned sk = PG8_LOW, sv = PG8_LOW;
   if (at.there) {
-    const typename P::held *ka = (const typename P::held*)(kp + at.row * PG_E + at.e),
-                           *va = (const typename P::held*)(vp + at.row * PG_E + at.e);
-    if (past) {                                                    // (the asm keeps this a branch of its own)
-      asm volatile("" ::: "memory");
-      kw = __builtin_nontemporal_load(ka);
-      vw = __builtin_nontemporal_load(va);
-      asm volatile("" ::: "memory");
-    } else {
-      kw = *ka;
-      vw = *va;
-    }
+    kw = *(const typename P::held*)(kp + at.row * PG_E + at.e);
+    vw = *(const typename P::held*)(vp + at.row * PG_E + at.e);
     sk = ks[at.row * (PG_E / 32) + at.e / 32];
     sv = vs[at.row * (PG_E / 32) + at.e / 32];
   }
@@ -236,9 +227,9 @@ __device__ __forceinline__ void pg8_read_body(T* __restrict__ k, T* __restrict__
   extern "C" __global__ __launch_bounds__(256) void name(                                                          \
       type* __restrict__ k, type* __restrict__ v, long krow, long khead, long vrow, long vhead, PG_POOL, int pages, \
       int shift, const int* __restrict__ table, int N, const int* __restrict__ starts,                             \
-      const int* __restrict__ lengths, int B, int M, int H, int past, unsigned* __restrict__ err) {                \
+      const int* __restrict__ lengths, int B, int M, int H, unsigned* __restrict__ err) {                          \
     pg8_read_body<type>(k, v, krow, khead, vrow, vhead, PG_POOL_ARGS, pages, shift, table, N, starts, lengths, B,  \
-                        M, H, past, err);                                                                          \
+                        M, H, err);                                                                                \
   }
 PG8_READ(pg_read16, unsigned short)
 PG8_READ(pg_read32, float)

@@ -32,7 +32,7 @@ from __future__ import annotations
 
 from pathlib import Path
 
-from .paged import BLOCK, KINDS, PAGED_SRC, SIGNATURES as SIGNATURES16, PagedCache, _collides, _overlap, kernels_of, loaded
+from .paged import BLOCK, KINDS, PAGED_SRC, ROWS, SIGNATURES as SIGNATURES16, PagedCache, _collides, _overlap, kernels_of, loaded
 from .prefill import MEM_CACHE_BYTES, PRELUDE_SRC
 
 FORM_SRC = Path(__file__).resolve().parent / 'hip' / 'form8.h'
@@ -41,10 +41,10 @@ FORMS = ('i8', 'e4m3')
 SCALED = 32                            # values of a power
 LEAST = {('i8', 'f16'): 109, ('i8', 'bf16'): 7, ('e4m3', 'f16'): 112, ('e4m3', 'bf16'): 10}    # bytes of the least powers
 
-# Bytes of elements from which a call reads the pool past the memory-side cache, which holds what later calls and layers
-# may read again (three pools in turn, through it / past it: 28,800 rows of 25 heads of 64, 92 MB each, 71.5 / 69.7 us; 8
-# heads of 128, 59 MB, 34.0 / 46.2; 12 heads of 64, 44 MB, 28.0 / 36.0).
-READ_PAST = MEM_CACHE_BYTES * 5 // 16
+# Bytes of elements in all layers' pools that a token's pass may read from which pg_attn loads them past the memory-side
+# cache, which cannot keep them until the next token's (through it / past it, 8 heads of 128: two of 209 MB 54.1 / 52.2 us,
+# one of 426 100.4 / 95.5; what fits is better kept: one of 209 45.1 / 52.0, of 304 63.1 / 67.5, of 333 75.2 / 75.7).
+ATTEND_PAST = MEM_CACHE_BYTES * 5 // 4
 # Heads of 128 whose 16-bit rows a wave of append takes together, one position's, where it has a multiple of them: its
 # place is found once, by scalar operations (12,900 rows of 8 heads, a head of eight rows / eight heads of one: 17.1 /
 # 15.5 us, 28,800: 44.4 / 41.3; in fp32 67.5 / 67.1).
@@ -54,11 +54,11 @@ _ATTENTION = ('pg_attn', 'pg_attn2', 'pg_attn8', 'pg_wide', 'pg_wide8')
 # the pools' two parameters are four here, with the powers'
 SIGNATURES = {name: SIGNATURES16[name] for name in ('pg_join', 'pg_wide_join', 'pg_take', 'pg_input')}
 SIGNATURES.update({name: SIGNATURES16[name][:5] + 'pp' + SIGNATURES16[name][5:] for name in _ATTENTION})
+SIGNATURES['pg_attn_past'] = SIGNATURES['pg_attn']
 SIGNATURES.update({name: 'ppllll' + 'pppp' + SIGNATURES16['pg_append16'][8:]
-                   for name in ('pg_append16', 'pg_append32', 'pg_append16x8')})
-SIGNATURES.update({name: SIGNATURES['pg_append16'][:-1] + 'ip' for name in ('pg_read16', 'pg_read32')})
+                   for name in ('pg_append16', 'pg_append32', 'pg_append16x8', 'pg_read16', 'pg_read32')})
 
-_OWN = {64: {'pg_read16', 'pg_read32'}, 128: {'pg_read16', 'pg_read32', 'pg_append16x8'}}      # beside kernels_of's
+_OWN = {'pg_read16', 'pg_read32', 'pg_attn_past'}              # beside kernels_of's
 
 
 def paged8_source(width: int, kind: str, form: str) -> str:
@@ -83,7 +83,7 @@ class PagedCache8(PagedCache):
     def _load(self, kind):
         return loaded(self.device.index, (self.width, kind, self.form),
                       lambda: paged8_source(self.width, kind, self.form),
-                      {name: SIGNATURES[name] for name in kernels_of(self.width, kind) | _OWN[self.width]
+                      {name: SIGNATURES[name] for name in kernels_of(self.width, kind) | _OWN | ({'pg_append16x8'} if self.width == 128 else set())
                        if name in SIGNATURES})
 
     def _shape(self, pages, heads, width, layers, page, dtype):
@@ -115,6 +115,13 @@ class PagedCache8(PagedCache):
         grid = self._blocks(M, 1024 // (self.width * heads), heads)
         return kn.pg_append32 if f32 else kn.pg_append16 if heads == 1 else kn.pg_append16x8, grid
 
+    def _layout(self, kn, B, N, M, G, wide, most):
+        attn, *rest = super()._layout(kn, B, N, M, G, wide, most)
+        if attn is kn.pg_attn and most * G <= ROWS:              # (each row is read once)
+            if 2 * self.layers * min(B * N, self.pages) * self.page * self.heads * self.width > ATTEND_PAST:
+                attn = kn.pg_attn_past
+        return attn, *rest
+
     def attend(self, q, table, starts, lengths, layer=0, scale=None, out=None, most=None):
         """As ``PagedCache.attend``, without weights: attention of the new
         tokens' queries ``q`` [M, G * heads, width] over what ``layer`` holds
@@ -145,11 +152,10 @@ class PagedCache8(PagedCache):
             return k, v
         kn = self._kind[self.dtype]
         grid = self._blocks(M, 1024 // (E * size), 1)
-        past = 2 * M * self.heads * E > READ_PAST
         stream, back = self._enter()
         try:
             (kn.pg_read32 if size == 4 else kn.pg_read16)(grid, BLOCK, stream, ks[0], vs[0], *ks[1:], *vs[1:], *at, *seqs,
-                                                          B, M, self.heads, past, self._err)
+                                                          B, M, self.heads, self._err)
         finally:
             self._leave(back)
         return k, v
