@@ -11,8 +11,8 @@
 //
 // Attention over such rows is hip/paged.hip's: rows are loaded as they are held and
 // opened on their way to registers or LDS. Long decodes take what the cache's bytes
-// take, half as many (two sequences after 120,001 of 8 heads of 128, 485 MB, in 100
-// us, 4.8 TB/s, where 16 bits take 180). Chunks of many rows are bound as 16-bit
+// take, half as many (two sequences after 120,001 of 8 heads of 128, 485 MB, in 96
+// us, 5.1 TB/s, where 16 bits take 180). Chunks of many rows are bound as 16-bit
 // ones are, with the opening on top: 4096 tokens after 18,001 in bf16 16 bits 1237 us,
 // e4m3 1240 (two operations for four values), whole numbers 1350 (eleven); in fp16
 // 1290, 1272 and 1355 (seven).

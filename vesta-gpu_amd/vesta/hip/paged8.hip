@@ -3,10 +3,10 @@
 // A wave takes rows of one head, so that what it reads or stores of the pool lies
 // together (a head's rows of a page do), the powers too: with rows of all heads,
 // whose powers reach memory two or four bytes at a time, 12,900 rows of 8 heads of
-// 128 took 22.8 us to append. Bound by memory: these rows 15.0 us (80 MB, 5.3 TB/s),
-// 28,800 rows of 25 heads of 64 appended in 67 and read back in 69.8 us (332 MB, 4.75
-// TB/s), of 8 heads of 128, whose pools the memory-side cache keeps, in 33.4 (6.4);
-// eight rows 3.6 us, a launch and the loads that wait for one another.
+// 128 took 22.8 us to append. Bound by memory: these rows 14.4 us (80 MB, 5.5 TB/s),
+// 28,800 rows of 25 heads of 64 appended in 67 and read back in 73.6 us (332 MB, 4.5
+// TB/s; in 54.5 where the memory-side cache holds the pool), of 8 heads of 128 in 46.5
+// (33 from the cache); eight rows 3.6 us, a launch and the loads that wait for one another.
 
 // A lane's neighbour in its two.
 __device__ __forceinline__ float pg8_other(float v) {
@@ -175,8 +175,8 @@ PG8_APPEND(pg_append16x8, unsigned short, 8)
 // A lane stores 16 bytes beside its neighbours', whole lines, past the caches, so
 // that the pool may stay in them; as 16 values a lane, two or four stores that leave
 // bytes out, they need the caches to put lines together, and push it out (28,800
-// rows, 25 heads of 64: 72.5 -> 69.8 us; 12 heads 39.3 -> 28.2, in fp32 62.5 -> 42.2; 8
-// heads of 128 50 -> 33.4; past the caches with what is left out 106).
+// rows, three pools in turn: 25 heads of 64 73 -> 72 us, 12 heads 39.3 -> 28.2, in fp32 62.5
+// -> 42.2; 8 heads of 128 50 -> 33.4; past the caches with what is left out 106).
 
 // A lane's elements, which are 16 bytes of values.
 template <typename T>
