@@ -272,3 +272,27 @@ def test_streams_and_graphs(layout):
         torch.cuda.synchronize()
         for got in (eager, *(got for _, got in graphs)):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('kind', DT)
+@pytest.mark.parametrize('V', (1, 2, 5, 64, 1000, 4097, 50257))
+def test_nans_from_the_first_id(layout, kind, V):
+    """NaNs of either sign come first, above +inf, by the lowest id: at id 0, every third, the whole row."""
+    from vesta.logprobs import logprobs
+    x = torch.randn(7, V, generator=_gen(V, 5), device='cuda').to(DT[kind])
+    x[0, 0] = math.nan
+    x[1] = math.nan
+    x[2, ::3] = math.nan
+    x[3, 0] = math.inf
+    x[3, V - 1] = math.nan
+    x[4] = math.inf
+    bits = x[5].view(torch.int32 if kind == 'f32' else torch.int16)
+    bits.fill_(-1)                                         # the NaN of all ones
+    given = torch.zeros(7, dtype=torch.int64, device='cuda')
+    rank = torch.where(x.isnan(), 2.0, torch.where(x == math.inf, 1.0, torch.atan(x.double()) / 2))
+    for top in sorted({1, min(V, 3), min(V, 64)}):
+        got = logprobs(x, given, top=top)
+        assert torch.equal(got.ids.long(), torch.sort(rank, dim=1, descending=True, stable=True).indices[:, :top])
+        for t in (got.given, got.entropy, got.top):
+            assert t[:6].isnan().all() and t[6].isfinite().all()
+        _check(x[6:], given[6:], top)

@@ -65,10 +65,10 @@ __device__ __forceinline__ void lp_unpack(vh_u32x4 w, float* v) {
 #endif
 }
 
-// An element's key, above 0; a value back from it.
+// An element's key, above 0 and below ~0 (a NaN of id 0 has a bit to spare); a value back from it.
 __device__ __forceinline__ unsigned lp_word(float v) {
   const unsigned b = __builtin_bit_cast(unsigned, v + 0.0f);       // (-0 is 0)
-  return v != v ? 0xffffffffu : b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+  return v != v ? 0xfffffffeu : b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ lp_key lp_key_of(float v, int id) { return (lp_key)lp_word(v) << 32 | (unsigned)~id; }
 __device__ __forceinline__ float lp_value(lp_key k) {
