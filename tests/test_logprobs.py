@@ -56,3 +56,15 @@ def test_layout(M, V, size, top):
         assert threads == 256 and each <= 256 * int(name[7:]) * (16 // size) and V >= 16 // size and each % (16 // size) == 0
     else:
         assert name == f'lp_rows{threads}'
+
+
+def test_tangents_refused():
+    """Forward-mode derivatives are not made either, and not dropped without a word; outside a level nothing has one."""
+    import torch.autograd.forward_ad as fwd
+    x = torch.zeros(3, 8)
+    with fwd.dual_level():
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad(), pytest.raises(ValueError, match='logits'):
+                lp.logprobs(_on(fwd.make_dual(x, torch.ones_like(x))))
+        with pytest.raises(ValueError, match='top'):       # (no tangent: on to the next check)
+            lp.logprobs(_on(x), top=9)

@@ -18,8 +18,8 @@ first one of its type of logits). Sums are fp32.
 A banned token (-inf) has the log probability -inf; a row that bans all has -inf
 throughout and the entropy 0. A NaN or +inf in a row makes its results NaN (ids
 are of its order then, NaN the largest). A given id outside the vocabulary has
-the log probability NaN. There is no backward pass: logits whose gradient is
-being recorded are refused.
+the log probability NaN. There is no backward pass, no forward-mode one either:
+logits whose gradient is being recorded, or that have a tangent, are refused.
 
 The reference's programs end in the largest logit's id (reference
 ``vesta/programs/gpt2.vst:78-82``).
@@ -127,6 +127,9 @@ def logprobs(logits, given=None, top=0):
         raise TypeError('logits: need a device tensor of float32, float16 or bfloat16')
     if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError('logits: no gradient is made of them; detach them, or call under torch.no_grad()')
+    forward = torch.autograd.forward_ad
+    if forward._current_level >= 0 and forward.unpack_dual(logits).tangent is not None:      # (the first: 0.3 us less)
+        raise ValueError('logits: no tangent is made of them; detach them')
     shape = logits.shape
     if len(shape) != 2 or not 1 <= shape[1] < 1 << 30:
         raise ValueError(f'logits: shape {tuple(shape)}, need rows of 1 to 2^30 logits')
