@@ -464,3 +464,26 @@ def test_a_lost_plane_shows():
     _, _, _, w, rel = pp.answer(x, 512.0)
     less = torch.exp2(-(512.0 - pp.cut(512.0 - x, 2))) / (1 + torch.exp2(-x))
     assert ((less - w).abs() > 1.5 * rel * w).all()
+
+
+def test_tangents_are_refused():
+    """Nothing here has a forward-mode derivative either: a tensor with a tangent is refused, in whatever mode of
+    recording; one without is taken inside a level too."""
+    import torch.autograd.forward_ad as forward
+    c = _Dry(8, 3)
+    table, starts, lengths = _batch()
+    q, w, to = _rows(5, 3), torch.zeros(2, 3, 192), torch.ones(2, 1, dtype=torch.int32)
+    with forward.dual_level():
+        d, dw = (forward.make_dual(t, torch.ones_like(t)) for t in (q, w))
+        for call in (lambda: c.append(d, q, table, starts, lengths), lambda: c.append(q, d, table, starts, lengths),
+                     lambda: c.attend(d, table, starts, lengths), lambda: c.attend(q, table, starts, lengths, out=d),
+                     lambda: c.attend(q, table, starts, lengths, weight=dw),
+                     lambda: c.attend(q, table, starts, lengths, weight=w, weight_out=dw),
+                     lambda: c.evict(dw[None], table, lengths, 5, to)):
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad(), pytest.raises(ValueError, match='tangent'):
+                    call()
+        assert not c.log
+        c.attend(d.detach(), table, starts, lengths)
+        c.append(q, q, table, starts, lengths)
+        assert c.log

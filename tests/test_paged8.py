@@ -176,3 +176,22 @@ def test_definition(form):
     if form == 'e4m3':                                   # torch's rounding of the scaled values
         want = (y.double() / held8.power2(byte.long() - 127)).float().to(torch.float8_e4m3fn).view(torch.uint8)
         assert torch.equal(code, want)
+
+
+def test_tangents_refused():
+    """Tensors with a forward-mode tangent are refused as ones whose gradient is recorded are."""
+    import torch.autograd.forward_ad as fwd
+    c = _Dry(8, 3)
+    table, starts, lengths = _batch()
+    k = _rows(5, 3)
+    with fwd.dual_level():
+        d = fwd.make_dual(k, torch.ones_like(k))
+        for call in (lambda: c.append(d, k, table, starts, lengths), lambda: c.append(k, d, table, starts, lengths),
+                     lambda: c.read(k, d, table, starts, lengths), lambda: c.attend(d, table, starts, lengths),
+                     lambda: c.attend(k, table, starts, lengths, out=d)):
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad(), pytest.raises(ValueError, match='tangent'):
+                    call()
+        assert not c.log
+        c.append(k, k, table, starts, lengths)
+        assert len(c.log) == 1

@@ -31,8 +31,8 @@ and ``lengths`` is checked on the device, where an impossible value is replaced
 by a possible one and raises an error word that ``check()`` reads: results, a
 weight updated in place among them, are then invalid. Nothing is appended for a
 sequence whose starts or length are impossible, so the cache's rows stay right.
-Nothing here has a backward pass: a tensor whose gradient is being recorded is
-refused (``ValueError``).
+Nothing here has a backward pass: a tensor whose gradient is being recorded, or
+that has a forward-mode tangent, is refused (``ValueError``).
 
 ``vesta.paged8.PagedCache8`` is the same with rows held in 8 bits.
 
@@ -315,7 +315,7 @@ class PagedCache:
         self._pools = [tuple(p[n].data_ptr() for p in pools) for n in range(self.layers)]      # each layer's
         self._index = self.keys.get_device()
         self._i32, self._f32, self._empty = torch.int32, torch.float32, torch.empty
-        self._recording = torch.is_grad_enabled
+        self._recording, self._forward = torch.is_grad_enabled, torch.autograd.forward_ad
         self._new = self.dtype, self._f32                          # types of new rows, and of queries
         self._queries = self._new if self._dt == 'f16' else (self.dtype,)
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -362,6 +362,8 @@ class PagedCache:
                              f'{tuple(like) if like is not None else ("rows", heads or "heads", self.width)}')
         if t.requires_grad and self._recording():
             self._no_gradient(name)
+        if self._forward._current_level >= 0 and self._forward.unpack_dual(t).tangent is not None:
+            raise ValueError(f'{name}: no tangent is made of it; detach it')
         row, head, one = t.stride()
         at = t.data_ptr()
         if (one != 1 or (row | head) & (3 if t.dtype is self._f32 else 7) or at & 15) and t.numel():
@@ -591,6 +593,8 @@ class PagedCache:
             raise TypeError(f'{name}: need a contiguous float32 tensor on {self.device}')
         if w.requires_grad and self._recording():
             self._no_gradient(name)
+        if self._forward._current_level >= 0 and self._forward.unpack_dual(w).tangent is not None:
+            raise ValueError(f'{name}: no tangent is made of it; detach it')
         if tuple(shape[:-1]) != lead or not least <= shape[-1] < 1 << 31:
             raise ValueError(f'{name}: shape {tuple(shape)}, need {lead} and {least} positions at least')
         return shape[-1]
