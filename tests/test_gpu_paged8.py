@@ -436,3 +436,20 @@ def test_other_stream_and_graph():
             assert all(torch.equal(x, y) for x, y in zip(got, want))
         b.lengths -= torch.tensor([1, 1, 0], dtype=torch.int32, device='cuda')
     b.cache.check()
+
+
+@pytest.mark.parametrize('form', FORMS)
+@pytest.mark.parametrize('dtype,new', [('f16', 'f16'), ('f16', 'f32'), ('bf16', 'bf16')])
+@pytest.mark.parametrize('width', (64, 128))
+def test_rows_behind_a_sequence_that_cannot_be(form, dtype, new, width):
+    """Rows behind the last sequence's stay as they are, whatever its length or first start says; its own become 0."""
+    b = Batch8([2, 3], [40, 20], 3, 1, width, 16, dtype, form)
+    for starts, lengths, text in ((b.starts, _ints([40, 1 << 30]), 'length'), (b.starts, _ints([40, -1]), 'length'),
+                                  (_ints([0, -2, 5]), b.lengths, 'starts')):
+        k, v = (torch.full((40, 3, width), 7.0, device='cuda', dtype=DT[new]) for _ in range(2))
+        b.cache.read(k, v, b.table, starts, lengths)
+        assert (k[5:] == 7).all() and (v[5:] == 7).all()
+        lost = slice(2, 5) if starts is b.starts else slice(0, 5)
+        assert not k[lost].any() and not v[lost].any()
+        with pytest.raises(RuntimeError, match=text):
+            b.cache.check()

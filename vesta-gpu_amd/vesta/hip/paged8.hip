@@ -102,7 +102,8 @@ struct Pg8At {
     if (ROWS > 1 && b + 1 < B && starts[b + 1] < first + ROWS) b = pg_owner(starts, B, i);
     const PgSeq s = pg_seq(starts, lengths, b, M, N << shift);
     const int j = i - s.first, pos = s.len - s.count + j;
-    ours = i < M && (s.bad != 0 || (j >= 0 && j < s.count));
+    // (starts that leave a sequence no row do not say which are behind it)
+    ours = i < M && ((j >= 0 && j < s.count) || (s.count == 0 && (s.bad & PG_ERR_STARTS)));
     bad = i < M ? s.bad : 0u;
     there = ours && s.bad == 0 && pos >= 0;
     row = 0;
