@@ -209,3 +209,25 @@ def test_refusals(hf):  # noqa: F811
         m.logprobs(top=V + 1)
     with pytest.raises(ValueError):
         m.logprobs(_ints([1, 2]))
+
+
+@pytest.mark.parametrize('scored', (None, 40))
+def test_given_of_many_rows(hf, alone, monkeypatch, scored):  # noqa: F811
+    """Given tokens of more rows than are scored at a time: the first text's and the last one's, whose rows are scored
+    last, against the model's own logits; one a row and two."""
+    from vesta import paged
+    from vesta.gpt2 import VestaGPT2
+    if scored:
+        monkeypatch.setattr(paged, 'SCORED', scored)
+    texts = [_prompt(60 + 3 * i, i) for i in range(9)]
+    M, last = sum(map(len, texts)), len(texts[-1])
+    assert M > paged.SCORED and (M % paged.SCORED or M > 2 * paged.SCORED)
+    given = _ints([[n, (7 * i + 3) % V] for i, n in enumerate(n for t in texts for n in t[1:] + [0])])
+    rows = {0: (slice(0, len(texts[0])), _each(alone, texts[0])), 8: (slice(M - last, M), _each(alone, texts[8]))}
+    m = VestaGPT2(hf, batch=1, tmax=32, engine='layered')
+    for ids in (given, given[:, 0].contiguous().long()):
+        _, _, got = Scorer(m, 9, pages=80).score(texts, ids, top=2)
+        for part, want in rows.values():
+            g = ids.view(M, -1)[part]
+            _check(type(got)(*(t[part].view(len(g), -1) if t is got.given else t[part] for t in got)), want, g, 2)
+    m.check()

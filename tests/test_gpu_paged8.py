@@ -453,3 +453,27 @@ def test_rows_behind_a_sequence_that_cannot_be(form, dtype, new, width):
         assert not k[lost].any() and not v[lost].any()
         with pytest.raises(RuntimeError, match=text):
             b.cache.check()
+
+
+@pytest.mark.parametrize('dtype,query', KINDS)
+def test_which_kernels_run(dtype, query, monkeypatch):
+    """Of a long decode on both sides of the rule, and of rows whose heads are taken together."""
+    from vesta import paged, paged8
+    call, names = paged._Launcher.__call__, []
+
+    def named(self, *a):
+        names.append(self.name)
+        return call(self, *a)
+
+    monkeypatch.setattr(paged._Launcher, '__call__', named)
+    b = Batch8([1, 1], [30000, 29000], 8, 1, 128, 64, dtype, 'i8', query)
+    size = 2 * min(b.table.numel(), b.cache.pages) * 64 * 8 * 128
+    for past, name in ((size, 'pg_attn'), (size - 1, 'pg_attn_past')):
+        monkeypatch.setattr(paged8, 'ATTEND_PAST', past)
+        b.cache.attend(b.q, b.table, b.starts, b.lengths, most=1)
+        assert names[0] == name, names
+        names.clear()
+    rows = b.q.float() if query == 'f32' else b.q
+    b.cache.append(rows, rows, b.table, b.starts, b.lengths)
+    assert names == ['pg_append32' if query == 'f32' else 'pg_append16x8']
+    b.cache.check()

@@ -195,3 +195,60 @@ def test_tangents_refused():
         assert not c.log
         c.append(k, k, table, starts, lengths)
         assert len(c.log) == 1
+
+
+class _Named(_Recorder):
+    """As on a device, where a kernel's launcher is the same object each time."""
+
+    def __getattr__(self, name):
+        launch = super().__getattr__(name)
+        setattr(self, name, launch)
+        return launch
+
+
+def _named(*a, **kw):
+    c = _Dry(*a, **kw)
+    c._kind = {dtype: _Named(c.log) for dtype in c._kind}
+    return c
+
+
+@pytest.mark.parametrize('heads', (3, 8, 12, 16))
+@pytest.mark.parametrize('width', (64, 128))
+@pytest.mark.parametrize('M', (1, 7, 64, 1001))
+def test_waves_of_append_and_read(heads, width, M):
+    """Eight heads of 128 in 16 bits are appended together, other rows a head at a time, and the waves are as many as
+    the kernels index."""
+    c = _named(40, heads, width=width)
+    table, starts, lengths = _batch(2, 20, M)
+    for dtype in (torch.float16, torch.float32):
+        k = _rows(M, heads, width, dtype)
+        c.append(k, k, table, starts, lengths)
+        together = width == 128 and heads % 8 == 0 and dtype == torch.float16
+        name, grid, block, _ = c.log[-1]
+        assert name == ('pg_append16x8' if together else 'pg_append16' if dtype == torch.float16 else 'pg_append32')
+        waves = M * heads // 8 if together else -(-M // (1024 // width)) * heads
+        assert block == 256 and 4 * grid >= waves > 4 * (grid - 1)
+        c.read(k, k.clone(), table, starts, lengths)
+        name, grid, block, _ = c.log[-1]
+        size = k.element_size()
+        waves = -(-M // (1024 // (width * size))) * heads
+        assert name == f'pg_read{8 * size}' and block == 256 and 4 * grid >= waves > 4 * (grid - 1)
+
+
+@pytest.mark.parametrize('layers,pages,N', [(1, 300, 100), (3, 300, 100), (1, 150, 100)])
+def test_rule_of_rows_past_the_cache(layers, pages, N, monkeypatch):
+    """Long decodes whose tables have room for more of all layers' rows than the rule says are loaded past the caches,
+    by any type of queries; a chunk whose rows are read again is not."""
+    c = _named(pages, 3, layers=layers)
+    table, starts, lengths = torch.zeros(2, N, dtype=torch.int32), _ints(0, 1, 2), _ints(1, 1)
+    size = 2 * layers * min(2 * N, pages) * 64 * 3 * 64
+    for dtype in (torch.float16, torch.float32):
+        q = _rows(2, 3, dtype=dtype)
+        for past, name in ((size, 'pg_attn'), (size - 1, 'pg_attn_past')):
+            monkeypatch.setattr(paged8, 'ATTEND_PAST', past)
+            c.log.clear()
+            c.attend(q, table, starts, lengths, most=1)
+            assert c.log[0][0] == name
+        c.log.clear()
+        c.attend(_rows(34, 3, dtype=dtype), table, _ints(0, 17, 34), lengths, most=17)
+        assert c.log[0][0] == 'pg_attn'
