@@ -296,3 +296,69 @@ def test_nans_from_the_first_id(layout, kind, V):
         for t in (got.given, got.entropy, got.top):
             assert t[:6].isnan().all() and t[6].isfinite().all()
         _check(x[6:], given[6:], top)
+
+
+@pytest.mark.parametrize('kind', DT)
+@pytest.mark.parametrize('V', (70, 1000, 5000, 50257))
+def test_masks_of_a_value(layout, kind, V):
+    """Rows whose masked tokens have a finite value: fewer allowed than are asked for, or as many; the rest by id."""
+    from vesta.logprobs import logprobs
+    gen = _gen(V, 11)
+    allowed = (0, 1, 3, 19, 30, 64, 65, 500)
+    for value in (-1e4, torch.finfo(DT[kind]).min, 7.0):
+        x = torch.full((len(allowed), V), value, device='cuda').to(DT[kind])
+        for row, n in zip(x, allowed):
+            ids = torch.randperm(V, generator=gen, device='cuda')[:n]
+            row[ids] = torch.randn(len(ids), generator=gen, device='cuda').mul_(3).to(row.dtype)
+        given = torch.randint(V, (len(x),), generator=gen, device='cuda')
+        for top in (1, 2, 5, 20, 64):
+            _check(x, given, top)
+        x[:, V // 2] = math.nan                            # (the same order behind a NaN)
+        order = torch.sort(torch.where(x.isnan(), math.inf, x), dim=1, descending=True, stable=True).indices
+        for top in (1, 2, 5, 64):
+            assert torch.equal(logprobs(x, given, top=top).ids.long(), order[:, :top])
+
+
+@pytest.mark.parametrize('kind', DT)
+@pytest.mark.parametrize('V', (2048, 50176, 131072))       # (64 parts of 2 loads in fp32: as many as are joined)
+def test_large_ones_in_few_places(layout, kind, V):
+    """The largest logits where one thread of each wave has them, or two: more than a row's list holds."""
+    vec = 4 if kind == 'f32' else 8
+    x = torch.randn(4, V, generator=_gen(V, 3), device='cuda')
+    load = torch.arange(V, device='cuda') // vec % 64
+    x[0, load == 5] += 40
+    x[1, load == 63] += 40
+    x[2, (load == 0) | (load == 31)] += 40
+    x[2, V // 3] = 50
+    x[3] = torch.where(load == 9, 40.0, -1e4)
+    x = x.to(DT[kind])
+    for top in (1, 3, 20, 64):
+        _check(x, None, top)
+
+
+def _us(call):
+    """The least of some calls' GPU times."""
+    call()
+    best = math.inf
+    for _ in range(5):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3)
+    return best
+
+
+@pytest.mark.parametrize('M,V,kind,top', [(2000, 50257, 'bf16', 64), (200, 128001, 'bf16', 20), (400, 50257, 'f32', 20)])
+def test_reads_of_a_row(M, V, kind, top):
+    """Ties, masks of a finite value and NaNs take a few readings of a row, not one for each alternative."""
+    from vesta.logprobs import logprobs
+    x = torch.randn(M, V, generator=_gen(M), device='cuda').to(DT[kind])
+    plain = _us(lambda: logprobs(x, top=top))
+    masked = torch.full_like(x, -1e4)
+    masked[:, 100:103] = x[:, 100:103]
+    flat, nan = torch.zeros_like(x), x.clone()
+    nan[:, 5] = math.nan
+    for y in (masked, flat, nan):
+        assert _us(lambda: logprobs(y, top=top)) < 8 * plain

@@ -227,15 +227,15 @@ __device__ __forceinline__ float lp_group(const float (*owns)[64], int lane) {
 }
 // -inf as a bound: fewer groups than k have anything else, and what else there is is listed.
 __device__ __forceinline__ float lp_least(float bound) { return fmaxf(bound, -3.402823466e38f); }
-// N of each lane's elements that reach the bound into the list, one of each lane
+// Those of each lane's N elements that reach a bound into the list, one of each lane
 // at a time; the lanes in this branch take places together. (Values are read
-// again: choosing a register takes more.)
-template <int N, typename F>
-__device__ __forceinline__ void lp_list(const lp_t* __restrict__ x, const float* v, float least, lp_key* list, int* listed,
-                                        F id_of) {
+// again: choosing a register takes more.) A full list's length goes on past
+// LP_LIST, by little.
+template <int N, typename R, typename F>
+__device__ __forceinline__ void lp_list(const lp_t* __restrict__ x, R reaches, lp_key* list, int* listed, F id_of) {
   lp_key in = 0;                                                   // bit N - 1 - j: element j
 #pragma unroll
-  for (int j = 0; j < N; ++j) in = in + in + (v[j] >= least ? 1 : 0);
+  for (int j = 0; j < N; ++j) in = in + in + (reaches(j) ? 1 : 0);
 #pragma nounroll
   while (in) {
     const int bit = 63 - __builtin_clzl(in), id = id_of(N - 1 - bit);
@@ -248,6 +248,7 @@ __device__ __forceinline__ void lp_list(const lp_t* __restrict__ x, const float*
       at = __hip_atomic_fetch_add(listed, __builtin_popcountl(lanes), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     at = __builtin_amdgcn_readfirstlane(at) + before;
     if (at < LP_LIST) list[at] = lp_key_of(lp_f(value), id);
+    else in = 0;
   }
 }
 // The listed ones' ranks, of which `found` gets those below k, 64 at a time. Of
@@ -298,6 +299,59 @@ __device__ __forceinline__ void lp_none(const lp_t* __restrict__ x, int n, int f
     at += __builtin_popcountl(all);
   }
   for (int i = at + lane; i < k; i += 64) found(i, 0);
+}
+// Where more reach the bound than are listed (a mask's finite value, a flat row), or
+// there are NaNs: the same with keys in the place of values. No two are equal,
+// and of equal values each group has its lowest id, so that the bound lies among the
+// lowest ids. `chunks` hands out N of a thread's keys (0 for none) and their ids; the row
+// is read twice more, where the largest key below the last, k times, reads it k times
+// (2000 rows of 50257 in bf16, three allowed, 64 asked for 2890 -> 240 us, with a NaN 2750
+// -> 187; 200 of 128001, 20: 354 -> 60, 314 -> 50). The largest alone is found in one
+// reading (8192 flat rows of 50257 in fp32, by keys / one by one: 879 / 662; two of
+// them 884 / 1186, of rows with a NaN 672 / 673).
+// False where these are more than are listed too: single groups have most of the large ones.
+template <int NT, int N, typename C, typename F>
+__device__ __forceinline__ bool lp_by_keys(const lp_t* __restrict__ x, C chunks, lp_key* list, int* listed, int* ranks,
+                                           int k, F found) {
+  static_assert(NT <= LP_LIST, "a key a thread");
+  const int tid = threadIdx.x, lane = tid & 63;
+  lp_key top = 0;
+  chunks([&](auto key, auto) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const lp_key o = key(j);
+      top = o > top ? o : top;
+    }
+  });
+  vh_lds_sync();                                                   // the list's length is read
+  list[tid] = top;
+  if (tid == 0) *listed = 0;
+  vh_lds_sync();
+  lp_key g = list[lane];
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) g = list[64 * w + lane] > g ? list[64 * w + lane] : g;
+  int above = 0;
+#pragma nounroll
+  for (int i = 0; i < 64; ++i) {
+    const unsigned hi = __builtin_amdgcn_readlane((int)(g >> 32), i), lo = __builtin_amdgcn_readlane((int)g, i);
+    above += ((lp_key)hi << 32 | lo) > g ? 1 : 0;
+  }
+  lp_key least = above < k ? g : ~(lp_key)0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const lp_key other = (lp_key)__shfl_xor((long)least, o, 64);
+    least = other < least ? other : least;
+  }
+  least = least ? least : 1;                                       // (fewer groups than k have any)
+  vh_lds_sync();                                                   // the groups are read
+  chunks([&](auto key, auto id) { lp_list<N>(x, [&](int j) { return key(j) >= least; }, list, listed, id); });
+  vh_lds_sync();
+  const int count = *listed;
+  if (count > LP_LIST) return false;
+  lp_order<NT>(list, ranks, count, k, found);
+  if (tid < 64)
+    for (int i = count + lane; i < k; i += 64) found(i, 0);
+  return true;
 }
 // The block's largest key.
 template <int NW>
@@ -387,7 +441,8 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
   const bool odd = a.s != a.s;                                     // a NaN or +inf: found one by one
   if (!odd && own >= least) {
     auto look = [&](int i, const float* v, int) {
-      lp_list<Span::N>(x, v, least, list, &listed, [&](int j) { return first + span.id_of(i, j); });
+      lp_list<Span::N>(x, [&](int j) { return v[j] >= least; }, list, &listed,
+                       [&](int j) { return first + span.id_of(i, j); });
     };
     if (other >= least) {
       span.visit(look);
@@ -410,17 +465,23 @@ __device__ __forceinline__ void lp_rows_body(const lp_t* __restrict__ X, long pi
     if (wave == 0) lp_none(x + first, n, first, count, k, found);
     return;
   }
-  // More reach the bound than are listed (many ties), or there are NaNs: the
-  // largest key below the last, k times.
+  auto chunks = [&](auto see) {
+    span.visit([&](int i, const float* v, int have) {
+      auto id = [&](int j) { return first + span.id_of(i, j); };
+      see([&](int j) { return j < have ? lp_key_of(v[j], id(j)) : (lp_key)0; }, id);
+    });
+  };
+  if (k > 1 && lp_by_keys<NT, Span::N>(x, chunks, list, &listed, ranks, k, found)) return;
+  // the largest key below the last, k times
   __shared__ lp_key best[NW];
   lp_key last = ~(lp_key)0;
   for (int rank = 0; rank < k; ++rank) {
     lp_key top = 0;
-    span.visit([&](int i, const float* v, int have) {
+    chunks([&](auto key, auto) {
 #pragma unroll
       for (int j = 0; j < Span::N; ++j) {
-        const lp_key key = j < have ? lp_key_of(v[j], first + span.id_of(i, j)) : 0;
-        if (key < last && key > top) top = key;
+        const lp_key o = key(j);
+        if (o < last && o > top) top = o;
       }
     });
     last = lp_block_best<NW>(top, best);
@@ -484,7 +545,7 @@ __device__ __forceinline__ void lp_part_body(const lp_t* __restrict__ X, long pi
   LpSums a = {wave_red_max(g), 0.0f, 0.0f};
   if (k) {
     const float least = lp_least(lp_kth(g, k));                    // (each wave by itself)
-    if (own >= least) lp_list<L * LP_VEC>(x, v, least, list, &listed, id_of);
+    if (own >= least) lp_list<L * LP_VEC>(x, [&](int j) { return v[j] >= least; }, list, &listed, id_of);
   }
   const float ref = lp_ref(a.m);
 #pragma unroll
@@ -505,24 +566,32 @@ __device__ __forceinline__ void lp_part_body(const lp_t* __restrict__ X, long pi
   }
   if (k == 0) return;
   const int count = listed;
+  auto found = [&](int rank, lp_key key) { mine[2 + rank] = key; };
   if (a.s == a.s && count <= LP_LIST) {
-    auto found = [&](int rank, lp_key key) { mine[2 + rank] = key; };
     lp_order<NT>(list, ranks, count, k, found);
     if (wave == 0) lp_none(x + first, end - first, first, count, k, found);
     return;
   }
+  auto chunks = [&](auto see) {
+    see([&](int j) {
+      const int e = first + (j / LP_VEC * NT + tid) * LP_VEC, early = e - (V - LP_VEC);
+      return e < end && j % LP_VEC >= early ? lp_key_of(v[j], id_of(j)) : (lp_key)0;
+    }, id_of);
+  };
+  if (k > 1 && lp_by_keys<NT, L * LP_VEC>(x, chunks, list, &listed, ranks, k, found)) return;
   __shared__ lp_key best[NW];
   lp_key last = ~(lp_key)0;
   for (int rank = 0; rank < k; ++rank) {
     lp_key top = 0;
+    chunks([&](auto key, auto) {
 #pragma unroll
-    for (int j = 0; j < L * LP_VEC; ++j) {
-      const int e = first + (j / LP_VEC * NT + tid) * LP_VEC, early = e - (V - LP_VEC);
-      const lp_key key = e < end && j % LP_VEC >= early ? lp_key_of(v[j], id_of(j)) : 0;
-      if (key < last && key > top) top = key;
-    }
+      for (int j = 0; j < L * LP_VEC; ++j) {
+        const lp_key o = key(j);
+        if (o < last && o > top) top = o;
+      }
+    });
     last = lp_block_best<NW>(top, best);
-    if (tid == 0) mine[2 + rank] = last;
+    if (tid == 0) found(rank, last);
     if (last == 0) last = 1;                                       // none left: none after it either
   }
 }

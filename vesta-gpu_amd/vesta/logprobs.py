@@ -13,7 +13,12 @@ with ``given``), and what a server answers with beside its tokens.
 
 Rows are read once, in one launch (two for few long rows), on torch's current
 stream; nothing is read back, so a call can be captured in a HIP graph (after a
-first one of its type of logits). Sums are fp32.
+first one of its type of logits). Sums are fp32. With alternatives asked for, a
+row is read two or three times more where over a thousand of its tokens tie for
+the last of them (a mask of a finite value that leaves fewer than are asked
+for, a flat row), or one is NaN or +inf; bans of -inf do not need that. Only where
+more than a thousand large ones lie in the same places of each 64 loads of 16
+bytes is it read once for each alternative.
 
 A banned token (-inf) has the log probability -inf; a row that bans all has -inf
 throughout and the entropy 0. A NaN or +inf in a row makes its results NaN (ids
