@@ -337,7 +337,8 @@ class VestaGPT2:
         ``vesta.logprobs.LogProbs`` of all M rows: the log probabilities of
         given[i] after row i (of a text, its own next tokens: how well the
         model, or one whose cache holds 8 bits, foretells it), the entropies
-        and the ``top`` most likely tokens.
+        and the ``top`` most likely tokens. Of rows that no sequence has
+        (behind ``starts[B]``) they mean nothing.
 
         Nothing is read back, so a call can be captured in a HIP graph, after
         one call of as many tokens and sequences. Calls share this object's

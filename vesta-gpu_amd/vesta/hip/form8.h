@@ -2,10 +2,12 @@
 // power of two, in the OCP microscaling formats' layout (a byte a block):
 //   PG_FORM 1  whole numbers of +-127: element q of a block with byte s stands for q 2^(s - 133)
 //   PG_FORM 2  e4m3 floats (up to 448): element x for x 2^(s - 127)
-// The power is the least with which a block's largest value rounds to an element,
-// within limits that make every value one of fp16 (bf16 where PG_KIND is), so
-// that opening an element is exact and what attention multiplies is what the
-// cache holds. A power of two costs e4m3 nothing and whole numbers half a bit on
+// The power is the least with which a block's largest value is below 127.5 or 464
+// steps of it, within limits that make every value one of fp16 (bf16 where PG_KIND is),
+// so that opening an element is exact and what attention multiplies is what the
+// cache holds. (Whole numbers read as bf16 end at 127 2^119, two powers below the
+// type's end: they are opened as (q + 128) f - 128 f, which the last power would make
+// an infinity.) A power of two costs e4m3 nothing and whole numbers half a bit on
 // average against any factor; a block of its own for 32 dims gains about as
 // much, and keeps the head's small dims apart from its large ones.
 //

@@ -69,7 +69,7 @@ BLOCK_BYTES = 128 << 10
 CU_ROWS = 256
 # Rows of more than so many bytes are dealt to blocks whose elements stay in registers (lp_part), and a second launch joins
 # them: it takes 5 us of the host's more, and for short rows saves less (whole / in parts; 8 x 50,257 7.0 / 4.9, k 5 9.1 /
-# 7.2, one call after another from Python 13.5 / 18.6) ...
+# 7.2, one call after another from Python 13.5 / 18.6). A captured call, which does without the host, is laid out alike ...
 PART_BYTES = 240 << 10
 # ... for up to so many rows (64 x 128,001 bf16, k 20: 19.1 / 13.5; 100: 19.9 / 18.4; 200: 20.6 / 26.6) ...
 PARTS_ROWS = 64

@@ -12,19 +12,24 @@ bytes, read half as many here.
 
 Each 32 values of a row are 8-bit elements and one power of two, the byte layout
 of the OCP microscaling formats. A block's power is the least with which its
-largest value rounds to an element; values are rounded to nearest, a tie to even.
+largest value is below 127.5 ('i8') or 464 ('e4m3') steps of it; values are
+rounded to nearest, a tie to even.
 
 * ``form='i8'``: whole numbers of +-127; a value is off by at most 1/127 of its
-  block's largest (1/255 where the largest is just below a power of two). A block
-  with an infinity or a NaN is held as NaNs.
+  block's largest (1/255 where that is just below 127.5/128 of a power of two). A
+  block with an infinity or a NaN is held as NaNs.
 * ``form='e4m3'``: floats of 4 bits exponent and 3 bits fraction; a value is off by
   at most 1/16 of itself, or by 2^-17.8 of its block's largest where that is more. An
   infinity or NaN is held as a NaN.
 
-Powers are limited such that every value is one of ``dtype``'s: over 'f16' steps
-of 2^-24 at least, sizes of 65024 ('i8') or 57344 ('e4m3') at most, larger ones
-held as these. So nothing is rounded after the cache: attention multiplies what
-it holds, in 16 bits ('f16': f16 or f32 queries; 'bf16': bf16).
+This holds within the powers that there are, which are limited such that every
+value is one of ``dtype``'s: over 'f16' steps of 2^-24 at least and sizes of 65024
+('i8') or 57344 ('e4m3') at most, over 'bf16' steps of 2^-126 and sizes of 127 2^119
+(8.4e37) or 448 2^119 (3.0e38); larger values are held as these. So what attention
+multiplies is what the cache holds, in 16 bits ('f16': f16 or f32 queries; 'bf16':
+bf16), its softmax weights rounded as over a 16-bit cache; under f16 and f32
+queries the products of values below 2^-14 are right to 2^-38 absolutely, not
+relatively.
 
 No weights are counted and nothing is evicted here.
 """
@@ -43,7 +48,9 @@ LEAST = {('i8', 'f16'): 109, ('i8', 'bf16'): 7, ('e4m3', 'f16'): 112, ('e4m3', '
 
 # Bytes of elements in all layers' pools that a token's pass may read from which pg_attn loads them past the memory-side
 # cache, which cannot keep them until the next token's (through it / past it, 8 heads of 128: two of 209 MB 54.1 / 52.2 us,
-# one of 426 100.4 / 95.5; what fits is better kept: one of 209 45.1 / 52.0, of 304 63.1 / 67.5, of 333 75.2 / 75.7).
+# one of 426 100.4 / 95.5; what fits is better kept: one of 209 45.1 / 52.0, of 304 63.1 / 67.5, of 333 75.2 / 75.7). The
+# bytes are those that the tables have room for: how many positions there are is known on the device only. A table much
+# wider than its sequences are long loses what the cache would have kept (45.1 / 52.0).
 ATTEND_PAST = MEM_CACHE_BYTES * 5 // 4
 # Heads of 128 whose 16-bit rows a wave of append takes together, one position's, where it has a multiple of them: its
 # place is found once, by scalar operations (12,900 rows of 8 heads, a head of eight rows / eight heads of one: 17.1 /
